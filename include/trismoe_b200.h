@@ -731,6 +731,142 @@ int tris_moe_layer_forward_static(const TrisMoeLayerView* layer, const void* x_f
                                   const float* router_logits, int32_t num_tokens, void* y_f16,
                                   float* router_logits_out, void* stream);
 
+/* ---- decode step around the experts ------------------------------------------------- */
+/* No reference counterpart: its attention, norms and sampling are stock PyTorch (MO:300-618, 1120-1200). */
+
+enum { TRIS_DTYPE_F16 = 0, TRIS_DTYPE_BF16 = 1, TRIS_DTYPE_F32 = 2, TRIS_DTYPE_E4M3 = 3 };
+
+/*
+ * Pages of one layer's key/value cache and the block table that says which of them a sequence has.  Element [p, s, h, d] of the
+ * keys is at k_pages[p * k_page_stride + s * k_token_stride + h * k_head_stride + d] (strides in elements, the head's dimensions side by
+ * side).  Bases, and strides in bytes, are multiples of 16.  Token i of sequence b is in slot i % page_size of page
+ * block_table[b * table_stride + i / page_size].
+ * e4m3 pages hold x / scale of their head, saturated at +-448; without scales that is 1.
+ * status_dev (optional device int32, sticky) is set to TRIS_ERR_CORRUPT where a needed page is outside [0, num_pages), a position outside the
+ * table or the rotation tables, or a length above table_width * page_size.  Such tokens are not written, read as zeros, or cut off.
+ */
+typedef struct TrisPagedKv {
+  void* k_pages;
+  void* v_pages;
+  int64_t k_page_stride, k_token_stride, k_head_stride;
+  int64_t v_page_stride, v_token_stride, v_head_stride;
+  const float* k_scale;             /* [num_kv_heads] or NULL; TRIS_DTYPE_E4M3 only       */
+  const float* v_scale;
+  const int32_t* block_table;       /* [num_sequences, table_width]                        */
+  int64_t table_stride;             /* entries between two sequences                       */
+  int32_t num_sequences;
+  int32_t table_width;              /* pages of a sequence                                 */
+  int32_t num_pages;
+  int32_t page_size;                /* tokens of a page, any number >= 1                   */
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t dtype;                    /* F16, BF16 (that of the rows) or E4M3                */
+  int32_t reserved0;
+  int32_t* status_dev;
+} TrisPagedKv;
+
+/*
+ * New tokens of a projection: row t of q / k / v has its heads of head_dim elements head_stride apart.  Token t belongs to sequence
+ * sequences[t] (NULL: t) and stands at positions[t]; a negative position is padding: nothing is written to the cache, its rows of q_out
+ * and k_out are zeros.  The first rotary_dim dimensions of q and k are rotated by the position's row of cos / sin
+ * [max_positions, rotary_dim / 2] - pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved - in fp32 and rounded once.
+ */
+typedef struct TrisPagedAppend {
+  const void* q;                    /* NULL (with num_q_heads 0): keys and values only     */
+  const void* k;
+  const void* v;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const float* cos;                 /* NULL: no rotation                                   */
+  const float* sin;
+  const void* positions;            /* [num_tokens] int32, or int64                        */
+  const int32_t* sequences;
+  void* q_out;                      /* [num_tokens, num_q_heads, head_dim]                 */
+  void* k_out;                      /* [num_tokens, num_kv_heads, head_dim] or NULL        */
+  int32_t num_tokens;
+  int32_t num_q_heads;
+  int32_t rotary_dim;               /* even, <= head_dim                                   */
+  int32_t max_positions;            /* rows of cos and sin                                 */
+  int32_t positions_are_64bit;
+  int32_t interleaved;
+  int32_t dtype;                    /* F16 or BF16                                         */
+  int32_t reserved0;
+} TrisPagedAppend;
+int tris_paged_kv_append(const TrisPagedKv* cache, const TrisPagedAppend* rows, void* stream);
+
+/*
+ * Attention of one new token per sequence over the cache: out = softmax(softmax_scale * q . k) . v over the tokens [lengths[b] - window, lengths[b])
+ * (window 0: all).  A sequence of length 0 gives zeros, and -inf for lse (natural logarithm of the softmax's sum).
+ * Query head h reads key/value head h / (num_q_heads / num_kv_heads).  head_dim is a multiple of 8 (E4M3: 16) up to 256.
+ */
+typedef struct TrisPagedAttention {
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  const int32_t* lengths;           /* [num_sequences]                                     */
+  void* out;                        /* [num_sequences, num_q_heads, head_dim], q's type    */
+  float* lse;                       /* [num_sequences, num_q_heads] or NULL                */
+  void* workspace;                  /* 16-byte aligned                                     */
+  int64_t workspace_bytes;
+  int32_t num_q_heads;
+  int32_t window;
+  int32_t dtype;                    /* F16 or BF16                                         */
+  float softmax_scale;
+} TrisPagedAttention;
+/* Scratch for any lengths that the table has room for; 0 for arguments that the call would refuse. */
+size_t tris_paged_decode_attention_workspace_bytes(const TrisPagedKv* cache, int32_t num_q_heads);
+int tris_paged_decode_attention(const TrisPagedKv* cache, const TrisPagedAttention* query, void* stream);
+
+/*
+ * h = residual + x; y = h / sqrt(mean(h^2) + eps) * weight, each row by itself in fp32 (h is rounded for residual_out only).
+ * y in the rows' type, or (dtype_out E4M3) as y / scale with one scale (largest magnitude / 448, 0 for zeros) per group of group_size
+ * columns: group_size is a multiple of 16 that divides hidden_size, or hidden_size.  residual and residual_out may be NULL, and the same.
+ */
+typedef struct TrisAddRmsNorm {
+  const void* x;
+  const void* residual;
+  const void* weight;               /* [hidden_size], the rows' type                       */
+  void* residual_out;
+  void* y;
+  float* scales;                    /* [rows, hidden_size / group_size], E4M3 only         */
+  int64_t x_stride, residual_stride, residual_out_stride, y_stride;   /* elements between rows */
+  int32_t rows;
+  int32_t hidden_size;
+  int32_t group_size;
+  int32_t dtype;                    /* F16 or BF16                                         */
+  int32_t dtype_out;                /* dtype, or E4M3                                      */
+  float eps;
+} TrisAddRmsNorm;
+int tris_add_rms_norm(const TrisAddRmsNorm* args, void* stream);
+
+/*
+ * Controls on logits before a token is chosen, in this order, each optional (NULL):
+ *   repetition[b] > 0: logits of tokens in tokens[b, 0 .. token_lengths[b]) are divided by it where positive, else multiplied
+ *   frequency[b], presence[b]: z -= frequency * n + presence * (n > 0), n = how often the token occurs from prompt_lengths[b] on
+ *   bias_ids / bias_values [rows, num_biases]: z += value (negative ids are skipped; repeated ids add up in their order)
+ *   allowed [rows, ceil(vocab / 32)], bit v % 32 of word v / 32: z = -inf where it is 0
+ * Token ids outside [0, vocab) are skipped.  out is fp32 and may be the logits themselves if they are.
+ */
+typedef struct TrisLogitControls {
+  const void* logits;
+  float* out;
+  const int32_t* tokens;
+  const int32_t* token_lengths;
+  const int32_t* prompt_lengths;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_ids;
+  const float* bias_values;
+  const int32_t* allowed;
+  int64_t logits_stride, out_stride, tokens_stride, bias_stride, allowed_stride;
+  int32_t rows;
+  int32_t vocab;
+  int32_t max_tokens;               /* columns of tokens                                   */
+  int32_t num_biases;
+  int32_t dtype;                    /* of the logits: F16, BF16 or F32                     */
+  int32_t reserved0;
+} TrisLogitControls;
+int tris_logit_controls(const TrisLogitControls* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

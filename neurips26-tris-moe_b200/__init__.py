@@ -44,9 +44,23 @@ from .ns_compensation import (  # noqa: F401
     run_grouped_ns_c1_forward,
     run_grouped_ns_compensation_forward,
 )
+from .decode_ops import (  # noqa: F401
+    add_rms_norm,
+    add_rms_norm_e4m3,
+    append_paged_kv,
+    apply_logit_controls,
+    paged_decode_attention,
+    raise_on_status,
+)
 from . import clocks, envflags, expert_parallel, synth  # noqa: F401
 
 __all__ = [
+    "add_rms_norm",
+    "add_rms_norm_e4m3",
+    "append_paged_kv",
+    "apply_logit_controls",
+    "paged_decode_attention",
+    "raise_on_status",
     "Packed4Linear",
     "build_grouped_ns_compensation_payload",
     "run_grouped_ns_c1_forward",

@@ -21,6 +21,7 @@ STATUS_NAMES = {
 
 _vp = C.c_void_p
 _i32 = C.c_int32
+_i64 = C.c_int64
 
 
 class TrisProjView(C.Structure):
@@ -98,6 +99,53 @@ class TrisSharedExpert(C.Structure):
     _fields_ = [("gate", _vp), ("up", _vp), ("down", _vp), ("gate_weight", _vp)]
 
 
+class TrisPagedKv(C.Structure):
+    _fields_ = [
+        ("k_pages", _vp), ("v_pages", _vp),
+        ("k_page_stride", _i64), ("k_token_stride", _i64), ("k_head_stride", _i64),
+        ("v_page_stride", _i64), ("v_token_stride", _i64), ("v_head_stride", _i64),
+        ("k_scale", _vp), ("v_scale", _vp), ("block_table", _vp), ("table_stride", _i64),
+        ("num_sequences", _i32), ("table_width", _i32), ("num_pages", _i32), ("page_size", _i32),
+        ("num_kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32), ("reserved0", _i32), ("status_dev", _vp),
+    ]
+
+
+class TrisPagedAppend(C.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp),
+        ("q_token_stride", _i64), ("q_head_stride", _i64), ("k_token_stride", _i64), ("k_head_stride", _i64),
+        ("v_token_stride", _i64), ("v_head_stride", _i64),
+        ("cos", _vp), ("sin", _vp), ("positions", _vp), ("sequences", _vp), ("q_out", _vp), ("k_out", _vp),
+        ("num_tokens", _i32), ("num_q_heads", _i32), ("rotary_dim", _i32), ("max_positions", _i32),
+        ("positions_are_64bit", _i32), ("interleaved", _i32), ("dtype", _i32), ("reserved0", _i32),
+    ]
+
+
+class TrisPagedAttention(C.Structure):
+    _fields_ = [
+        ("q", _vp), ("q_token_stride", _i64), ("q_head_stride", _i64), ("lengths", _vp), ("out", _vp), ("lse", _vp),
+        ("workspace", _vp), ("workspace_bytes", _i64), ("num_q_heads", _i32), ("window", _i32), ("dtype", _i32),
+        ("softmax_scale", C.c_float),
+    ]
+
+
+class TrisAddRmsNorm(C.Structure):
+    _fields_ = [
+        ("x", _vp), ("residual", _vp), ("weight", _vp), ("residual_out", _vp), ("y", _vp), ("scales", _vp),
+        ("x_stride", _i64), ("residual_stride", _i64), ("residual_out_stride", _i64), ("y_stride", _i64),
+        ("rows", _i32), ("hidden_size", _i32), ("group_size", _i32), ("dtype", _i32), ("dtype_out", _i32), ("eps", C.c_float),
+    ]
+
+
+class TrisLogitControls(C.Structure):
+    _fields_ = [
+        ("logits", _vp), ("out", _vp), ("tokens", _vp), ("token_lengths", _vp), ("prompt_lengths", _vp),
+        ("repetition", _vp), ("presence", _vp), ("frequency", _vp), ("bias_ids", _vp), ("bias_values", _vp), ("allowed", _vp),
+        ("logits_stride", _i64), ("out_stride", _i64), ("tokens_stride", _i64), ("bias_stride", _i64), ("allowed_stride", _i64),
+        ("rows", _i32), ("vocab", _i32), ("max_tokens", _i32), ("num_biases", _i32), ("dtype", _i32), ("reserved0", _i32),
+    ]
+
+
 # name -> (restype, argtypes); also the list of symbols include/trismoe_b200.h declares.
 _P = C.POINTER
 SIGNATURES = {
@@ -156,6 +204,12 @@ SIGNATURES = {
     "tris_moe_layer_forward_shared": (C.c_int, [_P(TrisMoeLayerView), _P(TrisSharedExpert), _vp, _vp, _i32, _vp, _vp, _vp, C.c_size_t, _vp, C.c_size_t, _vp]),
     "tris_paged_records_plan": (C.c_int, [_P(TrisProjView), _vp, _vp]),
     "tris_moe_layer_forward_paged": (C.c_int, [_P(TrisMoeLayerView), _P(TrisPagedLayer), _vp, _vp, _i32, _vp, _vp, _vp, C.c_size_t, _vp, _vp]),
+    # pointers to the structs above; packed bytes are passed on the way that counts (decode_ops.py)
+    "tris_paged_kv_append": (C.c_int, [_vp, _vp, _vp]),
+    "tris_paged_decode_attention_workspace_bytes": (C.c_size_t, [_vp, _i32]),
+    "tris_paged_decode_attention": (C.c_int, [_vp, _vp, _vp]),
+    "tris_add_rms_norm": (C.c_int, [_vp, _vp]),
+    "tris_logit_controls": (C.c_int, [_vp, _vp]),
     "tris_moe_layer_forward_static": (C.c_int, [_P(TrisMoeLayerView), _vp, _vp, _i32, _vp, _vp, _vp]),
 }
 STATIC_SCRATCH_BYTES = 8 << 20

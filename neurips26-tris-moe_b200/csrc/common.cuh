@@ -13,6 +13,8 @@ static_assert(sizeof(TrisRouteView) == 80, "TrisRouteView layout is part of the 
 static_assert(sizeof(TrisSharedExpert) == 32, "TrisSharedExpert layout is part of the ABI");
 static_assert(sizeof(TrisPageLaunch) == 24, "TrisPageLaunch layout is part of the ABI");
 static_assert(sizeof(TrisPagedLayer) == 1472, "TrisPagedLayer layout is part of the ABI");
+static_assert(sizeof(TrisPagedKv) == 136 && sizeof(TrisPagedAppend) == 152 && sizeof(TrisPagedAttention) == 80, "layouts are part of the ABI");
+static_assert(sizeof(TrisAddRmsNorm) == 104 && sizeof(TrisLogitControls) == 152, "layouts are part of the ABI");
 
 namespace tris {
 

@@ -1,0 +1,74 @@
+// What the kernels of the decode step around the experts share (paged_kv.cu, paged_attention.cu, rms_norm.cu, logit_controls.cu):
+// element types, loads and stores of eight values, page lookup.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace tris {
+
+constexpr float kE4m3Max = 448.f;
+
+template <typename T>
+struct Pair;  // two elements of a 16-bit type in one register
+template <>
+struct Pair<__half> {
+  static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 unpack(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ void store_float(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store_float(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store_float(__nv_fp8_e4m3* p, float v) { p->__x = __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
+
+// Eight elements by one 16-byte access (8 bytes of e4m3).
+template <typename T>
+__device__ __forceinline__ void load_8(const T* p, float (&v)[8]) {
+  const uint4 raw = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Pair<T>::unpack(w[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_8(T* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(Pair<T>::pack(v[0], v[1]), Pair<T>::pack(v[2], v[3]), Pair<T>::pack(v[4], v[5]), Pair<T>::pack(v[6], v[7]));
+}
+__device__ __forceinline__ uint32_t e4m3_pack4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+__device__ __forceinline__ void store_8(__nv_fp8_e4m3* p, const float (&v)[8]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(e4m3_pack4(v[0], v[1], v[2], v[3]), e4m3_pack4(v[4], v[5], v[6], v[7]));
+}
+
+// Maximum that keeps a NaN (fmaxf drops it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+inline int dtype_size(int dtype) { return dtype == TRIS_DTYPE_F32 ? 4 : dtype == TRIS_DTYPE_E4M3 ? 1 : 2; }
+int validate_paged_kv(const TrisPagedKv* cache, const char* what);  // paged_kv.cu
+
+}  // namespace tris

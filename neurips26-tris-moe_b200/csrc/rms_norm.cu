@@ -1,0 +1,220 @@
+// Residual addition and root-mean-square norm of rows in one pass, with an output in the rows' type or in e4m3 with scales.
+//
+// h = residual + x; y = h * w / sqrt(mean(h^2) + eps).  The mean needs the whole row before the first output, so a row stays in the registers of
+// the CTA that reads it: x and residual are read once, h and y written once.  Bound by bytes for many rows, by the chain load -> sum -> store for one.
+// The sums are fp32, h is not rounded before it is squared or scaled.  e4m3: y / s with s = max |y| / 448 of the group, so the group's largest
+// element is representable and none saturates; a second exchange between threads gives the maxima.
+#include "decode_step.cuh"
+
+namespace tris {
+namespace {
+
+constexpr int kMaxVectors = 8;  // of 8 columns that a thread keeps
+constexpr int most_threads(int vectors) { return vectors >= 4 ? 512 : 1024; }  // whose rows fit the registers
+
+__device__ __forceinline__ float block_sum(float v, float* red) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.f;
+  for (unsigned w = 0; w < blockDim.x / 32; ++w) v += red[w];
+  return v;
+}
+__device__ __forceinline__ float block_max(float v, float* red) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v = max_nan(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = red[0];
+  for (unsigned w = 1; w < blockDim.x / 32; ++w) v = max_nan(v, red[w]);
+  return v;
+}
+
+// Rows of at most 8 * VECS * blockDim columns, all pointers and strides at 16-byte boundaries.
+template <typename T, bool FP8, int VECS>
+__global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const __grid_constant__ TrisAddRmsNorm a) {
+  __shared__ float red[32], red_max[32];
+  extern __shared__ float vector_max[];  // groups that do not fit a warp: largest element of every vector
+  const int tid = threadIdx.x, vectors = a.hidden_size / 8;
+  const T* weight = static_cast<const T*>(a.weight);
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
+  float h[VECS][8], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int v = tid + i * blockDim.x;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) h[i][k] = 0.f;
+    if (v < vectors) {
+      load_8(x + 8 * v, h[i]);
+      if (res) {
+        float r[8];
+        load_8(res + 8 * v, r);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[i][k] += r[k];
+      }
+      if (a.residual_out) store_8(static_cast<T*>(a.residual_out) + row * a.residual_out_stride + 8 * v, h[i]);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += h[i][k] * h[i][k];
+  }
+  const float inv = 1.f / sqrtf(block_sum(sum, red) / a.hidden_size + a.eps);
+
+  if constexpr (!FP8) {
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int v = tid + i * blockDim.x;
+      if (v < vectors) {
+        float w[8];
+        load_8(weight + 8 * v, w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[i][k] = h[i][k] * inv * w[k];
+        store_8(static_cast<T*>(a.y) + row * a.y_stride + 8 * v, h[i]);
+      }
+    }
+  } else {
+    float top[VECS], all = 0.f;
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int v = tid + i * blockDim.x;
+      top[i] = 0.f;
+      if (v < vectors) {
+        float w[8];
+        load_8(weight + 8 * v, w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          h[i][k] = h[i][k] * inv * w[k];
+          top[i] = max_nan(top[i], fabsf(h[i][k]));
+        }
+      }
+      all = max_nan(all, top[i]);
+    }
+    const int per_group = a.group_size / 8;  // vectors
+    if (a.group_size == a.hidden_size) {
+      all = block_max(all, red_max);
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) top[i] = all;
+    } else if (per_group <= 32 && (per_group & (per_group - 1)) == 0) {
+      // neighbours in a warp; vectors past the row only meet one another
+      for (int d = per_group / 2; d; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) top[i] = max_nan(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], d));
+    } else {
+#pragma unroll
+      for (int i = 0; i < VECS; ++i)
+        if (tid + i * blockDim.x < vectors) vector_max[tid + i * blockDim.x] = top[i];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) {
+        const int v = tid + i * blockDim.x;
+        if (v < vectors)
+          for (int k = v / per_group * per_group, e = k + per_group; k < e; ++k) top[i] = max_nan(top[i], vector_max[k]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int v = tid + i * blockDim.x;
+      if (v < vectors) {
+        const float scale = top[i] / kE4m3Max;
+        const float div = scale == 0.f ? 1.f : scale;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[i][k] /= div;
+        store_8(static_cast<__nv_fp8_e4m3*>(a.y) + row * a.y_stride + 8 * v, h[i]);
+        if (v % per_group == 0) a.scales[row * (a.hidden_size / a.group_size) + v / per_group] = scale;
+      }
+    }
+  }
+}
+
+// Any width and alignment: element by element, the row read again for every use.  Each element is read and written by one thread, so the outputs
+// may lie on the inputs: what is read again after a store is not needed from there any more.
+template <typename T, bool FP8>
+__global__ void __launch_bounds__(1024) add_rms_norm_any_kernel(const __grid_constant__ TrisAddRmsNorm a) {
+  __shared__ float red[32], red_max[32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
+  const T* weight = static_cast<const T*>(a.weight);
+  auto sum_at = [&](int i) { return to_float(x[i]) + (res ? to_float(res[i]) : 0.f); };
+  float sum = 0.f;
+  for (int i = threadIdx.x; i < a.hidden_size; i += blockDim.x) {
+    const float h = sum_at(i);
+    sum += h * h;
+  }
+  const float inv = 1.f / sqrtf(block_sum(sum, red) / a.hidden_size + a.eps);
+  const int groups = FP8 ? a.hidden_size / a.group_size : 1, width = FP8 ? a.group_size : a.hidden_size;
+  for (int q = 0; q < groups; ++q) {
+    float div = 1.f;
+    if constexpr (FP8) {
+      float top = 0.f;
+      for (int i = q * width + threadIdx.x; i < (q + 1) * width; i += blockDim.x) top = max_nan(top, fabsf(sum_at(i) * inv * to_float(weight[i])));
+      __syncthreads();  // red_max of the group before
+      const float scale = block_max(top, red_max) / kE4m3Max;
+      div = scale == 0.f ? 1.f : scale;
+      if (threadIdx.x == 0) a.scales[row * groups + q] = scale;
+    }
+    for (int i = q * width + threadIdx.x; i < (q + 1) * width; i += blockDim.x) {
+      const float h = sum_at(i), y = h * inv * to_float(weight[i]);
+      if (a.residual_out) store_float(static_cast<T*>(a.residual_out) + row * a.residual_out_stride + i, h);
+      if constexpr (FP8)
+        store_float(static_cast<__nv_fp8_e4m3*>(a.y) + row * a.y_stride + i, y / div);
+      else
+        store_float(static_cast<T*>(a.y) + row * a.y_stride + i, y);
+    }
+  }
+}
+
+template <typename T, bool FP8>
+int launch_norm(const TrisAddRmsNorm& a, cudaStream_t stream) {
+  const int H = a.hidden_size;
+  const bool pdl = programmatic_launch_default();
+  const int64_t strides[4] = {a.x_stride, a.residual ? a.residual_stride : 0, a.residual_out ? a.residual_out_stride : 0, a.y_stride};
+  bool wide = H % 8 == 0 && H <= 8 * kMaxVectors * most_threads(kMaxVectors);
+  for (int64_t s : strides) wide = wide && s % 8 == 0;
+  for (const void* p : {a.x, a.residual, a.weight, static_cast<const void*>(a.residual_out), static_cast<const void*>(a.y)}) wide = wide && (!p || aligned_to(p, 16));
+  if (!wide) {
+    TRIS_CUDA(launch_kernel(add_rms_norm_any_kernel<T, FP8>, dim3(a.rows), dim3(H >= 1024 ? 1024 : (H + 31) / 32 * 32), 0, stream, pdl, 1, a));
+    return TRIS_OK;
+  }
+  const int vectors = H / 8;
+  // few rows: as many threads as vectors, the chain of one row is what counts; many: fewer threads with more loads in flight each
+  int vecs = 1;
+  while (vecs < kMaxVectors && (ceil_div(vectors, vecs) > most_threads(vecs) || (a.rows > 148 && ceil_div(vectors, vecs) > 256))) vecs *= 2;
+  const int threads = (ceil_div(vectors, vecs) + 31) / 32 * 32;
+  const int per_group = FP8 ? a.group_size / 8 : 0;
+  const bool in_warp = per_group <= 32 && (per_group & (per_group - 1)) == 0;
+  const size_t smem = FP8 && a.group_size != H && !in_warp ? sizeof(float) * vectors : 0;
+  auto kernel = vecs == 1 ? add_rms_norm_kernel<T, FP8, 1> : vecs == 2 ? add_rms_norm_kernel<T, FP8, 2> : vecs == 4 ? add_rms_norm_kernel<T, FP8, 4> : add_rms_norm_kernel<T, FP8, 8>;
+  TRIS_CUDA(launch_kernel(kernel, dim3(a.rows), dim3(threads), smem, stream, pdl, 1, a));
+  return TRIS_OK;
+}
+
+}  // namespace
+}  // namespace tris
+
+using namespace tris;
+
+extern "C" int tris_add_rms_norm(const TrisAddRmsNorm* args, void* stream) {
+  TRIS_REQUIRE(args, TRIS_ERR_INVALID_ARG, "add_rms_norm: null arguments");
+  const TrisAddRmsNorm& a = *args;
+  TRIS_REQUIRE(a.dtype == TRIS_DTYPE_F16 || a.dtype == TRIS_DTYPE_BF16, TRIS_ERR_INVALID_ARG, "add_rms_norm: rows are fp16 or bf16");
+  TRIS_REQUIRE(a.dtype_out == a.dtype || a.dtype_out == TRIS_DTYPE_E4M3, TRIS_ERR_INVALID_ARG, "add_rms_norm: the output has the rows' type or e4m3");
+  TRIS_REQUIRE(a.rows >= 0 && a.hidden_size >= 1, TRIS_ERR_INVALID_ARG, "add_rms_norm: negative sizes");
+  if (a.rows == 0) return TRIS_OK;
+  TRIS_REQUIRE(a.x && a.weight && a.y, TRIS_ERR_INVALID_ARG, "add_rms_norm: null x, weight or y");
+  const bool fp8 = a.dtype_out == TRIS_DTYPE_E4M3;
+  if (fp8) {
+    TRIS_REQUIRE(a.scales, TRIS_ERR_INVALID_ARG, "add_rms_norm: null scales");
+    TRIS_REQUIRE(a.group_size == a.hidden_size || (a.group_size > 0 && a.group_size % 16 == 0 && a.hidden_size % a.group_size == 0), TRIS_ERR_INVALID_ARG,
+                 "add_rms_norm: groups of %d columns do not divide rows of %d in multiples of 16", a.group_size, a.hidden_size);
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a.dtype == TRIS_DTYPE_F16) return fp8 ? launch_norm<__half, true>(a, s) : launch_norm<__half, false>(a, s);
+  return fp8 ? launch_norm<__nv_bfloat16, true>(a, s) : launch_norm<__nv_bfloat16, false>(a, s);
+}
