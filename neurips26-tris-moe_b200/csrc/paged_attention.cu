@@ -13,8 +13,7 @@
 // 8 columns, so that a step of 16 tokens costs two MMAs per 16 dimensions with up to 8 heads (with the heads as rows it would cost four, half
 // of them zeros).  No operand goes through a transposing load: the order of dimensions inside a product is free as long as both operands have the
 // same, so a lane's 16 bytes of a key row are its fragments as they are; of four value rows a lane has the same 8 dimensions, whose pairs of
-// tokens are put together by PRMT.  A lane therefore reads from shared memory exactly what it has itself copied there (cp.async): the ring
-// of a warp needs no barrier, and serves as a queue of loads in flight instead of registers.
+// tokens are put together by PRMT.  Each warp has a ring of its own in shared memory, filled by cp.async, and meets no other warp before it is done.
 #include <type_traits>
 
 #include "decode_step.cuh"
@@ -23,6 +22,7 @@ namespace tris {
 namespace {
 
 constexpr int kBlock = 16;  // tokens of a step
+constexpr int kWarps = 4;   // of a CTA
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnArgs {
@@ -32,10 +32,13 @@ struct AttnArgs {
   int row_tiles;    // tiles of kHeads query heads it takes
   int tile_heads;   // heads of a tile that exist at most
   int page_shift;   // log2(page_size), or -1
-  int min_run;      // blocks a warp takes at least
-  int workers;      // warps of the grid
-  float* part_o;    // [2 * workers][tile_heads][head_dim]
-  float* part_ml;   // [2 * workers][tile_heads][2]
+  int page_blocks;  // whether a block of 16 tokens never crosses a page
+  int wide_query;   // whether q's heads start on 16-byte boundaries
+  int ctas;         // of the first kernel
+  int resident;     // of them, at one time
+  int rows_together;  // whether a head's rows in a page are side by side
+  float* part_o;    // [2 * ctas][tile_heads][head_dim]
+  float* part_ml;   // [2 * ctas][tile_heads][2]
 };
 
 template <typename T>
@@ -56,10 +59,21 @@ __device__ __forceinline__ uint32_t e4m3_to_h2(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
   return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
 }
+__device__ __forceinline__ void cp_async_16_at(uint32_t dst, const void* src, int bytes) {  // bytes: 16, or 0 for zeros
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// 2^x; results below 2^-126 are 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
+// Tokens [lo, hi) of a sequence; its blocks begin at multiples of kBlock.
 struct Span {
-  int lo, hi;  // tokens [lo, hi)
-  __device__ __forceinline__ int blocks() const { return (hi - lo + kBlock - 1) / kBlock; }
+  int lo, hi;
+  __device__ __forceinline__ int first() const { return lo / kBlock; }
+  __device__ __forceinline__ int blocks() const { return hi > lo ? (hi - 1) / kBlock - lo / kBlock + 1 : 0; }
 };
 __device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
   const int64_t room = static_cast<int64_t>(a.cache.table_width) * a.cache.page_size;
@@ -68,17 +82,39 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
   return {a.query.window > 0 && hi > a.query.window ? hi - a.query.window : 0, hi};
 }
 
-// Blocks ahead of sequence `stop` (all lanes get the sum); the number of sequences is small and the lengths stay in L1.
-__device__ __forceinline__ int64_t blocks_before(const AttnArgs& a, int stop, int lane) {
-  int64_t sum = 0;
-  for (int b = lane; b < stop; b += 32) sum += span_of(a, b).blocks();
+// Blocks of sequences [32 i, 32 i + 32) up to and with each lane's own, times the items of a sequence.  (Block numbers fit 32 bits: the host sees to it.)
+__device__ __forceinline__ int scan_blocks(const AttnArgs& a, int i, int lane, int& mine) {
+  const int b = 32 * i + lane;
+  mine = b < a.cache.num_sequences ? span_of(a, b).blocks() * (a.cache.num_kv_heads * a.row_tiles) : 0;
+  int upto = mine;
 #pragma unroll
-  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-  return sum * a.cache.num_kv_heads * a.row_tiles;
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+    if (lane >= d) upto += v;
+  }
+  return upto;
 }
-__device__ __forceinline__ int64_t run_length(const AttnArgs& a, int64_t total) {
-  const int64_t even = (total + a.workers - 1) / a.workers;
-  return even > a.min_run ? even : a.min_run;
+// All blocks, and those ahead of sequence `stop`.
+__device__ __forceinline__ int count_blocks(const AttnArgs& a, int stop, int lane, int& before) {
+  int total = 0;
+  before = 0;
+  for (int i = 0; 32 * i < a.cache.num_sequences; ++i) {
+    int mine;
+    const int upto = scan_blocks(a, i, lane, mine);
+    if (stop / 32 == i) before = total + __shfl_sync(0xFFFFFFFFu, upto - mine, stop % 32);
+    total += __shfl_sync(0xFFFFFFFFu, upto, 31);
+  }
+  return total;
+}
+// Blocks that each warp takes.  The grid has as many CTAs as are resident twice over, so that an SM that is done early takes another one; where that
+// would leave a warp fewer than kMinRun blocks, half of them do the work.
+constexpr int kMinRun = 24;
+__device__ __forceinline__ int run_length(const AttnArgs& a, int total) {
+  const unsigned workers = static_cast<unsigned>(a.ctas) * kWarps;
+  const unsigned run = (static_cast<unsigned>(total) + workers - 1) / workers;
+  if (run >= kMinRun || a.resident >= a.ctas) return run;
+  const unsigned fewer = static_cast<unsigned>(a.resident) * kWarps;
+  return (static_cast<unsigned>(total) + fewer - 1) / fewer;
 }
 
 // Where a warp is in the numbering: block `blk` of `span`, head item `item` (head * row_tiles + tile) of sequence b.
@@ -101,6 +137,7 @@ struct Cursor {
     item = 0;
     if (b + 1 < a.cache.num_sequences) enter(a, b + 1);
   }
+  __device__ __forceinline__ int token() const { return (span.first() + blk) * kBlock; }
 };
 
 // T: type of q and out.  FP8: e4m3 pages, multiplied as fp16.  DP: head_dim rounded up to 64, 128 or 256.  NT: tiles of 8 query heads.
@@ -109,55 +146,76 @@ struct Shape {
   static constexpr int kElems = FP8 ? 16 : 8;                          // of a 16-byte chunk
   static constexpr int kKeyChunks = DP / kElems / 4;                   // of a key row that a lane has
   static constexpr int kValueChunks = DP / kElems / 8 ? DP / kElems / 8 : 1;
-  static constexpr int kSlots = 2 * kKeyChunks + 4 * kValueChunks;     // 16-byte pieces of a lane and step
-  static constexpr int kStageBytes = kSlots * 512;
-  static constexpr int kWarps = kStageBytes >= 16384 ? 4 : 8;
-  static constexpr int kStages = 24576 / kStageBytes > 6 ? 6 : (kWarps == 4 ? 49152 : 24576) / kStageBytes;
-  static constexpr int kSmem = kWarps * kStages * kStageBytes;
+  static constexpr int kRowBytes = DP * (FP8 ? 1 : 2);
+  static constexpr int kRowChunks = kRowBytes / 16;
+  static constexpr int kCopyRows = kRowChunks > 32 ? 1 : 32 / kRowChunks;  // rows that 32 lanes copy at once, 16 bytes each
+  static constexpr int kTile = kBlock * kRowBytes;                     // 16 rows of keys or of values
+  static constexpr int kStageBytes = 2 * kTile;
+  // Chunk that holds a row's chunk in shared memory, XORed: eight lanes that read together - keys: rows of both parities, four neighbouring
+  // chunks; values: rows 2 t, two neighbouring chunks - find eight different 16-byte columns.  (64-byte rows: two lanes a column for values.)
+  static __device__ __forceinline__ constexpr int key_swizzle(int row) { return kRowChunks >= 8 ? (row & 1) << 2 : 0; }
+  static __device__ __forceinline__ constexpr int value_swizzle(int row) { return kRowChunks >= 8 ? ((row >> 1) & 3) << 1 : ((row >> 1) & 1) << 1; }
   static constexpr int kSteps = DP / 16;                               // K = 16 steps of S
   static constexpr int kDimTiles = kValueChunks * kElems / 2;          // 16-dimension tiles of O
   static constexpr int kHeads = 8 * NT;
+  static constexpr int kPieceBytes = kHeads * (DP + 2) * 4;
+  // Two CTAs on an SM, of which one computes while the other starts or ends; with fp16 heads of 256 dimensions one, for the ring's sake.
+  static constexpr int kCtasPerSm = kStageBytes > 8192 ? 1 : 2;
+  static constexpr int kStagesThatFit = ((kCtasPerSm == 2 ? 115456 : 232000) / kWarps - kPieceBytes) / kStageBytes;
+  static constexpr int kStages = kStagesThatFit > 6 ? 6 : kStagesThatFit;
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kSmem = kRing + kWarps * kPieceBytes;
+  static_assert(kStages >= 2 && kPieceBytes <= kStages * kStageBytes, "ring");
+};
+constexpr float kLowest = -3.402823466e38f;  // the running maximum before any score
+
+// A warp's partial result of an item that another warp shares, left in shared memory: o [tile_heads][head_dim], then (m, l) of every head.
+struct Piece {
+  int b, item;
+  int starts, ends;  // whether the item's first and last block are in it
+  int used;
 };
 
 template <typename T, bool FP8, int DP, int NT>
-__global__ void __launch_bounds__(Shape<T, FP8, DP, NT>::kWarps * 32, 1) paged_attention_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm) paged_attention_kernel(const __grid_constant__ AttnArgs a) {
   using S = Shape<T, FP8, DP, NT>;
   using M = std::conditional_t<FP8, __half, T>;  // type of the products
   constexpr int kElt = FP8 ? 1 : 2;
   extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ Piece pieces[2 * kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const TrisPagedKv& c = a.cache;
+  const TrisPagedAttention& query = a.query;
+  const int D = c.head_dim;
   pdl_wait();
   pdl_launch_dependents();
 
-  const int worker = warp * gridDim.x + blockIdx.x;  // few blocks: on as many SMs as there are
-  const int D = c.head_dim;
-  const int per_seq = c.num_kv_heads * a.row_tiles;
-  const int64_t total = blocks_before(a, c.num_sequences, lane);
-  const int64_t run = run_length(a, total);
-  const int64_t first = worker * run;
-  if (first >= total) return;
-  const int count = static_cast<int>(min(run, total - first));
+  // this warp's run, and the sequence that holds its first block
+  int mine, upto = scan_blocks(a, 0, lane, mine);
+  int total = __shfl_sync(0xFFFFFFFFu, upto, 31);
+  for (int i = 1; 32 * i < c.num_sequences; ++i) {
+    int own;
+    total += __shfl_sync(0xFFFFFFFFu, scan_blocks(a, i, lane, own), 31);
+  }
+  const int run = run_length(a, total);
+  if (static_cast<int64_t>(blockIdx.x) * kWarps * run >= total) return;
+  const int64_t first_block = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * run;
+  const int first = static_cast<int>(first_block), count = first_block < total ? min(run, total - first) : 0;
+  if (lane < 2) pieces[2 * warp + lane].used = 0;
+  __syncwarp();
 
-  Cursor use;
-  {  // the sequence that holds block `first`
-    int64_t before = 0;
-    for (int b0 = 0;; b0 += 32) {
-      const int b = b0 + lane;
-      const int64_t mine = b < c.num_sequences ? static_cast<int64_t>(span_of(a, b).blocks()) * per_seq : 0;
-      int64_t upto = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-        if (lane >= d) upto += v;
-      }
+  Cursor use{};
+  if (count) {
+    int before = 0;
+    for (int i = 0;; ++i) {
+      if (i) upto = scan_blocks(a, i, lane, mine);
       const uint32_t beyond = __ballot_sync(0xFFFFFFFFu, before + upto > first);
       if (beyond) {
         const int l = __ffs(beyond) - 1;
-        const int64_t start = before + __shfl_sync(0xFFFFFFFFu, upto - mine, l);
-        use.enter(a, b0 + l);
-        use.item = static_cast<int>((first - start) / use.blocks);
-        use.blk = static_cast<int>((first - start) % use.blocks);
+        const int ahead = first - before - __shfl_sync(0xFFFFFFFFu, upto - mine, l);
+        use.enter(a, 32 * i + l);
+        use.item = static_cast<unsigned>(ahead) / static_cast<unsigned>(use.blocks);
+        use.blk = ahead - use.item * use.blocks;
         break;
       }
       before += __shfl_sync(0xFFFFFFFFu, upto, 31);
@@ -165,95 +223,55 @@ __global__ void __launch_bounds__(Shape<T, FP8, DP, NT>::kWarps * 32, 1) paged_a
   }
   bool owns_start = use.blk == 0;  // whether the current item begins in this run
 
-  Cursor load = use;
-  int left = count;  // blocks that are not asked for yet
-  // Lane l < 16: page of token l of the block that is asked for next.
-  auto page_of = [&](const Cursor& cur) {
-    const int tok = cur.span.lo + cur.blk * kBlock + (lane & 15);
-    if (tok >= cur.span.hi) return -1;
-    const int at = a.page_shift >= 0 ? tok >> a.page_shift : tok / c.page_size;
-    const int page = c.block_table[cur.b * c.table_stride + at];
-    if (page >= 0 && page < c.num_pages) return page;
-    if (c.status_dev) *c.status_dev = TRIS_ERR_CORRUPT;
-    return -1;
-  };
-  int page = page_of(load);
-  uint8_t* ring = smem + warp * (S::kStages * S::kStageBytes) + lane * 16;
-  auto issue = [&](int stage) {
-    if (left > 0) {
-      const int tok = load.span.lo + load.blk * kBlock + (lane & 15);
-      const int in_page = a.page_shift >= 0 ? tok & (c.page_size - 1) : tok % c.page_size;
-      const int head = load.item / a.row_tiles;
-      const int64_t k_off = page < 0 ? -1 : (page * c.k_page_stride + in_page * c.k_token_stride + head * c.k_head_stride) * kElt;
-      const int64_t v_off = page < 0 ? -1 : (page * c.v_page_stride + in_page * c.v_token_stride + head * c.v_head_stride) * kElt;
-      uint8_t* dst = ring + stage * S::kStageBytes;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {  // keys g and g + 8: chunks 4 j + t
-        const int64_t off = __shfl_sync(0xFFFFFFFFu, k_off, g + 8 * r);
-        const uint8_t* src = static_cast<const uint8_t*>(c.k_pages) + (off < 0 ? 0 : off);
-#pragma unroll
-        for (int j = 0; j < S::kKeyChunks; ++j) {
-          const bool ok = off >= 0 && (4 * j + t) * S::kElems < D;
-          cp_async_16(dst + (r * S::kKeyChunks + j) * 512, ok ? src + (4 * j + t) * 16 : static_cast<const uint8_t*>(c.k_pages), ok);
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {  // values 2 t, 2 t + 1, 2 t + 8, 2 t + 9: chunks 8 j + g
-        const int64_t off = __shfl_sync(0xFFFFFFFFu, v_off, 2 * t + (r & 1) + 8 * (r >> 1));
-        const uint8_t* src = static_cast<const uint8_t*>(c.v_pages) + (off < 0 ? 0 : off);
-#pragma unroll
-        for (int j = 0; j < S::kValueChunks; ++j) {
-          const bool ok = off >= 0 && (8 * j + g) * S::kElems < D;
-          cp_async_16(dst + (2 * S::kKeyChunks + r * S::kValueChunks + j) * 512, ok ? src + (8 * j + g) * 16 : static_cast<const uint8_t*>(c.v_pages), ok);
-        }
-      }
-      if (--left > 0) {
-        load.next(a);
-        page = page_of(load);
-      }
-    }
-    cp_async_commit();  // empty groups keep the count of groups in step
-  };
-#pragma unroll
-  for (int s = 0; s < S::kStages - 1; ++s) issue(s);
-
   uint32_t qf[NT][S::kSteps][2];
   float scale[NT][2];  // of heads 2 t and 2 t + 1 of a tile, to base 2
   float m[NT][2], l[NT][2], acc[S::kDimTiles][NT][4];
-  const TrisPagedAttention& query = a.query;
-
-  auto load_query = [&] {
+  auto fetch_query = [&] {
     const int head = use.item / a.row_tiles, tile = use.item % a.row_tiles;
-    const float base = query.softmax_scale * kLog2e * (FP8 && c.k_scale ? c.k_scale[head] : 1.f);
+    scale[0][0] = FP8 && c.k_scale ? c.k_scale[head] : 1.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = tile * S::kHeads + 8 * n + g;
       const T* src = static_cast<const T*>(query.q) + use.b * query.q_token_stride + (static_cast<int64_t>(head) * a.group + row) * query.q_head_stride;
-      float top = 0.f;
 #pragma unroll
       for (int j = 0; j < S::kKeyChunks; ++j) {
 #pragma unroll
-        for (int w = 0; w < S::kElems / 2; ++w) {
+        for (int w = 0; w < S::kElems / 2; w += 4) {
           const int d = (4 * j + t) * S::kElems + 2 * w;
-          uint32_t v = 0;
+          uint32_t v[4] = {0, 0, 0, 0};
           if (row < a.group && d < D) {
-            const uint16_t* p = reinterpret_cast<const uint16_t*>(src + d);
-            v = p[0] | (static_cast<uint32_t>(p[1]) << 16);
+            if (a.wide_query) {
+              const uint4 raw = *reinterpret_cast<const uint4*>(src + d);
+              v[0] = raw.x, v[1] = raw.y, v[2] = raw.z, v[3] = raw.w;
+            } else {
+              const uint16_t* p = reinterpret_cast<const uint16_t*>(src + d);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) v[i] = p[2 * i] | (static_cast<uint32_t>(p[2 * i + 1]) << 16);
+            }
           }
-          if constexpr (FP8 && !std::is_same_v<T, __half>) {
-            const float2 f = Pair<T>::unpack(v);
-            top = max_nan(top, max_nan(fabsf(f.x), fabsf(f.y)));
-          }
-          qf[n][j * (S::kElems / 4) + w / 2][w & 1] = v;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) qf[n][j * (S::kElems / 4) + (w + i) / 2][i & 1] = v[i];
         }
       }
-      float up = 1.f;  // bf16 queries against fp16 keys: a power of two brings a row's largest element to [1, 2)
+    }
+  };
+  auto start_item = [&] {
+    const float base = query.softmax_scale * kLog2e * scale[0][0];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float up = 1.f;
       if constexpr (FP8 && !std::is_same_v<T, __half>) {
-        top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        const int e = top > 0.f && top < INFINITY ? max(ilogbf(top), -100) : 0;
-        up = ldexpf(1.f, e);
-        const float down = ldexpf(1.f, -e);
+        // bf16 queries against fp16 keys: a power of two brings a row's largest element to [1, 2).  The magnitudes' bits order like the numbers.
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < S::kSteps; ++s)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) top = __vmaxu2(top, qf[n][s][i] & 0x7FFF7FFFu);
+        top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        const int e = min(max(max(top & 0xFFFFu, top >> 16) >> 7, 27u), 253u);  // biased exponent; zeros, infinities and NaN stay what they are
+        up = __uint_as_float(static_cast<uint32_t>(e) << 23);
+        const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
 #pragma unroll
         for (int s = 0; s < S::kSteps; ++s)
 #pragma unroll
@@ -264,7 +282,7 @@ __global__ void __launch_bounds__(Shape<T, FP8, DP, NT>::kWarps * 32, 1) paged_a
       }
       scale[n][0] = base * __shfl_sync(0xFFFFFFFFu, up, 8 * t);
       scale[n][1] = base * __shfl_sync(0xFFFFFFFFu, up, 8 * t + 4);
-      m[n][0] = m[n][1] = -INFINITY;
+      m[n][0] = m[n][1] = kLowest;
       l[n][0] = l[n][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < S::kDimTiles; ++i)
@@ -273,10 +291,85 @@ __global__ void __launch_bounds__(Shape<T, FP8, DP, NT>::kWarps * 32, 1) paged_a
     }
   };
 
-  auto finish_item = [&](bool owns_end) {
+  if (count) fetch_query();  // on its way while the first blocks are asked for
+
+  Cursor load = use;
+  int left = count;  // blocks that are not asked for yet
+  // Page of token `lane & 15` of the block that is asked for next; of the block itself where blocks do not cross pages.
+  auto page_of = [&](const Cursor& cur) {
+    int tok = cur.token();
+    if (!a.page_blocks) {
+      tok += lane & 15;
+      if (tok < cur.span.lo || tok >= cur.span.hi) return -1;
+    }
+    const int at = a.page_shift >= 0 ? tok >> a.page_shift : tok / c.page_size;
+    const int page = c.block_table[cur.b * c.table_stride + at];
+    if (page >= 0 && page < c.num_pages) return page;
+    if (c.status_dev) *c.status_dev = TRIS_ERR_CORRUPT;
+    return -1;
+  };
+  int page = left > 0 ? page_of(load) : -1;
+  uint8_t* ring = smem + warp * (S::kStages * S::kStageBytes);
+  const uint32_t ring_at = smem_u32(ring);
+  const uint8_t *k_pages = static_cast<const uint8_t*>(c.k_pages), *v_pages = static_cast<const uint8_t*>(c.v_pages);
+  const int64_t k_row = c.k_token_stride * kElt, v_row = c.v_token_stride * kElt;
+  // A copy takes 512 bytes of neighbouring rows, lane after lane.  (Lanes that copy what they need themselves - values: four rows, 128 bytes
+  // each, neighbouring lanes in different rows - reach 3.9 TB/s where this reaches 7.0.)
+  constexpr int kCopies = S::kTile / 512;
+  const int copy_row = lane / S::kRowChunks, copy_chunk = lane % S::kRowChunks;
+  const uint32_t k_to = copy_row * S::kRowBytes + ((copy_chunk ^ S::key_swizzle(copy_row)) << 4);
+  const uint32_t v_to = copy_row * S::kRowBytes + ((copy_chunk ^ S::value_swizzle(copy_row)) << 4);
+
+  auto issue = [&](int stage) {
+    if (left > 0) {
+      const int tok0 = load.token(), head = load.item / a.row_tiles;
+      const uint32_t dst = ring_at + stage * S::kStageBytes;
+      if (a.rows_together && page >= 0 && tok0 >= load.span.lo && tok0 + kBlock <= load.span.hi) {
+        // a whole block of one page, side by side in memory
+        const int in_page = a.page_shift >= 0 ? tok0 & (c.page_size - 1) : tok0 % c.page_size;
+        const uint8_t* k = k_pages + (page * c.k_page_stride + head * c.k_head_stride) * kElt + in_page * S::kRowBytes + lane * 16;
+        const uint8_t* v = v_pages + (page * c.v_page_stride + head * c.v_head_stride) * kElt + in_page * S::kRowBytes + lane * 16;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) cp_async_16_at(dst + (k_to ^ (S::key_swizzle(i * S::kCopyRows) << 4)) + i * 512, k + i * 512, 16);
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) cp_async_16_at(dst + (v_to ^ (S::value_swizzle(i * S::kCopyRows) << 4)) + S::kTile + i * 512, v + i * 512, 16);
+      } else {
+        const int tok = tok0 + (lane & 15);
+        const bool there = page >= 0 && tok >= load.span.lo && tok < load.span.hi;
+        const int in_page = a.page_shift >= 0 ? tok & (c.page_size - 1) : tok % c.page_size;
+        const int64_t k_off = there ? (page * c.k_page_stride + head * c.k_head_stride) * kElt + in_page * k_row : -1;
+        const int64_t v_off = there ? (page * c.v_page_stride + head * c.v_head_stride) * kElt + in_page * v_row : -1;
+        const bool in_row = copy_chunk * S::kElems < D;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          const int64_t off = __shfl_sync(0xFFFFFFFFu, k_off, i * S::kCopyRows + copy_row);
+          const bool ok = off >= 0 && in_row;
+          cp_async_16_at(dst + (k_to ^ (S::key_swizzle(i * S::kCopyRows) << 4)) + i * 512, ok ? k_pages + off + copy_chunk * 16 : k_pages, ok ? 16 : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          const int64_t off = __shfl_sync(0xFFFFFFFFu, v_off, i * S::kCopyRows + copy_row);
+          const bool ok = off >= 0 && in_row;
+          cp_async_16_at(dst + (v_to ^ (S::value_swizzle(i * S::kCopyRows) << 4)) + S::kTile + i * 512, ok ? v_pages + off + copy_chunk * 16 : v_pages, ok ? 16 : 0);
+        }
+      }
+      if (--left > 0) {
+        load.next(a);
+        page = page_of(load);
+      }
+    }
+    cp_async_commit();  // empty groups keep the count of groups in step
+  };
+  // where this lane's fragments are in a stage: keys g and g + 8, chunks 4 j + t; values 2 t, 2 t + 1, 2 t + 8, 2 t + 9, chunks 8 j + g
+  const uint32_t k_from = g * S::kRowBytes + ((t ^ S::key_swizzle(g)) << 4);
+  const uint32_t v_from = S::kTile + 2 * t * S::kRowBytes + ((g ^ S::value_swizzle(2 * t)) << 4);
+  const bool has_values = g < S::kRowChunks;
+#pragma unroll 1
+  for (int s = 0; s < S::kStages - 1; ++s) issue(s);
+
+  // The result of an item that this warp has had alone goes out; otherwise its piece is left for the other warps' (to != nullptr).
+  auto write_item = [&](float* to) {
     const int head = use.item / a.row_tiles, tile = use.item % a.row_tiles;
-    const bool whole = owns_start && owns_end;
-    const int64_t slot = 2 * static_cast<int64_t>(worker) + (owns_start ? 1 : 0);
     const float v_scale = FP8 && c.v_scale ? c.v_scale[head] : 1.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -288,7 +381,7 @@ __global__ void __launch_bounds__(Shape<T, FP8, DP, NT>::kWarps * 32, 1) paged_a
         const int in_tile = 8 * n + 2 * t + h, row = tile * S::kHeads + in_tile;
         if (row >= a.group) continue;
         const int64_t out_row = static_cast<int64_t>(use.b) * query.num_q_heads + head * a.group + row;
-        const float inv = whole ? (sum == 0.f ? 0.f : v_scale / sum) : v_scale;
+        const float inv = to ? v_scale : sum == 0.f ? 0.f : v_scale / sum;
 #pragma unroll
         for (int j = 0; j < S::kValueChunks; ++j) {
           const int d0 = (8 * j + g) * S::kElems;
@@ -301,142 +394,253 @@ __global__ void __launch_bounds__(Shape<T, FP8, DP, NT>::kWarps * 32, 1) paged_a
               v[2 * i] = acc[j * (S::kElems / 2) + 4 * q + i][n][h] * inv;
               v[2 * i + 1] = acc[j * (S::kElems / 2) + 4 * q + i][n][2 + h] * inv;
             }
-            if (whole) {
-              store_8(static_cast<T*>(query.out) + out_row * D + d0 + 8 * q, v);
-            } else {
-              float4* dst = reinterpret_cast<float4*>(a.part_o + (slot * a.tile_heads + in_tile) * D + d0 + 8 * q);
+            if (to) {
+              float4* dst = reinterpret_cast<float4*>(to + in_tile * D + d0 + 8 * q);
               dst[0] = make_float4(v[0], v[1], v[2], v[3]);
               dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+              store_8(static_cast<T*>(query.out) + out_row * D + d0 + 8 * q, v);
             }
           }
         }
         if (g == 0) {
-          if (!whole)
-            *reinterpret_cast<float2*>(a.part_ml + (slot * a.tile_heads + in_tile) * 2) = make_float2(m[n][h], sum);
+          if (to)
+            *reinterpret_cast<float2*>(to + a.tile_heads * D + 2 * in_tile) = make_float2(m[n][h], sum);
           else if (query.lse)
             query.lse[out_row] = sum == 0.f ? -INFINITY : (m[n][h] + log2f(sum)) * kLn2;
         }
       }
   };
-
-  load_query();
-  for (int i = 0; i < count; ++i) {
+  // Two pieces at most: of the item that another warp began (slot 0), and, with the warp's last block, of one that another warp ends (slot 1).
+  // The second one takes the ring's place, all of which has been read by then.
+  auto piece_at = [&](int slot) {
+    uint8_t* at = slot & 1 ? smem + (slot >> 1) * (S::kStages * S::kStageBytes) : smem + S::kRing + (slot >> 1) * S::kPieceBytes;
+    return reinterpret_cast<float*>(at);
+  };
+  bool fresh = true;  // an item begins
+  for (int i = 0, stage = 0; i < count; ++i) {
+    if (fresh) start_item();
+    fresh = false;
     cp_async_wait<S::kStages - 2>();
-    const uint8_t* src = ring + (i % S::kStages) * S::kStageBytes;
+    __syncwarp();  // all lanes' copies are there, and all lanes are done with the stage that is filled next
+    const uint8_t* src = ring + stage * S::kStageBytes;
 
-    float s[NT][4];
+    float s[NT][4], s_odd[NT][4];  // two sums: an MMA waits 20 cycles for the one before it
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[n][k] = s_odd[n][k] = 0.f;
 #pragma unroll
     for (int j = 0; j < S::kKeyChunks; ++j) {
-      const uint4 ka = *reinterpret_cast<const uint4*>(src + j * 512), kb = *reinterpret_cast<const uint4*>(src + (S::kKeyChunks + j) * 512);
+      const uint8_t* keys = src + (k_from ^ ((j & 1) << 6)) + ((j & ~1) << 6);
+      const uint4 ka = *reinterpret_cast<const uint4*>(keys), kb = *reinterpret_cast<const uint4*>(keys + 8 * S::kRowBytes);
       const uint32_t x[4] = {ka.x, ka.y, ka.z, ka.w}, y[4] = {kb.x, kb.y, kb.z, kb.w};
       if constexpr (FP8) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t a0 = e4m3_to_h2(x[w] & 0xFFFF), a2 = e4m3_to_h2(x[w] >> 16), a1 = e4m3_to_h2(y[w] & 0xFFFF), a3 = e4m3_to_h2(y[w] >> 16);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_16x8x16<M>(s[n], a0, a1, a2, a3, qf[n][4 * j + w][0], qf[n][4 * j + w][1]);
+          for (int n = 0; n < NT; ++n) mma_16x8x16<M>(w & 1 ? s_odd[n] : s[n], a0, a1, a2, a3, qf[n][4 * j + w][0], qf[n][4 * j + w][1]);
         }
       } else {
 #pragma unroll
         for (int w = 0; w < 2; ++w)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_16x8x16<M>(s[n], x[2 * w], y[2 * w], x[2 * w + 1], y[2 * w + 1], qf[n][2 * j + w][0], qf[n][2 * j + w][1]);
+          for (int n = 0; n < NT; ++n) mma_16x8x16<M>(w ? s_odd[n] : s[n], x[2 * w], y[2 * w], x[2 * w + 1], y[2 * w + 1], qf[n][2 * j + w][0], qf[n][2 * j + w][1]);
       }
     }
 
-    // tokens g and g + 8 of heads 2 t and 2 t + 1
-    const int tok = use.span.lo + use.blk * kBlock + g;
-    const bool in0 = tok < use.span.hi, in1 = tok + 8 < use.span.hi;
+    // Tokens g and g + 8 of heads 2 t and 2 t + 1.  Weights are 2^(s - m) with m no less than the largest score so far minus 8: m moves only when
+    // a score exceeds it by more than that, which is rare after the first blocks, and sums scaled by up to 2^8 are as exact.
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[n][k] = (s[n][k] + s_odd[n][k]) * scale[n][k & 1];
+    const int tok = use.token();
+    if (tok < use.span.lo || tok + kBlock > use.span.hi) {
+      const bool in0 = tok + g >= use.span.lo && tok + g < use.span.hi, in1 = tok + g + 8 >= use.span.lo && tok + g + 8 < use.span.hi;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (!in0) s[n][0] = s[n][1] = -INFINITY;
+        if (!in1) s[n][2] = s[n][3] = -INFINITY;
+      }
+    }
+    float x[NT][4];
+    bool above = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[n][k] = s[n][k] - m[n][k & 1];
+        above |= x[n][k] > 8.f;
+      }
+    if (__any_sync(0xFFFFFFFFu, above)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float old[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float top = fmaxf(s[n][h], s[n][2 + h]);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+          top = fmaxf(m[n][h], top);
+          old[h] = exp2_fast(m[n][h] - top);
+          m[n][h] = top;
+          l[n][h] *= old[h];
+          x[n][h] = s[n][h] - top;
+          x[n][2 + h] = s[n][2 + h] - top;
+        }
+#pragma unroll
+        for (int k = 0; k < S::kDimTiles; ++k) {
+          acc[k][n][0] *= old[0];
+          acc[k][n][1] *= old[1];
+          acc[k][n][2] *= old[0];
+          acc[k][n][3] *= old[1];
+        }
+      }
+    }
+    // The weights as the 8-column operand: pairs of tokens of one head.  Rounded to the values' type, as 16-bit operands are: 2^-8 (bf16) or
+    // 2^-11 (fp16) of a weight at most, independent from token to token; the sum l is of the weights before that.
     uint32_t p[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float old[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s[n][h] = in0 ? s[n][h] * scale[n][h] : -INFINITY;
-        s[n][2 + h] = in1 ? s[n][2 + h] * scale[n][h] : -INFINITY;
-        float top = fmaxf(s[n][h], s[n][2 + h]);
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-        const float now = fmaxf(m[n][h], top);
-        const float base = now == -INFINITY ? 0.f : now;  // nothing but -inf so far: weights of 0
-        old[h] = exp2f(m[n][h] - base);
-        m[n][h] = now;
-        s[n][h] = exp2f(s[n][h] - base);
-        s[n][2 + h] = exp2f(s[n][2 + h] - base);
-        l[n][h] = l[n][h] * old[h] + s[n][h] + s[n][2 + h];
-      }
-      // the weights as the 8-column operand: pairs of tokens of one head.  Rounded to the values' type, as 16-bit operands are: 2^-9 (bf16) or
-      // 2^-12 (fp16) of a weight, independent from token to token; the sum l is of the weights before that
-      p[n][0] = transpose_8x8(Pair<M>::pack(s[n][0], s[n][1]));
-      p[n][1] = transpose_8x8(Pair<M>::pack(s[n][2], s[n][3]));
-#pragma unroll
-      for (int k = 0; k < S::kDimTiles; ++k) {
-        acc[k][n][0] *= old[0];
-        acc[k][n][1] *= old[1];
-        acc[k][n][2] *= old[0];
-        acc[k][n][3] *= old[1];
-      }
+      for (int k = 0; k < 4; ++k) x[n][k] = exp2_fast(x[n][k]);
+      l[n][0] += x[n][0] + x[n][2];
+      l[n][1] += x[n][1] + x[n][3];
+      p[n][0] = transpose_8x8(Pair<M>::pack(x[n][0], x[n][1]));
+      p[n][1] = transpose_8x8(Pair<M>::pack(x[n][2], x[n][3]));
     }
 
-    const uint8_t* vals = src + 2 * S::kKeyChunks * 512;
+    const uint8_t* vals = src + v_from;
 #pragma unroll
     for (int j = 0; j < S::kValueChunks; ++j) {
       uint32_t v[4][4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(vals + (r * S::kValueChunks + j) * 512);
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (S::kRowChunks >= 8 || has_values) raw = *reinterpret_cast<const uint4*>(vals + ((r & 1) + 8 * (r >> 1)) * S::kRowBytes + j * 128);
         v[r][0] = raw.x, v[r][1] = raw.y, v[r][2] = raw.z, v[r][3] = raw.w;
       }
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
+        if constexpr (FP8) {
+          // bytes of two tokens side by side first, then two values at a time: {token 0, token 1} of dimensions 4 w + i
+          const uint32_t lo0 = prmt(v[0][w], v[1][w], 0x5140), hi0 = prmt(v[0][w], v[1][w], 0x7362);
+          const uint32_t lo1 = prmt(v[2][w], v[3][w], 0x5140), hi1 = prmt(v[2][w], v[3][w], 0x7362);
 #pragma unroll
-        for (int e = 0; e < (FP8 ? 2 : 1); ++e) {
-          uint32_t x[4];
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t u0 = e ? hi0 : lo0, u1 = e ? hi1 : lo1;
+            const uint32_t a0 = e4m3_to_h2(u0 & 0xFFFF), a1 = e4m3_to_h2(u0 >> 16), a2 = e4m3_to_h2(u1 & 0xFFFF), a3 = e4m3_to_h2(u1 >> 16);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = FP8 ? e4m3_to_h2(e ? v[r][w] >> 16 : v[r][w] & 0xFFFF) : v[r][w];
-          const uint32_t a0 = prmt(x[0], x[1], 0x5410), a1 = prmt(x[0], x[1], 0x7632), a2 = prmt(x[2], x[3], 0x5410), a3 = prmt(x[2], x[3], 0x7632);
-          const int tile = FP8 ? j * 8 + 2 * w + e : j * 4 + w;
+            for (int n = 0; n < NT; ++n) mma_16x8x16<M>(acc[j * 8 + 2 * w + e][n], a0, a1, a2, a3, p[n][0], p[n][1]);
+          }
+        } else {
+          const uint32_t a0 = prmt(v[0][w], v[1][w], 0x5410), a1 = prmt(v[0][w], v[1][w], 0x7632);
+          const uint32_t a2 = prmt(v[2][w], v[3][w], 0x5410), a3 = prmt(v[2][w], v[3][w], 0x7632);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_16x8x16<M>(acc[tile][n], a0, a1, a2, a3, p[n][0], p[n][1]);
+          for (int n = 0; n < NT; ++n) mma_16x8x16<M>(acc[j * 4 + w][n], a0, a1, a2, a3, p[n][0], p[n][1]);
         }
       }
     }
-    issue((i + S::kStages - 1) % S::kStages);
+    issue(stage == 0 ? S::kStages - 1 : stage - 1);
+    if (++stage == S::kStages) stage = 0;
 
-    const bool last = i + 1 == count;
-    if (last || use.blk + 1 == use.blocks) {
-      finish_item(use.blk + 1 == use.blocks);
+    const bool last = i + 1 == count, ends = use.blk + 1 == use.blocks;
+    if (last || ends) {
+      float* to = nullptr;
+      if (!(owns_start && ends)) {
+        const int slot = 2 * warp + (owns_start ? 1 : 0);
+        to = piece_at(slot);
+        if (lane == 0) pieces[slot] = {use.b, use.item, owns_start, ends, 1};
+        __syncwarp();
+      }
+      write_item(to);
       if (!last) {
         use.next(a);
-        owns_start = true;
-        load_query();
+        owns_start = fresh = true;
+        fetch_query();
       }
     } else {
       ++use.blk;
     }
   }
   cp_async_wait<0>();
+  __syncthreads();
+
+  // Neighbouring warps' pieces of one item are joined here; what other CTAs share goes to the workspace.
+  for (int s0 = 0; s0 < 2 * kWarps;) {
+    if (!pieces[s0].used) {
+      ++s0;
+      continue;
+    }
+    int s1 = s0;  // last piece of the item
+    for (int k = s0 + 1; !pieces[s1].ends && k < 2 * kWarps; ++k)
+      if (pieces[k].used) s1 = k;
+    const Piece item = pieces[s0];
+    const bool whole = item.starts && pieces[s1].ends;
+    const int head = item.item / a.row_tiles, tile = item.item % a.row_tiles;
+    const int heads = min(S::kHeads, a.group - tile * S::kHeads);
+    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (item.starts ? 1 : 0);
+    for (int h = warp; h < heads; h += kWarps) {
+      // an item's pieces are the second one of its first warp and the first ones of the next, so kWarps + 1 at most
+      float w[2 * kWarps], top = kLowest, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2 * kWarps; ++k) {
+        w[k] = kLowest;
+        if (k >= s0 && k <= s1 && pieces[k].used) w[k] = piece_at(k)[a.tile_heads * D + 2 * h];
+      }
+#pragma unroll
+      for (int k = 0; k < 2 * kWarps; ++k) top = fmaxf(top, w[k]);
+#pragma unroll
+      for (int k = 0; k < 2 * kWarps; ++k) {
+        const bool has = k >= s0 && k <= s1 && pieces[k].used;
+        w[k] = has ? exp2_fast(w[k] - top) : 0.f;
+        if (has) sum += w[k] * piece_at(k)[a.tile_heads * D + 2 * h + 1];
+      }
+      const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+      const int64_t out_row = static_cast<int64_t>(item.b) * query.num_q_heads + head * a.group + tile * S::kHeads + h;
+      for (int d = 4 * lane; d < D; d += 128) {
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 2 * kWarps; ++k) {
+          if (k >= s0 && k <= s1 && pieces[k].used) {
+            const float4 v = *reinterpret_cast<const float4*>(piece_at(k) + h * D + d);
+            o.x += w[k] * v.x, o.y += w[k] * v.y, o.z += w[k] * v.z, o.w += w[k] * v.w;
+          }
+        }
+        if (whole)
+          *reinterpret_cast<uint2*>(static_cast<T*>(query.out) + out_row * D + d) = make_uint2(Pair<T>::pack(o.x * inv, o.y * inv), Pair<T>::pack(o.z * inv, o.w * inv));
+        else
+          *reinterpret_cast<float4*>(a.part_o + (slot * a.tile_heads + h) * D + d) = o;
+      }
+      if (lane == 0) {
+        if (!whole)
+          *reinterpret_cast<float2*>(a.part_ml + (slot * a.tile_heads + h) * 2) = make_float2(top, sum);
+        else if (query.lse)
+          query.lse[out_row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+      }
+    }
+    s0 = s1 + 1;
+  }
 }
 
 // Joins the partial results of one query head of one sequence; zeros where there was nothing to attend to.
-constexpr int kJoinThreads = 128;
-constexpr int kMaxWorkers = 4096;
+constexpr int kJoinWarps = 4, kJoinThreads = 32 * kJoinWarps;
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const __grid_constant__ AttnArgs a, int tile_rows) {
-  __shared__ float weight[kMaxWorkers];
-  __shared__ float red[kJoinThreads / 32][2];
+  __shared__ float2 stats[kJoinThreads];
   __shared__ float4 sums[kJoinThreads];
   pdl_wait();
   pdl_launch_dependents();
   const TrisPagedKv& c = a.cache;
   const TrisPagedAttention& query = a.query;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int b = blockIdx.y, q_head = blockIdx.x, head = q_head / a.group, row = q_head % a.group;
   const int tile = row / tile_rows, in_tile = row % tile_rows, D = c.head_dim, D4 = D / 4;
   const int64_t out_row = static_cast<int64_t>(b) * query.num_q_heads + q_head;
+  int before;
+  const int total = count_blocks(a, b, lane, before);
   const Span span = span_of(a, b);
   const int blocks = span.blocks();
   T* out = static_cast<T*>(query.out) + out_row * D;
@@ -446,56 +650,64 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
     if (query.lse && tid == 0) query.lse[out_row] = -INFINITY;
     return;
   }
-  const int64_t run = run_length(a, blocks_before(a, c.num_sequences, lane));
-  const int64_t start = blocks_before(a, b, lane) + static_cast<int64_t>(head * a.row_tiles + tile) * blocks;
-  const int w0 = static_cast<int>(start / run), n = static_cast<int>((start + blocks - 1) / run) - w0 + 1;
-  if (n == 1) return;  // one warp had all of it
+  const unsigned run = run_length(a, total) * kWarps;  // of a CTA
+  const unsigned start = before + (head * a.row_tiles + tile) * blocks;
+  const int w0 = start / run, n = (start + blocks - 1) / run - w0 + 1;
+  if (n == 1) return;  // one CTA had all of it
   auto slot = [&](int i) { return (2 * static_cast<int64_t>(w0 + i) + (i == 0 ? 1 : 0)) * a.tile_heads + in_tile; };
 
-  float top = -INFINITY;
-  for (int i = tid; i < n; i += kJoinThreads) top = fmaxf(top, a.part_ml[slot(i) * 2]);
-#pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-  if (lane == 0) red[warp][0] = top;
-  __syncthreads();
-  for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, red[w][0]);
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int i = tid; i < n; i += kJoinThreads) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot(i) * 2);
-    const float w = exp2f(ml.x - base);
-    weight[i] = w;
-    sum += w * ml.y;
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-  if (lane == 0) red[warp][1] = sum;
-  __syncthreads();
-  sum = 0.f;
-  for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[w][1];
-
-  // a group of D / 4 threads per partial result; the groups' sums are added in their order
-  const int groups = kJoinThreads / D4, grp = tid / D4, col = tid % D4;
+  // A group of D / 4 threads takes every groups-th partial result, kBatch of them at a time so that their loads are in flight together;
+  // the groups' results are joined in their order.
+  constexpr int kBatch = 8;
+  const int groups = kJoinThreads / D4, grp = tid / D4, col = tid - grp * D4;
+  float top = kLowest, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float w, float2 ml, float4 v) {
+    sum += w * ml.y;
+    o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
+  };
+  auto rescale = [&](float to) {
+    const float w = exp2_fast(top - to);
+    sum *= w;
+    o.x *= w, o.y *= w, o.z *= w, o.w *= w;
+    top = to;
+  };
   if (grp < groups) {
-#pragma unroll 8
-    for (int i = grp; i < n; i += groups) {
-      const float4 v = *reinterpret_cast<const float4*>(a.part_o + slot(i) * D + 4 * col);
-      const float w = weight[i];
-      o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
+    for (int i0 = grp; i0 < n; i0 += kBatch * groups) {
+      float2 ml[kBatch];
+      float4 v[kBatch];
+      float to = top;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = i0 + k * groups;
+        ml[k] = make_float2(kLowest, 0.f);
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < n) {
+          ml[k] = *reinterpret_cast<const float2*>(a.part_ml + slot(i) * 2);
+          v[k] = *reinterpret_cast<const float4*>(a.part_o + slot(i) * D + 4 * col);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) to = fmaxf(to, ml[k].x);
+      rescale(to);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) add(exp2_fast(ml[k].x - top), ml[k], v[k]);
     }
     sums[tid] = o;
+    stats[tid] = make_float2(top, sum);
   }
   __syncthreads();
-  if (tid < D4) {
-    for (int k = 1; k < groups; ++k) {
-      const float4 v = sums[k * D4 + tid];
-      o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    uint2 packed = make_uint2(Pair<T>::pack(o.x * inv, o.y * inv), Pair<T>::pack(o.z * inv, o.w * inv));
-    *reinterpret_cast<uint2*>(out + 4 * tid) = packed;
+  if (tid >= D4) return;
+  const int used = n < groups ? n : groups;
+  float to = top;
+  for (int k = 1; k < used; ++k) to = fmaxf(to, stats[k * D4].x);
+  rescale(to);
+  for (int k = 1; k < used; ++k) {
+    const float2 ml = stats[k * D4];
+    add(exp2_fast(ml.x - top), ml, sums[k * D4 + tid]);
   }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint2*>(out + 4 * tid) = make_uint2(Pair<T>::pack(o.x * inv, o.y * inv), Pair<T>::pack(o.z * inv, o.w * inv));
   if (query.lse && tid == 0) query.lse[out_row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
@@ -514,24 +726,32 @@ int sm_count() {
 // Tiles of 8 query heads that share a key/value head's pass.  With heads of 256 dimensions the accumulators of two do not fit the registers.
 int head_tiles(int group, int head_dim) { return group > 8 && head_dim <= 128 ? 2 : 1; }
 
-size_t part_floats(int workers, int tile_heads, int head_dim) { return 2 * static_cast<size_t>(workers) * tile_heads * (head_dim + 2); }
+// CTAs of the first kernel: twice as many as are resident, but no more than there can be shares of one block for their warps.
+int attention_ctas(int resident, int64_t blocks) {
+  const int64_t ctas = (blocks + kWarps - 1) / kWarps;
+  return static_cast<int>(ctas < 1 ? 1 : ctas < 2 * resident ? ctas : 2 * resident);
+}
+int64_t most_blocks(const TrisPagedKv& c, int row_tiles) {
+  return static_cast<int64_t>(c.num_sequences) * c.num_kv_heads * row_tiles * ((static_cast<int64_t>(c.table_width) * c.page_size + kBlock - 1) / kBlock + 1);
+}
+size_t part_floats(int ctas, int tile_heads, int head_dim) { return 2 * static_cast<size_t>(ctas) * tile_heads * (head_dim + 2); }
 
 template <typename T, bool FP8, int DP, int NT>
 int launch_attention(AttnArgs& a, cudaStream_t stream) {
   using S = Shape<T, FP8, DP, NT>;
   auto kernel = paged_attention_kernel<T, FP8, DP, NT>;
-  TRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
   const TrisPagedKv& c = a.cache;
-  const int sms = sm_count();
-  TRIS_REQUIRE(sms > 0 && sms * S::kWarps <= kMaxWorkers, TRIS_ERR_CUDA, "paged_decode_attention: no device");
-  a.min_run = 1;
-  a.workers = sms * S::kWarps;
+  TRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  a.resident = sm_count() * S::kCtasPerSm;
+  a.ctas = attention_ctas(a.resident, most_blocks(c, a.row_tiles));
+  a.rows_together = a.page_blocks && c.head_dim == DP && c.k_token_stride == DP && c.v_token_stride == DP;
+  TRIS_REQUIRE(sm_count() > 0, TRIS_ERR_CUDA, "paged_decode_attention: no device");
   a.part_ml = static_cast<float*>(a.query.workspace);
-  a.part_o = a.part_ml + 4 * static_cast<size_t>(a.workers) * a.tile_heads;
-  const int64_t need = part_floats(a.workers, a.tile_heads, c.head_dim) * 4;
+  a.part_o = a.part_ml + 4 * static_cast<size_t>(a.ctas) * a.tile_heads;
+  const int64_t need = part_floats(a.ctas, a.tile_heads, c.head_dim) * 4;
   TRIS_REQUIRE(a.query.workspace && a.query.workspace_bytes >= need, TRIS_ERR_WORKSPACE, "paged_decode_attention: workspace of %lld bytes needed, got %lld",
                static_cast<long long>(need), static_cast<long long>(a.query.workspace_bytes));
-  TRIS_CUDA(launch_kernel(kernel, dim3(sms), dim3(S::kWarps * 32), S::kSmem, stream, programmatic_launch_default(), 1, a));
+  TRIS_CUDA(launch_kernel(kernel, dim3(a.ctas), dim3(kWarps * 32), S::kSmem, stream, programmatic_launch_default(), 1, a));
   TRIS_CUDA(launch_kernel(paged_attention_join_kernel<T>, dim3(a.query.num_q_heads, c.num_sequences), dim3(kJoinThreads), 0, stream, true, 1, a, S::kHeads));
   return TRIS_OK;
 }
@@ -552,7 +772,7 @@ extern "C" size_t tris_paged_decode_attention_workspace_bytes(const TrisPagedKv*
   if (num_q_heads < 1 || num_q_heads % cache->num_kv_heads) return 0;
   const int group = num_q_heads / cache->num_kv_heads, heads = 8 * head_tiles(group, cache->head_dim);
   const int sms = sm_count();
-  return sms > 0 ? part_floats(sms * 8, group < heads ? group : heads, cache->head_dim) * 4 : 0;
+  return sms > 0 ? part_floats(2 * 2 * sms, group < heads ? group : heads, cache->head_dim) * 4 : 0;
 }
 
 extern "C" int tris_paged_decode_attention(const TrisPagedKv* cache, const TrisPagedAttention* query, void* stream) {
@@ -577,6 +797,10 @@ extern "C" int tris_paged_decode_attention(const TrisPagedKv* cache, const TrisP
   const int heads = 8 * head_tiles(a.group, c.head_dim);
   a.row_tiles = ceil_div(a.group, heads);
   a.tile_heads = a.group < heads ? a.group : heads;
+  a.page_blocks = c.page_size % kBlock == 0;
+  a.wide_query = aligned_to(q.q, 16) && q.q_token_stride % 8 == 0 && q.q_head_stride % 8 == 0;
+  TRIS_REQUIRE(static_cast<int64_t>(c.table_width) * c.page_size < (1ll << 31) && most_blocks(c, a.row_tiles) < (1ll << 31), TRIS_ERR_UNSUPPORTED,
+               "paged_decode_attention: a block table for more than 2^31 blocks of %d tokens (all sequences and heads)", kBlock);
   a.page_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (c.page_size == 1 << s) a.page_shift = s;
