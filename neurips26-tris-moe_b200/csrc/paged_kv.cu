@@ -5,7 +5,8 @@
 // Bound by bytes for prompts, by the chain position -> page -> store for a decode step.
 //
 // A thread has one unit of two 16-byte chunks - the halves (i, i + rotary / 2) that rotate together - and walks over heads with it, so that its
-// eight cosines and sines are read once.  How many threads share a token's heads follows the number of tokens (heads_in_parallel).
+// eight cosines and sines are read once; four heads are asked for before the first of them is rotated.  How many threads share a token's heads follows
+// the number of tokens: all heads at once for a decode step, four heads and more to a thread where the GPU is full without that.
 #include "decode_step.cuh"
 
 namespace tris {
@@ -34,15 +35,37 @@ struct AppendArgs {
   int units, head_groups;
 };
 
+// VEC elements as they are in memory: one 16-byte access for eight.
 template <int VEC, typename T>
-__device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
-  if constexpr (VEC == 8) {
-    load_8(p, v);
-  } else {
+struct Chunk {
+  T v[VEC];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = to_float(p[i]);
+    for (int i = 0; i < VEC; ++i) store_float(v + i, 0.f);
   }
-}
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = p[i];
+  }
+  __device__ __forceinline__ void get(float (&f)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = to_float(v[i]);
+  }
+};
+template <typename T>
+struct Chunk<8, T> {
+  uint4 v;
+  __device__ __forceinline__ void clear() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 p = Pair<T>::unpack(w[i]);
+      f[2 * i] = p.x, f[2 * i + 1] = p.y;
+    }
+  }
+};
 template <int VEC, typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
   if constexpr (VEC == 8) {
@@ -102,68 +125,85 @@ __global__ void __launch_bounds__(128) paged_kv_append_kernel(const __grid_const
   float cs[VEC], sn[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) cs[i] = 1.f, sn[i] = 0.f;
-  if (r.cos && !padding) {
-    const float* cr = r.cos + pos * half;
-    const float* sr = r.sin + pos * half;
-    if (static_cast<int>(u) < pair_units) {
+  if (r.cos && !padding && (static_cast<int>(u) < pair_units || r.interleaved)) {
+    const int f0 = r.interleaved ? c0 * (VEC / 2) : c0 * VEC;
+    const float *cr = r.cos + pos * half + f0, *sr = r.sin + pos * half + f0;
+    constexpr int kStep = VEC == 8 ? 4 : 1;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) cs[i] = cr[c0 * VEC + i], sn[i] = sr[c0 * VEC + i];
-    } else if (r.interleaved) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int f = c0 * (VEC / 2) + i;
-        if (f < half) cs[i] = cr[f], sn[i] = sr[f];
+    for (int i = 0; i < VEC; i += kStep) {
+      if (f0 + i >= half) break;
+      if constexpr (VEC == 8) {
+        const float4 x = *reinterpret_cast<const float4*>(cr + i), y = *reinterpret_cast<const float4*>(sr + i);
+        cs[i] = x.x, cs[i + 1] = x.y, cs[i + 2] = x.z, cs[i + 3] = x.w;
+        sn[i] = y.x, sn[i + 1] = y.y, sn[i + 2] = y.z, sn[i + 3] = y.w;
+      } else {
+        cs[i] = cr[i], sn[i] = sr[i];
       }
     }
   }
 
-  for (int h = hg; h < hq + 2 * hkv; h += a.head_groups) {
-    const int kind = h < hq ? 0 : h < hq + hkv ? 1 : 2;
-    const int hh = kind == 0 ? h : kind == 1 ? h - hq : h - hq - hkv;
-    const T* src = kind == 0   ? static_cast<const T*>(r.q) + t * r.q_token_stride + hh * r.q_head_stride
-                   : kind == 1 ? static_cast<const T*>(r.k) + t * r.k_token_stride + hh * r.k_head_stride
-                               : static_cast<const T*>(r.v) + t * r.v_token_stride + hh * r.v_head_stride;
-    float x[VEC], y[VEC];
+  constexpr int kBatch = 4;
+  const int all = hq + 2 * hkv;
+  for (int h0 = hg; h0 < all; h0 += kBatch * a.head_groups) {
+    Chunk<VEC, T> in[kBatch][2];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = y[i] = 0.f;
-    if (!padding) {
-      load_vec<VEC>(src + c0 * VEC, x);
-      if (c1 >= 0) load_vec<VEC>(src + c1 * VEC, y);
-    }
-    if (kind < 2) {
-      if (static_cast<int>(u) < pair_units) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float p = x[i], q = y[i];
-          x[i] = p * cs[i] - q * sn[i];
-          y[i] = q * cs[i] + p * sn[i];
-        }
-      } else if (r.interleaved) {
-#pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) {
-          const float p = x[2 * i], q = x[2 * i + 1], v = y[2 * i], w = y[2 * i + 1];
-          x[2 * i] = p * cs[i] - q * sn[i];
-          x[2 * i + 1] = q * cs[i] + p * sn[i];
-          y[2 * i] = v * cs[VEC / 2 + i] - w * sn[VEC / 2 + i];
-          y[2 * i + 1] = w * cs[VEC / 2 + i] + v * sn[VEC / 2 + i];
-        }
+    for (int n = 0; n < kBatch; ++n) {
+      const int h = h0 + n * a.head_groups;
+      in[n][0].clear();
+      in[n][1].clear();
+      if (h < all && !padding) {
+        const T* src = h < hq         ? static_cast<const T*>(r.q) + t * r.q_token_stride + h * r.q_head_stride
+                       : h < hq + hkv ? static_cast<const T*>(r.k) + t * r.k_token_stride + (h - hq) * r.k_head_stride
+                                      : static_cast<const T*>(r.v) + t * r.v_token_stride + (h - hq - hkv) * r.v_head_stride;
+        in[n][0].load(src + c0 * VEC);
+        if (c1 >= 0) in[n][1].load(src + c1 * VEC);
       }
     }
-    if (kind == 0 || (kind == 1 && r.k_out)) {
-      T* dst = kind == 0 ? static_cast<T*>(r.q_out) + (static_cast<int64_t>(t) * hq + hh) * D : static_cast<T*>(r.k_out) + (static_cast<int64_t>(t) * hkv + hh) * D;
-      store_vec<VEC>(dst + c0 * VEC, x);
-      if (c1 >= 0) store_vec<VEC>(dst + c1 * VEC, y);
-    }
-    if (kind > 0 && fits) {
-      C* dst = kind == 1 ? static_cast<C*>(c.k_pages) + k_at + hh * c.k_head_stride : static_cast<C*>(c.v_pages) + v_at + hh * c.v_head_stride;
-      const float* scales = kind == 1 ? c.k_scale : c.v_scale;
-      if (sizeof(C) == 1 && scales) {
-        const float s = scales[hh];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) x[i] /= s, y[i] /= s;
+    for (int n = 0; n < kBatch; ++n) {
+      const int h = h0 + n * a.head_groups;
+      if (h >= all) break;
+      const int kind = h < hq ? 0 : h < hq + hkv ? 1 : 2, hh = kind == 0 ? h : kind == 1 ? h - hq : h - hq - hkv;
+      float x[VEC], y[VEC];
+      in[n][0].get(x);
+      in[n][1].get(y);
+      if (kind < 2) {
+        if (static_cast<int>(u) < pair_units) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float p = x[i], q = y[i];
+            x[i] = p * cs[i] - q * sn[i];
+            y[i] = q * cs[i] + p * sn[i];
+          }
+        } else if (r.interleaved) {
+#pragma unroll
+          for (int i = 0; i < VEC / 2; ++i) {
+            const float p = x[2 * i], q = x[2 * i + 1], v = y[2 * i], w = y[2 * i + 1];
+            x[2 * i] = p * cs[i] - q * sn[i];
+            x[2 * i + 1] = q * cs[i] + p * sn[i];
+            y[2 * i] = v * cs[VEC / 2 + i] - w * sn[VEC / 2 + i];
+            y[2 * i + 1] = w * cs[VEC / 2 + i] + v * sn[VEC / 2 + i];
+          }
+        }
       }
-      store_vec<VEC>(dst + c0 * VEC, x);
-      if (c1 >= 0) store_vec<VEC>(dst + c1 * VEC, y);
+      if (kind == 0 || (kind == 1 && r.k_out)) {
+        T* dst = kind == 0 ? static_cast<T*>(r.q_out) + (static_cast<int64_t>(t) * hq + hh) * D : static_cast<T*>(r.k_out) + (static_cast<int64_t>(t) * hkv + hh) * D;
+        store_vec<VEC>(dst + c0 * VEC, x);
+        if (c1 >= 0) store_vec<VEC>(dst + c1 * VEC, y);
+      }
+      if (kind > 0 && fits) {
+        C* dst = kind == 1 ? static_cast<C*>(c.k_pages) + k_at + hh * c.k_head_stride : static_cast<C*>(c.v_pages) + v_at + hh * c.v_head_stride;
+        const float* scales = kind == 1 ? c.k_scale : c.v_scale;
+        if (sizeof(C) == 1 && scales) {
+          const float s = scales[hh];
+          // the reciprocal may be one rounding off the quotient, which e4m3's four bits seldom show
+          const float up = 1.f / s;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) x[i] *= up, y[i] *= up;
+        }
+        store_vec<VEC>(dst + c0 * VEC, x);
+        if (c1 >= 0) store_vec<VEC>(dst + c1 * VEC, y);
+      }
     }
   }
 }
@@ -199,7 +239,7 @@ extern "C" int tris_paged_kv_append(const TrisPagedKv* cache, const TrisPagedApp
   AppendArgs a{c, r, 0, 1};
   a.rows.rotary_dim = rot;
   // 16-byte accesses need rows that start on such boundaries and chunks of 8 that do not straddle the halves or the rotated part
-  bool wide = c.head_dim % 8 == 0 && rot % (r.interleaved ? 8 : 16) == 0 && (!r.q_out || aligned_to(r.q_out, 16)) && (!r.k_out || aligned_to(r.k_out, 16));
+  bool wide = c.head_dim % 8 == 0 && rot % (r.interleaved ? 8 : 16) == 0 && aligned_to(r.cos, 16) && aligned_to(r.sin, 16) && (!r.q_out || aligned_to(r.q_out, 16)) && (!r.k_out || aligned_to(r.k_out, 16));
   const void* src[3] = {r.num_q_heads ? r.q : nullptr, r.k, r.v};
   const int64_t strides[3][2] = {{r.q_token_stride, r.q_head_stride}, {r.k_token_stride, r.k_head_stride}, {r.v_token_stride, r.v_head_stride}};
   for (int i = 0; i < 3; ++i)
@@ -208,8 +248,9 @@ extern "C" int tris_paged_kv_append(const TrisPagedKv* cache, const TrisPagedApp
   TRIS_REQUIRE(wide || r.interleaved || rot % 4 == 0, TRIS_ERR_UNSUPPORTED, "paged_kv_append: rotary_dim must be a multiple of 4");
   a.units = ceil_div(c.head_dim / vec, 2);
   const int heads = r.num_q_heads + 2 * c.num_kv_heads;
+  // threads for two rounds of all SMs, with 640 on each; beyond that a thread takes more heads with its cosines and sines
   a.head_groups = heads;
-  while (a.head_groups > 1 && static_cast<int64_t>(a.units) * a.head_groups * r.num_tokens > 148 * 2048) a.head_groups = ceil_div(a.head_groups, 2);
+  while (a.head_groups > 1 && static_cast<int64_t>(a.units) * a.head_groups * r.num_tokens > 2 * 148 * 640) a.head_groups = ceil_div(a.head_groups, 2);
   TRIS_REQUIRE(static_cast<int64_t>(a.units) * a.head_groups * r.num_tokens < (1ll << 31), TRIS_ERR_UNSUPPORTED, "paged_kv_append: too many tokens in one call");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool f16 = r.dtype == TRIS_DTYPE_F16, q8 = c.dtype == TRIS_DTYPE_E4M3;

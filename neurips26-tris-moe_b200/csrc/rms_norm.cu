@@ -2,6 +2,7 @@
 //
 // h = residual + x; y = h * w / sqrt(mean(h^2) + eps).  The mean needs the whole row before the first output, so a row stays in the registers of
 // the CTA that reads it: x and residual are read once, h and y written once.  Bound by bytes for many rows, by the chain load -> sum -> store for one.
+// CTAs take several rows, evenly, and ask for the next row before they add up the one they have; the weights stay in registers.
 // The sums are fp32, h is not rounded before it is squared or scaled.  e4m3: y / s with s = max |y| / 448 of the group, so the group's largest
 // element is representable and none saturates; a second exchange between threads gives the maxima.
 #include "decode_step.cuh"
@@ -9,9 +10,10 @@
 namespace tris {
 namespace {
 
-constexpr int kMaxVectors = 8;  // of 8 columns that a thread keeps
+constexpr int kMaxVectors = 4;  // of 8 columns that a thread keeps
 constexpr int most_threads(int vectors) { return vectors >= 4 ? 512 : 1024; }  // whose rows fit the registers
 
+// Over the CTA; red has a place for every warp.  A barrier lies between two uses of one red (two of them take turns).
 __device__ __forceinline__ float block_sum(float v, float* red) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
@@ -30,101 +32,124 @@ __device__ __forceinline__ float block_max(float v, float* red) {
   for (unsigned w = 1; w < blockDim.x / 32; ++w) v = max_nan(v, red[w]);
   return v;
 }
+template <typename T>
+__device__ __forceinline__ void unpack_8(const uint4& raw, float (&v)[8]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Pair<T>::unpack(w[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
 
 // Rows of at most 8 * VECS * blockDim columns, all pointers and strides at 16-byte boundaries.
 template <typename T, bool FP8, int VECS>
 __global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const __grid_constant__ TrisAddRmsNorm a) {
-  __shared__ float red[32], red_max[32];
+  __shared__ float red[2][32], red_max[2][32];
   extern __shared__ float vector_max[];  // groups that do not fit a warp: largest element of every vector
   const int tid = threadIdx.x, vectors = a.hidden_size / 8;
-  const T* weight = static_cast<const T*>(a.weight);
-  pdl_wait();
-  pdl_launch_dependents();
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-  const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
-  float h[VECS][8], sum = 0.f;
+  uint4 w[VECS], x[VECS], r[VECS];
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
     const int v = tid + i * blockDim.x;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) h[i][k] = 0.f;
-    if (v < vectors) {
-      load_8(x + 8 * v, h[i]);
-      if (res) {
-        float r[8];
-        load_8(res + 8 * v, r);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) h[i][k] += r[k];
-      }
-      if (a.residual_out) store_8(static_cast<T*>(a.residual_out) + row * a.residual_out_stride + 8 * v, h[i]);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) sum += h[i][k] * h[i][k];
+    w[i] = r[i] = make_uint4(0, 0, 0, 0);
+    if (v < vectors) w[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.weight) + 8 * v);
   }
-  const float inv = 1.f / sqrtf(block_sum(sum, red) / a.hidden_size + a.eps);
-
-  if constexpr (!FP8) {
+  pdl_wait();
+  pdl_launch_dependents();
+  auto fetch = [&](int64_t row) {
+    const T* xs = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* rs = static_cast<const T*>(a.residual) + row * a.residual_stride;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = tid + i * blockDim.x;
+      x[i] = make_uint4(0, 0, 0, 0);
       if (v < vectors) {
-        float w[8];
-        load_8(weight + 8 * v, w);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) h[i][k] = h[i][k] * inv * w[k];
-        store_8(static_cast<T*>(a.y) + row * a.y_stride + 8 * v, h[i]);
+        x[i] = *reinterpret_cast<const uint4*>(xs + 8 * v);
+        if (a.residual) r[i] = *reinterpret_cast<const uint4*>(rs + 8 * v);
       }
     }
-  } else {
-    float top[VECS], all = 0.f;
+  };
+  fetch(blockIdx.x);
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    float h[VECS][8], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      const int v = tid + i * blockDim.x;
-      top[i] = 0.f;
-      if (v < vectors) {
-        float w[8];
-        load_8(weight + 8 * v, w);
+      unpack_8<T>(x[i], h[i]);
+      if (a.residual) {
+        float f[8];
+        unpack_8<T>(r[i], f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          h[i][k] = h[i][k] * inv * w[k];
-          top[i] = max_nan(top[i], fabsf(h[i][k]));
-        }
+        for (int k = 0; k < 8; ++k) h[i][k] += f[k];
       }
-      all = max_nan(all, top[i]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += h[i][k] * h[i][k];
     }
-    const int per_group = a.group_size / 8;  // vectors
-    if (a.group_size == a.hidden_size) {
-      all = block_max(all, red_max);
-#pragma unroll
-      for (int i = 0; i < VECS; ++i) top[i] = all;
-    } else if (per_group <= 32 && (per_group & (per_group - 1)) == 0) {
-      // neighbours in a warp; vectors past the row only meet one another
-      for (int d = per_group / 2; d; d >>= 1)
-#pragma unroll
-        for (int i = 0; i < VECS; ++i) top[i] = max_nan(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], d));
-    } else {
-#pragma unroll
-      for (int i = 0; i < VECS; ++i)
-        if (tid + i * blockDim.x < vectors) vector_max[tid + i * blockDim.x] = top[i];
-      __syncthreads();
+    if (row + gridDim.x < a.rows) fetch(row + gridDim.x);
+    if (a.residual_out) {
 #pragma unroll
       for (int i = 0; i < VECS; ++i) {
         const int v = tid + i * blockDim.x;
-        if (v < vectors)
-          for (int k = v / per_group * per_group, e = k + per_group; k < e; ++k) top[i] = max_nan(top[i], vector_max[k]);
+        if (v < vectors) store_8(static_cast<T*>(a.residual_out) + row * a.residual_out_stride + 8 * v, h[i]);
       }
     }
+    const float inv = 1.f / sqrtf(block_sum(sum, red[turn]) / a.hidden_size + a.eps);
+    float top[VECS], all = 0.f;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      const int v = tid + i * blockDim.x;
-      if (v < vectors) {
-        const float scale = top[i] / kE4m3Max;
-        const float div = scale == 0.f ? 1.f : scale;
+      float f[8];
+      unpack_8<T>(w[i], f);
+      top[i] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) h[i][k] /= div;
-        store_8(static_cast<__nv_fp8_e4m3*>(a.y) + row * a.y_stride + 8 * v, h[i]);
-        if (v % per_group == 0) a.scales[row * (a.hidden_size / a.group_size) + v / per_group] = scale;
+      for (int k = 0; k < 8; ++k) {
+        h[i][k] = h[i][k] * inv * f[k];
+        if (FP8) top[i] = max_nan(top[i], fabsf(h[i][k]));
+      }
+      if (FP8) all = max_nan(all, tid + i * blockDim.x < vectors ? top[i] : 0.f);
+    }
+    if constexpr (!FP8) {
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) {
+        const int v = tid + i * blockDim.x;
+        if (v < vectors) store_8(static_cast<T*>(a.y) + row * a.y_stride + 8 * v, h[i]);
+      }
+    } else {
+      const int per_group = a.group_size / 8;  // vectors
+      if (a.group_size == a.hidden_size) {
+        all = block_max(all, red_max[turn]);
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) top[i] = all;
+      } else if (per_group <= 32 && (per_group & (per_group - 1)) == 0) {
+        // neighbours in a warp; vectors past the row only meet one another
+        for (int d = per_group / 2; d; d >>= 1)
+#pragma unroll
+          for (int i = 0; i < VECS; ++i) top[i] = max_nan(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], d));
+      } else {
+        __syncthreads();  // the row before has been read
+#pragma unroll
+        for (int i = 0; i < VECS; ++i)
+          if (tid + i * blockDim.x < vectors) vector_max[tid + i * blockDim.x] = top[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) {
+          const int v = tid + i * blockDim.x;
+          if (v < vectors)
+            for (int k = v / per_group * per_group, e = k + per_group; k < e; ++k) top[i] = max_nan(top[i], vector_max[k]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) {
+        const int v = tid + i * blockDim.x;
+        if (v < vectors) {
+          const float scale = top[i] / kE4m3Max;
+          // 1 / scale may be one rounding off the quotient, which e4m3's four bits seldom show; it overflows where scale is subnormal: divided there
+          const float up = 1.f / scale;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) h[i][k] = scale == 0.f ? h[i][k] : scale >= 1.2e-38f ? h[i][k] * up : h[i][k] / scale;
+          store_8(static_cast<__nv_fp8_e4m3*>(a.y) + row * a.y_stride + 8 * v, h[i]);
+          if (v % per_group == 0) a.scales[row * (a.hidden_size / a.group_size) + v / per_group] = scale;
+        }
       }
     }
   }
@@ -190,8 +215,10 @@ int launch_norm(const TrisAddRmsNorm& a, cudaStream_t stream) {
   const int per_group = FP8 ? a.group_size / 8 : 0;
   const bool in_warp = per_group <= 32 && (per_group & (per_group - 1)) == 0;
   const size_t smem = FP8 && a.group_size != H && !in_warp ? sizeof(float) * vectors : 0;
-  auto kernel = vecs == 1 ? add_rms_norm_kernel<T, FP8, 1> : vecs == 2 ? add_rms_norm_kernel<T, FP8, 2> : vecs == 4 ? add_rms_norm_kernel<T, FP8, 4> : add_rms_norm_kernel<T, FP8, 8>;
-  TRIS_CUDA(launch_kernel(kernel, dim3(a.rows), dim3(threads), smem, stream, pdl, 1, a));
+  auto kernel = vecs == 1 ? add_rms_norm_kernel<T, FP8, 1> : vecs == 2 ? add_rms_norm_kernel<T, FP8, 2> : add_rms_norm_kernel<T, FP8, 4>;
+  const int resident = 148 * (vecs == 1 ? 1280 : vecs == 2 ? 1024 : 512) / threads;  // by registers
+  const int turns = ceil_div(a.rows, resident < 1 ? 1 : resident);
+  TRIS_CUDA(launch_kernel(kernel, dim3(ceil_div(a.rows, turns)), dim3(threads), smem, stream, pdl, 1, a));
   return TRIS_OK;
 }
 
