@@ -1,22 +1,30 @@
 // Penalties for repeated tokens, biases and grammar masks on logits.
 //
-// A pass over the logits that reads each once and writes it once; which of them a penalty concerns is looked up in shared memory.  A CTA has a slice
-// of one row's vocabulary: it counts the history's tokens that lie in its slice (integer atomics, whose order does not matter) and then changes
-// its logits.  Those are few for every thread, and asked for before anything else, as are the first tokens of the history: the three ways to memory
-// overlap.  Every CTA of a row reads the row's history, which comes from L2; slices of 4096 logits keep that below what the slice itself takes for
-// histories of up to some thousand tokens.  Biases are few: they are added to what the CTA has written, one thread an entry.
+// A pass over the logits that reads each once and writes it once; which of them a penalty or a bias concerns is looked up in shared memory.  A CTA has
+// a slice of one row's vocabulary: it counts the history's tokens that lie in its slice (integer atomics, whose order does not matter) and then
+// streams over its logits, the next ones always on their way; the first, the mask and the first tokens of the history are asked for together.
+// Every CTA of a row reads the row's history, from L2, at some 24 instructions for 32 tokens: with slices of 4096 logits that was half of all work
+// (128 rows of 50304 logits and 3000 tokens 22 us), with four slices a row it is 17 us, 8 of them the stream.  Not kept: eight CTAs of a cluster that
+// count in one another's shared memory (31 us, two cluster barriers a CTA), a list of the logits concerned in place of the look-up (19 us), tokens of the slice
+// collected before they are counted (24 us).
 #include "decode_step.cuh"
 
 namespace tris {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 4;  // tokens of the history that a thread asks for at once
-constexpr uint32_t kHasBias = 0x80000000u, kInPrompt = 0x40000000u, kCount = 0x3FFFFFFFu;
+constexpr int kMostSlice = 12800;
+// A word counts the answer's occurrences in its low 16 bits and the prompt's in those above; in histories of more than 32767 tokens, where that could
+// overflow, the answer has 30 bits and the prompt's only set a bit.
+constexpr uint32_t kHasBias = 0x80000000u, kPrompt = 0x10000u, kLongPrompt = 0x40000000u;
+
 
 struct LogitArgs {
   TrisLogitControls c;
-  int wide;  // whether four logits can be read, and four results written, at once
+  int slice;        // logits of a CTA, a multiple of 32
+  int wide;         // whether four logits can be read, and four results written, at once
+  int wide_tokens;  // whether four tokens can
+  int short_history;
 };
 
 template <typename T>
@@ -31,108 +39,138 @@ __device__ __forceinline__ void load_4(const T* p, float (&z)[4]) {
   }
 }
 
-// VECS: groups of four logits that a thread has.
+// VECS: groups of four logits that a thread has at a time.
 template <typename T, int VECS>
 __global__ void __launch_bounds__(kThreads, 5) logit_controls_kernel(const __grid_constant__ LogitArgs a) {
-  constexpr int kSlice = kThreads * 4 * VECS;
-  __shared__ __align__(16) uint32_t words[kSlice];  // per logit: occurrences in the answer, whether in the prompt, whether it has a bias
-  __shared__ int repeated;                          // whether an id has two biases
+  extern __shared__ __align__(16) uint32_t words[];  // [slice] per logit: how often answer and prompt have it, and whether it has a bias
+  __shared__ int repeated;                           // whether an id has two biases
   const TrisLogitControls& c = a.c;
   const int64_t row = blockIdx.y;
-  const int v0 = blockIdx.x * kSlice, n = min(kSlice, c.vocab - v0), tid = threadIdx.x;
-  if (c.tokens || c.bias_ids) {
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) reinterpret_cast<uint4*>(words)[tid + i * kThreads] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) repeated = 0;
-  }
+  const int tid = threadIdx.x, v0 = blockIdx.x * a.slice, n = min(a.slice, c.vocab - v0);
+  const bool fast = a.wide && n % 4 == 0, marked = c.tokens || c.bias_ids;
   pdl_wait();
   pdl_launch_dependents();
   const T* in = static_cast<const T*>(c.logits) + row * c.logits_stride + v0;
   float* out = c.out + row * c.out_stride + v0;
   const int32_t* allowed = c.allowed ? c.allowed + row * c.allowed_stride + v0 / 32 : nullptr;
   const int32_t* tok = c.tokens ? c.tokens + row * c.tokens_stride : nullptr;
+  const int32_t* ids = c.bias_ids ? c.bias_ids + row * c.bias_stride : nullptr;
+  const float* values = c.bias_ids ? c.bias_values + row * c.bias_stride : nullptr;
 
-  int ahead[kAhead];
+  auto tokens_at = [&](int i) {  // four of them, -1 behind the last
+    if (a.wide_tokens && i + 4 <= c.max_tokens) return *reinterpret_cast<const int4*>(tok + i);
+    return make_int4(i < c.max_tokens ? tok[i] : -1, i + 1 < c.max_tokens ? tok[i + 1] : -1, i + 2 < c.max_tokens ? tok[i + 2] : -1,
+                     i + 3 < c.max_tokens ? tok[i + 3] : -1);
+  };
+  int4 now = make_int4(-1, -1, -1, -1);
+  if (tok) now = tokens_at(4 * tid);  // whether or not the history is that long
+  const int len = tok ? min(max(c.token_lengths[row], 0), c.max_tokens) : 0;
+  const int answer = tok && c.prompt_lengths ? c.prompt_lengths[row] : 0;  // first token that is counted
+  const int first_id = ids && tid < c.num_biases ? ids[tid] : -1;
+  float z[VECS][4], z_next[VECS][4];
+  uint32_t bits[VECS], bits_next[VECS];
+  // No branch between the loads, and nothing that waits for one: places behind the slice's end read its last ones.
+  auto fetch = [&](int base, float (&z)[VECS][4], uint32_t (&bits)[VECS]) {
+    if (fast) {
 #pragma unroll
-  for (int k = 0; k < kAhead; ++k) ahead[k] = tok && tid + k * kThreads < c.max_tokens ? tok[tid + k * kThreads] : -1;
-  float z[VECS][4];
-  uint32_t bits[VECS];
-#pragma unroll
-  for (int i = 0; i < VECS; ++i) {
-    const int at = 4 * (tid + i * kThreads);
-    bits[i] = allowed && at < n ? allowed[at / 32] >> (at & 31) : 0xFu;
-    if (a.wide && at + 4 <= n) {
-      load_4(in + at, z[i]);
+      for (int i = 0; i < VECS; ++i) load_4(in + min(base + 4 * (tid + i * kThreads), n - 4), z[i]);
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) z[i][k] = at + k < n ? to_float(in[at + k]) : 0.f;
+      for (int i = 0; i < VECS; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) z[i][k] = to_float(in[min(base + 4 * (tid + i * kThreads) + k, n - 1)]);
     }
-  }
+    if (allowed) {
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) bits[i] = allowed[min(base + 4 * (tid + i * kThreads), n - 1) / 32];
+    }
+  };
+  fetch(0, z, bits);
+  const float rep = c.repetition ? c.repetition[row] : 1.f, pres = c.presence ? c.presence[row] : 0.f, freq = c.frequency ? c.frequency[row] : 0.f;
 
-  if (c.tokens || c.bias_ids) {
-    const int len = tok ? min(max(c.token_lengths[row], 0), c.max_tokens) : 0;
-    const int prompt = c.prompt_lengths ? c.prompt_lengths[row] : 0;
+  if (marked) {
+    for (int i = tid; i < a.slice / 4; i += kThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) repeated = 0;
     __syncthreads();
-    for (int i0 = tid; i0 < len; i0 += kAhead * kThreads) {
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int i = i0 + k * kThreads;
-        const int id = ahead[k];
-        if (i < len && id >= v0 && id - v0 < n) {
-          if (i < prompt)
-            atomicOr(words + (id - v0), kInPrompt);
-          else
-            atomicAdd(words + (id - v0), 1u);
-        }
+    auto mark = [&](int id, int i) {
+      const uint32_t at = static_cast<uint32_t>(id) - static_cast<uint32_t>(v0);
+      if (at < static_cast<uint32_t>(n)) {
+        if (a.short_history || i >= answer)
+          atomicAdd(words + at, i >= answer ? 1u : kPrompt);
+        else
+          atomicOr(words + at, kLongPrompt);
       }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int i = i0 + (kAhead + k) * kThreads;
-        ahead[k] = i < len ? tok[i] : -1;
+    };
+    for (int i = 4 * tid; i < len;) {
+      const int next = i + 4 * kThreads;
+      int4 then = make_int4(-1, -1, -1, -1);
+      if (next < len) then = tokens_at(next);
+      if (i + 4 > len) {
+        if (i + 1 >= len) now.y = -1;
+        if (i + 2 >= len) now.z = -1;
+        now.w = -1;
       }
+      mark(now.x, i);
+      mark(now.y, i + 1);
+      mark(now.z, i + 2);
+      mark(now.w, i + 3);
+      now = then;
+      i = next;
     }
-    for (int i = tid; c.bias_ids && i < c.num_biases; i += kThreads) {
-      const int id = c.bias_ids[row * c.bias_stride + i];
+    for (int i = tid; ids && i < c.num_biases; i += kThreads) {
+      const int id = i == tid ? first_id : ids[i];
       if (id >= v0 && id - v0 < n && (atomicOr(words + (id - v0), kHasBias) & kHasBias)) repeated = 1;
     }
     __syncthreads();
   }
 
-  const float rep = c.repetition ? c.repetition[row] : 1.f, pres = c.presence ? c.presence[row] : 0.f, freq = c.frequency ? c.frequency[row] : 0.f;
+  const float less = 1.f / rep;  // z * less is z / rep to a rounding
+  const uint32_t in_answer = a.short_history ? kPrompt - 1 : kLongPrompt - 1;
+  for (int base = 0; base < n; base += 4 * VECS * kThreads) {
+    if (base + 4 * VECS * kThreads < n) fetch(base + 4 * VECS * kThreads, z_next, bits_next);
 #pragma unroll
-  for (int i = 0; i < VECS; ++i) {
-    const int at = 4 * (tid + i * kThreads);
-    if (at >= n) break;
-    if (tok) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(words + at);
-      const uint32_t w[4] = {raw.x & ~kHasBias, raw.y & ~kHasBias, raw.z & ~kHasBias, raw.w & ~kHasBias};
-      if (w[0] | w[1] | w[2] | w[3]) {
+    for (int i = 0; i < VECS; ++i) {
+      const int at = base + 4 * (tid + i * kThreads);
+      if (at >= n) break;
+      if (tok) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(words + at);
+        if ((raw.x | raw.y | raw.z | raw.w) & ~kHasBias) {
+          const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (w[k]) {
-            if (c.repetition) z[i][k] = z[i][k] > 0.f ? z[i][k] / rep : z[i][k] * rep;
-            if (w[k] & kCount) z[i][k] = z[i][k] - freq * static_cast<float>(w[k] & kCount) - pres;
+          for (int k = 0; k < 4; ++k) {
+            const float scaled = z[i][k] * (z[i][k] > 0.f ? less : rep);
+            if ((w[k] & ~kHasBias) && c.repetition) z[i][k] = scaled;
+            const uint32_t count = w[k] & in_answer;
+            const float lower = z[i][k] - freq * static_cast<float>(count) - pres;
+            if (count) z[i][k] = lower;
           }
         }
       }
+      if (allowed) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (!((bits[i] >> (at & 31)) & (1u << k))) z[i][k] = -INFINITY;
+      }
+      if (fast) {
+        *reinterpret_cast<float4*>(out + at) = make_float4(z[i][0], z[i][1], z[i][2], z[i][3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (at + k < n) out[at + k] = z[i][k];
+      }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (!((bits[i] >> k) & 1)) z[i][k] = -INFINITY;
-    if (a.wide && at + 4 <= n) {
-      *reinterpret_cast<float4*>(out + at) = make_float4(z[i][0], z[i][1], z[i][2], z[i][3]);
-    } else {
+    for (int i = 0; i < VECS; ++i) {
+      bits[i] = bits_next[i];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (at + k < n) out[at + k] = z[i][k];
+      for (int k = 0; k < 4; ++k) z[i][k] = z_next[i][k];
     }
   }
-  if (!c.bias_ids) return;
+  if (!ids) return;
+  // Biases are few: they are added to what has been written, one thread an entry.
   __syncthreads();
   for (int i = tid; i < c.num_biases; i += kThreads) {
-    const int32_t* ids = c.bias_ids + row * c.bias_stride;
-    const float* values = c.bias_values + row * c.bias_stride;
-    const int id = ids[i], at = id - v0;
+    const int id = i == tid ? first_id : ids[i], at = id - v0;
     if (id < v0 || at >= n) continue;
     float bias = values[i];
     if (repeated) {  // the first of an id's entries adds all of them, in their order
@@ -147,12 +185,16 @@ __global__ void __launch_bounds__(kThreads, 5) logit_controls_kernel(const __gri
 }
 
 template <int VECS>
-int launch_controls(const LogitArgs& a, cudaStream_t stream) {
+int launch_controls(LogitArgs& a, int most, cudaStream_t stream) {
   const TrisLogitControls& c = a.c;
+  const int slices = ceil_div(c.vocab, most);
+  a.slice = (ceil_div(c.vocab, slices) + 31) / 32 * 32;  // even ones
+  const size_t smem = c.tokens || c.bias_ids ? 4 * static_cast<size_t>(a.slice) : 0;
   auto kernel = c.dtype == TRIS_DTYPE_F16    ? logit_controls_kernel<__half, VECS>
                 : c.dtype == TRIS_DTYPE_BF16 ? logit_controls_kernel<__nv_bfloat16, VECS>
                                              : logit_controls_kernel<float, VECS>;
-  TRIS_CUDA(launch_kernel(kernel, dim3(ceil_div(c.vocab, kThreads * 4 * VECS), c.rows), dim3(kThreads), 0, stream, programmatic_launch_default(), 1, a));
+  TRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMostSlice));
+  TRIS_CUDA(launch_kernel(kernel, dim3(ceil_div(c.vocab, a.slice), c.rows), dim3(kThreads), smem, stream, programmatic_launch_default(), 1, a));
   return TRIS_OK;
 }
 
@@ -168,17 +210,17 @@ extern "C" int tris_logit_controls(const TrisLogitControls* args, void* stream) 
   TRIS_REQUIRE(c.rows >= 0 && c.vocab >= 0 && c.max_tokens >= 0 && c.num_biases >= 0, TRIS_ERR_INVALID_ARG, "logit_controls: negative sizes");
   if (c.rows == 0 || c.vocab == 0) return TRIS_OK;
   TRIS_REQUIRE(c.rows <= 65535, TRIS_ERR_UNSUPPORTED, "logit_controls: more than 65535 rows");
-  TRIS_REQUIRE(c.max_tokens < (1 << 30), TRIS_ERR_UNSUPPORTED, "logit_controls: histories of 2^30 tokens and more");
+  TRIS_REQUIRE(c.max_tokens < (1 << 30) && c.vocab < (1 << 30), TRIS_ERR_UNSUPPORTED, "logit_controls: histories or vocabularies of 2^30 tokens and more");
   TRIS_REQUIRE(c.logits && c.out, TRIS_ERR_INVALID_ARG, "logit_controls: null logits or out");
   TRIS_REQUIRE(!c.tokens || c.token_lengths, TRIS_ERR_INVALID_ARG, "logit_controls: tokens need token_lengths");
   TRIS_REQUIRE(c.tokens || c.max_tokens == 0 || !(c.repetition || c.presence || c.frequency), TRIS_ERR_INVALID_ARG, "logit_controls: penalties need tokens");
   TRIS_REQUIRE(!c.bias_ids == !c.bias_values, TRIS_ERR_INVALID_ARG, "logit_controls: bias_ids and bias_values go together");
   const int elt = dtype_size(c.dtype);
-  LogitArgs a{c, 0};
+  LogitArgs a{c, 0, 0, aligned_to(c.tokens, 16) && c.tokens_stride % 4 == 0, c.max_tokens < 32768};
   if (!(c.repetition || c.presence || c.frequency) || c.max_tokens == 0) a.c.tokens = nullptr;
   if (c.num_biases == 0) a.c.bias_ids = nullptr;
   a.wide = aligned_to(c.logits, 4 * elt) && aligned_to(c.out, 16) && c.logits_stride % 4 == 0 && c.out_stride % 4 == 0;
-  // slices of 4096 where that still gives every SM some, else of 1024
+  // slices of 1024 where larger ones would leave SMs without work
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return static_cast<int64_t>(ceil_div(c.vocab, 4096)) * c.rows >= 2 * 148 ? launch_controls<4>(a, s) : launch_controls<1>(a, s);
+  return static_cast<int64_t>(ceil_div(c.vocab, 4096)) * c.rows < 2 * 148 ? launch_controls<1>(a, 1024, s) : launch_controls<2>(a, kMostSlice, s);
 }

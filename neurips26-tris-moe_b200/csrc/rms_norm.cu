@@ -13,6 +13,13 @@ namespace {
 constexpr int kMaxVectors = 4;  // of 8 columns that a thread keeps
 constexpr int most_threads(int vectors) { return vectors >= 4 ? 512 : 1024; }  // whose rows fit the registers
 
+struct NormArgs {
+  TrisAddRmsNorm a;
+  float inv_hidden;
+  int groups;       // scales of a row
+  int group_shift;  // log2 of the vectors of a group where that is a power of two up to a warp's lanes, else -1
+};
+
 // Over the CTA; red has a place for every warp.  A barrier lies between two uses of one red (two of them take turns).
 __device__ __forceinline__ float block_sum(float v, float* red) {
 #pragma unroll
@@ -44,7 +51,8 @@ __device__ __forceinline__ void unpack_8(const uint4& raw, float (&v)[8]) {
 
 // Rows of at most 8 * VECS * blockDim columns, all pointers and strides at 16-byte boundaries.
 template <typename T, bool FP8, int VECS>
-__global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const __grid_constant__ TrisAddRmsNorm a) {
+__global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const __grid_constant__ NormArgs args) {
+  const TrisAddRmsNorm& a = args.a;
   __shared__ float red[2][32], red_max[2][32];
   extern __shared__ float vector_max[];  // groups that do not fit a warp: largest element of every vector
   const int tid = threadIdx.x, vectors = a.hidden_size / 8;
@@ -94,7 +102,7 @@ __global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const 
         if (v < vectors) store_8(static_cast<T*>(a.residual_out) + row * a.residual_out_stride + 8 * v, h[i]);
       }
     }
-    const float inv = 1.f / sqrtf(block_sum(sum, red[turn]) / a.hidden_size + a.eps);
+    const float inv = rsqrtf(block_sum(sum, red[turn]) * args.inv_hidden + a.eps);
     float top[VECS], all = 0.f;
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
@@ -120,7 +128,7 @@ __global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const 
         all = block_max(all, red_max[turn]);
 #pragma unroll
         for (int i = 0; i < VECS; ++i) top[i] = all;
-      } else if (per_group <= 32 && (per_group & (per_group - 1)) == 0) {
+      } else if (args.group_shift >= 0) {
         // neighbours in a warp; vectors past the row only meet one another
         for (int d = per_group / 2; d; d >>= 1)
 #pragma unroll
@@ -143,12 +151,18 @@ __global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const 
         const int v = tid + i * blockDim.x;
         if (v < vectors) {
           const float scale = top[i] / kE4m3Max;
-          // 1 / scale may be one rounding off the quotient, which e4m3's four bits seldom show; it overflows where scale is subnormal: divided there
-          const float up = 1.f / scale;
+          // times the reciprocal: at most one rounding off the quotient, which e4m3's four bits seldom show.  Of a subnormal scale the reciprocal
+          // overflows, so values and scale are raised first; a scale of 0 has nothing but zeros
+          const float lift = scale < 1.2e-38f ? 1.8446744e19f : 1.f;
+          const float up = scale == 0.f ? 0.f : 1.f / (scale * lift);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) h[i][k] = scale == 0.f ? h[i][k] : scale >= 1.2e-38f ? h[i][k] * up : h[i][k] / scale;
+          for (int k = 0; k < 8; ++k) h[i][k] = h[i][k] * lift * up;
           store_8(static_cast<__nv_fp8_e4m3*>(a.y) + row * a.y_stride + 8 * v, h[i]);
-          if (v % per_group == 0) a.scales[row * (a.hidden_size / a.group_size) + v / per_group] = scale;
+          if (args.group_shift >= 0) {
+            if ((v & (per_group - 1)) == 0) a.scales[row * args.groups + (v >> args.group_shift)] = scale;
+          } else if (v % per_group == 0) {
+            a.scales[row * args.groups + v / per_group] = scale;
+          }
         }
       }
     }
@@ -212,13 +226,14 @@ int launch_norm(const TrisAddRmsNorm& a, cudaStream_t stream) {
   int vecs = 1;
   while (vecs < kMaxVectors && (ceil_div(vectors, vecs) > most_threads(vecs) || (a.rows > 148 && ceil_div(vectors, vecs) > 256))) vecs *= 2;
   const int threads = (ceil_div(vectors, vecs) + 31) / 32 * 32;
-  const int per_group = FP8 ? a.group_size / 8 : 0;
-  const bool in_warp = per_group <= 32 && (per_group & (per_group - 1)) == 0;
-  const size_t smem = FP8 && a.group_size != H && !in_warp ? sizeof(float) * vectors : 0;
+  NormArgs args{a, 1.f / H, FP8 ? H / a.group_size : 1, -1};
+  for (int shift = 0; FP8 && shift <= 5; ++shift)
+    if (a.group_size == 8 << shift) args.group_shift = shift;
+  const size_t smem = FP8 && a.group_size != H && args.group_shift < 0 ? sizeof(float) * vectors : 0;
   auto kernel = vecs == 1 ? add_rms_norm_kernel<T, FP8, 1> : vecs == 2 ? add_rms_norm_kernel<T, FP8, 2> : add_rms_norm_kernel<T, FP8, 4>;
   const int resident = 148 * (vecs == 1 ? 1280 : vecs == 2 ? 1024 : 512) / threads;  // by registers
   const int turns = ceil_div(a.rows, resident < 1 ? 1 : resident);
-  TRIS_CUDA(launch_kernel(kernel, dim3(ceil_div(a.rows, turns)), dim3(threads), smem, stream, pdl, 1, a));
+  TRIS_CUDA(launch_kernel(kernel, dim3(ceil_div(a.rows, turns)), dim3(threads), smem, stream, pdl, 1, args));
   return TRIS_OK;
 }
 

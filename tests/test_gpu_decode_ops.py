@@ -472,7 +472,7 @@ def _controls_64(logits, c):
     return z, mag
 
 
-@pytest.mark.parametrize("rows,vocab,history", [(1, 50304, 700), (3, 1, 5), (5, 31, 40), (2, 1000, 0), (7, 32000, 3001), (130, 513, 64), (1, 131073, 9000)])
+@pytest.mark.parametrize("rows,vocab,history", [(1, 50304, 700), (3, 1, 5), (5, 31, 40), (2, 1000, 0), (7, 32000, 3001), (130, 513, 64), (1, 131073, 9000), (2, 4000, 40000)])
 @pytest.mark.parametrize("dtype", [F16, BF16, torch.float32], ids=["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("names", ["", "repetition", "presence frequency", "bias", "allowed", "repetition presence frequency bias allowed prompt"])
 def test_logit_controls(lib, rows, vocab, history, dtype, names):
