@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace tris {
@@ -67,6 +69,18 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
+// Lets a kernel use that much dynamic shared memory; asked of the driver once a device (0.5 us a call).
+template <auto KERNEL>
+inline int allow_shared_memory(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  TRIS_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return TRIS_OK;
+  TRIS_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return TRIS_OK;
+}
 inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline int dtype_size(int dtype) { return dtype == TRIS_DTYPE_F32 ? 4 : dtype == TRIS_DTYPE_E4M3 ? 1 : 2; }
 int validate_paged_kv(const TrisPagedKv* cache, const char* what);  // paged_kv.cu

@@ -184,18 +184,21 @@ __global__ void __launch_bounds__(kThreads, 5) logit_controls_kernel(const __gri
   }
 }
 
-template <int VECS>
+template <typename T, int VECS>
 int launch_controls(LogitArgs& a, int most, cudaStream_t stream) {
   const TrisLogitControls& c = a.c;
   const int slices = ceil_div(c.vocab, most);
   a.slice = (ceil_div(c.vocab, slices) + 31) / 32 * 32;  // even ones
   const size_t smem = c.tokens || c.bias_ids ? 4 * static_cast<size_t>(a.slice) : 0;
-  auto kernel = c.dtype == TRIS_DTYPE_F16    ? logit_controls_kernel<__half, VECS>
-                : c.dtype == TRIS_DTYPE_BF16 ? logit_controls_kernel<__nv_bfloat16, VECS>
-                                             : logit_controls_kernel<float, VECS>;
-  TRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMostSlice));
-  TRIS_CUDA(launch_kernel(kernel, dim3(ceil_div(c.vocab, a.slice), c.rows), dim3(kThreads), smem, stream, programmatic_launch_default(), 1, a));
+  if (int st = allow_shared_memory<logit_controls_kernel<T, VECS>>(4 * kMostSlice)) return st;
+  TRIS_CUDA(launch_kernel(logit_controls_kernel<T, VECS>, dim3(ceil_div(c.vocab, a.slice), c.rows), dim3(kThreads), smem, stream, programmatic_launch_default(), 1, a));
   return TRIS_OK;
+}
+// Slices of 1024 where larger ones would leave SMs without work.
+template <typename T>
+int launch_controls(LogitArgs& a, cudaStream_t stream) {
+  const bool few = static_cast<int64_t>(ceil_div(a.c.vocab, 4096)) * a.c.rows < 2 * 148;
+  return few ? launch_controls<T, 1>(a, 1024, stream) : launch_controls<T, 2>(a, kMostSlice, stream);
 }
 
 }  // namespace
@@ -220,7 +223,6 @@ extern "C" int tris_logit_controls(const TrisLogitControls* args, void* stream) 
   if (!(c.repetition || c.presence || c.frequency) || c.max_tokens == 0) a.c.tokens = nullptr;
   if (c.num_biases == 0) a.c.bias_ids = nullptr;
   a.wide = aligned_to(c.logits, 4 * elt) && aligned_to(c.out, 16) && c.logits_stride % 4 == 0 && c.out_stride % 4 == 0;
-  // slices of 1024 where larger ones would leave SMs without work
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return static_cast<int64_t>(ceil_div(c.vocab, 4096)) * c.rows < 2 * 148 ? launch_controls<1>(a, 1024, s) : launch_controls<2>(a, kMostSlice, s);
+  return c.dtype == TRIS_DTYPE_F16 ? launch_controls<__half>(a, s) : c.dtype == TRIS_DTYPE_BF16 ? launch_controls<__nv_bfloat16>(a, s) : launch_controls<float>(a, s);
 }

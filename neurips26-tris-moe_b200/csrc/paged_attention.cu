@@ -741,7 +741,7 @@ int launch_attention(AttnArgs& a, cudaStream_t stream) {
   using S = Shape<T, FP8, DP, NT>;
   auto kernel = paged_attention_kernel<T, FP8, DP, NT>;
   const TrisPagedKv& c = a.cache;
-  TRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  if (int st = allow_shared_memory<paged_attention_kernel<T, FP8, DP, NT>>(S::kSmem)) return st;
   a.resident = sm_count() * S::kCtasPerSm;
   a.ctas = attention_ctas(a.resident, most_blocks(c, a.row_tiles));
   a.rows_together = a.page_blocks && c.head_dim == DP && c.k_token_stride == DP && c.v_token_stride == DP;

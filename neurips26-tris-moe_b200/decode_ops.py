@@ -25,13 +25,23 @@ from . import _native
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2, torch.float8_e4m3fn: 3}
 _ROWS = (torch.float16, torch.bfloat16)
+_LOGIT_TYPES = (torch.float16, torch.bfloat16, torch.float32)
 # the structs of include/trismoe_b200.h, field by field (packing bytes takes a third of the time of a ctypes structure)
 _PAGED_KV = struct.Struct("@2Q6q3Qq8iQ")
 _APPEND = struct.Struct("@3Q6q6Q8i")
 _ATTENTION = struct.Struct("@Q2q4Qq3if")
 _NORM = struct.Struct("@6Q4q5if")
 _LOGITS = struct.Struct("@11Q5q6i")
-_workspace_bytes: dict = {}
+_scratch: dict = {}  # (device, heads) -> one byte seen as many, whose like is the scratch of a call
+
+
+def _scratch_like(key: tuple, cache: bytes, dev: torch.device) -> torch.Tensor:
+    with torch.cuda.device(dev):
+        need = int(_native.load().tris_paged_decode_attention_workspace_bytes(cache, key[1]))
+    byte = torch.empty((1,), dtype=torch.uint8, device=dev).expand(need)
+    if need:  # sizes that the call will refuse are not kept
+        _scratch[key] = byte
+    return byte
 
 
 def _fail(what: str, why: str):
@@ -39,38 +49,70 @@ def _fail(what: str, why: str):
 
 
 def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
-    _native.require_cuda(first, what)
     index = first.get_device()
+    if index < 0:
+        _native.require_cuda(first, what)
     for t in others:
         if t is not None and t.get_device() != index:
             _fail(what, "all tensors must live on one CUDA device")
     return first.device
 
 
-def _want(what: str, name: str, t: torch.Tensor, dtype, *shape) -> int:
+def _want(what: str, name: str, t: torch.Tensor, dtype, shape: tuple) -> int:
     """Address of a contiguous tensor of that type and shape."""
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         _fail(what, f"{name} must be contiguous {dtype} of shape {shape}, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
+def _matrix(what: str, name: str, t: torch.Tensor, dtype, rows: int, columns: Optional[int] = None) -> tuple:
+    """Address, row stride and columns of a matrix whose rows lie side by side in themselves."""
+    shape = t.shape
+    if len(shape) != 2 or t.dtype is not dtype or shape[0] != rows or (columns is not None and shape[1] != columns) or (t.stride(1) != 1 and shape[1] > 1):
+        _fail(what, f"{name} must be {dtype} [{rows}, {'any' if columns is None else columns}] with a row side by side, got {t.dtype} {tuple(shape)}")
+    return t.data_ptr(), t.stride(0), shape[1]
+
+
+def _new_like(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous, of t's shape, type and device (torch.empty with those spelled out takes twice as long)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _launch(what: str, name: str, dev: torch.device, *structs: bytes) -> None:
+    """Calls an entry point of the library on the device's current stream."""
+    entry = getattr(_native._lib or _native.load(), name)
+    if dev.index == torch._C._cuda_getDevice():
+        status = entry(*structs, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            status = entry(*structs, _native.stream_of(dev))
+    if status:
+        _native.check(status, what)
+
+
 def _cache(what: str, k_pages, v_pages, block_table, k_scale, v_scale, status) -> bytes:
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.dtype not in _DTYPES:
+    shape, dtype = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or shape != v_pages.shape or dtype is not v_pages.dtype or dtype not in _DTYPES:
         _fail(what, "k_pages and v_pages must have the same type and shape [num_pages, page_size, num_kv_heads, head_dim]")
-    pages, page_size, heads, dim = k_pages.shape
-    ks, vs, e4m3 = k_pages.stride(), v_pages.stride(), k_pages.dtype == torch.float8_e4m3fn
-    if ks[3] != 1 or vs[3] != 1:
+    pages, page_size, heads, dim = shape
+    k0, k1, k2, k3 = k_pages.stride()
+    v0, v1, v2, v3 = v_pages.stride()
+    if k3 != 1 or v3 != 1:
         _fail(what, "the dimensions of a head must be side by side")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        _fail(what, "block_table must be int32 [sequences, pages] with the pages of a sequence side by side")
-    if (k_scale is not None or v_scale is not None) and not e4m3:
+    if block_table.dim() != 2 or block_table.dtype is not torch.int32:
+        _fail(what, "block_table must be int32 [sequences, pages]")
+    sequences, width = block_table.shape
+    t0, t1 = block_table.stride()
+    if t1 != 1 and width > 1:
+        _fail(what, "block_table must have the pages of a sequence side by side")
+    if (k_scale is not None or v_scale is not None) and dtype is not torch.float8_e4m3fn:
         _fail(what, "scales belong to e4m3 pages")
     return _PAGED_KV.pack(
-        k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-        0 if k_scale is None else _want(what, "k_scale", k_scale, torch.float32, heads),
-        0 if v_scale is None else _want(what, "v_scale", v_scale, torch.float32, heads),
-        block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1], pages, page_size, heads, dim,
-        _DTYPES[k_pages.dtype], 0, 0 if status is None else _want(what, "status", status, torch.int32, 1))
+        k_pages.data_ptr(), v_pages.data_ptr(), k0, k1, k2, v0, v1, v2,
+        0 if k_scale is None else _want(what, "k_scale", k_scale, torch.float32, (heads,)),
+        0 if v_scale is None else _want(what, "v_scale", v_scale, torch.float32, (heads,)),
+        block_table.data_ptr(), t0, sequences, width, pages, page_size, heads, dim,
+        _DTYPES[dtype], 0, 0 if status is None else _want(what, "status", status, torch.int32, (1,)))
 
 
 def raise_on_status(status: torch.Tensor, what: str = "paged cache") -> None:
@@ -96,39 +138,38 @@ def append_paged_kv(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     with ``return_key`` a pair with the rotated keys."""
     what = "append_paged_kv"
     dev = _same_device(what, k, v, q, k_pages, v_pages, block_table, positions, sequences, cos, sin, k_scale, v_scale, status)
-    if k.dim() != 3 or v.shape != k.shape or k.dtype not in _ROWS or v.dtype != k.dtype or (k_pages.dim() == 4 and k.shape[1:] != k_pages.shape[2:]):
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 3 or v.shape != shape or dtype not in _ROWS or v.dtype is not dtype or shape[1:] != k_pages.shape[2:]:
         _fail(what, "k and v must be fp16 or bf16 [tokens, num_kv_heads, head_dim] of the cache")
-    tokens, kv_heads, dim = k.shape
-    if q is not None and (q.dim() != 3 or q.dtype != k.dtype or q.shape[0] != tokens or q.shape[2] != dim):
-        _fail(what, "q must be [tokens, q heads, head_dim] in the keys' type")
-    if positions.dtype not in (torch.int32, torch.int64):
-        _fail(what, "positions must be int32 or int64")
-    _want(what, "positions", positions, positions.dtype, tokens)
-    if sequences is not None:
-        _want(what, "sequences", sequences, torch.int32, tokens)
-    rotary, rows = 0, 0
-    if (cos is None) != (sin is None):
-        _fail(what, "cos and sin go together")
-    if cos is not None:
-        if cos.dim() != 2:
-            _fail(what, "cos and sin must be [positions, rotary_dim / 2]")
-        rows, rotary = cos.shape[0], 2 * cos.shape[1]
-        _want(what, "cos", cos, torch.float32, rows, rotary // 2)
-        _want(what, "sin", sin, torch.float32, rows, rotary // 2)
-    ks, vs, qs = k.stride(), v.stride(), (0, 0, 1) if q is None else q.stride()
-    if tokens and (ks[2] != 1 or vs[2] != 1 or qs[2] != 1):
-        _fail(what, "the dimensions of a head must be side by side")
+    tokens, _, dim = shape
     cache = _cache(what, k_pages, v_pages, block_table, k_scale, v_scale, status)
-    q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=dev)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev) if return_key else None
-    args = _APPEND.pack(
-        0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
-        0 if cos is None else cos.data_ptr(), 0 if cos is None else sin.data_ptr(), positions.data_ptr(),
-        0 if sequences is None else sequences.data_ptr(), 0 if q is None else q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(),
-        tokens, 0 if q is None else q.shape[1], rotary, rows, positions.dtype == torch.int64, bool(interleaved), _DTYPES[k.dtype], 0)
-    lib = _native.load()
-    with _native.on_device(dev):
-        _native.check(lib.tris_paged_kv_append(cache, args, _native.stream_of(dev)), what)
+    wide = positions.dtype is torch.int64
+    at = _want(what, "positions", positions, torch.int64 if wide else torch.int32, (tokens,))
+    sequence_at = 0 if sequences is None else _want(what, "sequences", sequences, torch.int32, (tokens,))
+    k0, k1, k2 = k.stride()
+    v0, v1, v2 = v.stride()
+    q_at = q0 = q1 = q_heads = out_at = 0
+    q2, q_out, k_out = 1, None, None
+    if q is not None:
+        if q.dim() != 3 or q.dtype is not dtype or q.shape[0] != tokens or q.shape[2] != dim:
+            _fail(what, "q must be [tokens, q heads, head_dim] in the keys' type")
+        q_at, q_heads = q.data_ptr(), q.shape[1]
+        q0, q1, q2 = q.stride()
+        q_out = _new_like(q)
+        out_at = q_out.data_ptr()
+    if (k2 != 1 or v2 != 1 or q2 != 1) and dim > 1:
+        _fail(what, "the dimensions of a head must be side by side")
+    rows = half = cos_at = sin_at = 0
+    if cos is not None or sin is not None:
+        if cos is None or sin is None or cos.dim() != 2:
+            _fail(what, "cos and sin go together, [positions, rotary_dim / 2] each")
+        rows, half = cos.shape
+        cos_at, sin_at = _want(what, "cos", cos, torch.float32, (rows, half)), _want(what, "sin", sin, torch.float32, (rows, half))
+    if return_key:
+        k_out = _new_like(k)
+    args = _APPEND.pack(q_at, k.data_ptr(), v.data_ptr(), q0, q1, k0, k1, v0, v1, cos_at, sin_at, at, sequence_at, out_at,
+                        0 if k_out is None else k_out.data_ptr(), tokens, q_heads, 2 * half, rows, wide, bool(interleaved), _DTYPES[dtype], 0)
+    _launch(what, "tris_paged_kv_append", dev, cache, args)
     return (q_out, k_out) if return_key else q_out
 
 
@@ -144,59 +185,59 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     [sequences, q heads], -inf for length 0)."""
     what = "paged_decode_attention"
     dev = _same_device(what, q, k_pages, v_pages, block_table, lengths, k_scale, v_scale, status)
-    if q.dim() != 3 or q.dtype not in _ROWS or q.stride(2) != 1:
-        _fail(what, "q must be fp16 or bf16 [sequences, q heads, head_dim] with the dimensions of a head side by side")
-    batch, heads, dim = q.shape
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3 or dtype not in _ROWS:
+        _fail(what, "q must be fp16 or bf16 [sequences, q heads, head_dim]")
+    batch, heads, dim = shape
+    q0, q1, q2 = q.stride()
+    if q2 != 1 and dim > 1:
+        _fail(what, "the dimensions of a head must be side by side")
     cache = _cache(what, k_pages, v_pages, block_table, k_scale, v_scale, status)
     if k_pages.shape[3] != dim or block_table.shape[0] != batch:
-        _fail(what, f"q {tuple(q.shape)} does not fit pages of head_dim {k_pages.shape[3]} and a block table of {block_table.shape[0]} sequences")
-    lengths_ptr = _want(what, "lengths", lengths, torch.int32, batch)
-    lib = _native.load()
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty((batch, heads), dtype=torch.float32, device=dev) if return_lse else None
-    with _native.on_device(dev):
-        key = (dev.index, heads, k_pages.shape[2], dim)
-        need = _workspace_bytes.get(key)
-        if need is None:
-            need = int(lib.tris_paged_decode_attention_workspace_bytes(cache, heads))
-            if need:
-                _workspace_bytes[key] = need
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev)
-        args = _ATTENTION.pack(q.data_ptr(), q.stride(0), q.stride(1), lengths_ptr, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-                               ws.data_ptr(), need, heads, int(window or 0), _DTYPES[q.dtype],
-                               dim ** -0.5 if softmax_scale is None else float(softmax_scale))
-        _native.check(lib.tris_paged_decode_attention(cache, args, _native.stream_of(dev)), what)
+        _fail(what, f"q {tuple(shape)} does not fit pages of head_dim {k_pages.shape[3]} and a block table of {block_table.shape[0]} sequences")
+    lengths_at = _want(what, "lengths", lengths, torch.int32, (batch,))
+    key = (dev.index, heads, k_pages.shape[2], dim)
+    scratch = _scratch.get(key)
+    if scratch is None:
+        scratch = _scratch_like(key, cache, dev)
+    ws = torch.empty_like(scratch, memory_format=torch.contiguous_format)
+    out, lse = _new_like(q), None
+    if return_lse:
+        lse = torch.empty((batch, heads), dtype=torch.float32, device=dev)
+    args = _ATTENTION.pack(q.data_ptr(), q0, q1, lengths_at, out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(),
+                           heads, window or 0, _DTYPES[dtype], dim ** -0.5 if softmax_scale is None else softmax_scale)
+    _launch(what, "tris_paged_decode_attention", dev, cache, args)
     return (out, lse) if return_lse else out
 
 
 def _norm(what: str, x, residual, weight, eps: float, group_size: Optional[int]):
     dev = _same_device(what, x, residual, weight)
-    if x.dim() < 1 or x.dtype not in _ROWS:
+    shape, dtype = x.shape, x.dtype
+    if not shape or dtype not in _ROWS:
         _fail(what, "x must be fp16 or bf16 [..., hidden]")
-    hidden = x.shape[-1]
-    _want(what, "weight", weight, x.dtype, hidden)
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        _fail(what, "residual must have x's shape and type")
-    x2 = x if x.dim() == 2 and x.stride(1) == 1 else x.reshape(-1, hidden).contiguous()
-    r2 = residual
-    if residual is not None and not (residual.dim() == 2 and residual.stride(1) == 1):
-        r2 = residual.reshape(-1, hidden).contiguous()
-    rows = x2.shape[0]
-    h = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
+    hidden = shape[-1]
+    weight_at = _want(what, "weight", weight, dtype, (hidden,))
+    rows_of = lambda t: t if t.dim() == 2 and t.stride(1) == 1 else t.reshape(-1, hidden).contiguous()
+    x2, h = rows_of(x), None
+    r_at = r_stride = h_at = scales_at = 0
+    if residual is not None:
+        if residual.shape != shape or residual.dtype is not dtype:
+            _fail(what, "residual must have x's shape and type")
+        r2, h = rows_of(residual), _new_like(x)
+        r_at, r_stride, h_at = r2.data_ptr(), r2.stride(0), h.data_ptr()
+    group, scales = hidden, None
     if group_size is None:
-        y, scales, group = torch.empty(x.shape, dtype=x.dtype, device=dev), None, hidden
+        y = _new_like(x)
     else:
-        group = int(group_size) or hidden
+        group = group_size or hidden
         if hidden == 0 or group < 0 or hidden % group:
             _fail(what, f"groups of {group} columns do not divide rows of {hidden}")
-        y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-        scales = torch.empty(x.shape[:-1] + (hidden // group,), dtype=torch.float32, device=dev)
-    args = _NORM.pack(x2.data_ptr(), 0 if r2 is None else r2.data_ptr(), weight.data_ptr(), 0 if h is None else h.data_ptr(), y.data_ptr(),
-                      0 if scales is None else scales.data_ptr(), x2.stride(0), 0 if r2 is None else r2.stride(0), hidden, hidden, rows, hidden,
-                      group, _DTYPES[x.dtype], _DTYPES[y.dtype], eps)
-    lib = _native.load()
-    with _native.on_device(dev):
-        _native.check(lib.tris_add_rms_norm(args, _native.stream_of(dev)), what)
+        y = torch.empty(shape, dtype=torch.float8_e4m3fn, device=dev)
+        scales = torch.empty(shape[:-1] + (hidden // group,), dtype=torch.float32, device=dev)
+        scales_at = scales.data_ptr()
+    args = _NORM.pack(x2.data_ptr(), r_at, weight_at, h_at, y.data_ptr(), scales_at, x2.stride(0), r_stride, hidden, hidden, x2.shape[0],
+                      hidden, group, _DTYPES[dtype], _DTYPES[y.dtype], eps)
+    _launch(what, "tris_add_rms_norm", dev, args)
     return y, scales, h
 
 
@@ -229,23 +270,14 @@ def apply_logit_controls(logits: torch.Tensor, *, tokens: Optional[torch.Tensor]
     ``tokens`` is int32 [rows, any]; ids outside the vocabulary are skipped.  ``out`` may be fp32 logits themselves."""
     what = "apply_logit_controls"
     dev = _same_device(what, logits, tokens, token_lengths, prompt_lengths, repetition, presence, frequency, bias_ids, bias_values, allowed, out)
-    if logits.dim() != 2 or logits.dtype not in _DTYPES or logits.dtype == torch.float8_e4m3fn or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    shape, dtype = logits.shape, logits.dtype
+    if len(shape) != 2 or dtype not in _LOGIT_TYPES or (logits.stride(1) != 1 and shape[1] > 1):
         _fail(what, "logits must be fp16, bf16 or fp32 [rows, vocab] with a row's logits side by side")
-    rows, vocab = logits.shape
+    rows, vocab = shape
     if out is None:
-        out = torch.empty((rows, vocab), dtype=torch.float32, device=dev)
-    elif out.dtype != torch.float32 or out.shape != logits.shape or (vocab > 1 and out.stride(1) != 1):
+        out = _new_like(logits) if dtype is torch.float32 else torch.empty(shape, dtype=torch.float32, device=dev)
+    elif out.dtype is not torch.float32 or out.shape != shape or (vocab > 1 and out.stride(1) != 1):
         _fail(what, "out must be fp32 of the logits' shape with a row side by side")
-
-    def matrix(name, t, dtype, columns=None):
-        if t is None:
-            return 0, 0, 0
-        if t.dim() != 2 or t.dtype != dtype or t.shape[0] != rows or (columns is not None and t.shape[1] != columns) or (t.shape[1] > 1 and t.stride(1) != 1):
-            _fail(what, f"{name} must be {dtype} [rows, {'any' if columns is None else columns}] with a row side by side, got {t.dtype} {tuple(t.shape)}")
-        return t.data_ptr(), t.stride(0), t.shape[1]
-
-    def column(name, t, dtype=torch.float32):
-        return 0 if t is None else _want(what, name, t, dtype, rows)
 
     if tokens is None and (repetition is not None or presence is not None or frequency is not None):
         _fail(what, "penalties need tokens")
@@ -253,17 +285,24 @@ def apply_logit_controls(logits: torch.Tensor, *, tokens: Optional[torch.Tensor]
         _fail(what, "tokens and token_lengths go together")
     if (bias_ids is None) != (bias_values is None):
         _fail(what, "bias_ids and bias_values go together")
-    tok, tok_stride, history = matrix("tokens", tokens, torch.int32)
-    ids, id_stride, biases = matrix("bias_ids", bias_ids, torch.int32)
-    values, value_stride, _ = matrix("bias_values", bias_values, torch.float32, biases)
-    if ids and biases and id_stride != value_stride:
-        _fail(what, "bias_ids and bias_values must have the same stride")
-    mask, mask_stride, _ = matrix("allowed", allowed, torch.int32, (vocab + 31) // 32)
-    args = _LOGITS.pack(logits.data_ptr(), out.data_ptr(), tok, column("token_lengths", token_lengths, torch.int32),
-                        column("prompt_lengths", prompt_lengths, torch.int32), column("repetition", repetition), column("presence", presence),
-                        column("frequency", frequency), ids, values, mask, logits.stride(0), out.stride(0), tok_stride, id_stride, mask_stride,
-                        rows, vocab, history, biases, _DTYPES[logits.dtype], 0)
-    lib = _native.load()
-    with _native.on_device(dev):
-        _native.check(lib.tris_logit_controls(args, _native.stream_of(dev)), what)
+    tok = tok_stride = history = ids = values = bias_stride = biases = mask = mask_stride = 0
+    if tokens is not None:
+        tok, tok_stride, history = _matrix(what, "tokens", tokens, torch.int32, rows)
+    if bias_ids is not None:
+        ids, bias_stride, biases = _matrix(what, "bias_ids", bias_ids, torch.int32, rows)
+        values, value_stride, _ = _matrix(what, "bias_values", bias_values, torch.float32, rows, biases)
+        if biases and bias_stride != value_stride:
+            _fail(what, "bias_ids and bias_values must have the same stride")
+    if allowed is not None:
+        mask, mask_stride, _ = _matrix(what, "allowed", allowed, torch.int32, rows, (vocab + 31) // 32)
+    each, f32, i32 = (rows,), torch.float32, torch.int32
+    args = _LOGITS.pack(logits.data_ptr(), out.data_ptr(), tok,
+                        0 if token_lengths is None else _want(what, "token_lengths", token_lengths, i32, each),
+                        0 if prompt_lengths is None else _want(what, "prompt_lengths", prompt_lengths, i32, each),
+                        0 if repetition is None else _want(what, "repetition", repetition, f32, each),
+                        0 if presence is None else _want(what, "presence", presence, f32, each),
+                        0 if frequency is None else _want(what, "frequency", frequency, f32, each),
+                        ids, values, mask, logits.stride(0), out.stride(0), tok_stride, bias_stride, mask_stride,
+                        rows, vocab, history, biases, _DTYPES[dtype], 0)
+    _launch(what, "tris_logit_controls", dev, args)
     return out
