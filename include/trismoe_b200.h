@@ -804,15 +804,15 @@ typedef struct TrisPagedAttention {
   const int32_t* lengths;           /* [num_sequences]                                     */
   void* out;                        /* [num_sequences, num_q_heads, head_dim], q's type    */
   float* lse;                       /* [num_sequences, num_q_heads] or NULL                */
-  void* workspace;                  /* 16-byte aligned                                     */
+  void* workspace;                  /* 16-byte aligned; NULL where none is needed          */
   int64_t workspace_bytes;
   int32_t num_q_heads;
   int32_t window;
   int32_t dtype;                    /* F16 or BF16                                         */
   float softmax_scale;
 } TrisPagedAttention;
-/* Scratch for any lengths that the table has room for; 0 for arguments that the call would refuse. */
-size_t tris_paged_decode_attention_workspace_bytes(const TrisPagedKv* cache, int32_t num_q_heads);
+/* Scratch for any lengths that the table has room for.  0: none is needed, or the call would refuse these arguments. */
+size_t tris_paged_decode_attention_workspace_bytes(const TrisPagedKv* cache, int32_t num_q_heads, int32_t window);
 int tris_paged_decode_attention(const TrisPagedKv* cache, const TrisPagedAttention* query, void* stream);
 
 /*

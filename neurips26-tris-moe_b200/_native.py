@@ -206,7 +206,7 @@ SIGNATURES = {
     "tris_moe_layer_forward_paged": (C.c_int, [_P(TrisMoeLayerView), _P(TrisPagedLayer), _vp, _vp, _i32, _vp, _vp, _vp, C.c_size_t, _vp, _vp]),
     # pointers to the structs above; packed bytes are passed on the way that counts (decode_ops.py)
     "tris_paged_kv_append": (C.c_int, [_vp, _vp, _vp]),
-    "tris_paged_decode_attention_workspace_bytes": (C.c_size_t, [_vp, _i32]),
+    "tris_paged_decode_attention_workspace_bytes": (C.c_size_t, [_vp, _i32, _i32]),
     "tris_paged_decode_attention": (C.c_int, [_vp, _vp, _vp]),
     "tris_add_rms_norm": (C.c_int, [_vp, _vp]),
     "tris_logit_controls": (C.c_int, [_vp, _vp]),

@@ -34,6 +34,7 @@ struct AttnArgs {
   int page_shift;   // log2(page_size), or -1
   int page_blocks;  // whether a block of 16 tokens never crosses a page
   int wide_query;   // whether q's heads start on 16-byte boundaries
+  int cluster;      // CTAs that share one item (a sequence's key/value head), or 0: the work is numbered through and cut evenly
   int ctas;         // of the first kernel
   int resident;     // of them, at one time
   int rows_together;  // whether a head's rows in a page are side by side
@@ -67,6 +68,26 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+constexpr int kMostCluster = 8;
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t local, uint32_t rank) {  // a shared-memory address in another CTA of the cluster
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ float4 load_cluster_4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 load_cluster_2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
 }
 
 // Tokens [lo, hi) of a sequence; its blocks begin at multiples of kBlock.
@@ -190,37 +211,61 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
   pdl_wait();
   pdl_launch_dependents();
 
-  // this warp's run, and the sequence that holds its first block
-  int mine, upto = scan_blocks(a, 0, lane, mine);
-  int total = __shfl_sync(0xFFFFFFFFu, upto, 31);
-  for (int i = 1; 32 * i < c.num_sequences; ++i) {
-    int own;
-    total += __shfl_sync(0xFFFFFFFFu, scan_blocks(a, i, lane, own), 31);
-  }
-  const int run = run_length(a, total);
-  if (static_cast<int64_t>(blockIdx.x) * kWarps * run >= total) return;
-  const int64_t first_block = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * run;
-  const int first = static_cast<int>(first_block), count = first_block < total ? min(run, total - first) : 0;
-  if (lane < 2) pieces[2 * warp + lane].used = 0;
-  __syncwarp();
-
+  // This warp's run: its part of the CTA's (cluster's) one item, or of the numbering, with the sequence that holds its first block.
   Cursor use{};
-  if (count) {
-    int before = 0;
-    for (int i = 0;; ++i) {
-      if (i) upto = scan_blocks(a, i, lane, mine);
-      const uint32_t beyond = __ballot_sync(0xFFFFFFFFu, before + upto > first);
-      if (beyond) {
-        const int l = __ffs(beyond) - 1;
-        const int ahead = first - before - __shfl_sync(0xFFFFFFFFu, upto - mine, l);
-        use.enter(a, 32 * i + l);
-        use.item = static_cast<unsigned>(ahead) / static_cast<unsigned>(use.blocks);
-        use.blk = ahead - use.item * use.blocks;
-        break;
+  int count = 0, shares = 1;  // shares: CTAs of the cluster that have a part
+  if (a.cluster) {
+    use.b = blockIdx.y;
+    use.item = blockIdx.x;
+    // the block table's row comes to L2 while the length is on its way
+    if (warp == 0 && lane * 32 < c.table_width) asm volatile("prefetch.global.L2 [%0];" ::"l"(c.block_table + use.b * c.table_stride + lane * 32));
+    use.span = span_of(a, use.b);
+    use.blocks = use.span.blocks();
+    if (query.lengths[use.b] > use.span.hi && c.status_dev) *c.status_dev = TRIS_ERR_CORRUPT;
+    const int run = (use.blocks + a.cluster * kWarps - 1) / (a.cluster * kWarps);
+    use.blk = (blockIdx.z * kWarps + warp) * run;
+    count = max(0, min(run, use.blocks - use.blk));
+    shares = run ? (use.blocks + kWarps * run - 1) / (kWarps * run) : 0;
+    if (use.blocks <= 1 && (blockIdx.z > 0 || use.blocks == 0)) {  // one block is its warp's alone; nothing at all gives zeros
+      if (use.blocks == 0 && blockIdx.z == 0) {
+        const int head = use.item / a.row_tiles, row0 = use.item % a.row_tiles * S::kHeads, rows = min(S::kHeads, a.group - row0);
+        const int64_t out_row = static_cast<int64_t>(use.b) * query.num_q_heads + head * a.group + row0;
+        for (int i = threadIdx.x; i < rows * D; i += kWarps * 32) store_float(static_cast<T*>(query.out) + out_row * D + i, 0.f);
+        for (int i = threadIdx.x; query.lse && i < rows; i += kWarps * 32) query.lse[out_row + i] = -INFINITY;
       }
-      before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+      return;  // the whole cluster: none of its CTAs has a piece
+    }
+  } else {
+    int mine, upto = scan_blocks(a, 0, lane, mine);
+    int total = __shfl_sync(0xFFFFFFFFu, upto, 31);
+    for (int i = 1; 32 * i < c.num_sequences; ++i) {
+      int own;
+      total += __shfl_sync(0xFFFFFFFFu, scan_blocks(a, i, lane, own), 31);
+    }
+    const int run = run_length(a, total);
+    if (static_cast<int64_t>(blockIdx.x) * kWarps * run >= total) return;
+    const int64_t first_block = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * run;
+    const int first = static_cast<int>(first_block);
+    count = first_block < total ? min(run, total - first) : 0;
+    if (count) {
+      int before = 0;
+      for (int i = 0;; ++i) {
+        if (i) upto = scan_blocks(a, i, lane, mine);
+        const uint32_t beyond = __ballot_sync(0xFFFFFFFFu, before + upto > first);
+        if (beyond) {
+          const int l = __ffs(beyond) - 1;
+          const int ahead = first - before - __shfl_sync(0xFFFFFFFFu, upto - mine, l);
+          use.enter(a, 32 * i + l);
+          use.item = static_cast<unsigned>(ahead) / static_cast<unsigned>(use.blocks);
+          use.blk = ahead - use.item * use.blocks;
+          break;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+      }
     }
   }
+  if (lane < 2) pieces[2 * warp + lane].used = 0;
+  __syncwarp();
   bool owns_start = use.blk == 0;  // whether the current item begins in this run
 
   uint32_t qf[NT][S::kSteps][2];
@@ -582,6 +627,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
     const int head = item.item / a.row_tiles, tile = item.item % a.row_tiles;
     const int heads = min(S::kHeads, a.group - tile * S::kHeads);
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (item.starts ? 1 : 0);
+    float* to_o = a.cluster ? piece_at(3) : a.part_o + slot * a.tile_heads * D;
+    float* to_ml = a.cluster ? piece_at(3) + a.tile_heads * D : a.part_ml + slot * a.tile_heads * 2;
     for (int h = warp; h < heads; h += kWarps) {
       // an item's pieces are the second one of its first warp and the first ones of the next, so kWarps + 1 at most
       float w[2 * kWarps], top = kLowest, sum = 0.f;
@@ -612,17 +659,50 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
         if (whole)
           *reinterpret_cast<uint2*>(static_cast<T*>(query.out) + out_row * D + d) = make_uint2(Pair<T>::pack(o.x * inv, o.y * inv), Pair<T>::pack(o.z * inv, o.w * inv));
         else
-          *reinterpret_cast<float4*>(a.part_o + (slot * a.tile_heads + h) * D + d) = o;
+          *reinterpret_cast<float4*>(to_o + h * D + d) = o;
       }
       if (lane == 0) {
         if (!whole)
-          *reinterpret_cast<float2*>(a.part_ml + (slot * a.tile_heads + h) * 2) = make_float2(top, sum);
+          *reinterpret_cast<float2*>(to_ml + h * 2) = make_float2(top, sum);
         else if (query.lse)
           query.lse[out_row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
       }
     }
     s0 = s1 + 1;
   }
+
+  if (a.cluster < 2 || shares < 2) return;  // all CTAs of a cluster agree on that
+  // The cluster's CTAs have left what they have of the item in the part of their rings that the item's second warp had; each joins some of it.
+  cluster_sync();
+  const int head = use.item / a.row_tiles, tile = use.item % a.row_tiles, heads = min(S::kHeads, a.group - tile * S::kHeads);
+  const uint32_t local = smem_u32(piece_at(3));
+  for (int i = blockIdx.z * kWarps * 32 + threadIdx.x; i < heads * (D / 4); i += a.cluster * kWarps * 32) {
+    const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
+    float2 ml[kMostCluster];
+    float4 v[kMostCluster];
+    float top = kLowest, sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < kMostCluster; ++r) {
+      const uint32_t at = in_cta(local, min(r, shares - 1));
+      ml[r] = load_cluster_2(at + (a.tile_heads * D + 2 * h) * 4);
+      v[r] = load_cluster_4(at + (h * D + d) * 4);
+    }
+#pragma unroll
+    for (int r = 0; r < kMostCluster; ++r) top = fmaxf(top, ml[r].x);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < kMostCluster; ++r) {
+      if (r >= shares) break;
+      const float w = exp2_fast(ml[r].x - top);
+      sum += w * ml[r].y;
+      o.x += w * v[r].x, o.y += w * v[r].y, o.z += w * v[r].z, o.w += w * v[r].w;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t out_row = static_cast<int64_t>(use.b) * query.num_q_heads + head * a.group + tile * S::kHeads + h;
+    *reinterpret_cast<uint2*>(static_cast<T*>(query.out) + out_row * D + d) = make_uint2(Pair<T>::pack(o.x * inv, o.y * inv), Pair<T>::pack(o.z * inv, o.w * inv));
+    if (d == 0 && query.lse) query.lse[out_row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  }
+  cluster_sync();  // nobody leaves while another reads its shared memory
 }
 
 // Joins the partial results of one query head of one sequence; zeros where there was nothing to attend to.
@@ -734,6 +814,20 @@ int attention_ctas(int resident, int64_t blocks) {
 int64_t most_blocks(const TrisPagedKv& c, int row_tiles) {
   return static_cast<int64_t>(c.num_sequences) * c.num_kv_heads * row_tiles * ((static_cast<int64_t>(c.table_width) * c.page_size + kBlock - 1) / kBlock + 1);
 }
+// CTAs that share an item, as many as still run at the same time for all items, up to kMostCluster; 0 where that leaves a warp more than
+// kMostShare blocks of the longest sequence that the table (or the window) has room for.  One launch instead of two and no numbering are worth 2 to 5 us -
+// 20 x 1 token 6.7 -> 4.8, 1 x 513 9.8 -> 8.0, 32 x 512-768 39 -> 36, 16 x 4096 in 8 bits 31 -> 26 -, but SMs that have no item stay idle, and
+// sequences of different lengths end at different times: 4 x 20580 44 -> 57, 13 x 49925 76 -> 104, 64 x 1-16384 293 -> 297 to 366.
+constexpr int kMostShare = 16;
+int cluster_size(const TrisPagedKv& c, int row_tiles, int window, int resident) {
+  const int64_t items = static_cast<int64_t>(c.num_sequences) * c.num_kv_heads * row_tiles;
+  int64_t tokens = static_cast<int64_t>(c.table_width) * c.page_size;
+  if (window > 0 && window < tokens) tokens = window + kBlock;
+  int size = kMostCluster;
+  while (size > 1 && items * size > resident) size /= 2;
+  return tokens <= static_cast<int64_t>(kMostShare) * kBlock * kWarps * size ? size : 0;
+}
+int resident_ctas(int head_dim, bool fp8) { return sm_count() * (head_dim > 128 && !fp8 ? 1 : 2); }
 size_t part_floats(int ctas, int tile_heads, int head_dim) { return 2 * static_cast<size_t>(ctas) * tile_heads * (head_dim + 2); }
 
 template <typename T, bool FP8, int DP, int NT>
@@ -742,16 +836,23 @@ int launch_attention(AttnArgs& a, cudaStream_t stream) {
   auto kernel = paged_attention_kernel<T, FP8, DP, NT>;
   const TrisPagedKv& c = a.cache;
   if (int st = allow_shared_memory<paged_attention_kernel<T, FP8, DP, NT>>(S::kSmem)) return st;
-  a.resident = sm_count() * S::kCtasPerSm;
-  a.ctas = attention_ctas(a.resident, most_blocks(c, a.row_tiles));
-  a.rows_together = a.page_blocks && c.head_dim == DP && c.k_token_stride == DP && c.v_token_stride == DP;
   TRIS_REQUIRE(sm_count() > 0, TRIS_ERR_CUDA, "paged_decode_attention: no device");
+  static_assert(S::kCtasPerSm == (DP > 128 && !FP8 ? 1 : 2), "resident_ctas");
+  a.resident = resident_ctas(c.head_dim, FP8);
+  a.rows_together = a.page_blocks && c.head_dim == DP && c.k_token_stride == DP && c.v_token_stride == DP;
+  const bool pdl = programmatic_launch_default();
+  a.cluster = cluster_size(c, a.row_tiles, a.query.window, a.resident);
+  if (a.cluster) {
+    TRIS_CUDA(launch_kernel(kernel, dim3(c.num_kv_heads * a.row_tiles, c.num_sequences, a.cluster), dim3(kWarps * 32), S::kSmem, stream, pdl, a.cluster, a));
+    return TRIS_OK;
+  }
+  a.ctas = attention_ctas(a.resident, most_blocks(c, a.row_tiles));
   a.part_ml = static_cast<float*>(a.query.workspace);
   a.part_o = a.part_ml + 4 * static_cast<size_t>(a.ctas) * a.tile_heads;
   const int64_t need = part_floats(a.ctas, a.tile_heads, c.head_dim) * 4;
   TRIS_REQUIRE(a.query.workspace && a.query.workspace_bytes >= need, TRIS_ERR_WORKSPACE, "paged_decode_attention: workspace of %lld bytes needed, got %lld",
                static_cast<long long>(need), static_cast<long long>(a.query.workspace_bytes));
-  TRIS_CUDA(launch_kernel(kernel, dim3(a.ctas), dim3(kWarps * 32), S::kSmem, stream, programmatic_launch_default(), 1, a));
+  TRIS_CUDA(launch_kernel(kernel, dim3(a.ctas), dim3(kWarps * 32), S::kSmem, stream, pdl, 1, a));
   TRIS_CUDA(launch_kernel(paged_attention_join_kernel<T>, dim3(a.query.num_q_heads, c.num_sequences), dim3(kJoinThreads), 0, stream, true, 1, a, S::kHeads));
   return TRIS_OK;
 }
@@ -767,12 +868,13 @@ int launch_shape(AttnArgs& a, cudaStream_t stream) {
 
 using namespace tris;
 
-extern "C" size_t tris_paged_decode_attention_workspace_bytes(const TrisPagedKv* cache, int32_t num_q_heads) {
+extern "C" size_t tris_paged_decode_attention_workspace_bytes(const TrisPagedKv* cache, int32_t num_q_heads, int32_t window) {
   if (validate_paged_kv(cache, "paged_decode_attention")) return 0;
-  if (num_q_heads < 1 || num_q_heads % cache->num_kv_heads) return 0;
-  const int group = num_q_heads / cache->num_kv_heads, heads = 8 * head_tiles(group, cache->head_dim);
-  const int sms = sm_count();
-  return sms > 0 ? part_floats(2 * 2 * sms, group < heads ? group : heads, cache->head_dim) * 4 : 0;
+  if (num_q_heads < 1 || num_q_heads % cache->num_kv_heads || window < 0 || sm_count() == 0) return 0;
+  const int group = num_q_heads / cache->num_kv_heads, heads = 8 * head_tiles(group, cache->head_dim), row_tiles = ceil_div(group, heads);
+  const int resident = resident_ctas(cache->head_dim, cache->dtype == TRIS_DTYPE_E4M3);
+  if (cluster_size(*cache, row_tiles, window, resident)) return 0;
+  return part_floats(attention_ctas(resident, most_blocks(*cache, row_tiles)), group < heads ? group : heads, cache->head_dim) * 4;
 }
 
 extern "C" int tris_paged_decode_attention(const TrisPagedKv* cache, const TrisPagedAttention* query, void* stream) {

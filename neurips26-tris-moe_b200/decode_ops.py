@@ -32,16 +32,8 @@ _APPEND = struct.Struct("@3Q6q6Q8i")
 _ATTENTION = struct.Struct("@Q2q4Qq3if")
 _NORM = struct.Struct("@6Q4q5if")
 _LOGITS = struct.Struct("@11Q5q6i")
-_scratch: dict = {}  # (device, heads) -> one byte seen as many, whose like is the scratch of a call
-
-
-def _scratch_like(key: tuple, cache: bytes, dev: torch.device) -> torch.Tensor:
-    with torch.cuda.device(dev):
-        need = int(_native.load().tris_paged_decode_attention_workspace_bytes(cache, key[1]))
-    byte = torch.empty((1,), dtype=torch.uint8, device=dev).expand(need)
-    if need:  # sizes that the call will refuse are not kept
-        _scratch[key] = byte
-    return byte
+# (device, sizes) -> a byte seen as many, whose like is the scratch of a call; None where there is none to have
+_scratch: dict = {}
 
 
 def _fail(what: str, why: str):
@@ -196,16 +188,23 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if k_pages.shape[3] != dim or block_table.shape[0] != batch:
         _fail(what, f"q {tuple(shape)} does not fit pages of head_dim {k_pages.shape[3]} and a block table of {block_table.shape[0]} sequences")
     lengths_at = _want(what, "lengths", lengths, torch.int32, (batch,))
-    key = (dev.index, heads, k_pages.shape[2], dim)
-    scratch = _scratch.get(key)
-    if scratch is None:
-        scratch = _scratch_like(key, cache, dev)
-    ws = torch.empty_like(scratch, memory_format=torch.contiguous_format)
+    window = window or 0
+    key = (dev.index, heads, k_pages.shape, k_pages.dtype, block_table.shape, window)
+    if key not in _scratch:
+        if len(_scratch) >= 4096:  # block tables may grow for ever
+            _scratch.clear()
+        with torch.cuda.device(dev):
+            need = int(_native.load().tris_paged_decode_attention_workspace_bytes(cache, heads, max(window, -1)))
+        _scratch[key] = torch.empty((1,), dtype=torch.uint8, device=dev).expand(need) if need else None
+    ws, ws_at, ws_bytes = _scratch[key], 0, 0
+    if ws is not None:
+        ws = _new_like(ws)
+        ws_at, ws_bytes = ws.data_ptr(), ws.numel()
     out, lse = _new_like(q), None
     if return_lse:
         lse = torch.empty((batch, heads), dtype=torch.float32, device=dev)
-    args = _ATTENTION.pack(q.data_ptr(), q0, q1, lengths_at, out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(),
-                           heads, window or 0, _DTYPES[dtype], dim ** -0.5 if softmax_scale is None else softmax_scale)
+    args = _ATTENTION.pack(q.data_ptr(), q0, q1, lengths_at, out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws_at, ws_bytes,
+                           heads, window, _DTYPES[dtype], dim ** -0.5 if softmax_scale is None else softmax_scale)
     _launch(what, "tris_paged_decode_attention", dev, cache, args)
     return (out, lse) if return_lse else out
 

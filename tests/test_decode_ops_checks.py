@@ -37,7 +37,7 @@ def test_caches_that_are_refused(lib, change, status, text):
                         ("tris_paged_decode_attention", n.TrisPagedAttention(q=A, out=A, lengths=A, workspace=A, num_q_heads=2))):
         st, message = _call(lib, entry, _cache(tm, **change), args)
         assert st == status and text in message, (entry, message)
-    assert lib.tris_paged_decode_attention_workspace_bytes(C.byref(_cache(tm, **change)), 2) == 0
+    assert lib.tris_paged_decode_attention_workspace_bytes(C.byref(_cache(tm, **change)), 2, 0) == 0
 
 
 def test_appends_that_are_refused(lib):
@@ -65,7 +65,7 @@ def test_attentions_that_are_refused(lib):
         assert st == status and text in message, message
     assert _call(lib, "tris_paged_decode_attention", _cache(tm, num_sequences=65536), tm._native.TrisPagedAttention(**good))[0] == 2
     assert _call(lib, "tris_paged_decode_attention", _cache(tm, num_sequences=0), tm._native.TrisPagedAttention(**good))[0] == 0
-    assert lib.tris_paged_decode_attention_workspace_bytes(C.byref(_cache(tm)), 3) == 0
+    assert lib.tris_paged_decode_attention_workspace_bytes(C.byref(_cache(tm)), 3, 0) == 0
 
 
 def test_norms_that_are_refused(lib):
