@@ -57,8 +57,9 @@ __device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&c)[4], uint32
 }
 // Two e4m3 values as fp16, exact.
 __device__ __forceinline__ uint32_t e4m3_to_h2(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
+  return h;
 }
 __device__ __forceinline__ void cp_async_16_at(uint32_t dst, const void* src, int bytes) {  // bytes: 16, or 0 for zeros
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -166,18 +167,20 @@ template <typename T, bool FP8, int DP, int NT>
 struct Shape {
   static constexpr int kElems = FP8 ? 16 : 8;                          // of a 16-byte chunk
   static constexpr int kKeyChunks = DP / kElems / 4;                   // of a key row that a lane has
-  static constexpr int kValueChunks = DP / kElems / 8 ? DP / kElems / 8 : 1;
+  static constexpr int kValueElems = FP8 && DP == 64 ? 8 : kElems;     // of a value row that a lane has at a time: eight lanes have the row
+  static constexpr int kValueChunks = DP / kValueElems / 8;
   static constexpr int kRowBytes = DP * (FP8 ? 1 : 2);
   static constexpr int kRowChunks = kRowBytes / 16;
   static constexpr int kCopyRows = kRowChunks > 32 ? 1 : 32 / kRowChunks;  // rows that 32 lanes copy at once, 16 bytes each
   static constexpr int kTile = kBlock * kRowBytes;                     // 16 rows of keys or of values
   static constexpr int kStageBytes = 2 * kTile;
   // Chunk that holds a row's chunk in shared memory, XORed: eight lanes that read together - keys: rows of both parities, four neighbouring
-  // chunks; values: rows 2 t, two neighbouring chunks - find eight different 16-byte columns.  (64-byte rows: two lanes a column for values.)
+  // chunks; values: rows 2 t, two neighbouring chunks - find eight different 16-byte columns.  (64-byte rows: two lanes a column for values, of which
+  // a lane has 8 bytes.)
   static __device__ __forceinline__ constexpr int key_swizzle(int row) { return kRowChunks >= 8 ? (row & 1) << 2 : 0; }
   static __device__ __forceinline__ constexpr int value_swizzle(int row) { return kRowChunks >= 8 ? ((row >> 1) & 3) << 1 : ((row >> 1) & 1) << 1; }
   static constexpr int kSteps = DP / 16;                               // K = 16 steps of S
-  static constexpr int kDimTiles = kValueChunks * kElems / 2;          // 16-dimension tiles of O
+  static constexpr int kDimTiles = kValueChunks * kValueElems / 2;        // 16-dimension tiles of O
   static constexpr int kHeads = 8 * NT;
   static constexpr int kPieceBytes = kHeads * (DP + 2) * 4;
   // Two CTAs on an SM, of which one computes while the other starts or ends; with fp16 heads of 256 dimensions one, for the ring's sake.
@@ -407,8 +410,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
   };
   // where this lane's fragments are in a stage: keys g and g + 8, chunks 4 j + t; values 2 t, 2 t + 1, 2 t + 8, 2 t + 9, chunks 8 j + g
   const uint32_t k_from = g * S::kRowBytes + ((t ^ S::key_swizzle(g)) << 4);
-  const uint32_t v_from = S::kTile + 2 * t * S::kRowBytes + ((g ^ S::value_swizzle(2 * t)) << 4);
-  const bool has_values = g < S::kRowChunks;
+  const uint32_t v_from = S::kTile + 2 * t * S::kRowBytes +
+                          (S::kValueElems == S::kElems ? (g ^ S::value_swizzle(2 * t)) << 4 : (((g >> 1) ^ S::value_swizzle(2 * t)) << 4) + 8 * (g & 1));
 #pragma unroll 1
   for (int s = 0; s < S::kStages - 1; ++s) issue(s);
 
@@ -429,15 +432,15 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
         const float inv = to ? v_scale : sum == 0.f ? 0.f : v_scale / sum;
 #pragma unroll
         for (int j = 0; j < S::kValueChunks; ++j) {
-          const int d0 = (8 * j + g) * S::kElems;
+          const int d0 = (8 * j + g) * S::kValueElems;
           if (d0 >= D) continue;
 #pragma unroll
-          for (int q = 0; q < S::kElems / 8; ++q) {
+          for (int q = 0; q < S::kValueElems / 8; ++q) {
             float v[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              v[2 * i] = acc[j * (S::kElems / 2) + 4 * q + i][n][h] * inv;
-              v[2 * i + 1] = acc[j * (S::kElems / 2) + 4 * q + i][n][2 + h] * inv;
+              v[2 * i] = acc[j * (S::kValueElems / 2) + 4 * q + i][n][h] * inv;
+              v[2 * i + 1] = acc[j * (S::kValueElems / 2) + 4 * q + i][n][2 + h] * inv;
             }
             if (to) {
               float4* dst = reinterpret_cast<float4*>(to + in_tile * D + d0 + 8 * q);
@@ -563,12 +566,17 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
       uint32_t v[4][4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (S::kRowChunks >= 8 || has_values) raw = *reinterpret_cast<const uint4*>(vals + ((r & 1) + 8 * (r >> 1)) * S::kRowBytes + j * 128);
-        v[r][0] = raw.x, v[r][1] = raw.y, v[r][2] = raw.z, v[r][3] = raw.w;
+        const uint8_t* at = vals + ((r & 1) + 8 * (r >> 1)) * S::kRowBytes + j * 128;
+        if constexpr (S::kValueElems == S::kElems) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(at);
+          v[r][0] = raw.x, v[r][1] = raw.y, v[r][2] = raw.z, v[r][3] = raw.w;
+        } else {
+          const uint2 raw = *reinterpret_cast<const uint2*>(at);
+          v[r][0] = raw.x, v[r][1] = raw.y;
+        }
       }
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < 4 * S::kValueElems / S::kElems; ++w) {
         if constexpr (FP8) {
           // bytes of two tokens side by side first, then two values at a time: {token 0, token 1} of dimensions 4 w + i
           const uint32_t lo0 = prmt(v[0][w], v[1][w], 0x5140), hi0 = prmt(v[0][w], v[1][w], 0x7362);
@@ -578,7 +586,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
             const uint32_t u0 = e ? hi0 : lo0, u1 = e ? hi1 : lo1;
             const uint32_t a0 = e4m3_to_h2(u0 & 0xFFFF), a1 = e4m3_to_h2(u0 >> 16), a2 = e4m3_to_h2(u1 & 0xFFFF), a3 = e4m3_to_h2(u1 >> 16);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_16x8x16<M>(acc[j * 8 + 2 * w + e][n], a0, a1, a2, a3, p[n][0], p[n][1]);
+            for (int n = 0; n < NT; ++n) mma_16x8x16<M>(acc[j * (S::kValueElems / 2) + 2 * w + e][n], a0, a1, a2, a3, p[n][0], p[n][1]);
           }
         } else {
           const uint32_t a0 = prmt(v[0][w], v[1][w], 0x5410), a1 = prmt(v[0][w], v[1][w], 0x7632);
