@@ -281,25 +281,28 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
     for (int n = 0; n < NT; ++n) {
       const int row = tile * S::kHeads + 8 * n + g;
       const T* src = static_cast<const T*>(query.q) + use.b * query.q_token_stride + (static_cast<int64_t>(head) * a.group + row) * query.q_head_stride;
+      const bool there = row < a.group;
+      if (a.wide_query) {
 #pragma unroll
-      for (int j = 0; j < S::kKeyChunks; ++j) {
+        for (int j = 0; j < S::kKeyChunks; ++j)
 #pragma unroll
-        for (int w = 0; w < S::kElems / 2; w += 4) {
-          const int d = (4 * j + t) * S::kElems + 2 * w;
-          uint32_t v[4] = {0, 0, 0, 0};
-          if (row < a.group && d < D) {
-            if (a.wide_query) {
-              const uint4 raw = *reinterpret_cast<const uint4*>(src + d);
-              v[0] = raw.x, v[1] = raw.y, v[2] = raw.z, v[3] = raw.w;
-            } else {
-              const uint16_t* p = reinterpret_cast<const uint16_t*>(src + d);
+          for (int w = 0; w < S::kElems / 2; w += 4) {
+            const int d = (4 * j + t) * S::kElems + 2 * w;
+            uint4 raw = make_uint4(0, 0, 0, 0);
+            if (there && d < D) raw = *reinterpret_cast<const uint4*>(src + d);
+            const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-              for (int i = 0; i < 4; ++i) v[i] = p[2 * i] | (static_cast<uint32_t>(p[2 * i + 1]) << 16);
-            }
+            for (int i = 0; i < 4; ++i) qf[n][j * (S::kElems / 4) + (w + i) / 2][i & 1] = v[i];
           }
+      } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) qf[n][j * (S::kElems / 4) + (w + i) / 2][i & 1] = v[i];
-        }
+        for (int j = 0; j < S::kKeyChunks; ++j)
+#pragma unroll
+          for (int w = 0; w < S::kElems / 2; ++w) {
+            const int d = (4 * j + t) * S::kElems + 2 * w;
+            const uint16_t* at = reinterpret_cast<const uint16_t*>(src + d);
+            qf[n][j * (S::kElems / 4) + w / 2][w & 1] = there && d < D ? at[0] | (static_cast<uint32_t>(at[1]) << 16) : 0;
+          }
       }
     }
   };
@@ -412,8 +415,6 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
   const uint32_t k_from = g * S::kRowBytes + ((t ^ S::key_swizzle(g)) << 4);
   const uint32_t v_from = S::kTile + 2 * t * S::kRowBytes +
                           (S::kValueElems == S::kElems ? (g ^ S::value_swizzle(2 * t)) << 4 : (((g >> 1) ^ S::value_swizzle(2 * t)) << 4) + 8 * (g & 1));
-#pragma unroll 1
-  for (int s = 0; s < S::kStages - 1; ++s) issue(s);
 
   // The result of an item that this warp has had alone goes out; otherwise its piece is left for the other warps' (to != nullptr).
   auto write_item = [&](float* to) {
@@ -465,8 +466,37 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
     uint8_t* at = slot & 1 ? smem + (slot >> 1) * (S::kStages * S::kStageBytes) : smem + S::kRing + (slot >> 1) * S::kPieceBytes;
     return reinterpret_cast<float*>(at);
   };
+  // Lanes 0 to 7 have the (m, l) of partial results: the largest m, the weight of each, and the weighted sum of the l.
+  auto weight_of = [](float2 ml, float& top, float& sum) {
+    top = ml.x;
+#pragma unroll
+    for (int k = 1; k < 8; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
+    const float weight = exp2_fast(ml.x - top);
+    sum = weight * ml.y;
+#pragma unroll
+    for (int k = 1; k < 8; k <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, k);
+    top = __shfl_sync(0xFFFFFFFFu, top, 0);
+    sum = __shfl_sync(0xFFFFFFFFu, sum, 0);
+    return weight;
+  };
+  static_assert(2 * kWarps <= 8 && kMostCluster <= 8, "weight_of");
+  auto store_result = [&](int b, int q_head, int d, float top, float sum, float4 o) {
+    const int64_t out_row = static_cast<int64_t>(b) * query.num_q_heads + q_head;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<uint2*>(static_cast<T*>(query.out) + out_row * D + d) = make_uint2(Pair<T>::pack(o.x * inv, o.y * inv), Pair<T>::pack(o.z * inv, o.w * inv));
+    if (d == 0 && query.lse) query.lse[out_row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  };
+
   bool fresh = true;  // an item begins
-  for (int i = 0, stage = 0; i < count; ++i) {
+  // The first turns only ask for blocks; every later one does its block and asks for another in the place of the one before.  (Code that runs once
+  // a CTA comes from far away: it is written once, and in loops.)
+  int stage = 0, place = 0;
+#pragma unroll 1
+  for (int i = count ? 1 - S::kStages : 0; i < count; ++i) {
+    if (i < 0) {
+      issue(place++);
+      continue;
+    }
     if (fresh) start_item();
     fresh = false;
     cp_async_wait<S::kStages - 2>();
@@ -596,7 +626,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
         }
       }
     }
-    issue(stage == 0 ? S::kStages - 1 : stage - 1);
+    issue(place);
+    if (++place == S::kStages) place = 0;
     if (++stage == S::kStages) stage = 0;
 
     const bool last = i + 1 == count, ends = use.blk + 1 == use.blocks;
@@ -621,62 +652,47 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
   cp_async_wait<0>();
   __syncthreads();
 
-  // Neighbouring warps' pieces of one item are joined here; what other CTAs share goes to the workspace.
-  for (int s0 = 0; s0 < 2 * kWarps;) {
-    if (!pieces[s0].used) {
-      ++s0;
-      continue;
-    }
-    int s1 = s0;  // last piece of the item
-    for (int k = s0 + 1; !pieces[s1].ends && k < 2 * kWarps; ++k)
-      if (pieces[k].used) s1 = k;
+  // Neighbouring warps' pieces of one item are joined here; what other CTAs share goes to the workspace, or is left for the cluster.
+  const uint32_t used = __ballot_sync(0xFFFFFFFFu, lane < 2 * kWarps && pieces[lane & (2 * kWarps - 1)].used);
+  const uint32_t last_ones = used & __ballot_sync(0xFFFFFFFFu, pieces[lane & (2 * kWarps - 1)].ends);
+#pragma unroll 1
+  for (uint32_t rest = used; rest;) {
+    const int s0 = __ffs(rest) - 1;
+    const uint32_t ends = last_ones & rest;
+    const uint32_t group = ends ? rest & (ends ^ (ends - 1)) : rest;  // up to the first piece that ends an item
+    rest &= ~group;
     const Piece item = pieces[s0];
-    const bool whole = item.starts && pieces[s1].ends;
+    const bool whole = item.starts && ends;
     const int head = item.item / a.row_tiles, tile = item.item % a.row_tiles;
     const int heads = min(S::kHeads, a.group - tile * S::kHeads);
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (item.starts ? 1 : 0);
     float* to_o = a.cluster ? piece_at(3) : a.part_o + slot * a.tile_heads * D;
     float* to_ml = a.cluster ? piece_at(3) + a.tile_heads * D : a.part_ml + slot * a.tile_heads * 2;
-    for (int h = warp; h < heads; h += kWarps) {
-      // an item's pieces are the second one of its first warp and the first ones of the next, so kWarps + 1 at most
-      float w[2 * kWarps], top = kLowest, sum = 0.f;
+    // a warp takes 128 dimensions of a head at a time
+#pragma unroll 1
+    for (int unit = warp; unit < heads * ((D + 127) / 128); unit += kWarps) {
+      const int h = D > 128 ? unit >> 1 : unit, d = (D > 128 ? (unit & 1) * 128 : 0) + 4 * lane;
+      // lane k has the weight of piece k
+      float2 ml = make_float2(kLowest, 0.f);
+      if ((group >> lane) & 1) ml = *reinterpret_cast<const float2*>(piece_at(lane) + a.tile_heads * D + 2 * h);
+      float top, sum;
+      const float weight = weight_of(ml, top, sum);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < 2 * kWarps; ++k) {
-        w[k] = kLowest;
-        if (k >= s0 && k <= s1 && pieces[k].used) w[k] = piece_at(k)[a.tile_heads * D + 2 * h];
+        if (!((group >> k) & 1)) continue;
+        const float4 v = *reinterpret_cast<const float4*>(piece_at(k) + h * D + min(d, D - 4));
+        const float w = __shfl_sync(0xFFFFFFFFu, weight, k);
+        o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
       }
-#pragma unroll
-      for (int k = 0; k < 2 * kWarps; ++k) top = fmaxf(top, w[k]);
-#pragma unroll
-      for (int k = 0; k < 2 * kWarps; ++k) {
-        const bool has = k >= s0 && k <= s1 && pieces[k].used;
-        w[k] = has ? exp2_fast(w[k] - top) : 0.f;
-        if (has) sum += w[k] * piece_at(k)[a.tile_heads * D + 2 * h + 1];
-      }
-      const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-      const int64_t out_row = static_cast<int64_t>(item.b) * query.num_q_heads + head * a.group + tile * S::kHeads + h;
-      for (int d = 4 * lane; d < D; d += 128) {
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < 2 * kWarps; ++k) {
-          if (k >= s0 && k <= s1 && pieces[k].used) {
-            const float4 v = *reinterpret_cast<const float4*>(piece_at(k) + h * D + d);
-            o.x += w[k] * v.x, o.y += w[k] * v.y, o.z += w[k] * v.z, o.w += w[k] * v.w;
-          }
-        }
-        if (whole)
-          *reinterpret_cast<uint2*>(static_cast<T*>(query.out) + out_row * D + d) = make_uint2(Pair<T>::pack(o.x * inv, o.y * inv), Pair<T>::pack(o.z * inv, o.w * inv));
-        else
-          *reinterpret_cast<float4*>(to_o + h * D + d) = o;
-      }
-      if (lane == 0) {
-        if (!whole)
-          *reinterpret_cast<float2*>(to_ml + h * 2) = make_float2(top, sum);
-        else if (query.lse)
-          query.lse[out_row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+      if (d >= D) continue;
+      if (whole) {
+        store_result(item.b, head * a.group + tile * S::kHeads + h, d, top, sum, o);
+      } else {
+        *reinterpret_cast<float4*>(to_o + h * D + d) = o;
+        if (d == 0) *reinterpret_cast<float2*>(to_ml + h * 2) = make_float2(top, sum);
       }
     }
-    s0 = s1 + 1;
   }
 
   if (a.cluster < 2 || shares < 2) return;  // all CTAs of a cluster agree on that
@@ -684,31 +700,22 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
   cluster_sync();
   const int head = use.item / a.row_tiles, tile = use.item % a.row_tiles, heads = min(S::kHeads, a.group - tile * S::kHeads);
   const uint32_t local = smem_u32(piece_at(3));
-  for (int i = blockIdx.z * kWarps * 32 + threadIdx.x; i < heads * (D / 4); i += a.cluster * kWarps * 32) {
-    const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
-    float2 ml[kMostCluster];
-    float4 v[kMostCluster];
-    float top = kLowest, sum = 0.f;
-#pragma unroll
-    for (int r = 0; r < kMostCluster; ++r) {
-      const uint32_t at = in_cta(local, min(r, shares - 1));
-      ml[r] = load_cluster_2(at + (a.tile_heads * D + 2 * h) * 4);
-      v[r] = load_cluster_4(at + (h * D + d) * 4);
-    }
-#pragma unroll
-    for (int r = 0; r < kMostCluster; ++r) top = fmaxf(top, ml[r].x);
+#pragma unroll 1
+  for (int unit = blockIdx.z * kWarps + warp; unit < heads * ((D + 127) / 128); unit += a.cluster * kWarps) {
+    const int h = D > 128 ? unit >> 1 : unit, d = (D > 128 ? (unit & 1) * 128 : 0) + 4 * lane, at = (h * D + min(d, D - 4)) * 4;
+    // lane r has the weight of CTA r
+    float2 ml = load_cluster_2(in_cta(local, min(lane, shares - 1)) + (a.tile_heads * D + 2 * h) * 4);
+    if (lane >= shares) ml = make_float2(kLowest, 0.f);
+    float top, sum;
+    const float weight = weight_of(ml, top, sum);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int r = 0; r < kMostCluster; ++r) {
-      if (r >= shares) break;
-      const float w = exp2_fast(ml[r].x - top);
-      sum += w * ml[r].y;
-      o.x += w * v[r].x, o.y += w * v[r].y, o.z += w * v[r].z, o.w += w * v[r].w;
+#pragma unroll 4
+    for (int r = 0; r < shares; ++r) {
+      const float4 v = load_cluster_4(in_cta(local, r) + at);
+      const float w = __shfl_sync(0xFFFFFFFFu, weight, r);
+      o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int64_t out_row = static_cast<int64_t>(use.b) * query.num_q_heads + head * a.group + tile * S::kHeads + h;
-    *reinterpret_cast<uint2*>(static_cast<T*>(query.out) + out_row * D + d) = make_uint2(Pair<T>::pack(o.x * inv, o.y * inv), Pair<T>::pack(o.z * inv, o.w * inv));
-    if (d == 0 && query.lse) query.lse[out_row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    if (d < D) store_result(use.b, head * a.group + tile * S::kHeads + h, d, top, sum, o);
   }
   cluster_sync();  // nobody leaves while another reads its shared memory
 }
