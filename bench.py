@@ -585,16 +585,19 @@ def run_extra(args):
     from trismoe_b200 import decode_harness as dh
 
     full = stack(synth.OLMOE, LAYERS, 1234)
-    model = dh.TrisDecoder(full, dh.DecoderShape(), max_length=512 + 256, max_batch=32, device=device, seed=0)
-    out["e2e_decode_olmoe_16_layers"] = []
-    for B in (1, 32):
-        ids = torch.randint(0, 50304, (B, 512), generator=torch.Generator().manual_seed(B)).to(device)
-        dh.run_exact_generation(model, ids, 8)  # warm-up
-        rec = dh.run_exact_generation(model, ids, 256)
-        out["e2e_decode_olmoe_16_layers"].append({k: (round(v, 3) if isinstance(v, float) else v) for k, v in rec.items() if k != "tokens"})
+    for name, page_size in (("e2e_decode_olmoe_16_layers", None), ("e2e_decode_olmoe_16_layers_paged", 16)):
+        model = dh.TrisDecoder(full, dh.DecoderShape(), max_length=512 + 256, max_batch=32, device=device, seed=0, page_size=page_size)
+        out[name] = []
+        for B in (1, 32):
+            ids = torch.randint(0, 50304, (B, 512), generator=torch.Generator().manual_seed(B)).to(device)
+            dh.run_exact_generation(model, ids, 8)  # warm-up
+            rec = dh.run_exact_generation(model, ids, 256)
+            out[name].append({k: (round(v, 3) if isinstance(v, float) else v) for k, v in rec.items() if k != "tokens"})
+        model.raise_on_kernel_status()
+        del model
     for blk in full:
         blk.raise_on_kernel_status()
-    del model, full
+    del full
     torch.cuda.empty_cache()
     # 4-bit backbones read in place (2048 x 2048, 128-column groups) against their fp16 expansion on the
     # skinny / tcgen05 GEMMs: 80 distinct matrices per pass (160 MB of nibbles, 640 MB of fp16: both beyond L2)

@@ -191,7 +191,7 @@ int launch_controls(LogitArgs& a, int most, cudaStream_t stream) {
   a.slice = (ceil_div(c.vocab, slices) + 31) / 32 * 32;  // even ones
   const size_t smem = c.tokens || c.bias_ids ? 4 * static_cast<size_t>(a.slice) : 0;
   if (int st = allow_shared_memory<logit_controls_kernel<T, VECS>>(4 * kMostSlice)) return st;
-  TRIS_CUDA(launch_kernel(logit_controls_kernel<T, VECS>, dim3(ceil_div(c.vocab, a.slice), c.rows), dim3(kThreads), smem, stream, programmatic_launch_default(), 1, a));
+  TRIS_CUDA(launch_step(logit_controls_kernel<T, VECS>, dim3(ceil_div(c.vocab, a.slice), c.rows), dim3(kThreads), smem, stream, programmatic_launch_default(), 1, a));
   return TRIS_OK;
 }
 // Slices of 1024 where larger ones would leave SMs without work.

@@ -858,7 +858,7 @@ int launch_attention(AttnArgs& a, cudaStream_t stream) {
   const bool pdl = programmatic_launch_default();
   a.cluster = cluster_size(c, a.row_tiles, a.query.window, a.resident);
   if (a.cluster) {
-    TRIS_CUDA(launch_kernel(kernel, dim3(c.num_kv_heads * a.row_tiles, c.num_sequences, a.cluster), dim3(kWarps * 32), S::kSmem, stream, pdl, a.cluster, a));
+    TRIS_CUDA(launch_step(kernel, dim3(c.num_kv_heads * a.row_tiles, c.num_sequences, a.cluster), dim3(kWarps * 32), S::kSmem, stream, pdl, a.cluster, a));
     return TRIS_OK;
   }
   a.ctas = attention_ctas(a.resident, most_blocks(c, a.row_tiles));
@@ -867,8 +867,8 @@ int launch_attention(AttnArgs& a, cudaStream_t stream) {
   const int64_t need = part_floats(a.ctas, a.tile_heads, c.head_dim) * 4;
   TRIS_REQUIRE(a.query.workspace && a.query.workspace_bytes >= need, TRIS_ERR_WORKSPACE, "paged_decode_attention: workspace of %lld bytes needed, got %lld",
                static_cast<long long>(need), static_cast<long long>(a.query.workspace_bytes));
-  TRIS_CUDA(launch_kernel(kernel, dim3(a.ctas), dim3(kWarps * 32), S::kSmem, stream, pdl, 1, a));
-  TRIS_CUDA(launch_kernel(paged_attention_join_kernel<T>, dim3(a.query.num_q_heads, c.num_sequences), dim3(kJoinThreads), 0, stream, true, 1, a, S::kHeads));
+  TRIS_CUDA(launch_step(kernel, dim3(a.ctas), dim3(kWarps * 32), S::kSmem, stream, pdl, 1, a));
+  TRIS_CUDA(launch_step(paged_attention_join_kernel<T>, dim3(a.query.num_q_heads, c.num_sequences), dim3(kJoinThreads), 0, stream, true, 1, a, S::kHeads));
   return TRIS_OK;
 }
 template <typename T, bool FP8>

@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(128) paged_kv_append_kernel(const __grid_const
 template <int VEC, typename T, typename C>
 int launch_append(const AppendArgs& a, cudaStream_t stream) {
   const int64_t threads = static_cast<int64_t>(a.units) * a.head_groups * a.rows.num_tokens;
-  TRIS_CUDA(launch_kernel(paged_kv_append_kernel<VEC, T, C>, dim3(static_cast<unsigned>((threads + 127) / 128)), dim3(128), 0, stream,
+  TRIS_CUDA(launch_step(paged_kv_append_kernel<VEC, T, C>, dim3(static_cast<unsigned>((threads + 127) / 128)), dim3(128), 0, stream,
                           programmatic_launch_default(), 1, a));
   return TRIS_OK;
 }

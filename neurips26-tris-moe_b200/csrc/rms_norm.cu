@@ -218,7 +218,7 @@ int launch_norm(const TrisAddRmsNorm& a, cudaStream_t stream) {
   for (int64_t s : strides) wide = wide && s % 8 == 0;
   for (const void* p : {a.x, a.residual, a.weight, static_cast<const void*>(a.residual_out), static_cast<const void*>(a.y)}) wide = wide && (!p || aligned_to(p, 16));
   if (!wide) {
-    TRIS_CUDA(launch_kernel(add_rms_norm_any_kernel<T, FP8>, dim3(a.rows), dim3(H >= 1024 ? 1024 : (H + 31) / 32 * 32), 0, stream, pdl, 1, a));
+    TRIS_CUDA(launch_step(add_rms_norm_any_kernel<T, FP8>, dim3(a.rows), dim3(H >= 1024 ? 1024 : (H + 31) / 32 * 32), 0, stream, pdl, 1, a));
     return TRIS_OK;
   }
   const int vectors = H / 8;
@@ -233,7 +233,7 @@ int launch_norm(const TrisAddRmsNorm& a, cudaStream_t stream) {
   auto kernel = vecs == 1 ? add_rms_norm_kernel<T, FP8, 1> : vecs == 2 ? add_rms_norm_kernel<T, FP8, 2> : add_rms_norm_kernel<T, FP8, 4>;
   const int resident = 148 * (vecs == 1 ? 1280 : vecs == 2 ? 1024 : 512) / threads;  // by registers
   const int turns = ceil_div(a.rows, resident < 1 ? 1 : resident);
-  TRIS_CUDA(launch_kernel(kernel, dim3(ceil_div(a.rows, turns)), dim3(threads), smem, stream, pdl, 1, args));
+  TRIS_CUDA(launch_step(kernel, dim3(ceil_div(a.rows, turns)), dim3(threads), smem, stream, pdl, 1, args));
   return TRIS_OK;
 }
 
