@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
       }
     }
     // The weights as the 8-column operand: pairs of tokens of one head.  Rounded to the values' type, as 16-bit operands are: 2^-8 (bf16) or
-    // 2^-11 (fp16) of a weight at most, independent from token to token; the sum l is of the weights before that.
+    // 2^-11 (fp16) of a weight at most, independent from token to token; the sum l is of the weights before that, so that lse is exact to fp32.
     uint32_t p[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {

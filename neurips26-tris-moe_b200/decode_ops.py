@@ -65,9 +65,9 @@ def _matrix(what: str, name: str, t: torch.Tensor, dtype, rows: int, columns: Op
     return t.data_ptr(), t.stride(0), shape[1]
 
 
-def _new_like(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous, of t's shape, type and device (torch.empty with those spelled out takes twice as long)."""
-    return torch.empty_like(t, memory_format=torch.contiguous_format)
+def _new_like(t: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """Contiguous, of t's shape and device, and t's type unless told otherwise (torch.empty with those spelled out takes twice as long)."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def _launch(what: str, name: str, dev: torch.device, *structs: bytes) -> None:
@@ -216,13 +216,16 @@ def _norm(what: str, x, residual, weight, eps: float, group_size: Optional[int])
         _fail(what, "x must be fp16 or bf16 [..., hidden]")
     hidden = shape[-1]
     weight_at = _want(what, "weight", weight, dtype, (hidden,))
-    rows_of = lambda t: t if t.dim() == 2 and t.stride(1) == 1 else t.reshape(-1, hidden).contiguous()
-    x2, h = rows_of(x), None
+    x2, h = x, None
+    if len(shape) != 2 or x.stride(1) != 1:
+        x2 = x.reshape(-1, hidden).contiguous()
     r_at = r_stride = h_at = scales_at = 0
     if residual is not None:
         if residual.shape != shape or residual.dtype is not dtype:
             _fail(what, "residual must have x's shape and type")
-        r2, h = rows_of(residual), _new_like(x)
+        r2, h = residual, _new_like(x)
+        if len(shape) != 2 or residual.stride(1) != 1:
+            r2 = residual.reshape(-1, hidden).contiguous()
         r_at, r_stride, h_at = r2.data_ptr(), r2.stride(0), h.data_ptr()
     group, scales = hidden, None
     if group_size is None:
@@ -231,7 +234,7 @@ def _norm(what: str, x, residual, weight, eps: float, group_size: Optional[int])
         group = group_size or hidden
         if hidden == 0 or group < 0 or hidden % group:
             _fail(what, f"groups of {group} columns do not divide rows of {hidden}")
-        y = torch.empty(shape, dtype=torch.float8_e4m3fn, device=dev)
+        y = _new_like(x, torch.float8_e4m3fn)
         scales = torch.empty(shape[:-1] + (hidden // group,), dtype=torch.float32, device=dev)
         scales_at = scales.data_ptr()
     args = _NORM.pack(x2.data_ptr(), r_at, weight_at, h_at, y.data_ptr(), scales_at, x2.stride(0), r_stride, hidden, hidden, x2.shape[0],
@@ -274,7 +277,7 @@ def apply_logit_controls(logits: torch.Tensor, *, tokens: Optional[torch.Tensor]
         _fail(what, "logits must be fp16, bf16 or fp32 [rows, vocab] with a row's logits side by side")
     rows, vocab = shape
     if out is None:
-        out = _new_like(logits) if dtype is torch.float32 else torch.empty(shape, dtype=torch.float32, device=dev)
+        out = _new_like(logits, torch.float32)
     elif out.dtype is not torch.float32 or out.shape != shape or (vocab > 1 and out.stride(1) != 1):
         _fail(what, "out must be fp32 of the logits' shape with a row side by side")
 
