@@ -163,6 +163,14 @@ struct Cursor {
 };
 
 // T: type of q and out.  FP8: e4m3 pages, multiplied as fp16.  DP: head_dim rounded up to 64, 128 or 256.  NT: tiles of 8 query heads.
+// CTAs on an SM, of which some compute while others start or end.  Pages in 8 bits are bound by instructions that wait for one another, so as many as
+// the registers allow (13 x 49925 tokens of heads of 64: 44 us with three or four, 64 with two); in 16 bits two with a deep ring (32 x 512-768 of heads
+// of 128: 34 us, 41 with three and two stages), and one where a step takes 16 KB.
+constexpr int ctas_per_sm(int dp, bool fp8, int nt) {
+  if (dp == 64) return fp8 && nt == 1 ? 4 : 3;
+  if (dp == 128) return fp8 && nt == 1 ? 3 : 2;
+  return fp8 ? 2 : 1;
+}
 template <typename T, bool FP8, int DP, int NT>
 struct Shape {
   static constexpr int kElems = FP8 ? 16 : 8;                          // of a 16-byte chunk
@@ -183,14 +191,15 @@ struct Shape {
   static constexpr int kDimTiles = kValueChunks * kValueElems / 2;        // 16-dimension tiles of O
   static constexpr int kHeads = 8 * NT;
   static constexpr int kPieceBytes = kHeads * (DP + 2) * 4;
-  // Two CTAs on an SM, of which one computes while the other starts or ends; with fp16 heads of 256 dimensions one, for the ring's sake.
-  static constexpr int kCtasPerSm = kStageBytes > 8192 ? 1 : 2;
-  static constexpr int kStagesThatFit = ((kCtasPerSm == 2 ? 115456 : 232000) / kWarps - kPieceBytes) / kStageBytes;
+  static constexpr int kCtasPerSm = ctas_per_sm(DP, FP8, NT);
+  static constexpr int kStagesThatFit = ((228 / kCtasPerSm - 1) * 1024 - 256 - kWarps * kPieceBytes) / (kWarps * kStageBytes);
   static constexpr int kStages = kStagesThatFit > 6 ? 6 : kStagesThatFit;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kSmem = kRing + kWarps * kPieceBytes;
+  static constexpr int kMostSmem = kRing + kWarps * kPieceBytes;
   static_assert(kStages >= 2 && kPieceBytes <= kStages * kStageBytes, "ring");
 };
+// A piece of that many heads; all of them start on 16-byte boundaries.
+__host__ __device__ __forceinline__ int piece_bytes(int heads, int head_dim) { return (heads * (head_dim + 2) * 4 + 15) / 16 * 16; }
 constexpr float kLowest = -3.402823466e38f;  // the running maximum before any score
 
 // A warp's partial result of an item that another warp shares, left in shared memory: o [tile_heads][head_dim], then (m, l) of every head.
@@ -463,7 +472,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
   // Two pieces at most: of the item that another warp began (slot 0), and, with the warp's last block, of one that another warp ends (slot 1).
   // The second one takes the ring's place, all of which has been read by then.
   auto piece_at = [&](int slot) {
-    uint8_t* at = slot & 1 ? smem + (slot >> 1) * (S::kStages * S::kStageBytes) : smem + S::kRing + (slot >> 1) * S::kPieceBytes;
+    uint8_t* at = slot & 1 ? smem + (slot >> 1) * (S::kStages * S::kStageBytes) : smem + S::kRing + (slot >> 1) * piece_bytes(a.tile_heads, D);
     return reinterpret_cast<float*>(at);
   };
   // Lanes 0 to 7 have the (m, l) of partial results: the largest m, the weight of each, and the weighted sum of the l.
@@ -842,7 +851,7 @@ int cluster_size(const TrisPagedKv& c, int row_tiles, int window, int resident) 
   while (size > 1 && items * size > resident) size /= 2;
   return tokens <= static_cast<int64_t>(kMostShare) * kBlock * kWarps * size ? size : 0;
 }
-int resident_ctas(int head_dim, bool fp8) { return sm_count() * (head_dim > 128 && !fp8 ? 1 : 2); }
+int resident_ctas(int head_dim, bool fp8, int tiles) { return sm_count() * ctas_per_sm(head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256, fp8, tiles); }
 size_t part_floats(int ctas, int tile_heads, int head_dim) { return 2 * static_cast<size_t>(ctas) * tile_heads * (head_dim + 2); }
 
 template <typename T, bool FP8, int DP, int NT>
@@ -850,15 +859,14 @@ int launch_attention(AttnArgs& a, cudaStream_t stream) {
   using S = Shape<T, FP8, DP, NT>;
   auto kernel = paged_attention_kernel<T, FP8, DP, NT>;
   const TrisPagedKv& c = a.cache;
-  if (int st = allow_shared_memory<paged_attention_kernel<T, FP8, DP, NT>>(S::kSmem)) return st;
+  if (int st = allow_shared_memory<paged_attention_kernel<T, FP8, DP, NT>>(S::kMostSmem)) return st;
   TRIS_REQUIRE(sm_count() > 0, TRIS_ERR_CUDA, "paged_decode_attention: no device");
-  static_assert(S::kCtasPerSm == (DP > 128 && !FP8 ? 1 : 2), "resident_ctas");
-  a.resident = resident_ctas(c.head_dim, FP8);
+  a.resident = resident_ctas(c.head_dim, FP8, NT);
   a.rows_together = a.page_blocks && c.head_dim == DP && c.k_token_stride == DP && c.v_token_stride == DP;
   const bool pdl = programmatic_launch_default();
   a.cluster = cluster_size(c, a.row_tiles, a.query.window, a.resident);
   if (a.cluster) {
-    TRIS_CUDA(launch_step(kernel, dim3(c.num_kv_heads * a.row_tiles, c.num_sequences, a.cluster), dim3(kWarps * 32), S::kSmem, stream, pdl, a.cluster, a));
+    TRIS_CUDA(launch_step(kernel, dim3(c.num_kv_heads * a.row_tiles, c.num_sequences, a.cluster), dim3(kWarps * 32), S::kRing + kWarps * piece_bytes(a.tile_heads, c.head_dim), stream, pdl, a.cluster, a));
     return TRIS_OK;
   }
   a.ctas = attention_ctas(a.resident, most_blocks(c, a.row_tiles));
@@ -867,7 +875,7 @@ int launch_attention(AttnArgs& a, cudaStream_t stream) {
   const int64_t need = part_floats(a.ctas, a.tile_heads, c.head_dim) * 4;
   TRIS_REQUIRE(a.query.workspace && a.query.workspace_bytes >= need, TRIS_ERR_WORKSPACE, "paged_decode_attention: workspace of %lld bytes needed, got %lld",
                static_cast<long long>(need), static_cast<long long>(a.query.workspace_bytes));
-  TRIS_CUDA(launch_step(kernel, dim3(a.ctas), dim3(kWarps * 32), S::kSmem, stream, pdl, 1, a));
+  TRIS_CUDA(launch_step(kernel, dim3(a.ctas), dim3(kWarps * 32), S::kRing + kWarps * piece_bytes(a.tile_heads, c.head_dim), stream, pdl, 1, a));
   TRIS_CUDA(launch_step(paged_attention_join_kernel<T>, dim3(a.query.num_q_heads, c.num_sequences), dim3(kJoinThreads), 0, stream, true, 1, a, S::kHeads));
   return TRIS_OK;
 }
@@ -886,8 +894,8 @@ using namespace tris;
 extern "C" size_t tris_paged_decode_attention_workspace_bytes(const TrisPagedKv* cache, int32_t num_q_heads, int32_t window) {
   if (validate_paged_kv(cache, "paged_decode_attention")) return 0;
   if (num_q_heads < 1 || num_q_heads % cache->num_kv_heads || window < 0 || sm_count() == 0) return 0;
-  const int group = num_q_heads / cache->num_kv_heads, heads = 8 * head_tiles(group, cache->head_dim), row_tiles = ceil_div(group, heads);
-  const int resident = resident_ctas(cache->head_dim, cache->dtype == TRIS_DTYPE_E4M3);
+  const int group = num_q_heads / cache->num_kv_heads, tiles = head_tiles(group, cache->head_dim), heads = 8 * tiles, row_tiles = ceil_div(group, heads);
+  const int resident = resident_ctas(cache->head_dim, cache->dtype == TRIS_DTYPE_E4M3, tiles);
   if (cluster_size(*cache, row_tiles, window, resident)) return 0;
   return part_floats(attention_ctas(resident, most_blocks(*cache, row_tiles)), group < heads ? group : heads, cache->head_dim) * 4;
 }
