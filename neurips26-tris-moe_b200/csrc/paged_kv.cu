@@ -225,11 +225,11 @@ extern "C" int tris_paged_kv_append(const TrisPagedKv* cache, const TrisPagedApp
   TRIS_REQUIRE(r.dtype == TRIS_DTYPE_F16 || r.dtype == TRIS_DTYPE_BF16, TRIS_ERR_INVALID_ARG, "paged_kv_append: rows are fp16 or bf16");
   TRIS_REQUIRE(c.dtype == TRIS_DTYPE_E4M3 || c.dtype == r.dtype, TRIS_ERR_INVALID_ARG, "paged_kv_append: pages hold the rows' type or e4m3");
   TRIS_REQUIRE(r.num_tokens >= 0 && r.num_q_heads >= 0, TRIS_ERR_INVALID_ARG, "paged_kv_append: negative sizes");
-  TRIS_REQUIRE((r.q && r.q_out) || r.num_q_heads == 0, TRIS_ERR_INVALID_ARG, "paged_kv_append: null q or q_out");
   TRIS_REQUIRE((r.cos == nullptr) == (r.sin == nullptr), TRIS_ERR_INVALID_ARG, "paged_kv_append: cos and sin go together");
   const int rot = r.cos ? r.rotary_dim : 0;
   TRIS_REQUIRE(rot % 2 == 0 && rot >= 0 && rot <= c.head_dim, TRIS_ERR_INVALID_ARG, "paged_kv_append: rotary_dim must be even and at most head_dim (got %d)", rot);
   if (r.num_tokens == 0) return TRIS_OK;
+  TRIS_REQUIRE((r.q && r.q_out) || r.num_q_heads == 0, TRIS_ERR_INVALID_ARG, "paged_kv_append: null q or q_out");
   TRIS_REQUIRE(r.k && r.v && r.positions, TRIS_ERR_INVALID_ARG, "paged_kv_append: null k, v or positions");
 
   AppendArgs a{c, r, 0, 1};

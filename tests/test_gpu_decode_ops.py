@@ -177,6 +177,78 @@ def test_attention_where_one_score_outweighs_all(lib):
     assert float(((out.double() - want).abs() - (2.0 ** -11 + 2.0 ** -11) * mag - 2.0 ** -11 * want.abs()).max()) <= 0
 
 
+@pytest.mark.parametrize("softmax_scale", [-0.2, 0.0, 3.0])
+def test_attention_with_any_scale(lib, softmax_scale):
+    import trismoe_b200 as tm
+
+    g, lengths = _gen(14), [1, 20, 333]
+    q = torch.randn((3, 4, 64), generator=g, device="cuda").half()
+    filled = _filled(g, lengths, 16, 2, 64, F16, LAYOUTS[0], scale=0.5)
+    _check_attention(tm, q, filled, lengths, softmax_scale=softmax_scale)
+
+
+def test_attention_of_queries_of_very_different_sizes(lib):
+    """8-bit pages: rows around 10^-20 and 10^20 in bf16, zeros, and elements far apart in one row."""
+    import trismoe_b200 as tm
+
+    g, lengths = _gen(15), [50, 50, 50, 50]
+    filled = _filled(g, lengths, 16, 1, 128, E4M3, LAYOUTS[0])
+    q = torch.randn((4, 2, 128), generator=g, device="cuda")
+    for b, size in enumerate((1e-20, 1e20, 0.0)):
+        q[b] *= size
+    q[3, :, ::2] *= 1e-6
+    for b, size in enumerate((1e20, 1e-20, 1.0, 1.0)):  # one scale for the call: a row at a time
+        one = lambda t: t[b: b + 1].contiguous()
+        k_pages, v_pages, table, rows = filled
+        _check_attention(tm, one(q.to(BF16)), (k_pages, v_pages, one(table), rows[b: b + 1]), [50], softmax_scale=size / 11.0)
+
+
+def test_calls_on_nothing(lib):
+    import trismoe_b200 as tm
+
+    new = lambda *s, dtype=F16: torch.zeros(s, dtype=dtype, device="cuda")
+    pages, i32 = new(4, 16, 2, 64), torch.int32
+    assert tm.paged_decode_attention(new(0, 4, 64), pages, pages, new(0, 3, dtype=i32), new(0, dtype=i32)).shape == (0, 4, 64)
+    out, lse = tm.paged_decode_attention(torch.ones_like(new(2, 4, 64)), pages, pages, new(2, 0, dtype=i32), new(2, dtype=i32), return_lse=True)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    assert tm.append_paged_kv(new(0, 4, 64), new(0, 2, 64), new(0, 2, 64), pages, pages, new(1, 4, dtype=i32), new(0, dtype=i32)).shape == (0, 4, 64)
+    assert tm.apply_logit_controls(new(0, 100)).shape == (0, 100) and tm.apply_logit_controls(new(3, 0)).shape == (3, 0)
+    x = torch.randn((2, 40), device="cuda")
+    empty = tm.apply_logit_controls(x, tokens=new(2, 0, dtype=i32), token_lengths=new(2, dtype=i32), repetition=new(2, dtype=torch.float32) + 2.0,
+                                    bias_ids=new(2, 0, dtype=i32), bias_values=new(2, 0, dtype=torch.float32))
+    assert torch.equal(empty, x)
+
+
+def test_arguments_that_the_python_layer_refuses(lib):
+    import trismoe_b200 as tm
+
+    new = lambda *s, dtype=F16: torch.zeros(s, dtype=dtype, device="cuda")
+    pages, i32 = new(4, 16, 2, 64), torch.int32
+    table, lens, pos, q, k = new(2, 3, dtype=i32), new(2, dtype=i32), new(2, dtype=i32), new(2, 4, 64), new(2, 2, 64)
+    attend = lambda q=q, k=pages, v=pages, t=table, n=lens, **m: tm.paged_decode_attention(q, k, v, t, n, **m)
+    append = lambda q=q, k=k, v=k, kp=pages, vp=pages, t=table, p=pos, s=None, **m: tm.append_paged_kv(q, k, v, kp, vp, t, p, s, **m)
+    f32 = lambda *s: new(*s, dtype=torch.float32)
+    logits = f32(2, 40)
+    for call, text in [
+        (lambda: attend(q=new(2, 3, 64)), "share"), (lambda: attend(q=new(2, 4, 32)), "head_dim"), (lambda: attend(q=q.float()), "fp16 or bf16"),
+        (lambda: attend(q=q.bfloat16()), "queries' type"), (lambda: attend(k=pages.bfloat16()), "same type"), (lambda: attend(t=table.long()), "int32"),
+        (lambda: attend(t=table[:1]), "sequences"), (lambda: attend(n=lens.long()), "lengths"), (lambda: attend(window=-1), "window"),
+        (lambda: attend(k_scale=f32(2)), "e4m3"), (lambda: attend(k=pages[..., ::2], v=pages[..., ::2], q=new(2, 4, 32)), "side by side"),
+        (lambda: attend(status=lens), "status"), (lambda: attend(n=lens.cpu()), "one CUDA device"),
+        (lambda: append(k=new(2, 1, 64)), "num_kv_heads"), (lambda: append(q=new(3, 4, 64)), "q must be"), (lambda: append(p=pos.float()), "positions"),
+        (lambda: append(s=pos.long()), "sequences"), (lambda: append(cos=f32(9, 32)), "go together"), (lambda: append(cos=f32(9, 64), sin=f32(9, 64)), "rotary_dim"),
+        (lambda: append(cos=f32(9, 32), sin=f32(8, 32)), "sin"), (lambda: append(k_scale=f32(2)), "e4m3"),
+        (lambda: tm.add_rms_norm(new(2, 64), new(2, 32), new(64)), "residual"), (lambda: tm.add_rms_norm(new(2, 64), None, new(32)), "weight"),
+        (lambda: tm.add_rms_norm(f32(2, 64), None, f32(64)), "fp16 or bf16"), (lambda: tm.add_rms_norm_e4m3(new(2, 64), None, new(64), group_size=24), "divide"),
+        (lambda: tm.add_rms_norm_e4m3(new(2, 64), None, new(64), group_size=8), "multiples of 16"),
+        (lambda: tm.apply_logit_controls(logits, repetition=f32(2)), "need tokens"), (lambda: tm.apply_logit_controls(logits, tokens=new(2, 5, dtype=i32)), "token_lengths"),
+        (lambda: tm.apply_logit_controls(logits, bias_ids=new(2, 5, dtype=i32)), "go together"), (lambda: tm.apply_logit_controls(logits, allowed=new(2, 1, dtype=i32)), "allowed"),
+        (lambda: tm.apply_logit_controls(logits, out=new(2, 40)), "out must be"), (lambda: tm.apply_logit_controls(logits.double()), "fp16, bf16 or fp32"),
+    ]:
+        with pytest.raises(RuntimeError, match=text):
+            call()
+
+
 def test_attention_offsets_beyond_32_bits(lib):
     import trismoe_b200 as tm
 
