@@ -62,13 +62,6 @@ __device__ __forceinline__ void store_8(__nv_fp8_e4m3* p, const float (&v)[8]) {
   *reinterpret_cast<uint2*>(p) = make_uint2(e4m3_pack4(v[0], v[1], v[2], v[3]), e4m3_pack4(v[4], v[5], v[6], v[7]));
 }
 
-// Maximum that keeps a NaN (fmaxf drops it).
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
 // launch_kernel, by the plain launch where nothing else is asked for: 0.6 us less of the host's time (2.8 against 3.4).
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_step(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl, int cluster_z, Args&&... args) {

@@ -20,24 +20,32 @@ struct NormArgs {
   int group_shift;  // log2 of the vectors of a group where that is a power of two up to a warp's lanes, else -1
 };
 
-// Over the CTA; red has a place for every warp.  A barrier lies between two uses of one red (two of them take turns).
+// Over the CTA, for all threads; red has a place for every warp.  A barrier lies between two uses of one red (two of them take turns).
 __device__ __forceinline__ float block_sum(float v, float* red) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  if (lane == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = 0.f;
-  for (unsigned w = 0; w < blockDim.x / 32; ++w) v += red[w];
+  v = lane < static_cast<int>(blockDim.x >> 5) ? red[lane] : 0.f;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
   return v;
 }
-__device__ __forceinline__ float block_max(float v, float* red) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v = max_nan(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
+// 1 / v to a rounding.
+__device__ __forceinline__ float reciprocal(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// Magnitudes as bits: they order like the numbers, and a NaN is the largest.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
+  v = __reduce_max_sync(0xFFFFFFFFu, v);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = red[0];
-  for (unsigned w = 1; w < blockDim.x / 32; ++w) v = max_nan(v, red[w]);
-  return v;
+  const int lane = threadIdx.x & 31;
+  return __reduce_max_sync(0xFFFFFFFFu, lane < static_cast<int>(blockDim.x >> 5) ? red[lane] : 0);
 }
 template <typename T>
 __device__ __forceinline__ void unpack_8(const uint4& raw, float (&v)[8]) {
@@ -53,8 +61,9 @@ __device__ __forceinline__ void unpack_8(const uint4& raw, float (&v)[8]) {
 template <typename T, bool FP8, int VECS>
 __global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const __grid_constant__ NormArgs args) {
   const TrisAddRmsNorm& a = args.a;
-  __shared__ float red[2][32], red_max[2][32];
-  extern __shared__ float vector_max[];  // groups that do not fit a warp: largest element of every vector
+  __shared__ float red[2][32];
+  __shared__ uint32_t red_max[2][32];
+  extern __shared__ uint32_t vector_max[];  // groups that do not fit a warp: largest element of every vector
   const int tid = threadIdx.x, vectors = a.hidden_size / 8;
   uint4 w[VECS], x[VECS], r[VECS];
 #pragma unroll
@@ -102,19 +111,24 @@ __global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const 
         if (v < vectors) store_8(static_cast<T*>(a.residual_out) + row * a.residual_out_stride + 8 * v, h[i]);
       }
     }
-    const float inv = rsqrtf(block_sum(sum, red[turn]) * args.inv_hidden + a.eps);
-    float top[VECS], all = 0.f;
+    sum = block_sum(sum, red[turn]);
+    const float inv = rsqrtf(sum * args.inv_hidden + a.eps);
+    uint32_t top[VECS];  // largest magnitude
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       float f[8];
       unpack_8<T>(w[i], f);
-      top[i] = 0.f;
+      float most = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         h[i][k] = h[i][k] * inv * f[k];
-        if (FP8) top[i] = max_nan(top[i], fabsf(h[i][k]));
+        if (FP8) most = fmaxf(most, fabsf(h[i][k]));
       }
-      if (FP8) all = max_nan(all, tid + i * blockDim.x < vectors ? top[i] : 0.f);
+      top[i] = __float_as_uint(most);
+      if (FP8 && !(sum < INFINITY)) {  // something is not finite: fmaxf drops a NaN
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top[i] = max(top[i], magnitude(h[i][k]));
+      }
     }
     if constexpr (!FP8) {
 #pragma unroll
@@ -125,14 +139,21 @@ __global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const 
     } else {
       const int per_group = a.group_size / 8;  // vectors
       if (a.group_size == a.hidden_size) {
+        uint32_t all = 0;
+#pragma unroll
+        for (int i = 0; i < VECS; ++i)
+          if (tid + i * blockDim.x < vectors) all = max(all, top[i]);
         all = block_max(all, red_max[turn]);
 #pragma unroll
         for (int i = 0; i < VECS; ++i) top[i] = all;
       } else if (args.group_shift >= 0) {
         // neighbours in a warp; vectors past the row only meet one another
-        for (int d = per_group / 2; d; d >>= 1)
 #pragma unroll
-          for (int i = 0; i < VECS; ++i) top[i] = max_nan(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], d));
+        for (int d = 16; d; d >>= 1)
+          if (d < per_group) {
+#pragma unroll
+            for (int i = 0; i < VECS; ++i) top[i] = max(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], d));
+          }
       } else {
         __syncthreads();  // the row before has been read
 #pragma unroll
@@ -143,20 +164,24 @@ __global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const 
         for (int i = 0; i < VECS; ++i) {
           const int v = tid + i * blockDim.x;
           if (v < vectors)
-            for (int k = v / per_group * per_group, e = k + per_group; k < e; ++k) top[i] = max_nan(top[i], vector_max[k]);
+            for (int k = v / per_group * per_group, e = k + per_group; k < e; ++k) top[i] = max(top[i], vector_max[k]);
         }
       }
 #pragma unroll
       for (int i = 0; i < VECS; ++i) {
         const int v = tid + i * blockDim.x;
         if (v < vectors) {
-          const float scale = top[i] / kE4m3Max;
-          // times the reciprocal: at most one rounding off the quotient, which e4m3's four bits seldom show.  Of a subnormal scale the reciprocal
-          // overflows, so values and scale are raised first; a scale of 0 has nothing but zeros
-          const float lift = scale < 1.2e-38f ? 1.8446744e19f : 1.f;
-          const float up = scale == 0.f ? 0.f : 1.f / (scale * lift);
+          // times reciprocals, of 448 and of the scale: at most two roundings off the quotients, which e4m3's four bits seldom show.  Of a subnormal
+          // scale the reciprocal overflows, so values and scale are raised first; a scale of 0 has nothing but zeros
+          const float scale = __uint_as_float(top[i]) * (1.f / kE4m3Max);
+          float times = scale == 0.f ? 0.f : reciprocal(scale);
+          if (scale < 1.2e-38f && scale != 0.f) {
+            times = reciprocal(scale * 1.8446744e19f);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) h[i][k] = h[i][k] * lift * up;
+            for (int k = 0; k < 8; ++k) h[i][k] *= 1.8446744e19f;
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) h[i][k] *= times;
           store_8(static_cast<__nv_fp8_e4m3*>(a.y) + row * a.y_stride + 8 * v, h[i]);
           if (args.group_shift >= 0) {
             if ((v & (per_group - 1)) == 0) a.scales[row * args.groups + (v >> args.group_shift)] = scale;
@@ -173,7 +198,8 @@ __global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const 
 // may lie on the inputs: what is read again after a store is not needed from there any more.
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(1024) add_rms_norm_any_kernel(const __grid_constant__ TrisAddRmsNorm a) {
-  __shared__ float red[32], red_max[32];
+  __shared__ float red[32];
+  __shared__ uint32_t red_max[32];
   pdl_wait();
   pdl_launch_dependents();
   const int64_t row = blockIdx.x;
@@ -191,10 +217,10 @@ __global__ void __launch_bounds__(1024) add_rms_norm_any_kernel(const __grid_con
   for (int q = 0; q < groups; ++q) {
     float div = 1.f;
     if constexpr (FP8) {
-      float top = 0.f;
-      for (int i = q * width + threadIdx.x; i < (q + 1) * width; i += blockDim.x) top = max_nan(top, fabsf(sum_at(i) * inv * to_float(weight[i])));
+      uint32_t top = 0;
+      for (int i = q * width + threadIdx.x; i < (q + 1) * width; i += blockDim.x) top = max(top, magnitude(sum_at(i) * inv * to_float(weight[i])));
       __syncthreads();  // red_max of the group before
-      const float scale = block_max(top, red_max) / kE4m3Max;
+      const float scale = __uint_as_float(block_max(top, red_max)) / kE4m3Max;
       div = scale == 0.f ? 1.f : scale;
       if (threadIdx.x == 0) a.scales[row * groups + q] = scale;
     }
