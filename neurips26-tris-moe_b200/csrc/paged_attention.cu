@@ -130,7 +130,7 @@ __device__ __forceinline__ int count_blocks(const AttnArgs& a, int stop, int lan
 }
 // Blocks that each warp takes.  The grid has as many CTAs as are resident twice over, so that an SM that is done early takes another one; where that
 // would leave a warp fewer than kMinRun blocks, half of them do the work.
-constexpr int kMinRun = 24;
+constexpr int kMinRun = 64;
 __device__ __forceinline__ int run_length(const AttnArgs& a, int total) {
   const unsigned workers = static_cast<unsigned>(a.ctas) * kWarps;
   const unsigned run = (static_cast<unsigned>(total) + workers - 1) / workers;
@@ -827,8 +827,6 @@ int sm_count() {
   return count[dev];
 }
 
-// Tiles of 8 query heads that share a key/value head's pass.  With heads of 256 dimensions the accumulators of two do not fit the registers.
-int head_tiles(int group, int head_dim) { return group > 8 && head_dim <= 128 ? 2 : 1; }
 
 // CTAs of the first kernel: twice as many as are resident, but no more than there can be shares of one block for their warps.
 int attention_ctas(int resident, int64_t blocks) {
@@ -838,20 +836,32 @@ int attention_ctas(int resident, int64_t blocks) {
 int64_t most_blocks(const TrisPagedKv& c, int row_tiles) {
   return static_cast<int64_t>(c.num_sequences) * c.num_kv_heads * row_tiles * ((static_cast<int64_t>(c.table_width) * c.page_size + kBlock - 1) / kBlock + 1);
 }
-// CTAs that share an item, as many as still run at the same time for all items, up to kMostCluster; 0 where that leaves a warp more than
-// kMostShare blocks of the longest sequence that the table (or the window) has room for.  One launch instead of two and no numbering are worth 2 to 5 us -
-// 20 x 1 token 6.7 -> 4.8, 1 x 513 9.8 -> 8.0, 32 x 512-768 39 -> 36, 16 x 4096 in 8 bits 31 -> 26 -, but SMs that have no item stay idle, and
-// sequences of different lengths end at different times: 4 x 20580 44 -> 57, 13 x 49925 76 -> 104, 64 x 1-16384 293 -> 297 to 366.
-constexpr int kMostShare = 16;
+// CTAs that share an item, as many as still run at the same time for all items, up to kMostCluster; 0: the work is numbered through.  One launch instead
+// of two and no numbering are worth 1 to 3 us (flat and clusters, us: 20 x 1 token 6.1 / 4.3, 1 x 513 8.7 / 7.4, 16 x 4096 in 8 bits 25.5 / 22.3), and
+// many short sequences gain more (32 x 512-768 37.6 / 34.7, 64 x 1-1024 44.6 / 34.9).  But a cluster's longest sequence ends last, and SMs without an
+// item stay idle: 64 x 1-2048 59.5 / 60.6, 1 x 8192 13.4 / 20.0, 1 x 4096 10.7 / 12.5, 64 x 1-16384 293 / 299.  So a warp may have up to
+// kMostShare blocks of the longest sequence that the table (or the window) has room for where clusters fill the GPU, and fewer as they fill less of it.
+constexpr int kMostShare = 24, kLeastShare = 4;
 int cluster_size(const TrisPagedKv& c, int row_tiles, int window, int resident) {
   const int64_t items = static_cast<int64_t>(c.num_sequences) * c.num_kv_heads * row_tiles;
   int64_t tokens = static_cast<int64_t>(c.table_width) * c.page_size;
   if (window > 0 && window < tokens) tokens = window + kBlock;
   int size = kMostCluster;
   while (size > 1 && items * size > resident) size /= 2;
-  return tokens <= static_cast<int64_t>(kMostShare) * kBlock * kWarps * size ? size : 0;
+  int64_t share = items * size >= resident ? kMostShare : kMostShare * items * size / resident;
+  if (share < kLeastShare) share = kLeastShare;
+  return tokens <= share * kBlock * kWarps * size ? size : 0;
 }
 int resident_ctas(int head_dim, bool fp8, int tiles) { return sm_count() * ctas_per_sm(head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256, fp8, tiles); }
+// Tiles of 8 query heads that share a key/value head's pass: two where a group has more than 8 - with heads of 256 dimensions the accumulators of two
+// do not fit the registers -, but where even so every tile has a cluster of its own of the largest size, one: the pages are read twice, by two
+// clusters, and what a warp does alone at its end is halved (group of 16, 8 x 1000 tokens 11.5 / 9.4 us, 32 x 1000 15.1 / 15.9, 128 x 1000 32 / 40).
+int head_tiles(const TrisPagedKv& c, int group, int window) {
+  if (group <= 8 || c.head_dim > 128) return 1;
+  const int singles = ceil_div(group, 8), resident = resident_ctas(c.head_dim, c.dtype == TRIS_DTYPE_E4M3, 1);
+  const bool room = static_cast<int64_t>(c.num_sequences) * c.num_kv_heads * singles * kMostCluster <= resident;
+  return room && cluster_size(c, singles, window, resident) ? 1 : 2;
+}
 size_t part_floats(int ctas, int tile_heads, int head_dim) { return 2 * static_cast<size_t>(ctas) * tile_heads * (head_dim + 2); }
 
 template <typename T, bool FP8, int DP, int NT>
@@ -880,9 +890,9 @@ int launch_attention(AttnArgs& a, cudaStream_t stream) {
   return TRIS_OK;
 }
 template <typename T, bool FP8>
-int launch_shape(AttnArgs& a, cudaStream_t stream) {
+int launch_shape(AttnArgs& a, int tiles, cudaStream_t stream) {
   const int d = a.cache.head_dim;
-  if (head_tiles(a.group, d) == 2) return d <= 64 ? launch_attention<T, FP8, 64, 2>(a, stream) : launch_attention<T, FP8, 128, 2>(a, stream);
+  if (tiles == 2) return d <= 64 ? launch_attention<T, FP8, 64, 2>(a, stream) : launch_attention<T, FP8, 128, 2>(a, stream);
   return d <= 64 ? launch_attention<T, FP8, 64, 1>(a, stream) : d <= 128 ? launch_attention<T, FP8, 128, 1>(a, stream) : launch_attention<T, FP8, 256, 1>(a, stream);
 }
 
@@ -894,7 +904,7 @@ using namespace tris;
 extern "C" size_t tris_paged_decode_attention_workspace_bytes(const TrisPagedKv* cache, int32_t num_q_heads, int32_t window) {
   if (validate_paged_kv(cache, "paged_decode_attention")) return 0;
   if (num_q_heads < 1 || num_q_heads % cache->num_kv_heads || window < 0 || sm_count() == 0) return 0;
-  const int group = num_q_heads / cache->num_kv_heads, tiles = head_tiles(group, cache->head_dim), heads = 8 * tiles, row_tiles = ceil_div(group, heads);
+  const int group = num_q_heads / cache->num_kv_heads, tiles = head_tiles(*cache, group, window), heads = 8 * tiles, row_tiles = ceil_div(group, heads);
   const int resident = resident_ctas(cache->head_dim, cache->dtype == TRIS_DTYPE_E4M3, tiles);
   if (cluster_size(*cache, row_tiles, window, resident)) return 0;
   return part_floats(attention_ctas(resident, most_blocks(*cache, row_tiles)), group < heads ? group : heads, cache->head_dim) * 4;
@@ -919,7 +929,7 @@ extern "C" int tris_paged_decode_attention(const TrisPagedKv* cache, const TrisP
   a.cache = c;
   a.query = q;
   a.group = q.num_q_heads / c.num_kv_heads;
-  const int heads = 8 * head_tiles(a.group, c.head_dim);
+  const int tiles = head_tiles(c, a.group, q.window), heads = 8 * tiles;
   a.row_tiles = ceil_div(a.group, heads);
   a.tile_heads = a.group < heads ? a.group : heads;
   a.page_blocks = c.page_size % kBlock == 0;
@@ -931,6 +941,6 @@ extern "C" int tris_paged_decode_attention(const TrisPagedKv* cache, const TrisP
     if (c.page_size == 1 << s) a.page_shift = s;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool q8 = c.dtype == TRIS_DTYPE_E4M3;
-  if (q.dtype == TRIS_DTYPE_F16) return q8 ? launch_shape<__half, true>(a, s) : launch_shape<__half, false>(a, s);
-  return q8 ? launch_shape<__nv_bfloat16, true>(a, s) : launch_shape<__nv_bfloat16, false>(a, s);
+  if (q.dtype == TRIS_DTYPE_F16) return q8 ? launch_shape<__half, true>(a, tiles, s) : launch_shape<__half, false>(a, tiles, s);
+  return q8 ? launch_shape<__nv_bfloat16, true>(a, tiles, s) : launch_shape<__nv_bfloat16, false>(a, tiles, s);
 }
