@@ -2,18 +2,23 @@
 //
 // out = sum_t exp(s_t - m) v_t / sum_t exp(s_t - m), s_t = scale * q . k_t, m the largest s so far: one pass over keys and values, in which the
 // sums are scaled down whenever m grows.  Two such partial results (m, l, o) of different tokens join by the same rule, so a sequence can be cut
-// anywhere.  Every cached byte is read once and used for as many query heads as share it: bound by bytes.
+// anywhere.  Every cached byte is read once and used for as many query heads as share it: bound by bytes where there are many (64 sequences of 1 to
+// 16384 tokens, 32/8 heads of 128 in bf16, 1.8 GB: 290 us, 6.2 TB/s; one of 131071 in fp16 96 us, 5.6), by the chain length - page - rows - join
+// where there are few (513 tokens of 16 heads 7.4 us), and by the conversion's instructions where pages are in 8 bits (heads of 256, 66 MB: 22 us).
 //
-// Work.  The tokens of every (sequence, key/value head) are cut into blocks of 16, all blocks are numbered through, and each warp of the grid
+// Work.  Short sequences: a cluster of CTAs has one key/value head of one sequence and cuts its tokens evenly (cluster_size has the rule).
+// Long ones: the tokens of every (sequence, key/value head) are cut into blocks of 16, all blocks are numbered through, and each warp of the grid
 // takes an equal run of them, whatever sequences it crosses: lengths may differ by any factor, change from one replay of a graph to the next,
-// and a single long sequence still occupies every SM.  A warp that has all of a sequence's blocks writes its result; others write partial
-// results to the workspace (at most two a warp), which the second kernel joins in the order of the tokens.
+// and a single long sequence still occupies every SM.  A warp that has all of an item's blocks writes its result; others leave partial
+// results that are joined in the order of the tokens: first those of a CTA's warps in shared memory, then those of a cluster's CTAs over distributed
+// shared memory or, of numbered blocks, by a second kernel from the workspace (at most two a CTA).
 //
 // One warp's step.  S^T = K Q^T and O^T = V^T P^T by mma.sync m16n8k16: the cached rows are the 16-row operand and the query heads of a group the
 // 8 columns, so that a step of 16 tokens costs two MMAs per 16 dimensions with up to 8 heads (with the heads as rows it would cost four, half
 // of them zeros).  No operand goes through a transposing load: the order of dimensions inside a product is free as long as both operands have the
 // same, so a lane's 16 bytes of a key row are its fragments as they are; of four value rows a lane has the same 8 dimensions, whose pairs of
-// tokens are put together by PRMT.  Each warp has a ring of its own in shared memory, filled by cp.async, and meets no other warp before it is done.
+// tokens are put together by PRMT.  A step's MMAs take a tenth of the time its bytes take (heads of 128: 16 at two cycles of an SM, 8 KB at 23 bytes a
+// cycle), so nothing waits for the tensor pipe; tcgen05 tiles have 128 rows and their second operand in shared memory.  Each warp has a ring of its own in shared memory, filled by cp.async, and meets no other warp before it is done.
 #include <type_traits>
 
 #include "decode_step.cuh"
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
       const int tok0 = load.token(), head = load.item / a.row_tiles;
       const uint32_t dst = ring_at + stage * S::kStageBytes;
       if (a.rows_together && page >= 0 && tok0 >= load.span.lo && tok0 + kBlock <= load.span.hi) {
-        // a whole block of one page, side by side in memory
+        // a whole block of one page, side by side in memory: addresses are one base and constants (32 x 512-768: 34.6 us, 36.9 without)
         const int in_page = a.page_shift >= 0 ? tok0 & (c.page_size - 1) : tok0 % c.page_size;
         const uint8_t* k = k_pages + (page * c.k_page_stride + head * c.k_head_stride) * kElt + in_page * S::kRowBytes + lane * 16;
         const uint8_t* v = v_pages + (page * c.v_page_stride + head * c.v_head_stride) * kElt + in_page * S::kRowBytes + lane * 16;
