@@ -27,7 +27,7 @@ namespace tris {
 namespace {
 
 constexpr int kBlock = 16;  // tokens of a step
-constexpr int kWarps = 4;   // of a CTA
+constexpr int kWarps = 4;   // of a CTA (W); 2 for many very short sequences
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnArgs {
@@ -176,7 +176,7 @@ constexpr int ctas_per_sm(int dp, bool fp8, int nt) {
   if (dp == 128) return fp8 && nt == 1 ? 3 : 2;
   return fp8 ? 2 : 1;
 }
-template <typename T, bool FP8, int DP, int NT>
+template <typename T, bool FP8, int DP, int NT, int W>
 struct Shape {
   static constexpr int kElems = FP8 ? 16 : 8;                          // of a 16-byte chunk
   static constexpr int kKeyChunks = DP / kElems / 4;                   // of a key row that a lane has
@@ -196,11 +196,11 @@ struct Shape {
   static constexpr int kDimTiles = kValueChunks * kValueElems / 2;        // 16-dimension tiles of O
   static constexpr int kHeads = 8 * NT;
   static constexpr int kPieceBytes = kHeads * (DP + 2) * 4;
-  static constexpr int kCtasPerSm = ctas_per_sm(DP, FP8, NT);
-  static constexpr int kStagesThatFit = ((228 / kCtasPerSm - 1) * 1024 - 256 - kWarps * kPieceBytes) / (kWarps * kStageBytes);
+  static constexpr int kCtasPerSm = ctas_per_sm(DP, FP8, NT) * (kWarps / W);
+  static constexpr int kStagesThatFit = ((228 / kCtasPerSm - 1) * 1024 - 256 - (W == kWarps ? W * kPieceBytes : 0)) / (W * kStageBytes);
   static constexpr int kStages = kStagesThatFit > 6 ? 6 : kStagesThatFit;
-  static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kMostSmem = kRing + kWarps * kPieceBytes;
+  static constexpr int kRing = W * kStages * kStageBytes;
+  static constexpr int kMostSmem = kRing + (W == kWarps ? W * kPieceBytes : 0);
   static_assert(kStages >= 2 && kPieceBytes <= kStages * kStageBytes, "ring");
 };
 // A piece of that many heads; all of them start on 16-byte boundaries.
@@ -214,13 +214,13 @@ struct Piece {
   int used;
 };
 
-template <typename T, bool FP8, int DP, int NT>
-__global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm) paged_attention_kernel(const __grid_constant__ AttnArgs a) {
-  using S = Shape<T, FP8, DP, NT>;
+template <typename T, bool FP8, int DP, int NT, int W>
+__global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) paged_attention_kernel(const __grid_constant__ AttnArgs a) {
+  using S = Shape<T, FP8, DP, NT, W>;
   using M = std::conditional_t<FP8, __half, T>;  // type of the products
   constexpr int kElt = FP8 ? 1 : 2;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ Piece pieces[2 * kWarps];
+  __shared__ Piece pieces[2 * W];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const TrisPagedKv& c = a.cache;
   const TrisPagedAttention& query = a.query;
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
   // This warp's run: its part of the CTA's (cluster's) one item, or of the numbering, with the sequence that holds its first block.
   Cursor use{};
   int count = 0, shares = 1;  // shares: CTAs of the cluster that have a part
-  if (a.cluster) {
+  if (W < kWarps || a.cluster) {
     use.b = blockIdx.y;
     use.item = blockIdx.x;
     // the block table's row comes to L2 while the length is on its way
@@ -239,20 +239,20 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
     use.span = span_of(a, use.b);
     use.blocks = use.span.blocks();
     if (query.lengths[use.b] > use.span.hi && c.status_dev) *c.status_dev = TRIS_ERR_CORRUPT;
-    const int run = (use.blocks + a.cluster * kWarps - 1) / (a.cluster * kWarps);
-    use.blk = (blockIdx.z * kWarps + warp) * run;
+    const int run = (use.blocks + a.cluster * W - 1) / (a.cluster * W);
+    use.blk = (blockIdx.z * W + warp) * run;
     count = max(0, min(run, use.blocks - use.blk));
-    shares = run ? (use.blocks + kWarps * run - 1) / (kWarps * run) : 0;
+    shares = run ? (use.blocks + W * run - 1) / (W * run) : 0;
     if (use.blocks <= 1 && (blockIdx.z > 0 || use.blocks == 0)) {  // one block is its warp's alone; nothing at all gives zeros
       if (use.blocks == 0 && blockIdx.z == 0) {
         const int head = use.item / a.row_tiles, row0 = use.item % a.row_tiles * S::kHeads, rows = min(S::kHeads, a.group - row0);
         const int64_t out_row = static_cast<int64_t>(use.b) * query.num_q_heads + head * a.group + row0;
-        for (int i = threadIdx.x; i < rows * D; i += kWarps * 32) store_float(static_cast<T*>(query.out) + out_row * D + i, 0.f);
-        for (int i = threadIdx.x; query.lse && i < rows; i += kWarps * 32) query.lse[out_row + i] = -INFINITY;
+        for (int i = threadIdx.x; i < rows * D; i += W * 32) store_float(static_cast<T*>(query.out) + out_row * D + i, 0.f);
+        for (int i = threadIdx.x; query.lse && i < rows; i += W * 32) query.lse[out_row + i] = -INFINITY;
       }
       return;  // the whole cluster: none of its CTAs has a piece
     }
-  } else {
+  } else if constexpr (W == kWarps) {
     int mine, upto = scan_blocks(a, 0, lane, mine);
     int total = __shfl_sync(0xFFFFFFFFu, upto, 31);
     for (int i = 1; 32 * i < c.num_sequences; ++i) {
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
   // Two pieces at most: of the item that another warp began (slot 0), and, with the warp's last block, of one that another warp ends (slot 1).
   // The second one takes the ring's place, all of which has been read by then.
   auto piece_at = [&](int slot) {
-    uint8_t* at = slot & 1 ? smem + (slot >> 1) * (S::kStages * S::kStageBytes) : smem + S::kRing + (slot >> 1) * piece_bytes(a.tile_heads, D);
+    uint8_t* at = slot & 1 || W < kWarps ? smem + (slot >> 1) * (S::kStages * S::kStageBytes) : smem + S::kRing + (slot >> 1) * piece_bytes(a.tile_heads, D);
     return reinterpret_cast<float*>(at);
   };
   // Lanes 0 to 7 have the (m, l) of partial results: the largest m, the weight of each, and the weighted sum of the l.
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
     sum = __shfl_sync(0xFFFFFFFFu, sum, 0);
     return weight;
   };
-  static_assert(2 * kWarps <= 8 && kMostCluster <= 8, "weight_of");
+  static_assert(2 * W <= 8 && kMostCluster <= 8, "weight_of");
   auto store_result = [&](int b, int q_head, int d, float top, float sum, float4 o) {
     const int64_t out_row = static_cast<int64_t>(b) * query.num_q_heads + q_head;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -667,8 +667,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
   __syncthreads();
 
   // Neighbouring warps' pieces of one item are joined here; what other CTAs share goes to the workspace, or is left for the cluster.
-  const uint32_t used = __ballot_sync(0xFFFFFFFFu, lane < 2 * kWarps && pieces[lane & (2 * kWarps - 1)].used);
-  const uint32_t last_ones = used & __ballot_sync(0xFFFFFFFFu, pieces[lane & (2 * kWarps - 1)].ends);
+  const uint32_t used = __ballot_sync(0xFFFFFFFFu, lane < 2 * W && pieces[lane & (2 * W - 1)].used);
+  const uint32_t last_ones = used & __ballot_sync(0xFFFFFFFFu, pieces[lane & (2 * W - 1)].ends);
 #pragma unroll 1
   for (uint32_t rest = used; rest;) {
     const int s0 = __ffs(rest) - 1;
@@ -680,11 +680,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
     const int head = item.item / a.row_tiles, tile = item.item % a.row_tiles;
     const int heads = min(S::kHeads, a.group - tile * S::kHeads);
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (item.starts ? 1 : 0);
-    float* to_o = a.cluster ? piece_at(3) : a.part_o + slot * a.tile_heads * D;
-    float* to_ml = a.cluster ? piece_at(3) + a.tile_heads * D : a.part_ml + slot * a.tile_heads * 2;
+    float* to_o = W < kWarps || a.cluster ? piece_at(3) : a.part_o + slot * a.tile_heads * D;
+    float* to_ml = W < kWarps || a.cluster ? piece_at(3) + a.tile_heads * D : a.part_ml + slot * a.tile_heads * 2;
     // a warp takes 128 dimensions of a head at a time
 #pragma unroll 1
-    for (int unit = warp; unit < heads * ((D + 127) / 128); unit += kWarps) {
+    for (int unit = warp; unit < heads * ((D + 127) / 128); unit += W) {
       const int h = D > 128 ? unit >> 1 : unit, d = (D > 128 ? (unit & 1) * 128 : 0) + 4 * lane;
       // lane k has the weight of piece k
       float2 ml = make_float2(kLowest, 0.f);
@@ -693,7 +693,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
       const float weight = weight_of(ml, top, sum);
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < 2 * kWarps; ++k) {
+      for (int k = 0; k < 2 * W; ++k) {
         if (!((group >> k) & 1)) continue;
         const float4 v = *reinterpret_cast<const float4*>(piece_at(k) + h * D + min(d, D - 4));
         const float w = __shfl_sync(0xFFFFFFFFu, weight, k);
@@ -709,13 +709,13 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<T, FP8, DP, NT>::kCtasPerSm
     }
   }
 
-  if (a.cluster < 2 || shares < 2) return;  // all CTAs of a cluster agree on that
+  if (W < kWarps || a.cluster < 2 || shares < 2) return;  // all CTAs of a cluster agree on that
   // The cluster's CTAs have left what they have of the item in the part of their rings that the item's second warp had; each joins some of it.
   cluster_sync();
   const int head = use.item / a.row_tiles, tile = use.item % a.row_tiles, heads = min(S::kHeads, a.group - tile * S::kHeads);
   const uint32_t local = smem_u32(piece_at(3));
 #pragma unroll 1
-  for (int unit = blockIdx.z * kWarps + warp; unit < heads * ((D + 127) / 128); unit += a.cluster * kWarps) {
+  for (int unit = blockIdx.z * W + warp; unit < heads * ((D + 127) / 128); unit += a.cluster * W) {
     const int h = D > 128 ? unit >> 1 : unit, d = (D > 128 ? (unit & 1) * 128 : 0) + 4 * lane, at = (h * D + min(d, D - 4)) * 4;
     // lane r has the weight of CTA r
     float2 ml = load_cluster_2(in_cta(local, min(lane, shares - 1)) + (a.tile_heads * D + 2 * h) * 4);
@@ -857,6 +857,14 @@ int cluster_size(const TrisPagedKv& c, int row_tiles, int window, int resident) 
   if (share < kLeastShare) share = kLeastShare;
   return tokens <= share * kBlock * kWarps * size ? size : 0;
 }
+// More items than CTAs that run at one time, of at most kShort tokens: start and end of a CTA are all there is, and CTAs of two warps, of which twice
+// as many run, halve the rounds.  Four and two warps, us: 42 x 16 tokens of 8 heads 7.3 / 4.5, 128 x 64 19.6 / 14.1, 64 x 256 18.4 / 17.0; 64 x 512 27.0 / 29.3, and
+// for 42 x 128 in 8 bits, all of whose CTAs run, 7.5 / 8.5.
+constexpr int kShort = 256;
+bool two_warps(const TrisPagedKv& c, int row_tiles, int window, int resident) {
+  const int64_t items = static_cast<int64_t>(c.num_sequences) * c.num_kv_heads * row_tiles;
+  return items > resident && (static_cast<int64_t>(c.table_width) * c.page_size <= kShort || (window > 0 && window <= kShort - kBlock));
+}
 int resident_ctas(int head_dim, bool fp8, int tiles) { return sm_count() * ctas_per_sm(head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256, fp8, tiles); }
 // Tiles of 8 query heads that share a key/value head's pass: two where a group has more than 8 - with heads of 256 dimensions the accumulators of two
 // do not fit the registers -, but where even so every tile has a cluster of its own of the largest size, one: the pages are read twice, by two
@@ -871,17 +879,24 @@ size_t part_floats(int ctas, int tile_heads, int head_dim) { return 2 * static_c
 
 template <typename T, bool FP8, int DP, int NT>
 int launch_attention(AttnArgs& a, cudaStream_t stream) {
-  using S = Shape<T, FP8, DP, NT>;
-  auto kernel = paged_attention_kernel<T, FP8, DP, NT>;
+  using S = Shape<T, FP8, DP, NT, kWarps>;
+  auto kernel = paged_attention_kernel<T, FP8, DP, NT, kWarps>;
   const TrisPagedKv& c = a.cache;
-  if (int st = allow_shared_memory<paged_attention_kernel<T, FP8, DP, NT>>(S::kMostSmem)) return st;
+  if (int st = allow_shared_memory<paged_attention_kernel<T, FP8, DP, NT, kWarps>>(S::kMostSmem)) return st;
   TRIS_REQUIRE(sm_count() > 0, TRIS_ERR_CUDA, "paged_decode_attention: no device");
   a.resident = resident_ctas(c.head_dim, FP8, NT);
   a.rows_together = a.page_blocks && c.head_dim == DP && c.k_token_stride == DP && c.v_token_stride == DP;
   const bool pdl = programmatic_launch_default();
   a.cluster = cluster_size(c, a.row_tiles, a.query.window, a.resident);
+  const dim3 items(c.num_kv_heads * a.row_tiles, c.num_sequences, a.cluster);
+  if (a.cluster == 1 && two_warps(c, a.row_tiles, a.query.window, a.resident)) {
+    using P = Shape<T, FP8, DP, NT, 2>;
+    if (int st = allow_shared_memory<paged_attention_kernel<T, FP8, DP, NT, 2>>(P::kMostSmem)) return st;
+    TRIS_CUDA(launch_step(paged_attention_kernel<T, FP8, DP, NT, 2>, items, dim3(64), P::kMostSmem, stream, pdl, 1, a));
+    return TRIS_OK;
+  }
   if (a.cluster) {
-    TRIS_CUDA(launch_step(kernel, dim3(c.num_kv_heads * a.row_tiles, c.num_sequences, a.cluster), dim3(kWarps * 32), S::kRing + kWarps * piece_bytes(a.tile_heads, c.head_dim), stream, pdl, a.cluster, a));
+    TRIS_CUDA(launch_step(kernel, items, dim3(kWarps * 32), S::kRing + kWarps * piece_bytes(a.tile_heads, c.head_dim), stream, pdl, a.cluster, a));
     return TRIS_OK;
   }
   a.ctas = attention_ctas(a.resident, most_blocks(c, a.row_tiles));

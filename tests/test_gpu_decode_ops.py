@@ -103,11 +103,12 @@ SHAPES = [  # q heads, kv heads, head_dim, rows, cache
     (2, 2, 8, F16, F16), (9, 1, 64, BF16, E4M3), (20, 1, 112, F16, E4M3), (3, 1, 192, BF16, BF16), (2, 1, 16, F16, E4M3), (17, 1, 256, BF16, E4M3),
 ]
 # short ones are attended to by clusters, long ones by numbered blocks; the last ones keep two tiles of heads together in clusters, too
-LENGTHS = [[1], [0], [16, 0, 1, 17, 15], [33, 300, 1, 0, 129, 1000, 64], [2500], [9000, 1, 0, 40], [(13 * i) % 70 for i in range(100)]]
+LENGTHS = [[1], [0], [16, 0, 1, 17, 15], [33, 300, 1, 0, 129, 1000, 64], [2500], [9000, 1, 0, 40], [(13 * i) % 70 for i in range(100)],
+           [(29 * i) % 200 for i in range(700)]]  # more than run at a time: CTAs of two warps
 
 
 @pytest.mark.parametrize("heads,kv,dim,rows,cache", SHAPES, ids=lambda v: str(v).replace("torch.", ""))
-@pytest.mark.parametrize("lengths", LENGTHS, ids=lambda v: "-".join(map(str, v[:7])))
+@pytest.mark.parametrize("lengths", LENGTHS, ids=lambda v: f"{len(v)}-" + "-".join(map(str, v[:7])))
 def test_attention_over_lengths(lib, heads, kv, dim, rows, cache, lengths):
     import trismoe_b200 as tm
 
@@ -115,7 +116,7 @@ def test_attention_over_lengths(lib, heads, kv, dim, rows, cache, lengths):
     scales = [None, None]
     if cache == E4M3:
         scales = [0.5 + torch.rand((kv,), generator=g, device="cuda") for _ in range(2)]
-    page = {1: 16, 4: 32, 5: 8, 7: 48, 100: 16}[len(lengths)]
+    page = {1: 16, 4: 32, 5: 8, 7: 48, 100: 16, 700: 16}[len(lengths)]
     filled = _filled(g, lengths, page, kv, dim, cache, LAYOUTS[heads % 3])
     q = (torch.randn((len(lengths), heads, dim), generator=g, device="cuda") * 2.0).to(rows)
     _check_attention(tm, q, filled, lengths, k_scale=scales[0], v_scale=scales[1])
