@@ -844,8 +844,9 @@ int64_t most_blocks(const TrisPagedKv& c, int row_tiles) {
 // CTAs that share an item, as many as still run at the same time for all items, up to kMostCluster; 0: the work is numbered through.  One launch instead
 // of two and no numbering are worth 1 to 3 us (flat and clusters, us: 20 x 1 token 6.1 / 4.3, 1 x 513 8.7 / 7.4, 16 x 4096 in 8 bits 25.5 / 22.3), and
 // many short sequences gain more (32 x 512-768 37.6 / 34.7, 64 x 1-1024 44.6 / 34.9).  But a cluster's longest sequence ends last, and SMs without an
-// item stay idle: 64 x 1-2048 59.5 / 60.6, 1 x 8192 13.4 / 20.0, 1 x 4096 10.7 / 12.5, 64 x 1-16384 293 / 299.  So a warp may have up to
-// kMostShare blocks of the longest sequence that the table (or the window) has room for where clusters fill the GPU, and fewer as they fill less of it.
+// item stay idle: 1 x 8192 13.4 / 20.0, 1 x 4096 10.7 / 12.5, 64 x 1-2048 59.1 / 60.3, 64 x 1-3000 79 / 84, 64 x 1-16384 293 / 299.  Where the items take many
+// rounds their ends even out: 128 x 1-4096 197 / 183, 128 x 1-8192 354 / 355, 200 x 1-8192 560 / 540.  So a warp may have up to kMostShare blocks
+// of the longest sequence that the table (or the window) has room for, times the rounds, or the part of one, that the items take.
 constexpr int kMostShare = 24, kLeastShare = 4;
 int cluster_size(const TrisPagedKv& c, int row_tiles, int window, int resident) {
   const int64_t items = static_cast<int64_t>(c.num_sequences) * c.num_kv_heads * row_tiles;
@@ -853,7 +854,7 @@ int cluster_size(const TrisPagedKv& c, int row_tiles, int window, int resident) 
   if (window > 0 && window < tokens) tokens = window + kBlock;
   int size = kMostCluster;
   while (size > 1 && items * size > resident) size /= 2;
-  int64_t share = items * size >= resident ? kMostShare : kMostShare * items * size / resident;
+  int64_t share = kMostShare * items * size / resident;
   if (share < kLeastShare) share = kLeastShare;
   return tokens <= share * kBlock * kWarps * size ? size : 0;
 }
