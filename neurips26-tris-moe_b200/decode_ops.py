@@ -82,7 +82,8 @@ def _launch(what: str, name: str, dev: torch.device, *structs: bytes) -> None:
         _native.check(status, what)
 
 
-def _cache(what: str, k_pages, v_pages, block_table, k_scale, v_scale, status) -> bytes:
+def _cache(what: str, k_pages, v_pages, block_table, k_scale, v_scale, status) -> tuple:
+    """The cache as the library takes it, and (dtype, heads, head_dim, sequences, table width, page size) of it."""
     shape, dtype = k_pages.shape, k_pages.dtype
     if len(shape) != 4 or shape != v_pages.shape or dtype is not v_pages.dtype or dtype not in _DTYPES:
         _fail(what, "k_pages and v_pages must have the same type and shape [num_pages, page_size, num_kv_heads, head_dim]")
@@ -99,12 +100,13 @@ def _cache(what: str, k_pages, v_pages, block_table, k_scale, v_scale, status) -
         _fail(what, "block_table must have the pages of a sequence side by side")
     if (k_scale is not None or v_scale is not None) and dtype is not torch.float8_e4m3fn:
         _fail(what, "scales belong to e4m3 pages")
-    return _PAGED_KV.pack(
+    packed = _PAGED_KV.pack(
         k_pages.data_ptr(), v_pages.data_ptr(), k0, k1, k2, v0, v1, v2,
         0 if k_scale is None else _want(what, "k_scale", k_scale, torch.float32, (heads,)),
         0 if v_scale is None else _want(what, "v_scale", v_scale, torch.float32, (heads,)),
         block_table.data_ptr(), t0, sequences, width, pages, page_size, heads, dim,
         _DTYPES[dtype], 0, 0 if status is None else _want(what, "status", status, torch.int32, (1,)))
+    return packed, (dtype, heads, dim, sequences, width, page_size)
 
 
 def raise_on_status(status: torch.Tensor, what: str = "paged cache") -> None:
@@ -130,11 +132,13 @@ def append_paged_kv(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     with ``return_key`` a pair with the rotated keys."""
     what = "append_paged_kv"
     dev = _same_device(what, k, v, q, k_pages, v_pages, block_table, positions, sequences, cos, sin, k_scale, v_scale, status)
+    cache, (_, cache_heads, cache_dim, _, _, _) = _cache(what, k_pages, v_pages, block_table, k_scale, v_scale, status)
     shape, dtype = k.shape, k.dtype
-    if len(shape) != 3 or v.shape != shape or dtype not in _ROWS or v.dtype is not dtype or shape[1:] != k_pages.shape[2:]:
-        _fail(what, "k and v must be fp16 or bf16 [tokens, num_kv_heads, head_dim] of the cache")
-    tokens, _, dim = shape
-    cache = _cache(what, k_pages, v_pages, block_table, k_scale, v_scale, status)
+    if len(shape) != 3 or v.shape != shape or dtype not in _ROWS or v.dtype is not dtype:
+        _fail(what, "k and v must be fp16 or bf16 [tokens, num_kv_heads, head_dim]")
+    tokens, heads, dim = shape
+    if heads != cache_heads or dim != cache_dim:
+        _fail(what, f"k {tuple(shape)} does not fit pages of num_kv_heads {cache_heads} and head_dim {cache_dim}")
     wide = positions.dtype is torch.int64
     at = _want(what, "positions", positions, torch.int64 if wide else torch.int32, (tokens,))
     sequence_at = 0 if sequences is None else _want(what, "sequences", sequences, torch.int32, (tokens,))
@@ -153,10 +157,11 @@ def append_paged_kv(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         _fail(what, "the dimensions of a head must be side by side")
     rows = half = cos_at = sin_at = 0
     if cos is not None or sin is not None:
-        if cos is None or sin is None or cos.dim() != 2:
-            _fail(what, "cos and sin go together, [positions, rotary_dim / 2] each")
+        if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()) \
+                or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
+            _fail(what, "cos and sin go together, contiguous fp32 [positions, rotary_dim / 2] each")
         rows, half = cos.shape
-        cos_at, sin_at = _want(what, "cos", cos, torch.float32, (rows, half)), _want(what, "sin", sin, torch.float32, (rows, half))
+        cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
     if return_key:
         k_out = _new_like(k)
     args = _APPEND.pack(q_at, k.data_ptr(), v.data_ptr(), q0, q1, k0, k1, v0, v1, cos_at, sin_at, at, sequence_at, out_at,
@@ -184,21 +189,20 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     q0, q1, q2 = q.stride()
     if q2 != 1 and dim > 1:
         _fail(what, "the dimensions of a head must be side by side")
-    cache = _cache(what, k_pages, v_pages, block_table, k_scale, v_scale, status)
-    if k_pages.shape[3] != dim or block_table.shape[0] != batch:
-        _fail(what, f"q {tuple(shape)} does not fit pages of head_dim {k_pages.shape[3]} and a block table of {block_table.shape[0]} sequences")
+    cache, sizes = _cache(what, k_pages, v_pages, block_table, k_scale, v_scale, status)
+    if sizes[2] != dim or sizes[3] != batch:
+        _fail(what, f"q {tuple(shape)} does not fit pages of head_dim {sizes[2]} and a block table of {sizes[3]} sequences")
     lengths_at = _want(what, "lengths", lengths, torch.int32, (batch,))
     window = window or 0
-    key = (dev.index, heads, k_pages.shape, k_pages.dtype, block_table.shape, window)
-    if key not in _scratch:
-        if len(_scratch) >= 4096:  # block tables may grow for ever
-            _scratch.clear()
+    key = (dev.index, heads, window, sizes)
+    like, ws_at, ws_bytes = _scratch.get(key, False), 0, 0
+    known = like is not False
+    if not known:
         with torch.cuda.device(dev):
             need = int(_native.load().tris_paged_decode_attention_workspace_bytes(cache, heads, max(window, -1)))
-        _scratch[key] = torch.empty((1,), dtype=torch.uint8, device=dev).expand(need) if need else None
-    ws, ws_at, ws_bytes = _scratch[key], 0, 0
-    if ws is not None:
-        ws = _new_like(ws)
+        like = torch.empty((1,), dtype=torch.uint8, device=dev).expand(need) if need else None
+    if like is not None:
+        ws = _new_like(like)
         ws_at, ws_bytes = ws.data_ptr(), ws.numel()
     out, lse = _new_like(q), None
     if return_lse:
@@ -206,6 +210,10 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     args = _ATTENTION.pack(q.data_ptr(), q0, q1, lengths_at, out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws_at, ws_bytes,
                            heads, window, _DTYPES[dtype], dim ** -0.5 if softmax_scale is None else softmax_scale)
     _launch(what, "tris_paged_decode_attention", dev, cache, args)
+    if not known:  # a call that was refused says nothing of what the next one needs
+        if len(_scratch) >= 4096:  # block tables may grow for ever
+            _scratch.clear()
+        _scratch[key] = like
     return (out, lse) if return_lse else out
 
 

@@ -251,6 +251,22 @@ def test_arguments_that_the_python_layer_refuses(lib):
             call()
 
 
+def test_a_refused_call_does_not_spoil_the_next(lib):
+    """Long caches need scratch; what a refused call of the same sizes needed is not remembered."""
+    import trismoe_b200 as tm
+
+    g, lengths = _gen(16), [20000]
+    k_pages, v_pages, table, rows = _filled(g, lengths, 16, 1, 40, F16, LAYOUTS[1])
+    q = torch.randn((1, 1, 40), generator=g, device="cuda").half()
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    flat = torch.zeros((k_pages.numel() + 1,), dtype=F16, device="cuda")
+    off = flat[1:].view(k_pages.shape)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="16-byte boundary"):
+            tm.paged_decode_attention(q, off, off, table, lens)
+    _check_attention(tm, q, (k_pages, v_pages, table, rows), lengths)
+
+
 def test_attention_offsets_beyond_32_bits(lib):
     import trismoe_b200 as tm
 
