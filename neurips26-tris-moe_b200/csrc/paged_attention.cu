@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
       const uint32_t dst = ring_at + stage * S::kStageBytes;
       if (a.rows_together && page >= 0 && tok0 >= load.span.lo && tok0 + kBlock <= load.span.hi) {
         // a whole block of one page, side by side in memory: addresses are one base and constants (32 x 512-768: 34.6 us, 36.9 without)
-        const int in_page = a.page_shift >= 0 ? tok0 & (c.page_size - 1) : tok0 % c.page_size;
+        const int64_t in_page = a.page_shift >= 0 ? tok0 & (c.page_size - 1) : tok0 % c.page_size;
         const uint8_t* k = k_pages + (page * c.k_page_stride + head * c.k_head_stride) * kElt + in_page * S::kRowBytes + lane * 16;
         const uint8_t* v = v_pages + (page * c.v_page_stride + head * c.v_head_stride) * kElt + in_page * S::kRowBytes + lane * 16;
 #pragma unroll
@@ -821,17 +821,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
 }
 
 int sm_count() {
-  static int count[64] = {};
+  static std::atomic<int> count[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  if (!count[dev]) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    count[dev] = n;
-  }
-  return count[dev];
+  int n = count[dev].load(std::memory_order_relaxed);
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) count[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
-
 
 // CTAs of the first kernel: twice as many as are resident, but no more than there can be shares of one block for their warps.
 int attention_ctas(int resident, int64_t blocks) {
@@ -955,7 +951,7 @@ extern "C" int tris_paged_decode_attention(const TrisPagedKv* cache, const TrisP
   a.tile_heads = a.group < heads ? a.group : heads;
   a.page_blocks = c.page_size % kBlock == 0;
   a.wide_query = aligned_to(q.q, 16) && q.q_token_stride % 8 == 0 && q.q_head_stride % 8 == 0;
-  TRIS_REQUIRE(static_cast<int64_t>(c.table_width) * c.page_size < (1ll << 31) && most_blocks(c, a.row_tiles) < (1ll << 31), TRIS_ERR_UNSUPPORTED,
+  TRIS_REQUIRE(static_cast<int64_t>(c.table_width) * c.page_size < (1ll << 31) - kBlock && most_blocks(c, a.row_tiles) < (1ll << 31), TRIS_ERR_UNSUPPORTED,
                "paged_decode_attention: a block table for more than 2^31 blocks of %d tokens (all sequences and heads)", kBlock);
   a.page_shift = -1;
   for (int s = 0; s < 31; ++s)

@@ -282,6 +282,23 @@ def test_attention_offsets_beyond_32_bits(lib):
     _check_attention(tm, q[:1], (k_pages, v_pages, table, [(k.double(), v.double())]), [48])
 
 
+@pytest.mark.parametrize("dtype", [F16, E4M3], ids=["fp16", "e4m3"])
+def test_attention_in_a_page_of_more_than_4_gb(lib, dtype):
+    """One page a sequence, 9 (18) million tokens of 512 (256) bytes; only the window at its end is ever written or read."""
+    import trismoe_b200 as tm
+
+    g, tokens, window = _gen(17), 9_000_000 if dtype == F16 else 18_000_000, 100
+    pages = [torch.empty((1, 1, tokens, 256), dtype=dtype, device="cuda").transpose(1, 2) for _ in range(2)]
+    k, v = (torch.randn((window, 1, 256), generator=g, device="cuda") for _ in range(2))
+    table = torch.zeros((1, 1), dtype=torch.int32, device="cuda")
+    where = torch.arange(tokens - window, tokens, device="cuda")
+    q = tm.append_paged_kv(torch.randn((window, 2, 256), generator=g, device="cuda").half(), k.half(), v.half(), pages[0], pages[1], table, where,
+                           torch.zeros((window,), dtype=torch.int32, device="cuda"))
+    held = [(p[0, where].double()) for p in pages]
+    assert torch.equal(held[1], v.half().to(dtype).double())
+    _check_attention(tm, q[:1].contiguous(), (pages[0], pages[1], table, [tuple(held)]), [tokens], window=window)
+
+
 def test_attention_reports_what_does_not_fit(lib):
     import trismoe_b200 as tm
 
