@@ -18,7 +18,8 @@
 // of them zeros).  No operand goes through a transposing load: the order of dimensions inside a product is free as long as both operands have the
 // same, so a lane's 16 bytes of a key row are its fragments as they are; of four value rows a lane has the same 8 dimensions, whose pairs of
 // tokens are put together by PRMT.  A step's MMAs take a tenth of the time its bytes take (heads of 128: 16 at two cycles of an SM, 8 KB at 23 bytes a
-// cycle), so nothing waits for the tensor pipe; tcgen05 tiles have 128 rows and their second operand in shared memory.  Each warp has a ring of its own in shared memory, filled by cp.async, and meets no other warp before it is done.
+// cycle), so nothing waits for the tensor pipe; tcgen05 tiles have 128 rows and their second operand in shared memory.  Each warp has a ring of its
+// own in shared memory, filled by cp.async, and meets no other warp before it is done.
 #include <type_traits>
 
 #include "decode_step.cuh"
