@@ -206,7 +206,7 @@ struct Shape {
 };
 // A piece of that many heads; all of them start on 16-byte boundaries.
 __host__ __device__ __forceinline__ int piece_bytes(int heads, int head_dim) { return (heads * (head_dim + 2) * 4 + 15) / 16 * 16; }
-constexpr float kLowest = -3.402823466e38f;  // the running maximum before any score
+constexpr float kLowest = -3.402823466e38f;  // m before any score
 
 // A warp's partial result of an item that another warp shares, left in shared memory: o [tile_heads][head_dim], then (m, l) of every head.
 struct Piece {
@@ -220,6 +220,8 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
   using S = Shape<T, FP8, DP, NT, W>;
   using M = std::conditional_t<FP8, __half, T>;  // type of the products
   constexpr int kElt = FP8 ? 1 : 2;
+  // Range of the weights, to base 2.  bf16 ones are not lifted: they lose nothing below 1, and values may go up to the end of 32 bits themselves.
+  constexpr float kLift = std::is_same_v<M, __half> ? 7.f : 0.f, kMostWeight = kLift + 8.f;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Piece pieces[2 * W];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -543,8 +545,9 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
       }
     }
 
-    // Tokens g and g + 8 of heads 2 t and 2 t + 1.  Weights are 2^(s - m) with m no less than the largest score so far minus 8: m moves only when
-    // a score exceeds it by more than that, which is rare after the first blocks, and sums scaled by up to 2^8 are as exact.
+    // Tokens g and g + 8 of heads 2 t and 2 t + 1.  Weights are 2^(s - m); m is the largest score so far less kLift when it moves, and moves only when
+    // a score exceeds it by more than kMostWeight, which is rare after the first blocks.  Of fp16 the largest weight is so between 2^7 and
+    // 2^15 (the type ends below 2^16), and weights down to 2^-21 of it have all of its bits; sums in 32 bits are as exact at any scale.
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -565,7 +568,7 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         x[n][k] = s[n][k] - m[n][k & 1];
-        above |= x[n][k] > 8.f;
+        above |= x[n][k] > kMostWeight;
       }
     if (__any_sync(0xFFFFFFFFu, above)) {
 #pragma unroll
@@ -576,7 +579,7 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
           float top = fmaxf(s[n][h], s[n][2 + h]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-          top = fmaxf(m[n][h], top);
+          top = fmaxf(m[n][h], top - kLift);
           old[h] = exp2_fast(m[n][h] - top);
           m[n][h] = top;
           l[n][h] *= old[h];

@@ -179,6 +179,26 @@ def test_attention_where_one_score_outweighs_all(lib):
     assert float(((out.double() - want).abs() - (2.0 ** -11 + 2.0 ** -11) * mag - 2.0 ** -11 * want.abs()).max()) <= 0
 
 
+@pytest.mark.parametrize("rows,cache", [(F16, F16), (BF16, BF16), (F16, E4M3), (BF16, E4M3)], ids=lambda v: str(v).replace("torch.", ""))
+def test_attention_of_small_weights_beside_a_large_one_on_nothing(lib, rows, cache):
+    import trismoe_b200 as tm
+
+    # the token that has almost all of the weight has values of zero: the result is made of weights from 2^-17 to 2^-19 of it
+    g, lengths, page, dim = _gen(9), [2, 3, 40, 300], 16, 64
+    k_pages, v_pages, table, kept = _filled(g, lengths, page, 2, dim, cache, LAYOUTS[0])
+    for b, n in enumerate(lengths):
+        k, v = kept[b]
+        k[..., 0] = -torch.rand((n, 2), generator=g, device="cuda").to(cache).double()
+        at = (5 * b) % n
+        k[at, :, 0], v[at] = 12.0, 0.0
+        place = torch.arange(n, device="cuda")
+        page_of = table[b, place // page].long()
+        k_pages[page_of, place % page], v_pages[page_of, place % page] = k.to(cache), v.to(cache)
+    q = torch.zeros((4, 6, dim), dtype=rows, device="cuda")
+    q[..., 0] = 1.0
+    _check_attention(tm, q, (k_pages, v_pages, table, kept), lengths, softmax_scale=1.0)
+
+
 @pytest.mark.parametrize("softmax_scale", [-0.2, 0.0, 3.0])
 def test_attention_with_any_scale(lib, softmax_scale):
     import trismoe_b200 as tm
