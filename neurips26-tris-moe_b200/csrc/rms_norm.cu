@@ -67,14 +67,14 @@ __global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const 
   extern __shared__ uint32_t vector_max[];  // groups that do not fit a warp: largest element of every vector
   const int tid = threadIdx.x, vectors = a.hidden_size / 8;
   uint4 w[VECS], x[VECS], r[VECS];
+  pdl_wait();  // ahead of the weight, too: it may be what the launch before has made (1 + w)
+  pdl_launch_dependents();
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
     const int v = tid + i * blockDim.x;
     w[i] = r[i] = make_uint4(0, 0, 0, 0);
     if (v < vectors) w[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.weight) + 8 * v);
   }
-  pdl_wait();
-  pdl_launch_dependents();
   auto fetch = [&](int64_t row) {
     const T* xs = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* rs = static_cast<const T*>(a.residual) + row * a.residual_stride;

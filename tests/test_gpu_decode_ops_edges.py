@@ -1,0 +1,81 @@
+"""GPU tests of the decode step's operators where they could go wrong unnoticed: launches that overlap, dimensions and rows that a call must not
+touch, quotients that end half way between two results, numbers that are not finite, sizes that lead to each variant.
+
+Definitions in 64 bits and the bounds' parts (U, SUB) are those of test_gpu_decode_ops.py; further bounds are derived where they stand."""
+import pytest
+import torch
+
+from test_gpu_decode_ops import F16, LAYOUTS, _filled, _gen
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- launches that overlap ------------------------------------------------------------------
+@pytest.fixture
+def overlapping(lib):
+    """Programmatic launches for the stand-alone entry points, as they were before afterwards."""
+    previous = lib.tris_set_programmatic_launch(1)
+    try:
+        yield lib
+    finally:
+        torch.cuda.synchronize()
+        lib.tris_set_programmatic_launch(previous)
+
+
+@pytest.mark.parametrize("quantized", [False, True], ids=["16 bit", "e4m3"])
+@pytest.mark.parametrize("rows,hidden", [(1, 2048), (300, 4096), (3, 1001)])
+def test_norm_of_a_weight_that_the_launch_before_writes(overlapping, rows, hidden, quantized):
+    """A weight in the form 1 + w, made by the kernel just ahead, or by a norm whose output it is."""
+    import trismoe_b200 as tm
+
+    g = _gen(rows + hidden)
+    x, r = (torch.randn((rows, hidden), generator=g, device="cuda").half() for _ in range(2))
+    norm = (lambda w: tm.add_rms_norm_e4m3(x, r, w)[0].view(torch.uint8)) if quantized else (lambda w: tm.add_rms_norm(x, r, w)[0])
+    deltas = [torch.randn((hidden,), generator=g, device="cuda").half() for _ in range(20)]
+    one, weight = torch.ones((hidden,), dtype=F16, device="cuda"), torch.zeros((hidden,), dtype=F16, device="cuda")
+    got = []
+    for d in deltas:
+        torch.add(d, 1.0, out=weight)
+        got.append(norm(weight))
+        got.append(norm(tm.add_rms_norm(d, None, one)[0]))
+    torch.cuda.synchronize()
+    for i, d in enumerate(deltas):
+        weight = d + 1.0
+        torch.cuda.synchronize()
+        first = norm(weight)
+        weight = tm.add_rms_norm(d, None, one)[0]
+        torch.cuda.synchronize()
+        assert torch.equal(got[2 * i], first) and torch.equal(got[2 * i + 1], norm(weight))
+
+
+@pytest.mark.parametrize("longest", [60, 20000], ids=["clusters", "numbered"])
+def test_a_chain_of_overlapping_launches_equals_one_that_does_not(overlapping, longest):
+    import trismoe_b200 as tm
+
+    g, lengths, hidden, vocab = _gen(longest), [longest, 1, 17], 512, 4000
+    k_pages, v_pages, table, _ = _filled(g, [n + 30 for n in lengths], 16, 2, 64, F16, LAYOUTS[0])
+    kept = k_pages.clone(), v_pages.clone()
+    cos, sin = (torch.rand((longest + 40, 32), generator=g, device="cuda") for _ in range(2))
+    w, wqkv, head = ((torch.randn(s, generator=g, device="cuda") / 16).half() for s in ((hidden,), (12 * 64, hidden), (vocab, hidden)))
+    start = torch.randn((3, hidden), generator=g, device="cuda").half()
+    tokens = torch.randint(0, vocab, (3, 50), generator=g, device="cuda", dtype=torch.int32)
+    known, penalty = torch.full((3,), 50, dtype=torch.int32, device="cuda"), torch.full((3,), 1.25, device="cuda")
+    places = [torch.tensor([n + step for n in lengths], dtype=torch.int32, device="cuda") for step in range(5)]
+
+    def chain():
+        k_pages.copy_(kept[0])
+        v_pages.copy_(kept[1])
+        x, h, out = start, start, []
+        for at in places:
+            x, h = tm.add_rms_norm(x, h, w)
+            qkv = torch.nn.functional.linear(x, wqkv).view(3, 12, 64)
+            q = tm.append_paged_kv(qkv[:, :8], qkv[:, 8:10], qkv[:, 10:], k_pages, v_pages, table, at, cos=cos, sin=sin)
+            x = tm.paged_decode_attention(q, k_pages, v_pages, table, at + 1).flatten(1)
+            y, h = tm.add_rms_norm(x, h, w)
+            out.append(tm.apply_logit_controls(torch.nn.functional.linear(y, head), tokens=tokens, token_lengths=known, repetition=penalty))
+        return out + [x, h, k_pages.nan_to_num().clone(), v_pages.nan_to_num().clone()]
+
+    on = chain()
+    overlapping.tris_set_programmatic_launch(0)
+    off = chain()
+    assert all(torch.equal(a, b) for a, b in zip(on, off))
