@@ -172,13 +172,22 @@ __global__ void __launch_bounds__(128) paged_kv_append_kernel(const __grid_const
             y[i] = q * cs[i] + p * sn[i];
           }
         } else if (r.interleaved) {
+          // chunks behind the rotated dimensions stay as they are: by a cosine of 1 and a sine of 0 an infinity would spoil its neighbour
+          if (c0 * VEC < r.rotary_dim) {
 #pragma unroll
-          for (int i = 0; i < VEC / 2; ++i) {
-            const float p = x[2 * i], q = x[2 * i + 1], v = y[2 * i], w = y[2 * i + 1];
-            x[2 * i] = p * cs[i] - q * sn[i];
-            x[2 * i + 1] = q * cs[i] + p * sn[i];
-            y[2 * i] = v * cs[VEC / 2 + i] - w * sn[VEC / 2 + i];
-            y[2 * i + 1] = w * cs[VEC / 2 + i] + v * sn[VEC / 2 + i];
+            for (int i = 0; i < VEC / 2; ++i) {
+              const float p = x[2 * i], q = x[2 * i + 1];
+              x[2 * i] = p * cs[i] - q * sn[i];
+              x[2 * i + 1] = q * cs[i] + p * sn[i];
+            }
+          }
+          if (c1 * VEC < r.rotary_dim) {
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+              const float v = y[2 * i], w = y[2 * i + 1];
+              y[2 * i] = v * cs[VEC / 2 + i] - w * sn[VEC / 2 + i];
+              y[2 * i + 1] = w * cs[VEC / 2 + i] + v * sn[VEC / 2 + i];
+            }
           }
         }
       }

@@ -2,6 +2,8 @@
 touch, quotients that end half way between two results, numbers that are not finite, sizes that lead to each variant.
 
 Definitions in 64 bits and the bounds' parts (U, SUB) are those of test_gpu_decode_ops.py; further bounds are derived where they stand."""
+import math
+
 import pytest
 import torch
 
@@ -79,3 +81,30 @@ def test_a_chain_of_overlapping_launches_equals_one_that_does_not(overlapping, l
     overlapping.tris_set_programmatic_launch(0)
     off = chain()
     assert all(torch.equal(a, b) for a, b in zip(on, off))
+
+
+# ---- append ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("extra", [0, 1], ids=["wide", "element by element"])
+@pytest.mark.parametrize("dim,rot", [(64, 16), (128, 120), (48, 4), (80, 0), (256, 8)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_leaves_dimensions_that_do_not_rotate_as_they_are(lib, dim, rot, interleaved, extra):
+    """Infinities, NaN and zeros of both signs beside one another, behind the rotated dimensions."""
+    import trismoe_b200 as tm
+
+    g, tokens = _gen(dim + rot), 9
+    k_pages, v_pages, table, _ = _filled(g, [tokens], 16, 2, dim, F16, LAYOUTS[0])
+    flat = torch.randn((tokens, 8 * dim + extra), generator=g, device="cuda").half()
+    rows = flat[:, extra:].unflatten(1, (8, dim))
+    odd = torch.tensor([math.inf, 1.0, -0.0, -math.inf, math.nan, 2.0, -0.0, -0.0, 3.0, math.inf], device="cuda").half()
+    rows[..., rot:] = odd[(torch.arange(tokens * 8 * (dim - rot), device="cuda") % 10).view(tokens, 8, dim - rot)]
+    cos = sin = None
+    if rot:
+        angle = torch.rand((tokens, rot // 2), generator=g, device="cuda") * 6.0
+        cos, sin = angle.cos(), angle.sin()
+    q, k = tm.append_paged_kv(rows[:, :4], rows[:, 4:6], rows[:, 6:], k_pages, v_pages, table, torch.arange(tokens, device="cuda"),
+                              torch.zeros((tokens,), dtype=torch.int32, device="cuda"), cos=cos, sin=sin, interleaved=interleaved, return_key=True)
+    bits = lambda t: torch.where(t.isnan(), torch.full_like(t, math.nan), t).contiguous().view(torch.int16)
+    held = k_pages[table[0, 0].long(), :tokens]
+    for got, want in ((q, rows[:, :4]), (k, rows[:, 4:6]), (held, rows[:, 4:6])):
+        assert torch.equal(bits(got[..., rot:]), bits(want[..., rot:]))
+        assert bool(torch.isfinite(got[..., :rot]).all())
