@@ -6,6 +6,7 @@ The reference leaves these to stock PyTorch (attention, norms and rotation of it
 modeling_olmoe.py:300-618, 1120-1200; greedy argmax in tools/benchmark_e2e_grid.py:325-420).  All of
 them run on the current stream, allocate only what they return (and scratch), and never synchronise,
 so they can be captured in a CUDA graph.  There is no CPU path: tensors must live on a CUDA device.
+Nor is there a backward pass: where gradients are recorded, inputs that require one are refused.
 
 Pages.  ``k_pages`` and ``v_pages`` are ``[num_pages, page_size, num_kv_heads, head_dim]`` with any
 strides that are multiples of 16 bytes and the head's dimensions side by side; fastest is one where a head's tokens of a page
@@ -32,6 +33,7 @@ _APPEND = struct.Struct("@3Q6q6Q8i")
 _ATTENTION = struct.Struct("@Q2q4Qq3if")
 _NORM = struct.Struct("@6Q4q5if")
 _LOGITS = struct.Struct("@11Q5q6i")
+_NO_GRADIENT = "an input requires a gradient, and there is none: call it under torch.no_grad(), or with detached tensors"
 # (device, sizes) -> a byte seen as many, whose like is the scratch of a call; None where there is none to have
 _scratch: dict = {}
 
@@ -44,9 +46,15 @@ def _same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]
     index = first.get_device()
     if index < 0:
         _native.require_cuda(first, what)
+    grad = torch.is_grad_enabled()
+    if grad and first.requires_grad:
+        _fail(what, _NO_GRADIENT)
     for t in others:
-        if t is not None and t.get_device() != index:
-            _fail(what, "all tensors must live on one CUDA device")
+        if t is not None:
+            if t.get_device() != index:
+                _fail(what, "all tensors must live on one CUDA device")
+            if grad and t.requires_grad:
+                _fail(what, _NO_GRADIENT)
     return first.device
 
 

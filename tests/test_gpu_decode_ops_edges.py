@@ -83,6 +83,29 @@ def test_a_chain_of_overlapping_launches_equals_one_that_does_not(overlapping, l
     assert all(torch.equal(a, b) for a, b in zip(on, off))
 
 
+def test_inputs_that_require_a_gradient_are_refused(lib):
+    """Nothing here has a gradient: a call that would drop one says so."""
+    import trismoe_b200 as tm
+
+    new = lambda *s, dtype=F16: torch.zeros(s, dtype=dtype, device="cuda")
+    asks = lambda *s, dtype=F16: new(*s, dtype=dtype).requires_grad_()
+    i32, f32 = torch.int32, torch.float32
+    table, lens, pos, pages = new(2, 3, dtype=i32), new(2, dtype=i32), new(2, dtype=i32), new(4, 16, 2, 64)
+    q, k = new(2, 4, 64), new(2, 2, 64)
+    calls = [
+        lambda: tm.append_paged_kv(asks(2, 4, 64), k, k, pages, pages, table, pos), lambda: tm.append_paged_kv(q, k, asks(2, 2, 64), pages, pages, table, pos),
+        lambda: tm.paged_decode_attention(asks(2, 4, 64), pages, pages, table, lens), lambda: tm.paged_decode_attention(q, pages, asks(4, 16, 2, 64), table, lens),
+        lambda: tm.add_rms_norm(asks(2, 64), None, new(64)), lambda: tm.add_rms_norm(new(2, 64), None, asks(64)), lambda: tm.add_rms_norm_e4m3(new(2, 64), asks(2, 64), new(64)),
+        lambda: tm.apply_logit_controls(asks(2, 40, dtype=f32)),
+        lambda: tm.apply_logit_controls(new(2, 40, dtype=f32), bias_ids=new(2, 1, dtype=i32), bias_values=asks(2, 1, dtype=f32)),
+    ]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+
+
 # ---- append ---------------------------------------------------------------------------------
 @pytest.mark.parametrize("extra", [0, 1], ids=["wide", "element by element"])
 @pytest.mark.parametrize("dim,rot", [(64, 16), (128, 120), (48, 4), (80, 0), (256, 8)])
