@@ -329,7 +329,9 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
     for (int n = 0; n < NT; ++n) {
       float up = 1.f;
       if constexpr (FP8 && !std::is_same_v<T, __half>) {
-        // bf16 queries against fp16 keys: a power of two brings a row's largest element to [1, 2).  The magnitudes' bits order like the numbers.
+        // bf16 queries against fp16 keys: a power of two brings a row's largest element to [2^14, 2^15), so that elements down to 2^-31 of it keep all
+        // their bits; sums are in 32 bits and keys at most 448.  The magnitudes' bits order like the numbers.
+        constexpr uint32_t kRaise = 14;
         uint32_t top = 0;
 #pragma unroll
         for (int s = 0; s < S::kSteps; ++s)
@@ -337,9 +339,9 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
           for (int i = 0; i < 2; ++i) top = __vmaxu2(top, qf[n][s][i] & 0x7FFF7FFFu);
         top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
         top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        const int e = min(max(max(top & 0xFFFFu, top >> 16) >> 7, 27u), 253u);  // biased exponent; zeros, infinities and NaN stay what they are
-        up = __uint_as_float(static_cast<uint32_t>(e) << 23);
-        const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+        const uint32_t e = min(max(max(top & 0xFFFFu, top >> 16) >> 7, 27u), 253u);  // biased exponent; zeros, infinities and NaN stay what they are
+        up = __uint_as_float((e - kRaise) << 23);
+        const float down = __uint_as_float((254 - e + kRaise) << 23);
 #pragma unroll
         for (int s = 0; s < S::kSteps; ++s)
 #pragma unroll

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_decode_ops import F16, LAYOUTS, _filled, _gen
+from test_gpu_decode_ops import BF16, E4M3, F16, LAYOUTS, _check_attention, _filled, _gen
 
 pytestmark = pytest.mark.gpu
 
@@ -131,3 +131,20 @@ def test_append_leaves_dimensions_that_do_not_rotate_as_they_are(lib, dim, rot, 
     for got, want in ((q, rows[:, :4]), (k, rows[:, 4:6]), (held, rows[:, 4:6])):
         assert torch.equal(bits(got[..., rot:]), bits(want[..., rot:]))
         assert bool(torch.isfinite(got[..., :rot]).all())
+
+
+# ---- attention ------------------------------------------------------------------------------
+@pytest.mark.parametrize("small", [2.0 ** -14, 2.0 ** -20, 2.0 ** -26])
+def test_small_elements_of_a_query_over_8_bit_pages(lib, small):
+    """Keys are zero where the query is large, so the scores are made of what is small in it: no bit of it may be lost beside the large element."""
+    import trismoe_b200 as tm
+
+    g, lengths, dim = _gen(40), [1, 16, 200], 64
+    k_pages, v_pages, table, kept = _filled(g, lengths, 16, 1, dim, E4M3, LAYOUTS[0])
+    for b, n in enumerate(lengths):
+        kept[b][0][..., 0] = 0.0
+        place = torch.arange(n, device="cuda")
+        k_pages[table[b, place // 16].long(), place % 16] = kept[b][0].to(E4M3)
+    q = torch.randn((3, 4, dim), generator=g, device="cuda") * small
+    q[..., 0] = 1.75
+    _check_attention(tm, q.to(BF16), (k_pages, v_pages, table, kept), lengths, softmax_scale=0.25 / small)
