@@ -62,6 +62,31 @@ __device__ __forceinline__ void store_8(__nv_fp8_e4m3* p, const float (&v)[8]) {
   *reinterpret_cast<uint2*>(p) = make_uint2(e4m3_pack4(v[0], v[1], v[2], v[3]), e4m3_pack4(v[4], v[5], v[6], v[7]));
 }
 
+// x / s of many x by one s, rounded to 32 bits as a division rounds it (but for quotients within some 2^-46 of half way between two numbers, none
+// of which is one): the reciprocal in two parts, two instructions an element where a division takes some ten.  Scales for which the parts are not exact, and
+// infinite elements, which have no sum of two products, are divided.  (Prompts of 8188 tokens, 48 heads of 128, to e4m3: 33.4 us, 41.3 with a division for
+// all; 31.6 by the reciprocal alone, which is one step of e4m3 off where it falls on the other side of half way.)
+struct DivideBy {
+  float s, hi, lo;
+  bool parts;
+  __device__ __forceinline__ explicit DivideBy(float scale) : s(scale), hi(1.f / scale), parts(fabsf(scale) >= 0x1p-80f && fabsf(scale) <= 0x1p80f) {
+    lo = fmaf(-hi, scale, 1.f) * hi;
+  }
+  template <int N>
+  __device__ __forceinline__ void operator()(float (&x)[N]) const {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(x[i]));
+    if (parts && top < INFINITY) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = fmaf(x[i], hi, x[i] * lo);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] /= s;
+    }
+  }
+};
+
 // launch_kernel, by the plain launch where nothing else is asked for: 0.6 us less of the host's time (2.8 against 3.4).
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_step(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl, int cluster_z, Args&&... args) {

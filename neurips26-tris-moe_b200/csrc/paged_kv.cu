@@ -200,11 +200,9 @@ __global__ void __launch_bounds__(128) paged_kv_append_kernel(const __grid_const
         C* dst = kind == 1 ? static_cast<C*>(c.k_pages) + k_at + hh * c.k_head_stride : static_cast<C*>(c.v_pages) + v_at + hh * c.v_head_stride;
         const float* scales = kind == 1 ? c.k_scale : c.v_scale;
         if (sizeof(C) == 1 && scales) {
-          const float s = scales[hh];
-          // the reciprocal may be one rounding off the quotient, which e4m3's four bits seldom show
-          const float up = 1.f / s;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) x[i] *= up, y[i] *= up;
+          const DivideBy divide(scales[hh]);
+          divide(x);
+          divide(y);
         }
         store_vec<VEC>(dst + c0 * VEC, x);
         if (c1 >= 0) store_vec<VEC>(dst + c1 * VEC, y);

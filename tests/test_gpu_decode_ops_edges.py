@@ -133,6 +133,60 @@ def test_append_leaves_dimensions_that_do_not_rotate_as_they_are(lib, dim, rot, 
         assert bool(torch.isfinite(got[..., :rot]).all())
 
 
+@pytest.mark.parametrize("extra", [0, 1], ids=["wide", "element by element"])
+@pytest.mark.parametrize("rows,odd", [(F16, 7), (F16, 63), (BF16, 7)], ids=["fp16 7", "fp16 63", "bf16 7"])
+def test_append_to_8_bits_rounds_the_quotient(lib, rows, odd, extra):
+    """Half way between two e4m3 values the result is the even one.  x / scale is exact there, x * (1 / scale) need not be."""
+    import trismoe_b200 as tm
+
+    half_way = (torch.arange(16, 32, device="cuda") / 16.0).repeat(4) * torch.tensor([1.0, -1.0, 16.0, -8.0], device="cuda").repeat_interleave(16)
+    scale = torch.tensor([odd / 64.0, 1.0], device="cuda")
+    flat = torch.zeros((1, 2 * 64 + extra), dtype=rows, device="cuda")
+    x = flat[:, extra:].view(1, 2, 64)
+    x.copy_((half_way * scale[:, None])[None])
+    assert torch.equal(x[0].double() / scale.double()[:, None], half_way.double().expand(2, 64))
+    pages = [torch.zeros((1, 2, 16, 64), dtype=E4M3, device="cuda").transpose(1, 2) for _ in range(2)]
+    table, zero = torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.zeros((1,), dtype=torch.int32, device="cuda")
+    tm.append_paged_kv(None, x, x, *pages, table, zero, k_scale=scale, v_scale=scale)
+    for p in pages:
+        assert torch.equal(p[0, 0].float(), half_way.to(E4M3).float().expand(2, 64))
+
+
+def test_append_to_8_bits_with_a_scale_whose_reciprocal_overflows(lib):
+    import trismoe_b200 as tm
+
+    x = torch.tensor([0.0, -0.0, 1.0, -2.0 ** -24] * 16, device="cuda").half().view(1, 1, 64)
+    pages = [torch.ones((1, 1, 16, 64), dtype=F16, device="cuda").to(E4M3).transpose(1, 2) for _ in range(2)]
+    table, zero = torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.zeros((1,), dtype=torch.int32, device="cuda")
+    scale = torch.full((1,), 2.0 ** -140, device="cuda")
+    tm.append_paged_kv(None, x, x, *pages, table, zero, k_scale=scale, v_scale=scale)
+    for p in pages:
+        assert torch.equal(p[0, 0, 0].float(), torch.tensor([0.0, -0.0, 448.0, -448.0] * 16, device="cuda"))
+
+
+@pytest.mark.parametrize("rows", [F16, BF16], ids=["fp16", "bf16"])
+def test_append_to_8_bits_divides_numbers_of_any_size(lib, rows):
+    """Bit for bit the quotient in 32 bits, saturated and rounded: scales from 2^-149 to 2^127, and rows with everything that is not finite."""
+    import trismoe_b200 as tm
+
+    g = _gen(49)
+    scale = torch.cat([2.0 ** torch.arange(-149.0, 128.0, 4.0, dtype=torch.float64), 2.0 ** torch.tensor([-81.0, -80.0, 80.0, 81.0]).double()]).float().cuda()
+    scale = scale * (1.0 + torch.rand(scale.shape, generator=g, device="cuda")).clamp(max=1.99)
+    heads, tokens, dim = scale.numel(), 64, 128
+    x = torch.randn((tokens, heads, dim), generator=g, device="cuda") * 10.0
+    x[1::2] *= scale.clamp(1e-6, 1e6)[:, None]
+    x[::2] *= 2.0 ** torch.randint(-40, 40, (tokens // 2, heads, dim), generator=g, device="cuda").float()
+    x[5, :, :6] = torch.tensor([math.inf, -math.inf, math.nan, 0.0, -0.0, 65504.0], device="cuda")
+    x = x.to(rows)
+    pages = [torch.zeros((4, heads, 16, dim), dtype=E4M3, device="cuda").transpose(1, 2) for _ in range(2)]
+    table, zero = torch.arange(4, dtype=torch.int32, device="cuda")[None], torch.zeros((tokens,), dtype=torch.int32, device="cuda")
+    tm.append_paged_kv(None, x, x, *pages, table, torch.arange(tokens, device="cuda"), zero, k_scale=scale, v_scale=scale)
+    want = (x.float() / scale[:, None]).clamp(-448.0, 448.0).to(E4M3).float()
+    for p in pages:
+        got = p.reshape(tokens, heads, dim).float()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
 # ---- attention ------------------------------------------------------------------------------
 @pytest.mark.parametrize("small", [2.0 ** -14, 2.0 ** -20, 2.0 ** -26])
 def test_small_elements_of_a_query_over_8_bit_pages(lib, small):
