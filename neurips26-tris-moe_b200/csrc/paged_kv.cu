@@ -201,8 +201,11 @@ __global__ void __launch_bounds__(128) paged_kv_append_kernel(const __grid_const
         const float* scales = kind == 1 ? c.k_scale : c.v_scale;
         if (sizeof(C) == 1 && scales) {
           const DivideBy divide(scales[hh]);
-          divide(x);
-          divide(y);
+          float top = 0.f;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) top = fmaxf(top, fmaxf(fabsf(x[i]), fabsf(y[i])));
+          divide(x, top);
+          divide(y, top);
         }
         store_vec<VEC>(dst + c0 * VEC, x);
         if (c1 >= 0) store_vec<VEC>(dst + c1 * VEC, y);

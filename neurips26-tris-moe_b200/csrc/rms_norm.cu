@@ -3,7 +3,7 @@
 // h = residual + x; y = h * w / sqrt(mean(h^2) + eps).  The mean needs the whole row before the first output, so a row stays in the registers of
 // the CTA that reads it: x and residual are read once, h and y written once.  Bound by bytes for many rows, by the chain load -> sum -> store for one.
 // CTAs take several rows, evenly, and ask for the next row before they add up the one they have; the weights stay in registers.
-// 2047 x 4096 bf16 to e4m3 with a scale for 128 columns: 12.4 us, 9.0 of them its 59 MB at the rate of a copy; in bf16 10.0 us (67 MB).
+// 2047 x 4096 bf16 to e4m3 with a scale for 128 columns: 12.9 us, 9.0 of them its 59 MB at the rate of a copy; in bf16 10.0 us (67 MB).
 // The sums are fp32, h is not rounded before it is squared or scaled.  e4m3: y / s with s = max |y| / 448 of the group, so the group's largest
 // element is representable and none saturates; a second exchange between threads gives the maxima.
 #include "decode_step.cuh"
@@ -13,6 +13,9 @@ namespace {
 
 constexpr int kMaxVectors = 4;  // of 8 columns that a thread keeps
 constexpr int most_threads(int vectors) { return vectors >= 4 ? 512 : 1024; }  // whose rows fit the registers
+// With two registers more for one vector a thread, an SM would have four CTAs of 256 in place of five (2047 x 2048 to e4m3: 8.1 us, 7.2 so).
+constexpr int registers(int vectors) { return vectors >= 4 ? 128 : vectors == 2 ? 64 : 48; }
+constexpr int threads_on_sm(int vectors) { return 65536 / registers(vectors) / 256 * 256; }
 
 struct NormArgs {
   TrisAddRmsNorm a;
@@ -33,12 +36,6 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
   return v;
 }
-// 1 / v to a rounding.
-__device__ __forceinline__ float reciprocal(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 // Magnitudes as bits: they order like the numbers, and a NaN is the largest.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
@@ -47,6 +44,21 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
   __syncthreads();
   const int lane = threadIdx.x & 31;
   return __reduce_max_sync(0xFFFFFFFFu, lane < static_cast<int>(blockDim.x >> 5) ? red[lane] : 0);
+}
+// A vector of a group whose largest magnitude has these bits, in place, by the group's scale, and that.  Two-part reciprocals of 448 and of the scale give
+// both quotients as divisions round them, at nine instructions a vector and one an element; a scale of 0 has nothing but zeros.
+__device__ __forceinline__ float quantize_8(float (&y)[8], uint32_t top) {
+  constexpr float hi = 1.f / kE4m3Max, lo = static_cast<float>(1.0 / kE4m3Max - hi);
+  constexpr uint32_t least = 67u << 23, most = 187u << 23;  // 2^-60 and 2^60
+  const float largest = __uint_as_float(top);
+  if (top - least <= most - least) {
+    const float scale = fmaf(largest, hi, largest * lo), up = reciprocal(scale);
+    DivideBy::by_parts(y, up, DivideBy::second_part(up, scale));
+    return scale;
+  }
+  const float scale = largest / kE4m3Max;
+  if (scale != 0.f) DivideBy{scale}(y, largest);
+  return scale;
 }
 template <typename T>
 __device__ __forceinline__ void unpack_8(const uint4& raw, float (&v)[8]) {
@@ -60,7 +72,7 @@ __device__ __forceinline__ void unpack_8(const uint4& raw, float (&v)[8]) {
 
 // Rows of at most 8 * VECS * blockDim columns, all pointers and strides at 16-byte boundaries.
 template <typename T, bool FP8, int VECS>
-__global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const __grid_constant__ NormArgs args) {
+__global__ void __maxnreg__(registers(VECS)) add_rms_norm_kernel(const __grid_constant__ NormArgs args) {
   const TrisAddRmsNorm& a = args.a;
   __shared__ float red[2][32];
   __shared__ uint32_t red_max[2][32];
@@ -172,17 +184,7 @@ __global__ void __launch_bounds__(most_threads(VECS)) add_rms_norm_kernel(const 
       for (int i = 0; i < VECS; ++i) {
         const int v = tid + i * blockDim.x;
         if (v < vectors) {
-          // times reciprocals, of 448 and of the scale: at most two roundings off the quotients, which e4m3's four bits seldom show.  Of a subnormal
-          // scale the reciprocal overflows, so values and scale are raised first; a scale of 0 has nothing but zeros
-          const float scale = __uint_as_float(top[i]) * (1.f / kE4m3Max);
-          float times = scale == 0.f ? 0.f : reciprocal(scale);
-          if (scale < 1.2e-38f && scale != 0.f) {
-            times = reciprocal(scale * 1.8446744e19f);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) h[i][k] *= 1.8446744e19f;
-          }
-#pragma unroll
-          for (int k = 0; k < 8; ++k) h[i][k] *= times;
+          const float scale = quantize_8(h[i], top[i]);
           store_8(static_cast<__nv_fp8_e4m3*>(a.y) + row * a.y_stride + 8 * v, h[i]);
           if (args.group_shift >= 0) {
             if ((v & (per_group - 1)) == 0) a.scales[row * args.groups + (v >> args.group_shift)] = scale;
@@ -259,7 +261,7 @@ int launch_norm(const TrisAddRmsNorm& a, cudaStream_t stream) {
     if (a.group_size == 8 << shift) args.group_shift = shift;
   const size_t smem = FP8 && a.group_size != H && args.group_shift < 0 ? sizeof(float) * vectors : 0;
   auto kernel = vecs == 1 ? add_rms_norm_kernel<T, FP8, 1> : vecs == 2 ? add_rms_norm_kernel<T, FP8, 2> : add_rms_norm_kernel<T, FP8, 4>;
-  const int resident = 148 * (vecs == 1 ? 1280 : vecs == 2 ? 1024 : 512) / threads;  // by registers
+  const int resident = 148 * threads_on_sm(vecs) / threads;
   const int turns = ceil_div(a.rows, resident < 1 ? 1 : resident);
   TRIS_CUDA(launch_step(kernel, dim3(ceil_div(a.rows, turns)), dim3(threads), smem, stream, pdl, 1, args));
   return TRIS_OK;

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_decode_ops import BF16, E4M3, F16, LAYOUTS, _check_attention, _filled, _gen
+from test_gpu_decode_ops import BF16, E4M3, F16, LAYOUTS, SUB, U, _check_attention, _filled, _gen
 
 pytestmark = pytest.mark.gpu
 
@@ -202,3 +202,43 @@ def test_small_elements_of_a_query_over_8_bit_pages(lib, small):
     q = torch.randn((3, 4, dim), generator=g, device="cuda") * small
     q[..., 0] = 1.75
     _check_attention(tm, q.to(BF16), (k_pages, v_pages, table, kept), lengths, softmax_scale=0.25 / small)
+
+
+# ---- norm -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("extra", [0, 1], ids=["wide", "element by element"])
+@pytest.mark.parametrize("dtype,odd", [(F16, 7), (F16, 63), (BF16, 7)], ids=["fp16 7", "fp16 63", "bf16 7"])
+@pytest.mark.parametrize("group", [0, 32, 96])
+def test_norm_to_8_bits_rounds_the_quotients(lib, dtype, odd, group, extra):
+    """Rows of +-1 have a mean square of 1, so with eps 0 y is the weight; weights half way between two e4m3 values times the scale."""
+    import trismoe_b200 as tm
+
+    scale = odd / 64.0
+    part = torch.cat([torch.tensor([448.0], device="cuda"), torch.arange(16, 32, device="cuda") / 16.0, torch.arange(17, 32, device="cuda") / 2.0])
+    values = part.repeat(9)  # 288 columns, every 32 of them with the largest
+    w = (values * scale).to(dtype)
+    assert torch.equal(w.double(), values.double() * scale)
+    sign = torch.where(torch.rand((5, 288), generator=_gen(45), device="cuda") < 0.5, -1.0, 1.0)
+    x = torch.empty((5, 288 + extra), dtype=dtype, device="cuda")[:, extra:]
+    x.copy_(sign)
+    got, scales, _ = tm.add_rms_norm_e4m3(x, None, w, 0.0, group_size=group)
+    assert bool((scales == scale).all())
+    assert torch.equal(got.float(), sign * values.to(E4M3).float())
+
+
+@pytest.mark.parametrize("size", [2.0 ** -130, 2.0 ** -126, 2.0 ** -100, 2.0 ** -60, 1.0, 2.0 ** 60, 2.0 ** 120])
+def test_norm_to_8_bits_over_the_range_of_scales(lib, size):
+    """bf16 weights of any size: values are right to a rounding to e4m3, scales to a rounding to fp32 (of a subnormal scale: to 2^-149)."""
+    import trismoe_b200 as tm
+
+    w = (torch.randn((512,), generator=_gen(46), device="cuda").double() * size).to(BF16)
+    x = torch.ones((2, 512), dtype=BF16, device="cuda")
+    values, scales, _ = tm.add_rms_norm_e4m3(x, None, w, 0.0, group_size=128)
+    want = w.double().abs().view(4, 128).amax(1) / 448.0
+    assert float(((scales.double() - want).abs() - 2.0 ** -22 * want - 2.0 ** -149).max()) <= 0
+    part, back = w.double().view(4, 128), values.double().view(2, 4, 128)
+    # of a scale of few bits the quotient by the scale as it is stored
+    quotient = part / scales.double()[..., None]
+    bound = (U[E4M3] + 2.0 ** -20) * quotient.abs().clamp(max=480.0) + SUB[E4M3]
+    held = scales.double()[..., None] > 2.0 ** -140
+    assert float((((back - quotient.clamp(-448.0, 448.0)).abs() - bound) * held).max()) <= 0
+    assert bool(torch.isfinite(back).all())
