@@ -242,3 +242,29 @@ def test_norm_to_8_bits_over_the_range_of_scales(lib, size):
     held = scales.double()[..., None] > 2.0 ** -140
     assert float((((back - quotient.clamp(-448.0, 448.0)).abs() - bound) * held).max()) <= 0
     assert bool(torch.isfinite(back).all())
+
+
+# ---- logits ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,vocab", [(2, 4000), (40, 50304)], ids=["small slices", "large slices"])
+def test_repetition_divides(lib, rows, vocab):
+    """Positive logits are the quotients to the last bit."""
+    import trismoe_b200 as tm
+
+    logits = 1.0 + torch.randint(0, 2000, (rows, vocab), generator=_gen(60), device="cuda").float()
+    repetition = 1.0 + torch.arange(rows, device="cuda") * 2.0 + 46.0
+    tokens = torch.arange(vocab, dtype=torch.int32, device="cuda").expand(rows, vocab).contiguous()
+    lengths = torch.full((rows,), vocab, dtype=torch.int32, device="cuda")
+    out = tm.apply_logit_controls(logits, tokens=tokens, token_lengths=lengths, repetition=repetition)
+    assert torch.equal(out, (logits.double() / repetition.double()[:, None]).float())
+    out = tm.apply_logit_controls(-logits, tokens=tokens, token_lengths=lengths, repetition=repetition)
+    assert torch.equal(out, -logits * repetition[:, None])
+
+
+def test_repetition_whose_reciprocal_is_not_finite(lib):
+    import trismoe_b200 as tm
+
+    logits = torch.tensor([[2.0 ** -100, -1.0, 2.0 ** -140, 0.0]], device="cuda")
+    tokens = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    out = tm.apply_logit_controls(logits, tokens=tokens, token_lengths=torch.full((1,), 4, dtype=torch.int32, device="cuda"),
+                                  repetition=torch.full((1,), 2.0 ** -130, device="cuda"))
+    assert torch.equal(out, torch.tensor([[2.0 ** 30, -(2.0 ** -130), 2.0 ** -10, 0.0]], device="cuda"))
