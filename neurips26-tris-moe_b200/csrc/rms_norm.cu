@@ -36,6 +36,12 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
   return v;
 }
+// The larger magnitude, or NaN where there is one.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float m;
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
 // Magnitudes as bits: they order like the numbers, and a NaN is the largest.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
@@ -135,13 +141,9 @@ __global__ void __maxnreg__(registers(VECS)) add_rms_norm_kernel(const __grid_co
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         h[i][k] = h[i][k] * inv * f[k];
-        if (FP8) most = fmaxf(most, fabsf(h[i][k]));
+        if (FP8) most = max_or_nan(most, h[i][k]);
       }
-      top[i] = __float_as_uint(most);
-      if (FP8 && !(sum < INFINITY)) {  // something is not finite: fmaxf drops a NaN
-#pragma unroll
-        for (int k = 0; k < 8; ++k) top[i] = max(top[i], magnitude(h[i][k]));
-      }
+      top[i] = magnitude(most);
     }
     if constexpr (!FP8) {
 #pragma unroll

@@ -244,6 +244,33 @@ def test_norm_to_8_bits_over_the_range_of_scales(lib, size):
     assert bool(torch.isfinite(back).all())
 
 
+@pytest.mark.parametrize("group", [0, 16, 48, 96])
+def test_norm_to_8_bits_of_what_is_not_a_number(lib, group):
+    """A NaN makes its group's scale one, wherever it comes from - a weight, an infinite weight on zero, a row of zeros without eps, a negative eps -,
+    in both kernels."""
+    import trismoe_b200 as tm
+
+    g = _gen(44)
+    x = torch.randn((4, 288), generator=g, device="cuda").half()
+    x[1] = 0.0
+    x[2, 100] = 0.0
+    off = torch.empty((4, 289), dtype=F16, device="cuda")[:, 1:]  # element by element
+    off.copy_(x)
+    w = torch.ones((288,), dtype=F16, device="cuda")
+    for place, weight, eps in ((5, math.nan, 1e-5), (100, math.inf, 1e-5), (100, -math.inf, 1e-5), (0, 1.0, 0.0), (0, 1.0, -1e3)):
+        w.fill_(1.0)
+        w[place] = weight
+        h = x.double()
+        y = h / (h.square().mean(-1, keepdim=True) + eps).sqrt() * w.double()
+        want = y.view(4, -1, group or 288).abs().amax(-1) / 448.0
+        assert bool(want.isnan().any())
+        for rows in (x, off):
+            values, scales, _ = tm.add_rms_norm_e4m3(rows, None, w, eps, group_size=group)
+            assert torch.equal(scales.isnan(), want.isnan())
+            assert torch.equal(scales.isinf(), want.isinf())
+            assert bool(values.float().isnan()[y.isnan()].all())
+
+
 # ---- logits ---------------------------------------------------------------------------------
 @pytest.mark.parametrize("rows,vocab", [(2, 4000), (40, 50304)], ids=["small slices", "large slices"])
 def test_repetition_divides(lib, rows, vocab):
