@@ -14,10 +14,10 @@
 // shared memory or, of numbered blocks, by a second kernel from the workspace (at most two a CTA).
 //
 // One warp's step.  S^T = K Q^T and O^T = V^T P^T by mma.sync m16n8k16: the cached rows are the 16-row operand and the query heads of a group the
-// 8 columns, so that a step of 16 tokens costs two MMAs per 16 dimensions with up to 8 heads (with the heads as rows it would cost four, half
-// of them zeros).  No operand goes through a transposing load: the order of dimensions inside a product is free as long as both operands have the
+// 8 columns, so that a step of 16 tokens costs three MMAs per 16 dimensions with up to 8 heads - one for the scores, two for the two parts of a
+// weight - (with the heads as rows it would cost six, half of them zeros).  No operand goes through a transposing load: the order of dimensions inside a product is free as long as both operands have the
 // same, so a lane's 16 bytes of a key row are its fragments as they are; of four value rows a lane has the same 8 dimensions, whose pairs of
-// tokens are put together by PRMT.  A step's MMAs take a tenth of the time its bytes take (heads of 128: 16 at two cycles of an SM, 8 KB at 23 bytes a
+// tokens are put together by PRMT.  A step's MMAs take a seventh of the time its bytes take (heads of 128: 24 at two cycles of an SM, 8 KB at 23 bytes a
 // cycle), so nothing waits for the tensor pipe; tcgen05 tiles have 128 rows and their second operand in shared memory.  Each warp has a ring of its
 // own in shared memory, filled by cp.async, and meets no other warp before it is done.
 #include <type_traits>
@@ -75,6 +75,26 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two weights as sums of two 16-bit numbers: off by 2^-16 (bf16) or 2^-21 (fp16) of a weight, where one number is off by 2^-9 or 2^-12 - as much as the
+// result's own rounding, but for results in bf16 over 8-bit pages, whose weights are single fp16 numbers.  (One number and two, us: 32 x 512-768 34.8 and 35.3,
+// 1 x 131071 94.3 and 94.5, 64 x 1-16384 287.5 and 288.0, 8 x 8192 of fp16 queries over 8 bits 53.1 and 55.4; 64 x 1-16384 of bf16 over 8 bits 153.4, with two 162.)
+// Neither number is zero or negative, so that an infinite value gives an infinity and not NaN: the first is rounded from a little less than the weight.
+// (In fp16 that ends with weights of 2^-23, 2^-30 of the largest, whose first number is zero.)
+template <typename M>
+__device__ __forceinline__ void two_parts(float a, float b, uint32_t& most, uint32_t& rest) {
+  if constexpr (std::is_same_v<M, __half>) {
+    constexpr float kLess = 1.f - 0x1p-10f, kTiny = -0x1p-23f;
+    most = Pair<M>::pack(fmaxf(fmaf(a, kLess, kTiny), 0.f), fmaxf(fmaf(b, kLess, kTiny), 0.f));
+    const float2 f = Pair<M>::unpack(most);
+    rest = Pair<M>::pack(a - f.x, b - f.y);
+  } else {
+    constexpr float kLess = 1.f - 0x1p-12f;
+    const uint32_t x = __float_as_uint(a * kLess), y = __float_as_uint(b * kLess);
+    most = prmt(x, y, 0x7632);  // rounded towards zero
+    rest = Pair<M>::pack(a - __uint_as_float(x & 0xFFFF0000u), b - __uint_as_float(y & 0xFFFF0000u));
+  }
 }
 
 constexpr int kMostCluster = 8;
@@ -222,6 +242,7 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
   constexpr int kElt = FP8 ? 1 : 2;
   // Range of the weights, to base 2.  bf16 ones are not lifted: they lose nothing below 1, and values may go up to the end of 32 bits themselves.
   constexpr float kLift = std::is_same_v<M, __half> ? 7.f : 0.f, kMostWeight = kLift + 8.f;
+  constexpr bool kTwoParts = !FP8 || std::is_same_v<T, __half>;  // of a weight
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Piece pieces[2 * W];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -597,17 +618,25 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
         }
       }
     }
-    // The weights as the 8-column operand: pairs of tokens of one head.  Rounded to the values' type, as 16-bit operands are: 2^-8 (bf16) or
-    // 2^-11 (fp16) of a weight at most, independent from token to token; the sum l is of the weights before that, so that lse is exact to fp32.
-    uint32_t p[NT][2];
+    // The weights as the 8-column operand: pairs of tokens of one head, each weight a 16-bit number or the sum of two (two_parts), whose products with the
+    // values add up in the same accumulators.  The sum l is of the weights as they are.
+    uint32_t p[NT][2], rest[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[n][k] = exp2_fast(x[n][k]);
       l[n][0] += x[n][0] + x[n][2];
       l[n][1] += x[n][1] + x[n][3];
-      p[n][0] = transpose_8x8(Pair<M>::pack(x[n][0], x[n][1]));
-      p[n][1] = transpose_8x8(Pair<M>::pack(x[n][2], x[n][3]));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if constexpr (kTwoParts) {
+          two_parts<M>(x[n][2 * k], x[n][2 * k + 1], p[n][k], rest[n][k]);
+          rest[n][k] = transpose_8x8(rest[n][k]);
+        } else {
+          p[n][k] = Pair<M>::pack(x[n][2 * k], x[n][2 * k + 1]);
+        }
+        p[n][k] = transpose_8x8(p[n][k]);
+      }
     }
 
     const uint8_t* vals = src + v_from;
@@ -636,13 +665,19 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
             const uint32_t u0 = e ? hi0 : lo0, u1 = e ? hi1 : lo1;
             const uint32_t a0 = e4m3_to_h2(u0 & 0xFFFF), a1 = e4m3_to_h2(u0 >> 16), a2 = e4m3_to_h2(u1 & 0xFFFF), a3 = e4m3_to_h2(u1 >> 16);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_16x8x16<M>(acc[j * (S::kValueElems / 2) + 2 * w + e][n], a0, a1, a2, a3, p[n][0], p[n][1]);
+            for (int n = 0; n < NT; ++n) {
+              mma_16x8x16<M>(acc[j * (S::kValueElems / 2) + 2 * w + e][n], a0, a1, a2, a3, p[n][0], p[n][1]);
+              if constexpr (kTwoParts) mma_16x8x16<M>(acc[j * (S::kValueElems / 2) + 2 * w + e][n], a0, a1, a2, a3, rest[n][0], rest[n][1]);
+            }
           }
         } else {
           const uint32_t a0 = prmt(v[0][w], v[1][w], 0x5410), a1 = prmt(v[0][w], v[1][w], 0x7632);
           const uint32_t a2 = prmt(v[2][w], v[3][w], 0x5410), a3 = prmt(v[2][w], v[3][w], 0x7632);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_16x8x16<M>(acc[j * 4 + w][n], a0, a1, a2, a3, p[n][0], p[n][1]);
+          for (int n = 0; n < NT; ++n) {
+            mma_16x8x16<M>(acc[j * 4 + w][n], a0, a1, a2, a3, p[n][0], p[n][1]);
+            if constexpr (kTwoParts) mma_16x8x16<M>(acc[j * 4 + w][n], a0, a1, a2, a3, rest[n][0], rest[n][1]);
+          }
         }
       }
     }

@@ -3,7 +3,7 @@
 // h = residual + x; y = h * w / sqrt(mean(h^2) + eps).  The mean needs the whole row before the first output, so a row stays in the registers of
 // the CTA that reads it: x and residual are read once, h and y written once.  Bound by bytes for many rows, by the chain load -> sum -> store for one.
 // CTAs take several rows, evenly, and ask for the next row before they add up the one they have; the weights stay in registers.
-// 2047 x 4096 bf16 to e4m3 with a scale for 128 columns: 12.9 us, 9.0 of them its 59 MB at the rate of a copy; in bf16 10.0 us (67 MB).
+// 2047 x 4096 bf16 to e4m3 with a scale for 128 columns: 12.7 us, 9.0 of them its 59 MB at the rate of a copy; in bf16 10.0 us (67 MB).
 // The sums are fp32, h is not rounded before it is squared or scaled.  e4m3: y / s with s = max |y| / 448 of the group, so the group's largest
 // element is representable and none saturates; a second exchange between threads gives the maxima.
 #include "decode_step.cuh"

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_decode_ops import BF16, E4M3, F16, LAYOUTS, SUB, U, _check_attention, _filled, _gen
+from test_gpu_decode_ops import BF16, E4M3, F16, LAYOUTS, SUB, U, _attend_64, _check_attention, _filled, _gen
 
 pytestmark = pytest.mark.gpu
 
@@ -202,6 +202,58 @@ def test_small_elements_of_a_query_over_8_bit_pages(lib, small):
     q = torch.randn((3, 4, dim), generator=g, device="cuda") * small
     q[..., 0] = 1.75
     _check_attention(tm, q.to(BF16), (k_pages, v_pages, table, kept), lengths, softmax_scale=0.25 / small)
+
+
+@pytest.mark.parametrize("rows,cache", [(F16, F16), (BF16, BF16), (F16, E4M3), (BF16, E4M3)], ids=lambda v: str(v).replace("torch.", ""))
+@pytest.mark.parametrize("lengths", [[3, 2, 5, 64], [700, 1000], [20000]], ids=["short", "clusters", "numbered"])
+def test_attention_keeps_more_of_a_weight_than_16_bits(lib, rows, cache, lengths):
+    """Values of +-1 that cancel: the result is small beside the sum of magnitudes, so a rounding of the weights would show.
+    Weights have the error of their scores (at most 2^-17: sums of 64 products in 32 bits) and of two roundings to 8 bits (2^-16) at most; of one to 11 bits (2^-12) in addition
+    where the result is in bf16, whose own rounding is eight times as large, and pages are in 8 bits."""
+    import trismoe_b200 as tm
+
+    g, heads, dim = _gen(41), 8, 64
+    k_pages, v_pages, table, kept = _filled(g, lengths, 16, 2, dim, cache, LAYOUTS[0])
+    for b, n in enumerate(lengths):
+        kept[b][1].sign_()
+        place = torch.arange(n, device="cuda")
+        v_pages[table[b, place // 16].long(), place % 16] = kept[b][1].to(cache)
+    q = torch.randn((len(lengths), heads, dim), generator=g, device="cuda").to(rows)
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out = tm.paged_decode_attention(q, k_pages, v_pages, table, lens)
+    want, _, mag = _attend_64(q, kept, 0, dim ** -0.5, None, None)
+    bound = (2.0 ** -15 + (2.0 ** -12 if rows == BF16 and cache == E4M3 else 0.0)) * mag + U[rows] * want.abs() + SUB[rows]
+    assert float(((out.double() - want).abs() - bound).max()) <= 0
+
+
+@pytest.mark.parametrize("rows,cache", [(F16, F16), (BF16, BF16), (BF16, E4M3)], ids=lambda v: str(v).replace("torch.", ""))
+@pytest.mark.parametrize("lengths", [[1, 2, 64, 700], [20000]], ids=["clusters", "numbered"])
+def test_an_infinite_value_gives_an_infinity_whatever_its_weight(lib, rows, cache, lengths):
+    """Weights that are a power of two, or a number of 16 bits, exactly, and others; what has no infinity stands in with e4m3's largest number."""
+    import trismoe_b200 as tm
+
+    g, heads, dim, n = _gen(51), 4, 64, len(lengths)
+    k_pages, v_pages, table, kept = _filled(g, lengths, 16, 1, dim, cache, LAYOUTS[0], scale=0.5)
+    q = torch.randn((n, heads, dim), generator=g, device="cuda").to(rows)
+    q[:, 0] = 0.0  # equal weights
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    if cache == E4M3:
+        v_pages.copy_(torch.full_like(v_pages, 448.0, dtype=torch.float32))
+        out = tm.paged_decode_attention(q, k_pages, v_pages, table, lens)
+        assert float((out.double() - 448.0).abs().max()) <= 2.0 ** -8 * 448.0
+        return
+    for b, length in enumerate(lengths):
+        for i, sign in ((0, 1.0), (length // 2, -1.0), (length - 1, 1.0)):
+            v_pages[table[b, i // 16].long(), i % 16, 0, 3 * i % 61] = sign * math.inf
+    out = tm.paged_decode_attention(q, k_pages, v_pages, table, lens)
+    for b, length in enumerate(lengths):
+        want = torch.zeros((dim,), device="cuda", dtype=torch.float64)
+        for i in (0, length // 2, length - 1):
+            want[3 * i % 61] += v_pages[table[b, i // 16].long(), i % 16, 0, 3 * i % 61].double()
+        odd = ~torch.isfinite(want)
+        assert bool(odd.any()) and bool(torch.isfinite(out[b][:, ~odd]).all())
+        for h in range(heads):
+            assert torch.equal(out[b, h][odd].double().nan_to_num(nan=7.0), want[odd].nan_to_num(nan=7.0))
 
 
 # ---- norm -----------------------------------------------------------------------------------
