@@ -767,7 +767,7 @@ typedef struct TrisPagedKv {
 
 /*
  * New tokens of a projection: row t of q / k / v has its heads of head_dim elements head_stride apart.  Token t belongs to sequence
- * sequences[t] (NULL: t) and stands at positions[t]; a negative position is padding: nothing is written to the cache, its rows of q_out
+ * sequences[t] (NULL: t; num_tokens is at most num_sequences then) and stands at positions[t]; a negative position is padding: nothing is written to the cache, its rows of q_out
  * and k_out are zeros.  The first rotary_dim dimensions of q and k are rotated by the position's row of cos / sin
  * [max_positions, rotary_dim / 2] - pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved - in fp32 and rounded once.
  */

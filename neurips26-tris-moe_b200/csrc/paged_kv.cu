@@ -259,6 +259,7 @@ extern "C" int tris_paged_kv_append(const TrisPagedKv* cache, const TrisPagedApp
   a.head_groups = heads;
   while (a.head_groups > 1 && static_cast<int64_t>(a.units) * a.head_groups * r.num_tokens > 2 * 148 * 640) a.head_groups = ceil_div(a.head_groups, 2);
   TRIS_REQUIRE(static_cast<int64_t>(a.units) * a.head_groups * r.num_tokens < (1ll << 31), TRIS_ERR_UNSUPPORTED, "paged_kv_append: too many tokens in one call");
+  TRIS_REQUIRE(r.sequences || r.num_tokens <= c.num_sequences, TRIS_ERR_INVALID_ARG, "paged_kv_append: %d tokens without sequences for a block table of %d", r.num_tokens, c.num_sequences);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool f16 = r.dtype == TRIS_DTYPE_F16, q8 = c.dtype == TRIS_DTYPE_E4M3;
   if (wide) {

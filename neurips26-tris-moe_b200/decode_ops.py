@@ -133,14 +133,14 @@ def append_paged_kv(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     """Rotates queries and keys by their positions and writes keys and values to the cache.
 
     ``q`` [tokens, q heads, head_dim] (or None), ``k`` and ``v`` [tokens, kv heads, head_dim]: views into one projection's output are
-    fine.  Token ``t`` belongs to sequence ``sequences[t]`` (int32; default: ``t``) and stands at ``positions[t]`` (int32 or
+    fine.  Token ``t`` belongs to sequence ``sequences[t]`` (int32; default: ``t``, of which the block table must have as many) and stands at ``positions[t]`` (int32 or
     int64; negative: padding, not written).  ``cos`` and ``sin`` [positions, rotary_dim / 2] in fp32 rotate the first ``rotary_dim``
     dimensions, pairs ``(i, i + rotary_dim / 2)`` or, ``interleaved``, ``(2 i, 2 i + 1)``; None: no rotation.  e4m3 pages get
     ``x / scale``, saturated.  Tokens of one call must have different places.  Returns the rotated queries (None without ``q``),
     with ``return_key`` a pair with the rotated keys."""
     what = "append_paged_kv"
     dev = _same_device(what, k, v, q, k_pages, v_pages, block_table, positions, sequences, cos, sin, k_scale, v_scale, status)
-    cache, (_, cache_heads, cache_dim, _, _, _) = _cache(what, k_pages, v_pages, block_table, k_scale, v_scale, status)
+    cache, (_, cache_heads, cache_dim, table_sequences, _, _) = _cache(what, k_pages, v_pages, block_table, k_scale, v_scale, status)
     shape, dtype = k.shape, k.dtype
     if len(shape) != 3 or v.shape != shape or dtype not in _ROWS or v.dtype is not dtype:
         _fail(what, "k and v must be fp16 or bf16 [tokens, num_kv_heads, head_dim]")
@@ -149,7 +149,12 @@ def append_paged_kv(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         _fail(what, f"k {tuple(shape)} does not fit pages of num_kv_heads {cache_heads} and head_dim {cache_dim}")
     wide = positions.dtype is torch.int64
     at = _want(what, "positions", positions, torch.int64 if wide else torch.int32, (tokens,))
-    sequence_at = 0 if sequences is None else _want(what, "sequences", sequences, torch.int32, (tokens,))
+    if sequences is not None:
+        sequence_at = _want(what, "sequences", sequences, torch.int32, (tokens,))
+    elif tokens <= table_sequences:
+        sequence_at = 0
+    else:
+        _fail(what, f"{tokens} tokens without sequences do not fit a block table of {table_sequences} sequences")
     k0, k1, k2 = k.stride()
     v0, v1, v2 = v.stride()
     q_at = q0 = q1 = q_heads = out_at = 0

@@ -187,6 +187,17 @@ def test_append_to_8_bits_divides_numbers_of_any_size(lib, rows):
         assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
 
 
+def test_append_of_tokens_that_have_no_sequence_is_refused(lib):
+    import trismoe_b200 as tm
+
+    pages = torch.zeros((4, 16, 2, 64), dtype=F16, device="cuda")
+    x = torch.zeros((3, 2, 64), dtype=F16, device="cuda")
+    table, at = torch.zeros((2, 2), dtype=torch.int32, device="cuda"), torch.zeros((3,), dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="sequences"):
+        tm.append_paged_kv(x, x, x, pages, pages, table, at)
+    tm.append_paged_kv(x[:2], x[:2], x[:2], pages, pages, table, at[:2])
+
+
 # ---- attention ------------------------------------------------------------------------------
 @pytest.mark.parametrize("small", [2.0 ** -14, 2.0 ** -20, 2.0 ** -26])
 def test_small_elements_of_a_query_over_8_bit_pages(lib, small):
