@@ -743,7 +743,7 @@ enum { TRIS_DTYPE_F16 = 0, TRIS_DTYPE_BF16 = 1, TRIS_DTYPE_F32 = 2, TRIS_DTYPE_E
  * block_table[b * table_stride + i / page_size].
  * e4m3 pages hold x / scale of their head, saturated at +-448; without scales that is 1.
  * status_dev (optional device int32, sticky) is set to TRIS_ERR_CORRUPT where a needed page is outside [0, num_pages), a position outside the
- * table or the rotation tables, or a length above table_width * page_size.  Such tokens are not written, read as zeros, or cut off.
+ * table or the rotation tables, or a length negative or above table_width * page_size.  Such tokens are not written, read as zeros, or cut off.
  */
 typedef struct TrisPagedKv {
   void* k_pages;

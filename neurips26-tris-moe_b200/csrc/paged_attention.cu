@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
     if (warp == 0 && lane * 32 < c.table_width) asm volatile("prefetch.global.L2 [%0];" ::"l"(c.block_table + use.b * c.table_stride + lane * 32));
     use.span = span_of(a, use.b);
     use.blocks = use.span.blocks();
-    if (query.lengths[use.b] > use.span.hi && c.status_dev) *c.status_dev = TRIS_ERR_CORRUPT;
+    if (query.lengths[use.b] != use.span.hi && c.status_dev) *c.status_dev = TRIS_ERR_CORRUPT;
     const int run = (use.blocks + a.cluster * W - 1) / (a.cluster * W);
     use.blk = (blockIdx.z * W + warp) * run;
     count = max(0, min(run, use.blocks - use.blk));
@@ -794,7 +794,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
   const Span span = span_of(a, b);
   const int blocks = span.blocks();
   T* out = static_cast<T*>(query.out) + out_row * D;
-  if (query.lengths[b] > span.hi && c.status_dev && q_head == 0 && tid == 0) *c.status_dev = TRIS_ERR_CORRUPT;
+  if (query.lengths[b] != span.hi && c.status_dev && q_head == 0 && tid == 0) *c.status_dev = TRIS_ERR_CORRUPT;
   if (blocks == 0) {
     for (int d = tid; d < D; d += kJoinThreads) store_float(out + d, 0.f);
     if (query.lse && tid == 0) query.lse[out_row] = -INFINITY;

@@ -267,6 +267,22 @@ def test_an_infinite_value_gives_an_infinity_whatever_its_weight(lib, rows, cach
             assert torch.equal(out[b, h][odd].double().nan_to_num(nan=7.0), want[odd].nan_to_num(nan=7.0))
 
 
+def test_a_negative_length_is_reported(lib):
+    import trismoe_b200 as tm
+
+    g = _gen(42)
+    for longest in (40, 20000):  # by clusters and numbered
+        k_pages, v_pages, table, _ = _filled(g, [longest, 20], 16, 1, 64, F16, LAYOUTS[0])
+        q = torch.randn((2, 2, 64), generator=g, device="cuda").half()
+        status = torch.zeros((1,), dtype=torch.int32, device="cuda")
+        good = tm.paged_decode_attention(q, k_pages, v_pages, table, torch.tensor([longest, 20], dtype=torch.int32, device="cuda"), status=status)
+        tm.raise_on_status(status)
+        out = tm.paged_decode_attention(q, k_pages, v_pages, table, torch.tensor([longest, -1], dtype=torch.int32, device="cuda"), status=status)
+        with pytest.raises(RuntimeError, match="CORRUPT"):
+            tm.raise_on_status(status)
+        assert torch.equal(out[0], good[0]) and bool((out[1] == 0).all())
+
+
 # ---- norm -----------------------------------------------------------------------------------
 @pytest.mark.parametrize("extra", [0, 1], ids=["wide", "element by element"])
 @pytest.mark.parametrize("dtype,odd", [(F16, 7), (F16, 63), (BF16, 7)], ids=["fp16 7", "fp16 63", "bf16 7"])
