@@ -142,6 +142,15 @@ inline int allow_shared_memory(int bytes) {
   done.fetch_or(bit, std::memory_order_relaxed);
   return TRIS_OK;
 }
+// SMs of the current device, 0 where there is none; asked of the driver once a device.
+inline int sm_count() {
+  static std::atomic<int> count[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  int n = count[dev].load(std::memory_order_relaxed);
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) count[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
 inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline int dtype_size(int dtype) { return dtype == TRIS_DTYPE_F32 ? 4 : dtype == TRIS_DTYPE_E4M3 ? 1 : 2; }
 int validate_paged_kv(const TrisPagedKv* cache, const char* what);  // paged_kv.cu

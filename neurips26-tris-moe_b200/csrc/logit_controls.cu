@@ -208,7 +208,7 @@ int launch_controls(LogitArgs& a, int most, cudaStream_t stream) {
 // 9.2 and 8.2 for 32, 15.2 and 9.2 for 64.
 template <typename T>
 int launch_controls(LogitArgs& a, cudaStream_t stream) {
-  const bool few = static_cast<int64_t>(ceil_div(a.c.vocab, 4096)) * a.c.rows < 2 * 148;
+  const bool few = static_cast<int64_t>(ceil_div(a.c.vocab, 4096)) * a.c.rows < 2 * sm_count();
   return few ? launch_controls<T, 1>(a, 1024, stream) : launch_controls<T, 2>(a, kMostSlice, stream);
 }
 

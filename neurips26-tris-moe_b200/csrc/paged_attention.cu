@@ -861,15 +861,6 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
   if (query.lse && tid == 0) query.lse[out_row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
-int sm_count() {
-  static std::atomic<int> count[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  int n = count[dev].load(std::memory_order_relaxed);
-  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) count[dev].store(n, std::memory_order_relaxed);
-  return n;
-}
-
 // CTAs of the first kernel: twice as many as are resident, but no more than there can be shares of one block for their warps.
 int attention_ctas(int resident, int64_t blocks) {
   const int64_t ctas = (blocks + kWarps - 1) / kWarps;

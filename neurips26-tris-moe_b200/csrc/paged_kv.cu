@@ -257,7 +257,8 @@ extern "C" int tris_paged_kv_append(const TrisPagedKv* cache, const TrisPagedApp
   // threads for two rounds of all SMs, with 640 on each; beyond that a thread takes more heads with its cosines and sines (8188 tokens of 48 heads of
   // 128: 36 us, 45 with half as many threads, 40 with twice and with eight times as many; 2048 tokens 11.1, 14.7, 12.3, 20.7)
   a.head_groups = heads;
-  while (a.head_groups > 1 && static_cast<int64_t>(a.units) * a.head_groups * r.num_tokens > 2 * 148 * 640) a.head_groups = ceil_div(a.head_groups, 2);
+  const int64_t enough = 2 * 640 * static_cast<int64_t>(sm_count());
+  while (a.head_groups > 1 && static_cast<int64_t>(a.units) * a.head_groups * r.num_tokens > enough) a.head_groups = ceil_div(a.head_groups, 2);
   TRIS_REQUIRE(static_cast<int64_t>(a.units) * a.head_groups * r.num_tokens < (1ll << 31), TRIS_ERR_UNSUPPORTED, "paged_kv_append: too many tokens in one call");
   TRIS_REQUIRE(r.sequences || r.num_tokens <= c.num_sequences, TRIS_ERR_INVALID_ARG, "paged_kv_append: %d tokens without sequences for a block table of %d", r.num_tokens, c.num_sequences);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

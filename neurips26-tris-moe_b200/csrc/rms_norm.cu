@@ -255,15 +255,16 @@ int launch_norm(const TrisAddRmsNorm& a, cudaStream_t stream) {
   const int vectors = H / 8;
   // few rows: as many threads as vectors, the chain of one row is what counts (100 x 8192: 3.4 us, 4.1 with 256 threads); many: fewer threads with more
   // loads in flight each (2047 x 4096: 10.0 us, 13.8 with a vector a thread, 10.7 with 128 threads)
+  const int sms = sm_count();
   int vecs = 1;
-  while (vecs < kMaxVectors && (ceil_div(vectors, vecs) > most_threads(vecs) || (a.rows > 148 && ceil_div(vectors, vecs) > 256))) vecs *= 2;
+  while (vecs < kMaxVectors && (ceil_div(vectors, vecs) > most_threads(vecs) || (a.rows > sms && ceil_div(vectors, vecs) > 256))) vecs *= 2;
   const int threads = (ceil_div(vectors, vecs) + 31) / 32 * 32;
   NormArgs args{a, 1.f / H, FP8 ? H / a.group_size : 1, -1};
   for (int shift = 0; FP8 && shift <= 5; ++shift)
     if (a.group_size == 8 << shift) args.group_shift = shift;
   const size_t smem = FP8 && a.group_size != H && args.group_shift < 0 ? sizeof(float) * vectors : 0;
   auto kernel = vecs == 1 ? add_rms_norm_kernel<T, FP8, 1> : vecs == 2 ? add_rms_norm_kernel<T, FP8, 2> : add_rms_norm_kernel<T, FP8, 4>;
-  const int resident = 148 * threads_on_sm(vecs) / threads;
+  const int resident = sms * threads_on_sm(vecs) / threads;
   const int turns = ceil_div(a.rows, resident < 1 ? 1 : resident);
   TRIS_CUDA(launch_step(kernel, dim3(ceil_div(a.rows, turns)), dim3(threads), smem, stream, pdl, 1, args));
   return TRIS_OK;
