@@ -212,6 +212,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     known = like is not False
     if not known:
         with torch.cuda.device(dev):
+            capturing = torch.cuda.is_current_stream_capturing()  # what is allocated now belongs to a graph
             need = int(_native.load().tris_paged_decode_attention_workspace_bytes(cache, heads, max(window, -1)))
         like = torch.empty((1,), dtype=torch.uint8, device=dev).expand(need) if need else None
     if like is not None:
@@ -223,7 +224,7 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     args = _ATTENTION.pack(q.data_ptr(), q0, q1, lengths_at, out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws_at, ws_bytes,
                            heads, window, _DTYPES[dtype], dim ** -0.5 if softmax_scale is None else softmax_scale)
     _launch(what, "tris_paged_decode_attention", dev, cache, args)
-    if not known:  # a call that was refused says nothing of what the next one needs
+    if not known and not capturing:  # a call that was refused says nothing of what the next one needs
         if len(_scratch) >= 4096:  # block tables may grow for ever
             _scratch.clear()
         _scratch[key] = like

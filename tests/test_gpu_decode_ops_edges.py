@@ -283,6 +283,26 @@ def test_a_negative_length_is_reported(lib):
         assert torch.equal(out[0], good[0]) and bool((out[1] == 0).all())
 
 
+def test_a_capture_leaves_no_scratch_behind_in_its_pool(lib):
+    """What a first call inside a capture allocates goes with the graph."""
+    import trismoe_b200 as tm
+    from trismoe_b200 import decode_ops
+
+    g, lengths = _gen(43), [20011]
+    k_pages, v_pages, table, _ = _filled(g, lengths, 16, 1, 72, F16, LAYOUTS[0])
+    q = torch.randn((1, 1, 72), generator=g, device="cuda").half()
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    known = dict(decode_ops._scratch)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = tm.paged_decode_attention(q, k_pages, v_pages, table, lens)
+    graph.replay()
+    assert decode_ops._scratch == known
+    eager = tm.paged_decode_attention(q, k_pages, v_pages, table, lens)
+    assert torch.equal(out, eager) and len(decode_ops._scratch) == len(known) + 1
+
+
 # ---- norm -----------------------------------------------------------------------------------
 @pytest.mark.parametrize("extra", [0, 1], ids=["wide", "element by element"])
 @pytest.mark.parametrize("dtype,odd", [(F16, 7), (F16, 63), (BF16, 7)], ids=["fp16 7", "fp16 63", "bf16 7"])
