@@ -179,18 +179,42 @@ __global__ void __launch_bounds__(kThreads, 5) logit_controls_kernel(const __gri
   if (!ids) return;
   // Biases are few: they are added to what has been written, one thread an entry.
   __syncthreads();
-  for (int i = tid; i < c.num_biases; i += kThreads) {
-    const int id = i == tid ? first_id : ids[i], at = id - v0;
-    if (id < v0 || at >= n) continue;
-    float bias = i == tid ? first_value : values[i];
-    if (repeated) {  // the first of an id's entries adds all of them, in their order
-      bool first = true;
-      for (int k = 0; k < i; ++k) first = first && ids[k] != id;
-      if (!first) continue;
-      for (int k = i + 1; k < c.num_biases; ++k)
-        if (ids[k] == id) bias += values[k];
+  if (!repeated) {
+    for (int i = tid; i < c.num_biases; i += kThreads) {
+      const int id = i == tid ? first_id : ids[i], at = id - v0;
+      if (id < v0 || at >= n) continue;
+      const float bias = i == tid ? first_value : values[i];
+      if (!allowed || (allowed[at / 32] >> (at & 31)) & 1) out[at] += bias;
     }
-    if (!allowed || (allowed[at / 32] >> (at & 31)) & 1) out[at] += bias;
+    return;
+  }
+  // Some ids are there more than once.  The list is taken as many entries at a time as there are threads: of a warp's entries of one id the first adds up all, in
+  // their order, and of several warps' the lowest goes first, which the words tell that have done their service.  Time grows with the list's length, not its square.
+#pragma unroll 1
+  for (int base = 0; base < c.num_biases; base += kThreads) {
+    const int i = base + tid, lane = tid & 31;
+    const int id = i < c.num_biases ? ids[i] : -1, at = id - v0;
+    const bool here = id >= v0 && at < n;
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, here ? at : -1);
+    const float value = here ? values[i] : 0.f;
+    float bias = value;
+    if (__any_sync(0xFFFFFFFFu, here && (same & (same - 1)))) {
+      for (int k = 1; k < 32; ++k) {
+        const float v = __shfl_sync(0xFFFFFFFFu, value, k);
+        if (k > lane && ((same >> k) & 1)) bias += v;
+      }
+    }
+    bool pending = here && __ffs(same) - 1 == lane && (!allowed || (allowed[at / 32] >> (at & 31)) & 1);
+    while (__syncthreads_or(pending)) {
+      if (pending) words[at] = kThreads;
+      __syncthreads();
+      if (pending) atomicMin(words + at, tid);
+      __syncthreads();
+      if (pending && words[at] == tid) {
+        out[at] += bias;
+        pending = false;
+      }
+    }
   }
 }
 

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_decode_ops import BF16, E4M3, F16, LAYOUTS, SUB, U, _attend_64, _check_attention, _filled, _gen
+from test_gpu_decode_ops import BF16, E4M3, F16, LAYOUTS, SUB, U, _attend_64, _check_attention, _controls_64, _filled, _gen
 
 pytestmark = pytest.mark.gpu
 
@@ -394,3 +394,50 @@ def test_repetition_whose_reciprocal_is_not_finite(lib):
     out = tm.apply_logit_controls(logits, tokens=tokens, token_lengths=torch.full((1,), 4, dtype=torch.int32, device="cuda"),
                                   repetition=torch.full((1,), 2.0 ** -130, device="cuda"))
     assert torch.equal(out, torch.tensor([[2.0 ** 30, -(2.0 ** -130), 2.0 ** -10, 0.0]], device="cuda"))
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("rows,vocab,biases", [(2, 1000, 700), (1, 50304, 9000), (40, 50304, 600), (3, 37, 5000)])
+def test_repeated_biases_add_up_in_their_order(lib, rows, vocab, biases, masked):
+    """Ids that occur once, a few times and very often, in any order; sums in 32 bits, one entry after the other."""
+    import trismoe_b200 as tm
+
+    g = _gen(biases)
+    ids = torch.randint(-3, vocab + 3, (rows, biases), generator=g, device="cuda", dtype=torch.int32)
+    ids[:, biases // 3: biases // 2] = vocab // 2
+    ids[:, : biases // 3: 2] = ids[:, biases // 2: biases // 2 + len(range(0, biases // 3, 2))]
+    values = torch.randn((rows, biases), generator=g, device="cuda") * 3.0
+    logits = torch.randn((rows, vocab), generator=g, device="cuda")
+    c = {"bias_ids": ids, "bias_values": values}
+    if masked:
+        c["allowed"] = torch.randint(-2 ** 31, 2 ** 31, (rows, -(-vocab // 32)), generator=g, device="cuda", dtype=torch.int64).to(torch.int32)
+    want, mag = _controls_64(logits, c)
+    got = tm.apply_logit_controls(logits, **c)
+    assert torch.equal(got, tm.apply_logit_controls(logits, **c))
+    finite = torch.isfinite(want)
+    assert torch.equal(got[~finite].double(), want[~finite])
+    # as many roundings as an id has entries, each at most 2^-24 of the magnitudes
+    entries = torch.zeros((rows, vocab), device="cuda", dtype=torch.float64)
+    ok = (ids >= 0) & (ids < vocab)
+    entries.scatter_add_(1, torch.where(ok, ids, 0).long(), ok.double())
+    assert float(((got.double() - want).abs() - (2 + entries) * 2.0 ** -24 * mag)[finite].max()) <= 0
+
+
+def test_a_long_list_of_biases_with_a_repeated_id_takes_time_by_its_length(lib):
+    """25000 entries, one of them twice: some 60 us; milliseconds would be a search of the list for each of its entries."""
+    import trismoe_b200 as tm
+
+    ids = torch.randperm(50304, generator=_gen(52), device="cuda")[None, :25000].int()
+    ids[0, -1] = ids[0, 0]
+    c = {"bias_ids": ids, "bias_values": torch.randn((1, 25000), generator=_gen(53), device="cuda")}
+    logits = torch.randn((1, 50304), generator=_gen(54), device="cuda")
+    tm.apply_logit_controls(logits, **c)
+    times = []
+    for _ in range(5):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        tm.apply_logit_controls(logits, **c)
+        end.record()
+        torch.cuda.synchronize()
+        times.append(start.elapsed_time(end))
+    assert min(times) < 3.0
