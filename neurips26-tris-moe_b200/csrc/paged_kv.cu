@@ -20,9 +20,10 @@ int validate_paged_kv(const TrisPagedKv* c, const char* what) {
   TRIS_REQUIRE(c->block_table || c->num_sequences == 0 || c->table_width == 0, TRIS_ERR_INVALID_ARG, "%s: null block table", what);
   const int elt = dtype_size(c->dtype);
   TRIS_REQUIRE(c->head_dim * elt % 16 == 0 && c->head_dim <= 256, TRIS_ERR_UNSUPPORTED, "%s: a head takes a multiple of 16 bytes and up to 256 dimensions (got %d)", what, c->head_dim);
-  const int64_t strides[6] = {c->k_page_stride, c->k_token_stride, c->k_head_stride, c->v_page_stride, c->v_token_stride, c->v_head_stride};
-  for (int64_t s : strides)
-    TRIS_REQUIRE(s >= 0 && s * elt % 16 == 0, TRIS_ERR_UNSUPPORTED, "%s: strides of the pages must be multiples of 16 bytes", what);
+  const int64_t strides[6] = {c->k_page_stride, c->v_page_stride, c->k_token_stride, c->v_token_stride, c->k_head_stride, c->v_head_stride};
+  const int sizes[3] = {c->num_pages, c->page_size, c->num_kv_heads};
+  for (int i = 0; i < 6; ++i)  // of a size of 1 the stride is of no account
+    TRIS_REQUIRE(sizes[i / 2] <= 1 || (strides[i] >= 0 && strides[i] * elt % 16 == 0), TRIS_ERR_UNSUPPORTED, "%s: strides of the pages must be multiples of 16 bytes", what);
   TRIS_REQUIRE(aligned_to(c->k_pages, 16) && aligned_to(c->v_pages, 16), TRIS_ERR_UNSUPPORTED, "%s: pages must start on a 16-byte boundary", what);
   return TRIS_OK;
 }

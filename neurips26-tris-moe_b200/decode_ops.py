@@ -315,7 +315,7 @@ def apply_logit_controls(logits: torch.Tensor, *, tokens: Optional[torch.Tensor]
     if bias_ids is not None:
         ids, bias_stride, biases = _matrix(what, "bias_ids", bias_ids, torch.int32, rows)
         values, value_stride, _ = _matrix(what, "bias_values", bias_values, torch.float32, rows, biases)
-        if biases and bias_stride != value_stride:
+        if biases and rows > 1 and bias_stride != value_stride:
             _fail(what, "bias_ids and bias_values must have the same stride")
     if allowed is not None:
         mask, mask_stride, _ = _matrix(what, "allowed", allowed, torch.int32, rows, (vocab + 31) // 32)

@@ -441,3 +441,25 @@ def test_a_long_list_of_biases_with_a_repeated_id_takes_time_by_its_length(lib):
         torch.cuda.synchronize()
         times.append(start.elapsed_time(end))
     assert min(times) < 3.0
+
+
+def test_strides_of_sizes_of_one_are_of_no_account(lib):
+    """A dimension of size 1 may have any stride: one head, one page, pages of one token; one row of biases."""
+    import trismoe_b200 as tm
+
+    g = _gen(50)
+    for pages, page, heads in ((5, 4, 1), (1, 40, 2), (20, 1, 2)):
+        k_pages, v_pages, table, rows = _filled(g, [17], page, heads, 64, F16, LAYOUTS[1], spare=pages - -(-17 // page))
+        assert k_pages.shape == (pages, page, heads, 64)
+        strides = [3 if n == 1 else s for n, s in zip(k_pages.shape, k_pages.stride())]
+        odd = [p.as_strided(p.shape, strides) for p in (k_pages, v_pages)]
+        q = torch.randn((1, 4, 64), generator=g, device="cuda").half()
+        _check_attention(tm, q, (*odd, table, rows), [17])
+        new = torch.randn((1, heads, 64), generator=g, device="cuda").half()
+        tm.append_paged_kv(None, new, new, *odd, table, torch.tensor([16], dtype=torch.int32, device="cuda"))
+        assert torch.equal(k_pages[table[0, 16 // page].long(), 16 % page], new[0]) and torch.equal(v_pages[table[0, 16 // page].long(), 16 % page], new[0])
+    ids = torch.tensor([[3, 7, -1, 3, 9]], dtype=torch.int32, device="cuda")[:, :4]
+    values = torch.ones((1, 40), device="cuda")[:, 10:14]
+    want = torch.zeros((1, 40), device="cuda")
+    want[0, 3], want[0, 7] = 2.0, 1.0
+    assert torch.equal(tm.apply_logit_controls(torch.zeros((1, 40), device="cuda"), bias_ids=ids, bias_values=values), want)
