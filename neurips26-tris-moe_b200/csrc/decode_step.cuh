@@ -1,5 +1,5 @@
 // What the kernels of the decode step around the experts share (paged_kv.cu, paged_attention.cu, rms_norm.cu, logit_controls.cu):
-// element types, loads and stores of eight values, page lookup.
+// element types, conversions and stores of eight values, quotients by a scale.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -37,16 +37,14 @@ __device__ __forceinline__ void store_float(__half* p, float v) { *p = __float2h
 __device__ __forceinline__ void store_float(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_float(__nv_fp8_e4m3* p, float v) { p->__x = __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
 
-// Eight elements by one 16-byte access (8 bytes of e4m3).
+// Eight elements that have been read, and stored by one access of 16 bytes (8 of e4m3).
 template <typename T>
-__device__ __forceinline__ void load_8(const T* p, float (&v)[8]) {
-  const uint4 raw = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void unpack_8(const uint4& raw, float (&v)[8]) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = Pair<T>::unpack(w[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
   }
 }
 template <typename T>

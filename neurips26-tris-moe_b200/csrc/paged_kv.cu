@@ -53,14 +53,7 @@ template <typename T>
 struct Chunk<8, T> {
   uint4 v;
   __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 p = Pair<T>::unpack(w[i]);
-      f[2 * i] = p.x, f[2 * i + 1] = p.y;
-    }
-  }
+  __device__ __forceinline__ void get(float (&f)[8]) const { unpack_8<T>(v, f); }
 };
 template <int VEC, typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {

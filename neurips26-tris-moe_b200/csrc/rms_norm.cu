@@ -66,16 +66,6 @@ __device__ __forceinline__ float quantize_8(float (&y)[8], uint32_t top) {
   if (scale != 0.f) DivideBy{scale}(y, largest);
   return scale;
 }
-template <typename T>
-__device__ __forceinline__ void unpack_8(const uint4& raw, float (&v)[8]) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = Pair<T>::unpack(w[i]);
-    v[2 * i] = f.x, v[2 * i + 1] = f.y;
-  }
-}
-
 // Rows of at most 8 * VECS * blockDim columns, all pointers and strides at 16-byte boundaries.
 template <typename T, bool FP8, int VECS>
 __global__ void __maxnreg__(registers(VECS)) add_rms_norm_kernel(const __grid_constant__ NormArgs args) {
