@@ -463,3 +463,122 @@ def test_strides_of_sizes_of_one_are_of_no_account(lib):
     want = torch.zeros((1, 40), device="cuda")
     want[0, 3], want[0, 7] = 2.0, 1.0
     assert torch.equal(tm.apply_logit_controls(torch.zeros((1, 40), device="cuda"), bias_ids=ids, bias_values=values), want)
+
+
+# ---- sizes that lead to each variant --------------------------------------------------------
+def test_lse_of_small_scores(lib):
+    """Scores below 1 and few tokens: products are exact, sums, exponentials and logarithm a few roundings of 2^-23 each; a weight of 16 bits would be
+    off by 2^-12."""
+    import trismoe_b200 as tm
+
+    g, lengths = _gen(47), [1, 2, 3, 5, 9, 40]
+    for rows in (F16, BF16):
+        k_pages, v_pages, table, kept = _filled(g, lengths, 16, 1, 64, rows, LAYOUTS[0])
+        q = (torch.randn((6, 8, 64), generator=g, device="cuda") * 0.25).to(rows)
+        _, lse = tm.paged_decode_attention(q, k_pages, v_pages, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), return_lse=True)
+        _, want, _ = _attend_64(q, kept, 0, 0.125, None, None)
+        assert float((lse.double() - want).abs().max()) <= 2.0 ** -18
+
+
+def _workspace(lib, q, k_pages, table, window=0):
+    from trismoe_b200 import decode_ops
+
+    packed, _ = decode_ops._cache("test", k_pages, k_pages, table, None, None, None)
+    return lib.tris_paged_decode_attention_workspace_bytes(packed, q.shape[1], window)
+
+
+def test_attention_of_so_many_blocks_that_a_warp_has_a_long_run(lib):
+    """Numbered blocks, 64 and more to a warp of the doubled grid: 148 SMs x 3 CTAs x 2 x 4 warps x 64 are 227 000 blocks."""
+    import trismoe_b200 as tm
+
+    g, lengths = _gen(48), [150000, 0, 1, 90001, 63, 70000, 16, 33333, 130000]
+    k_pages, v_pages, table, kept = _filled(g, lengths, 16, 8, 16, F16, LAYOUTS[0])
+    q = torch.randn((9, 8, 16), generator=g, device="cuda").half()
+    assert sum(-(-n // 16) for n in lengths) * 8 > 230_000 and _workspace(lib, q, k_pages, table) > 0
+    _check_attention(tm, q, (k_pages, v_pages, table, kept), lengths)
+
+
+@pytest.mark.parametrize("window", [4096, 4111, 9999])
+@pytest.mark.parametrize("rows,cache", [(F16, F16), (BF16, E4M3)], ids=["fp16", "e4m3"])
+def test_attention_in_a_window_over_numbered_blocks(lib, rows, cache, window):
+    import trismoe_b200 as tm
+
+    g, lengths = _gen(window), [20000, 5000, 0, 17, 4096]
+    filled = _filled(g, lengths, 16, 1, 128, cache, LAYOUTS[0])
+    q = torch.randn((5, 4, 128), generator=g, device="cuda").to(rows)
+    assert _workspace(lib, q, filled[0], filled[2], window) > 0
+    _check_attention(tm, q, filled, lengths, window=window)
+
+
+@pytest.mark.parametrize("width", [512, 8192])
+@pytest.mark.parametrize("lengths", [[513], [1, 0, 70, 300]], ids=["one", "four"])
+def test_attention_of_short_sequences_in_a_wide_table(lib, lengths, width):
+    """A table with room for 8192 or 131072 tokens, as a server has."""
+    import trismoe_b200 as tm
+
+    g = _gen(width)
+    k_pages, v_pages, table, kept = _filled(g, lengths, 16, 4, 128, F16, LAYOUTS[0])
+    wide = torch.full((len(lengths), width), -1, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    q = torch.randn((len(lengths), 8, 128), generator=g, device="cuda").half()
+    _check_attention(tm, q, (k_pages, v_pages, wide, kept), lengths)
+
+
+@pytest.mark.parametrize("rows,hidden,groups", [(2047, 2048, (0, 128, 512)), (2047, 4096, (0, 128, 1024)), (1000, 8192, (0, 128, 2048)), (3, 768, (48, 384)),
+                                                (1200, 768, (48, 384)), (2, 1680, (240, 560)), (700, 1680, (240,)), (2000, 256, (0, 16, 64))])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+def test_norm_of_many_rows_and_odd_groups(lib, rows, hidden, groups, dtype):
+    """Several rows to a CTA in each variant, groups wider than a warp and not of a power of two, rows off 16-byte boundaries too."""
+    import trismoe_b200 as tm
+
+    g = _gen(rows + hidden)
+    x, res = (s * torch.randn((rows, hidden), generator=g, device="cuda") for s in (1.0, 3.0))
+    x, res = x.to(dtype), res.to(dtype)
+    w = (1.0 + 0.2 * torch.randn((hidden,), generator=g, device="cuda")).to(dtype)
+    h64 = x.double() + res.double()
+    want = h64 / (h64.square().mean(-1, keepdim=True) + 1e-5).sqrt() * w.double()
+    off = torch.empty((rows, hidden + 1), dtype=dtype, device="cuda")[:, 1:]
+    off.copy_(x)
+    for rows_ in (x, off):
+        y, h = tm.add_rms_norm(rows_, res, w, 1e-5)
+        assert torch.equal(h, h64.to(dtype))
+        assert float(((y.double() - want).abs() - (U[dtype] + 2.0 ** -17) * want.abs() - SUB[dtype]).max()) <= 0
+        for group in groups:
+            values, scales, h8 = tm.add_rms_norm_e4m3(rows_, res, w, 1e-5, group_size=group)
+            parts = want.view(rows, -1, group or hidden)
+            want_scale = parts.abs().amax(-1) / 448.0
+            assert torch.equal(h8, h) and float(((scales.double() - want_scale).abs() - 2.0 ** -16 * want_scale).max()) <= 0
+            back = values.double().view(parts.shape) * scales.double()[..., None]
+            assert float(((back - parts).abs() - (U[E4M3] + 2.0 ** -15) * parts.abs() - 1.01 * SUB[E4M3] * want_scale[..., None]).max()) <= 0
+
+
+@pytest.mark.parametrize("rows,vocab,history", [(40, 50304, 3000), (300, 4001, 64), (90, 20000, 40000), (25, 65536, 500)])
+@pytest.mark.parametrize("dtype", [F16, torch.float32], ids=["fp16", "fp32"])
+def test_logit_controls_in_large_slices(lib, rows, vocab, history, dtype):
+    """More than two CTAs an SM would have with slices of 4096: large slices, over which a CTA streams in several turns."""
+    import trismoe_b200 as tm
+
+    assert -(-vocab // 4096) * rows >= 2 * 148
+    g = _gen(rows + vocab)
+    rand = lambda *s: torch.rand(s, generator=g, device="cuda")
+    ints = lambda low, high, *s: torch.randint(low, high, s, generator=g, device="cuda", dtype=torch.int32)
+    logits = (torch.randn((rows, vocab + 3), generator=g, device="cuda") * 5.0).to(dtype)[:, 1: vocab + 1]
+    tokens = ints(-2, vocab + 2, rows, history)
+    tokens[:, : history // 2] %= vocab // 50
+    ids = ints(-2, vocab + 1, rows, 37)
+    ids[:, 20:] = ids[:, :17]
+    c = {"tokens": tokens, "token_lengths": ints(-1, history + 5, rows), "prompt_lengths": ints(0, history + 2, rows), "repetition": 0.5 + rand(rows),
+         "presence": rand(rows), "frequency": rand(rows), "bias_ids": ids, "bias_values": torch.randn((rows, 37), generator=g, device="cuda"),
+         "allowed": torch.randint(-2 ** 31, 2 ** 31, (rows, -(-vocab // 32)), generator=g, device="cuda", dtype=torch.int64).to(torch.int32)}
+    c["allowed"][0] = 0
+    for aligned in (False, True):
+        src = logits.contiguous() if aligned else logits
+        want, mag = _controls_64(src, c)
+        got = tm.apply_logit_controls(src, **c)
+        finite = torch.isfinite(want)
+        assert torch.equal(got[~finite].double(), want[~finite])
+        # each of some ten roundings is at most 2^-24 of the magnitudes added up
+        assert float(((got.double() - want).abs() - 12 * 2.0 ** -24 * mag)[finite].max()) <= 0
+        if dtype == torch.float32:
+            same = src.clone()
+            assert torch.equal(tm.apply_logit_controls(same, out=same, **c), got) and bool((got == same).all())
