@@ -879,7 +879,7 @@ constexpr int kMostShare = 24, kLeastShare = 4;
 int cluster_size(const TrisPagedKv& c, int row_tiles, int window, int resident) {
   const int64_t items = static_cast<int64_t>(c.num_sequences) * c.num_kv_heads * row_tiles;
   int64_t tokens = static_cast<int64_t>(c.table_width) * c.page_size;
-  if (window > 0 && window < tokens) tokens = window + kBlock;
+  if (window > 0 && window < tokens) tokens = static_cast<int64_t>(window) + kBlock;
   int size = kMostCluster;
   while (size > 1 && items * size > resident) size /= 2;
   int64_t share = kMostShare * items * size / resident;

@@ -206,14 +206,14 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if sizes[2] != dim or sizes[3] != batch:
         _fail(what, f"q {tuple(shape)} does not fit pages of head_dim {sizes[2]} and a block table of {sizes[3]} sequences")
     lengths_at = _want(what, "lengths", lengths, torch.int32, (batch,))
-    window = window or 0
+    window = max(-1, min(window or 0, 2 ** 31 - 1))  # as a 32-bit number; no cache is longer
     key = (dev.index, heads, window, sizes)
     like, ws_at, ws_bytes = _scratch.get(key, False), 0, 0
     known = like is not False
     if not known:
         with torch.cuda.device(dev):
             capturing = torch.cuda.is_current_stream_capturing()  # what is allocated now belongs to a graph
-            need = int(_native.load().tris_paged_decode_attention_workspace_bytes(cache, heads, max(window, -1)))
+            need = int(_native.load().tris_paged_decode_attention_workspace_bytes(cache, heads, window))
         like = torch.empty((1,), dtype=torch.uint8, device=dev).expand(need) if need else None
     if like is not None:
         ws = _new_like(like)

@@ -465,6 +465,21 @@ def test_strides_of_sizes_of_one_are_of_no_account(lib):
     assert torch.equal(tm.apply_logit_controls(torch.zeros((1, 40), device="cuda"), bias_ids=ids, bias_values=values), want)
 
 
+def test_a_window_of_any_size(lib):
+    """A window beyond 32 bits is no window; a negative one is refused."""
+    import trismoe_b200 as tm
+
+    g, lengths = _gen(55), [300, 7]
+    k_pages, v_pages, table, _ = _filled(g, lengths, 16, 2, 64, F16, LAYOUTS[0])
+    q = torch.randn((2, 4, 64), generator=g, device="cuda").half()
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    want = tm.paged_decode_attention(q, k_pages, v_pages, table, lens)
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 40):
+        assert torch.equal(tm.paged_decode_attention(q, k_pages, v_pages, table, lens, window=window), want)
+    with pytest.raises(RuntimeError, match="window"):
+        tm.paged_decode_attention(q, k_pages, v_pages, table, lens, window=-2 ** 40)
+
+
 # ---- sizes that lead to each variant --------------------------------------------------------
 def test_lse_of_small_scores(lib):
     """Scores below 1 and few tokens: products are exact, sums, exponentials and logarithm a few roundings of 2^-23 each; a weight of 16 bits would be
