@@ -300,8 +300,8 @@ def apply_logit_controls(logits: torch.Tensor, *, tokens: Optional[torch.Tensor]
     rows, vocab = shape
     if out is None:
         out = _new_like(logits, torch.float32)
-    elif out.dtype is not torch.float32 or out.shape != shape or (vocab > 1 and out.stride(1) != 1):
-        _fail(what, "out must be fp32 of the logits' shape with a row side by side")
+    elif out.dtype is not torch.float32 or out.shape != shape or (vocab > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < vocab):
+        _fail(what, "out must be fp32 of the logits' shape with a row side by side, and the next one behind it")
 
     if tokens is None and (repetition is not None or presence is not None or frequency is not None):
         _fail(what, "penalties need tokens")

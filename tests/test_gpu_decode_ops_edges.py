@@ -480,6 +480,16 @@ def test_a_window_of_any_size(lib):
         tm.paged_decode_attention(q, k_pages, v_pages, table, lens, window=-2 ** 40)
 
 
+def test_an_output_whose_rows_overlap_is_refused(lib):
+    import trismoe_b200 as tm
+
+    logits = torch.randn((3, 40), generator=_gen(55), device="cuda")
+    for out in (torch.empty((1, 40), device="cuda").expand(3, 40), torch.empty((200,), device="cuda").as_strided((3, 40), (39, 1))):
+        with pytest.raises(RuntimeError, match="out must be"):
+            tm.apply_logit_controls(logits, out=out)
+    assert torch.equal(tm.apply_logit_controls(logits[:1], out=torch.empty((1, 40), device="cuda").as_strided((1, 40), (0, 1))), logits[:1])
+
+
 # ---- sizes that lead to each variant --------------------------------------------------------
 def test_lse_of_small_scores(lib):
     """Scores below 1 and few tokens: products are exact, sums, exponentials and logarithm a few roundings of 2^-23 each; a weight of 16 bits would be
