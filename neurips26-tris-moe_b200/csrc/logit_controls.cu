@@ -4,9 +4,9 @@
 // a slice of one row's vocabulary: it counts the history's tokens that lie in its slice (integer atomics, whose order does not matter) and then
 // streams over its logits, the next ones always on their way; the first, the mask and the first tokens of the history are asked for together.
 // Every CTA of a row reads the row's history, from L2, at some 24 instructions for 32 tokens: with slices of 4096 logits that was half of all work
-// (128 rows of 50304 logits and 3000 tokens 22 us), with four slices a row it is 17 us, 8 of them the stream.  Not kept: eight CTAs of a cluster that
+// (128 rows of 50304 logits, 3000 tokens and 64 biases 22 us), with four slices a row it is 16 us, 8 of them the stream.  Not kept: eight CTAs of a cluster that
 // count in one another's shared memory (31 us, two cluster barriers a CTA), a list of the logits concerned in place of the look-up (19 us), tokens of the slice
-// collected before they are counted (24 us).
+// collected before they are counted (24 us; all beside 17 us).
 #include <float.h>
 
 #include "decode_step.cuh"
@@ -127,8 +127,8 @@ __global__ void __launch_bounds__(kThreads, 5) logit_controls_kernel(const __gri
     __syncthreads();
   }
 
-  // z / rep by the reciprocal's two parts (128 rows of 50304 logits: 17.0 us; 17.4 by a division, 16.7 by one part, which is a rounding off); an infinite z
-  // has no second product, and no rep of 0 or without end a second part
+  // z / rep by the reciprocal's two parts (128 rows of 50304 logits without biases: 14.5 us; 15.9 by a division; 13.8 by one part, which is a rounding
+  // off).  An infinite z has no second product, a rep of 0 or without end no second part.
   const DivideBy divide(rep);
   const float less_lo = divide.lo == divide.lo ? divide.lo : 0.f;
   auto penalised = [&](float z) {

@@ -4,7 +4,8 @@
 // sums are scaled down whenever m grows.  Two such partial results (m, l, o) of different tokens join by the same rule, so a sequence can be cut
 // anywhere.  Every cached byte is read once and used for as many query heads as share it: bound by bytes where there are many (64 sequences of 1 to
 // 16384 tokens, 32/8 heads of 128 in bf16, 1.8 GB: 290 us, 6.2 TB/s; one of 131071 in fp16 96 us, 5.6), by the chain length - page - rows - join
-// where there are few (513 tokens of 16 heads 7.4 us), and by the conversion's instructions where pages are in 8 bits (heads of 256, 66 MB: 22 us).
+// where there are few (513 tokens of 16 heads 8 us).  16 sequences of 4096 in 8 bits (heads of 256, 66 MB) take 22 us: of a CTA's 37 800 cycles the eight
+// steps of a warp take 21 500, nine tenths of the rate of a copy, the reads ahead of them, which depend on one another, 6 600, and the joins 9 700.
 //
 // Work.  Short sequences: a cluster of CTAs has one key/value head of one sequence and cuts its tokens evenly (cluster_size has the rule).
 // Long ones: the tokens of every (sequence, key/value head) are cut into blocks of 16, all blocks are numbered through, and each warp of the grid
@@ -15,9 +16,9 @@
 //
 // One warp's step.  S^T = K Q^T and O^T = V^T P^T by mma.sync m16n8k16: the cached rows are the 16-row operand and the query heads of a group the
 // 8 columns, so that a step of 16 tokens costs three MMAs per 16 dimensions with up to 8 heads - one for the scores, two for the two parts of a
-// weight - (with the heads as rows it would cost six, half of them zeros).  No operand goes through a transposing load: the order of dimensions inside a product is free as long as both operands have the
-// same, so a lane's 16 bytes of a key row are its fragments as they are; of four value rows a lane has the same 8 dimensions, whose pairs of
-// tokens are put together by PRMT.  A step's MMAs take a seventh of the time its bytes take (heads of 128: 24 at two cycles of an SM, 8 KB at 23 bytes a
+// weight - (with the heads as rows it would cost six, half of them zeros).  No operand goes through a transposing load: the order of dimensions
+// inside a product is free as long as both operands have the same, so a lane's 16 bytes of a key row are its fragments as they are; of four value
+// rows a lane has the same 8 dimensions, whose pairs of tokens are put together by PRMT.  A step's MMAs take a seventh of the time its bytes take (heads of 128: 24 at two cycles of an SM, 8 KB at 23 bytes a
 // cycle), so nothing waits for the tensor pipe; tcgen05 tiles have 128 rows and their second operand in shared memory.  Each warp has a ring of its
 // own in shared memory, filled by cp.async, and meets no other warp before it is done.
 #include <type_traits>
@@ -875,6 +876,8 @@ int64_t most_blocks(const TrisPagedKv& c, int row_tiles) {
 // item stay idle: 1 x 8192 13.4 / 20.0, 1 x 4096 10.7 / 12.5, 64 x 1-2048 59.1 / 60.3, 64 x 1-3000 79 / 84, 64 x 1-16384 293 / 299.  Where the items take many
 // rounds their ends even out: 128 x 1-4096 197 / 183, 128 x 1-8192 354 / 355, 200 x 1-8192 560 / 540.  So a warp may have up to kMostShare blocks
 // of the longest sequence that the table (or the window) has room for, times the rounds, or the part of one, that the items take.
+// The host knows that room, not the lengths: short sequences in a table for 8192 tokens or 131072 are numbered (tight and wide tables, us: 1 x 513
+// 8.0 / 9.0, 8 x 513 11.8 / 14.6, 32 x 512-768 35.5 / 36.9).
 constexpr int kMostShare = 24, kLeastShare = 4;
 int cluster_size(const TrisPagedKv& c, int row_tiles, int window, int resident) {
   const int64_t items = static_cast<int64_t>(c.num_sequences) * c.num_kv_heads * row_tiles;

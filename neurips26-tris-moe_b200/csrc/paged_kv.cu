@@ -3,6 +3,7 @@
 // A dimension pair (a, b) of a token at position p becomes (a cos - b sin, b cos + a sin) with its frequency's row of the tables: a pass over
 // the projection's output that reads every element once and writes it once - queries to rows of their own, keys and values to their slots.
 // 8188 tokens of 16/16 heads of 128 (202 MB): 36 us, 5.6 TB/s.  Bound by bytes for prompts, by the chain position -> page -> store for a decode step.
+// To e4m3 with scales 32 us (168 MB): pages get the quotients (DivideBy has their cost).
 //
 // A thread has one unit of two 16-byte chunks - the halves (i, i + rotary / 2) that rotate together - and walks over heads with it, so that its
 // eight cosines and sines are read once; two heads are asked for before the first of them is rotated.  How many threads share a token's heads follows
