@@ -838,6 +838,44 @@ typedef struct TrisAddRmsNorm {
 int tris_add_rms_norm(const TrisAddRmsNorm* args, void* stream);
 
 /*
+ * Rows (group_rows 1) or weights (group_rows 128) in 8 bits: values = x / scale in e4m3 and a scale - the largest magnitude / 448, 0 for zeros - for each
+ * 128 columns of group_rows rows; the last groups may be smaller.
+ */
+typedef struct TrisQuantizeE4m3 {
+  const void* x;
+  void* values;
+  float* scales;                    /* [ceil(rows / group_rows), ceil(columns / 128)]      */
+  int64_t x_stride, values_stride, scales_stride;   /* elements between rows              */
+  int32_t rows;
+  int32_t columns;
+  int32_t group_rows;
+  int32_t dtype;                    /* of x: F16 or BF16                                   */
+} TrisQuantizeE4m3;
+int tris_quantize_e4m3(const TrisQuantizeE4m3* args, void* stream);
+
+/*
+ * out[t, n] = sum over k of x[t, k] * x_scales[t, k / 128] * weight[n, k] * weight_scales[n / 128, k / 128], plus bias[n]: e4m3 values, sums in fp32, one
+ * rounding.  Rows of x and weight start on 16-byte boundaries; any sizes from one column on.
+ */
+typedef struct TrisE4m3Linear {
+  const void* x;                    /* e4m3 [rows, in_features]                            */
+  const float* x_scales;            /* [rows, ceil(in_features / 128)]                     */
+  const void* weight;               /* e4m3 [out_features, in_features]                    */
+  const float* weight_scales;       /* [ceil(out_features / 128), ceil(in_features / 128)] */
+  const void* bias;                 /* [out_features] or NULL                              */
+  void* out;                        /* [rows, out_features]                                */
+  int32_t* status_dev;              /* optional, sticky: TRIS_ERR_TIMEOUT where a bounded wait ran out; the tile is NaN then */
+  int64_t x_stride, x_scales_stride, weight_stride, weight_scales_stride, out_stride;
+  int32_t rows;
+  int32_t in_features;
+  int32_t out_features;
+  int32_t dtype;                    /* of out: F16, BF16 or F32                            */
+  int32_t bias_dtype;               /* F16, BF16 or F32                                    */
+  int32_t reserved0;
+} TrisE4m3Linear;
+int tris_e4m3_linear(const TrisE4m3Linear* args, void* stream);
+
+/*
  * Controls on logits before a token is chosen, in this order, each optional (NULL):
  *   repetition[b] > 0: logits of tokens in tokens[b, 0 .. token_lengths[b]) are divided by it where positive, else multiplied
  *   frequency[b], presence[b]: z -= frequency * n + presence * (n > 0), n = how often the token occurs from prompt_lengths[b] on

@@ -52,6 +52,7 @@ from .decode_ops import (  # noqa: F401
     paged_decode_attention,
     raise_on_status,
 )
+from .e4m3_ops import linear_e4m3, quantize_e4m3  # noqa: F401
 from . import clocks, envflags, expert_parallel, synth  # noqa: F401
 
 __all__ = [
@@ -59,7 +60,9 @@ __all__ = [
     "add_rms_norm_e4m3",
     "append_paged_kv",
     "apply_logit_controls",
+    "linear_e4m3",
     "paged_decode_attention",
+    "quantize_e4m3",
     "raise_on_status",
     "Packed4Linear",
     "build_grouped_ns_compensation_payload",

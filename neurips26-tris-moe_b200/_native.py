@@ -137,6 +137,21 @@ class TrisAddRmsNorm(C.Structure):
     ]
 
 
+class TrisQuantizeE4m3(C.Structure):
+    _fields_ = [
+        ("x", _vp), ("values", _vp), ("scales", _vp), ("x_stride", _i64), ("values_stride", _i64), ("scales_stride", _i64),
+        ("rows", _i32), ("columns", _i32), ("group_rows", _i32), ("dtype", _i32),
+    ]
+
+
+class TrisE4m3Linear(C.Structure):
+    _fields_ = [
+        ("x", _vp), ("x_scales", _vp), ("weight", _vp), ("weight_scales", _vp), ("bias", _vp), ("out", _vp), ("status_dev", _vp),
+        ("x_stride", _i64), ("x_scales_stride", _i64), ("weight_stride", _i64), ("weight_scales_stride", _i64), ("out_stride", _i64),
+        ("rows", _i32), ("in_features", _i32), ("out_features", _i32), ("dtype", _i32), ("bias_dtype", _i32), ("reserved0", _i32),
+    ]
+
+
 class TrisLogitControls(C.Structure):
     _fields_ = [
         ("logits", _vp), ("out", _vp), ("tokens", _vp), ("token_lengths", _vp), ("prompt_lengths", _vp),
@@ -209,6 +224,8 @@ SIGNATURES = {
     "tris_paged_decode_attention_workspace_bytes": (C.c_size_t, [_vp, _i32, _i32]),
     "tris_paged_decode_attention": (C.c_int, [_vp, _vp, _vp]),
     "tris_add_rms_norm": (C.c_int, [_vp, _vp]),
+    "tris_quantize_e4m3": (C.c_int, [_vp, _vp]),
+    "tris_e4m3_linear": (C.c_int, [_vp, _vp]),
     "tris_logit_controls": (C.c_int, [_vp, _vp]),
     "tris_moe_layer_forward_static": (C.c_int, [_P(TrisMoeLayerView), _vp, _vp, _i32, _vp, _vp, _vp]),
 }

@@ -1,4 +1,5 @@
-// What the kernels of the decode step around the experts share (paged_kv.cu, paged_attention.cu, rms_norm.cu, logit_controls.cu):
+// What the kernels of the decode step around the experts share (paged_kv.cu, paged_attention.cu, rms_norm.cu, logit_controls.cu,
+// e4m3_linear.cu, quantize_e4m3.cu, sample_tokens.cu):
 // element types, conversions and stores of eight values, quotients by a scale.
 #pragma once
 #include <cuda_bf16.h>
@@ -118,6 +119,54 @@ struct DivideBy {
     }
   }
 };
+
+// The larger magnitude, or NaN where there is one.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float m;
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+// Magnitudes as bits: they order like the numbers, and a NaN is the largest.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+// A vector of a group whose largest magnitude has these bits, in place, by the group's scale, and that.  Two-part reciprocals of 448 and of the scale give
+// both quotients as divisions round them, at nine instructions a vector and one an element; a scale of 0 has nothing but zeros.
+__device__ __forceinline__ float quantize_8(float (&y)[8], uint32_t top) {
+  constexpr float hi = 1.f / kE4m3Max, lo = static_cast<float>(1.0 / kE4m3Max - hi);
+  constexpr uint32_t least = 67u << 23, most = 187u << 23;  // 2^-60 and 2^60
+  const float largest = __uint_as_float(top);
+  if (top - least <= most - least) {
+    const float scale = fmaf(largest, hi, largest * lo), up = reciprocal(scale);
+    DivideBy::by_parts(y, up, DivideBy::second_part(up, scale));
+    return scale;
+  }
+  const float scale = largest / kE4m3Max;
+  if (scale != 0.f) DivideBy{scale}(y, largest);
+  return scale;
+}
+// A cluster of CTAs and one another's shared memory.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t local, uint32_t rank) {  // a shared-memory address in another CTA of the cluster
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ float4 load_cluster_4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 load_cluster_2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float load_cluster(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
 
 // launch_kernel, by the plain launch where nothing else is asked for: 0.6 us less of the host's time (2.8 against 3.4).
 template <typename... KArgs, typename... Args>

@@ -99,24 +99,6 @@ __device__ __forceinline__ void two_parts(float a, float b, uint32_t& most, uint
 }
 
 constexpr int kMostCluster = 8;
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t in_cta(uint32_t local, uint32_t rank) {  // a shared-memory address in another CTA of the cluster
-  uint32_t at;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
-  return at;
-}
-__device__ __forceinline__ float4 load_cluster_4(uint32_t at) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ float2 load_cluster_2(uint32_t at) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
-  return v;
-}
 
 // Tokens [lo, hi) of a sequence; its blocks begin at multiples of kBlock.
 struct Span {

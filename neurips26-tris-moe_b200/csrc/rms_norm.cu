@@ -36,35 +36,12 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
   return v;
 }
-// The larger magnitude, or NaN where there is one.
-__device__ __forceinline__ float max_or_nan(float a, float b) {
-  float m;
-  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
-  return m;
-}
-// Magnitudes as bits: they order like the numbers, and a NaN is the largest.
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
   v = __reduce_max_sync(0xFFFFFFFFu, v);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   const int lane = threadIdx.x & 31;
   return __reduce_max_sync(0xFFFFFFFFu, lane < static_cast<int>(blockDim.x >> 5) ? red[lane] : 0);
-}
-// A vector of a group whose largest magnitude has these bits, in place, by the group's scale, and that.  Two-part reciprocals of 448 and of the scale give
-// both quotients as divisions round them, at nine instructions a vector and one an element; a scale of 0 has nothing but zeros.
-__device__ __forceinline__ float quantize_8(float (&y)[8], uint32_t top) {
-  constexpr float hi = 1.f / kE4m3Max, lo = static_cast<float>(1.0 / kE4m3Max - hi);
-  constexpr uint32_t least = 67u << 23, most = 187u << 23;  // 2^-60 and 2^60
-  const float largest = __uint_as_float(top);
-  if (top - least <= most - least) {
-    const float scale = fmaf(largest, hi, largest * lo), up = reciprocal(scale);
-    DivideBy::by_parts(y, up, DivideBy::second_part(up, scale));
-    return scale;
-  }
-  const float scale = largest / kE4m3Max;
-  if (scale != 0.f) DivideBy{scale}(y, largest);
-  return scale;
 }
 // Rows of at most 8 * VECS * blockDim columns, all pointers and strides at 16-byte boundaries.
 template <typename T, bool FP8, int VECS>
