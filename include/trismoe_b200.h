@@ -905,6 +905,29 @@ typedef struct TrisLogitControls {
 } TrisLogitControls;
 int tris_logit_controls(const TrisLogitControls* args, void* stream);
 
+/*
+ * A token of each row.  In the order of falling logits (equal ones by rising index) a token is kept while its place is below top_k, the weights ahead of it
+ * are less than top_p times those of the first top_k, and its weight w = exp((z - max) / temperature) is at least min_p; of those kept, in the order of
+ * the vocabulary, the first is drawn whose running sum exceeds random times the whole.  temperature <= 0: the first of the largest.  Off: top_k <= 0,
+ * top_p >= 1, min_p <= 0, and NULL (temperature 1).  Weights are counted in units of 2^-46 of the largest (vocabularies beyond 65536: 2^-(62 - log2)).
+ * Logits of -inf and NaN are never drawn; a row without others gives -1.
+ */
+typedef struct TrisSampleTokens {
+  const void* logits;               /* [rows, vocab]                                       */
+  const float* random;              /* [rows], in [0, 1)                                   */
+  const float* temperature;         /* [rows] each, or NULL                                */
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t* out;                     /* [rows]                                              */
+  int64_t logits_stride;
+  int32_t rows;
+  int32_t vocab;
+  int32_t dtype;                    /* of the logits: F16, BF16 or F32                     */
+  int32_t reserved0;
+} TrisSampleTokens;
+int tris_sample_tokens(const TrisSampleTokens* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -51,6 +51,7 @@ from .decode_ops import (  # noqa: F401
     apply_logit_controls,
     paged_decode_attention,
     raise_on_status,
+    sample_tokens,
 )
 from .e4m3_ops import linear_e4m3, quantize_e4m3  # noqa: F401
 from . import clocks, envflags, expert_parallel, synth  # noqa: F401
@@ -64,6 +65,7 @@ __all__ = [
     "paged_decode_attention",
     "quantize_e4m3",
     "raise_on_status",
+    "sample_tokens",
     "Packed4Linear",
     "build_grouped_ns_compensation_payload",
     "run_grouped_ns_c1_forward",

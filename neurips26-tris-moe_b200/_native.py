@@ -161,6 +161,13 @@ class TrisLogitControls(C.Structure):
     ]
 
 
+class TrisSampleTokens(C.Structure):
+    _fields_ = [
+        ("logits", _vp), ("random", _vp), ("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp), ("out", _vp),
+        ("logits_stride", _i64), ("rows", _i32), ("vocab", _i32), ("dtype", _i32), ("reserved0", _i32),
+    ]
+
+
 # name -> (restype, argtypes); also the list of symbols include/trismoe_b200.h declares.
 _P = C.POINTER
 SIGNATURES = {
@@ -227,6 +234,7 @@ SIGNATURES = {
     "tris_quantize_e4m3": (C.c_int, [_vp, _vp]),
     "tris_e4m3_linear": (C.c_int, [_vp, _vp]),
     "tris_logit_controls": (C.c_int, [_vp, _vp]),
+    "tris_sample_tokens": (C.c_int, [_vp, _vp]),
     "tris_moe_layer_forward_static": (C.c_int, [_P(TrisMoeLayerView), _vp, _vp, _i32, _vp, _vp, _vp]),
 }
 STATIC_SCRATCH_BYTES = 8 << 20

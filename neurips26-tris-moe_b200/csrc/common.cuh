@@ -14,7 +14,7 @@ static_assert(sizeof(TrisSharedExpert) == 32, "TrisSharedExpert layout is part o
 static_assert(sizeof(TrisPageLaunch) == 24, "TrisPageLaunch layout is part of the ABI");
 static_assert(sizeof(TrisPagedLayer) == 1472, "TrisPagedLayer layout is part of the ABI");
 static_assert(sizeof(TrisPagedKv) == 136 && sizeof(TrisPagedAppend) == 152 && sizeof(TrisPagedAttention) == 80, "layouts are part of the ABI");
-static_assert(sizeof(TrisQuantizeE4m3) == 64 && sizeof(TrisE4m3Linear) == 120, "layouts are part of the ABI");
+static_assert(sizeof(TrisQuantizeE4m3) == 64 && sizeof(TrisE4m3Linear) == 120 && sizeof(TrisSampleTokens) == 80, "layouts are part of the ABI");
 static_assert(sizeof(TrisAddRmsNorm) == 104 && sizeof(TrisLogitControls) == 152, "layouts are part of the ABI");
 
 namespace tris {

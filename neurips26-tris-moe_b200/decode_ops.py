@@ -33,6 +33,7 @@ _APPEND = struct.Struct("@3Q6q6Q8i")
 _ATTENTION = struct.Struct("@Q2q4Qq3if")
 _NORM = struct.Struct("@6Q4q5if")
 _LOGITS = struct.Struct("@11Q5q6i")
+_SAMPLE = struct.Struct("@7Qq4i")
 _NO_GRADIENT = "an input requires a gradient, and there is none: call it under torch.no_grad(), or with detached tensors"
 # (device, sizes) -> a byte seen as many, whose like is the scratch of a call; None where there is none to have
 _scratch: dict = {}
@@ -329,4 +330,35 @@ def apply_logit_controls(logits: torch.Tensor, *, tokens: Optional[torch.Tensor]
                         ids, values, mask, logits.stride(0), out.stride(0), tok_stride, bias_stride, mask_stride,
                         rows, vocab, history, biases, _DTYPES[dtype], 0)
     _launch(what, "tris_logit_controls", dev, args)
+    return out
+
+
+def sample_tokens(logits: torch.Tensor, random: torch.Tensor, *, temperature: Optional[torch.Tensor] = None, top_k: Optional[torch.Tensor] = None,
+                  top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A token of each row of ``logits`` [rows, vocab] (fp16, bf16 or fp32), drawn by ``random`` (fp32 [rows], in [0, 1)): int64 [rows].
+
+    A token's weight is ``exp((z - max) / temperature)``.  In the order of falling logits, equal ones by rising index, a token is kept while each of these
+    holds, and of those kept the first one in the vocabulary's order is drawn whose running sum of weights exceeds ``random`` times the whole:
+
+    * ``top_k`` (int32 [rows]): fewer than ``top_k`` tokens are ahead of it; 0 or less: off;
+    * ``top_p`` (fp32 [rows]): the weights ahead of it are less than ``top_p`` times those that ``top_k`` leaves; 1 or more: off, the first is always kept;
+    * ``min_p`` (fp32 [rows]): its weight is at least ``min_p`` times the largest; 0 or less: off.
+
+    ``temperature`` (fp32 [rows], default 1): 0 or less takes the first of the largest logits.  Weights are counted in units of 2^-46 of the
+    largest, so the sums are exact and a draw is the same on every run.  Logits of -inf and NaN are never drawn; a row without any other gives -1."""
+    what = "sample_tokens"
+    dev = _same_device(what, logits, random, temperature, top_k, top_p, min_p)
+    shape, dtype = logits.shape, logits.dtype
+    if len(shape) != 2 or dtype not in _LOGIT_TYPES or (logits.stride(1) != 1 and shape[1] > 1):
+        _fail(what, "logits must be fp16, bf16 or fp32 [rows, vocab] with a row's logits side by side")
+    rows, vocab = shape
+    out = torch.empty((rows,), dtype=torch.int64, device=dev)
+    each, f32 = (rows,), torch.float32
+    args = _SAMPLE.pack(logits.data_ptr(), _want(what, "random", random, f32, each),
+                        0 if temperature is None else _want(what, "temperature", temperature, f32, each),
+                        0 if top_k is None else _want(what, "top_k", top_k, torch.int32, each),
+                        0 if top_p is None else _want(what, "top_p", top_p, f32, each),
+                        0 if min_p is None else _want(what, "min_p", min_p, f32, each),
+                        out.data_ptr(), logits.stride(0), rows, vocab, _DTYPES[dtype], 0)
+    _launch(what, "tris_sample_tokens", dev, args)
     return out
