@@ -742,6 +742,8 @@ enum { TRIS_DTYPE_F16 = 0, TRIS_DTYPE_BF16 = 1, TRIS_DTYPE_F32 = 2, TRIS_DTYPE_E
  * side).  Bases, and strides in bytes, are multiples of 16.  Token i of sequence b is in slot i % page_size of page
  * block_table[b * table_stride + i / page_size].
  * e4m3 pages hold x / scale of their head, saturated at +-448; without scales that is 1.
+ * With scale_tokens both scales are [num_pages, page_size / scale_tokens, num_kv_heads], one for each block of that many tokens of a page and head, and belong to the cache:
+ * an append writes them.  They are positive, from 2^-64 to 2^64.
  * status_dev (optional device int32, sticky) is set to TRIS_ERR_CORRUPT where a needed page is outside [0, num_pages), a position outside the
  * table or the rotation tables, or a length negative or above table_width * page_size.  Such tokens are not written, read as zeros, or cut off.
  */
@@ -750,7 +752,7 @@ typedef struct TrisPagedKv {
   void* v_pages;
   int64_t k_page_stride, k_token_stride, k_head_stride;
   int64_t v_page_stride, v_token_stride, v_head_stride;
-  const float* k_scale;             /* [num_kv_heads] or NULL; TRIS_DTYPE_E4M3 only       */
+  const float* k_scale;             /* [num_kv_heads] or NULL, or as scale_tokens says; TRIS_DTYPE_E4M3 only */
   const float* v_scale;
   const int32_t* block_table;       /* [num_sequences, table_width]                        */
   int64_t table_stride;             /* entries between two sequences                       */
@@ -761,7 +763,7 @@ typedef struct TrisPagedKv {
   int32_t num_kv_heads;
   int32_t head_dim;
   int32_t dtype;                    /* F16, BF16 (that of the rows) or E4M3                */
-  int32_t reserved0;
+  int32_t scale_tokens;             /* 0: a scale for each head; else tokens of a block, of which page_size is a multiple */
   int32_t* status_dev;
 } TrisPagedKv;
 
@@ -770,6 +772,9 @@ typedef struct TrisPagedKv {
  * sequences[t] (NULL: t; num_tokens is at most num_sequences then) and stands at positions[t]; a negative position is padding: nothing is written to the cache, its rows of q_out
  * and k_out are zeros.  The first rotary_dim dimensions of q and k are rotated by the position's row of cos / sin
  * [max_positions, rotary_dim / 2] - pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved - in fp32 and rounded once.
+ * Scales of blocks: a block's scale is the smallest power of two by which its finite values stay within 448.  A token at the block's first place begins it anew;
+ * one behind makes the scale larger where it has to, and the tokens ahead of it are brought to the new scale (exact, but for what falls below
+ * the smallest number of e4m3).  The tokens of one block follow one another in the call, in the order of their positions.
  */
 typedef struct TrisPagedAppend {
   const void* q;                    /* NULL (with num_q_heads 0): keys and values only     */

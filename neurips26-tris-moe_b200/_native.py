@@ -106,7 +106,7 @@ class TrisPagedKv(C.Structure):
         ("v_page_stride", _i64), ("v_token_stride", _i64), ("v_head_stride", _i64),
         ("k_scale", _vp), ("v_scale", _vp), ("block_table", _vp), ("table_stride", _i64),
         ("num_sequences", _i32), ("table_width", _i32), ("num_pages", _i32), ("page_size", _i32),
-        ("num_kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32), ("reserved0", _i32), ("status_dev", _vp),
+        ("num_kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32), ("scale_tokens", _i32), ("status_dev", _vp),
     ]
 
 

@@ -1,4 +1,4 @@
-// What the kernels of the decode step around the experts share (paged_kv.cu, paged_attention.cu, rms_norm.cu, logit_controls.cu,
+// What the kernels of the decode step around the experts share (paged_kv.cu, paged_kv_blocks.cu, paged_attention.cu, rms_norm.cu, logit_controls.cu,
 // e4m3_linear.cu, quantize_e4m3.cu, sample_tokens.cu):
 // element types, conversions and stores of eight values, quotients by a scale.
 #pragma once
@@ -201,5 +201,6 @@ inline int sm_count() {
 inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline int dtype_size(int dtype) { return dtype == TRIS_DTYPE_F32 ? 4 : dtype == TRIS_DTYPE_E4M3 ? 1 : 2; }
 int validate_paged_kv(const TrisPagedKv* cache, const char* what);  // paged_kv.cu
+int append_block_scaled(const TrisPagedKv& cache, const TrisPagedAppend& rows, int rotary_dim, cudaStream_t stream);  // paged_kv_blocks.cu
 
 }  // namespace tris

@@ -45,6 +45,8 @@ struct AttnArgs {
   int ctas;         // of the first kernel
   int resident;     // of them, at one time
   int rows_together;  // whether a head's rows in a page are side by side
+  int scale_shift;    // log2 of the tokens of a scale, or -1
+  int page_scales;    // scales of a page and head
   float* part_o;    // [2 * ctas][tile_heads][head_dim]
   float* part_ml;   // [2 * ctas][tile_heads][2]
 };
@@ -70,6 +72,9 @@ __device__ __forceinline__ uint32_t e4m3_to_h2(uint32_t two) {
 }
 __device__ __forceinline__ void cp_async_16_at(uint32_t dst, const void* src, int bytes) {  // bytes: 16, or 0 for zeros
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_4_at(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 // 2^x; results below 2^-126 are 0.
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -171,7 +176,7 @@ struct Cursor {
   __device__ __forceinline__ int token() const { return (span.first() + blk) * kBlock; }
 };
 
-// T: type of q and out.  FP8: e4m3 pages, multiplied as fp16.  DP: head_dim rounded up to 64, 128 or 256.  NT: tiles of 8 query heads.
+// T: type of q and out.  FP8: e4m3 pages, multiplied as fp16.  SB: their scales belong to blocks of tokens and heads, not to heads.  DP: head_dim rounded up to 64, 128 or 256.  NT: tiles of 8 query heads.
 // CTAs on an SM, of which some compute while others start or end.  Pages in 8 bits are bound by instructions that wait for one another, so as many as
 // the registers allow (13 x 49925 tokens of heads of 64: 44 us with three or four, 64 with two); in 16 bits two with a deep ring (32 x 512-768 of heads
 // of 128: 34 us, 41 with three and two stages), and one where a step takes 16 KB.
@@ -180,7 +185,7 @@ constexpr int ctas_per_sm(int dp, bool fp8, int nt) {
   if (dp == 128) return fp8 && nt == 1 ? 3 : 2;
   return fp8 ? 2 : 1;
 }
-template <typename T, bool FP8, int DP, int NT, int W>
+template <typename T, bool FP8, bool SB, int DP, int NT, int W>
 struct Shape {
   static constexpr int kElems = FP8 ? 16 : 8;                          // of a 16-byte chunk
   static constexpr int kKeyChunks = DP / kElems / 4;                   // of a key row that a lane has
@@ -190,7 +195,8 @@ struct Shape {
   static constexpr int kRowChunks = kRowBytes / 16;
   static constexpr int kCopyRows = kRowChunks > 32 ? 1 : 32 / kRowChunks;  // rows that 32 lanes copy at once, 16 bytes each
   static constexpr int kTile = kBlock * kRowBytes;                     // 16 rows of keys or of values
-  static constexpr int kStageBytes = 2 * kTile;
+  static constexpr int kScales = 2 * kTile;                            // where a stage has its 16 tokens' scales, of keys and of values
+  static constexpr int kStageBytes = kScales + (SB ? 2 * kBlock * 4 : 0);
   // Chunk that holds a row's chunk in shared memory, XORed: eight lanes that read together - keys: rows of both parities, four neighbouring
   // chunks; values: rows 2 t, two neighbouring chunks - find eight different 16-byte columns.  (64-byte rows: two lanes a column for values, of which
   // a lane has 8 bytes.)
@@ -218,9 +224,9 @@ struct Piece {
   int used;
 };
 
-template <typename T, bool FP8, int DP, int NT, int W>
-__global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) paged_attention_kernel(const __grid_constant__ AttnArgs a) {
-  using S = Shape<T, FP8, DP, NT, W>;
+template <typename T, bool FP8, bool SB, int DP, int NT, int W>
+__global__ void __launch_bounds__(W * 32, Shape<T, FP8, SB, DP, NT, W>::kCtasPerSm) paged_attention_kernel(const __grid_constant__ AttnArgs a) {
+  using S = Shape<T, FP8, SB, DP, NT, W>;
   using M = std::conditional_t<FP8, __half, T>;  // type of the products
   constexpr int kElt = FP8 ? 1 : 2;
   // Range of the weights, to base 2.  bf16 ones are not lifted: they lose nothing below 1, and values may go up to the end of 32 bits themselves.
@@ -297,7 +303,7 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
   float m[NT][2], l[NT][2], acc[S::kDimTiles][NT][4];
   auto fetch_query = [&] {
     const int head = use.item / a.row_tiles, tile = use.item % a.row_tiles;
-    scale[0][0] = FP8 && c.k_scale ? c.k_scale[head] : 1.f;
+    scale[0][0] = FP8 && !SB && c.k_scale ? c.k_scale[head] : 1.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int row = tile * S::kHeads + 8 * n + g;
@@ -427,6 +433,15 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
           cp_async_16_at(dst + (v_to ^ (S::value_swizzle(i * S::kCopyRows) << 4)) + S::kTile + i * 512, ok ? v_pages + off + copy_chunk * 16 : v_pages, ok ? 16 : 0);
         }
       }
+      if constexpr (SB) {
+        // each lane brings the scale of one token: keys' in the first half, values' in the other
+        const int tok = tok0 + (lane & 15);
+        const bool there = page >= 0 && tok >= load.span.lo && tok < load.span.hi;
+        const int in_page = a.page_shift >= 0 ? tok & (c.page_size - 1) : tok % c.page_size;
+        const int block = a.scale_shift >= 0 ? in_page >> a.scale_shift : in_page / c.scale_tokens;
+        const float* src = (lane < 16 ? c.k_scale : c.v_scale) + (there ? (static_cast<int64_t>(page) * a.page_scales + block) * c.num_kv_heads + head : 0);
+        cp_async_4_at(dst + S::kScales + 4 * lane, src, there ? 4 : 0);
+      }
       if (--left > 0) {
         load.next(a);
         page = page_of(load);
@@ -442,7 +457,7 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
   // The result of an item that this warp has had alone goes out; otherwise its piece is left for the other warps' (to != nullptr).
   auto write_item = [&](float* to) {
     const int head = use.item / a.row_tiles, tile = use.item % a.row_tiles;
-    const float v_scale = FP8 && c.v_scale ? c.v_scale[head] : 1.f;
+    const float v_scale = FP8 && !SB && c.v_scale ? c.v_scale[head] : 1.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -554,10 +569,26 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
     // Tokens g and g + 8 of heads 2 t and 2 t + 1.  Weights are 2^(s - m); m is the largest score so far less kLift when it moves, and moves only when
     // a score exceeds it by more than kMostWeight, which is rare after the first blocks.  Of fp16 the largest weight is so between 2^7 and
     // 2^15 (the type ends below 2^16), and weights down to 2^-21 of it have all of its bits; sums in 32 bits are as exact at any scale.
+    // With scales of blocks a token's weight in the sum over the values has its value scale in it, 2^e * f with f in [1/2, 1): m follows s + e, so that it is that
+    // weight which keeps its bits, whatever the scales of other blocks are; the sum l is of 2^(s - m).
+    float key_scale[2] = {1.f, 1.f}, value_part[2] = {1.f, 1.f}, lift[2] = {0.f, 0.f};
+    if constexpr (SB) {
+      const float* scales = reinterpret_cast<const float*>(src + S::kScales);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        key_scale[h] = scales[g + 8 * h];
+        const uint32_t bits = __float_as_uint(fminf(fmaxf(scales[kBlock + g + 8 * h], 0x1p-64f), 0x1p64f));
+        lift[h] = static_cast<float>(static_cast<int>(bits >> 23) - 126);
+        value_part[h] = __uint_as_float((bits & 0x7FFFFFu) | (126u << 23));
+      }
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s[n][k] = (s[n][k] + s_odd[n][k]) * scale[n][k & 1];
+      for (int k = 0; k < 4; ++k) {
+        s[n][k] = (s[n][k] + s_odd[n][k]) * scale[n][k & 1];
+        if constexpr (SB) s[n][k] = fmaf(s[n][k], key_scale[k >> 1], lift[k >> 1]);
+      }
     const int tok = use.token();
     if (tok < use.span.lo || tok + kBlock > use.span.hi) {
       const bool in0 = tok + g >= use.span.lo && tok + g < use.span.hi, in1 = tok + g + 8 >= use.span.lo && tok + g + 8 < use.span.hi;
@@ -606,10 +637,21 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, DP, NT, W>::kCtasPerSm) 
     uint32_t p[NT][2], rest[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      if constexpr (SB) {
+        float plain[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[n][k] = exp2_fast(x[n][k]);
-      l[n][0] += x[n][0] + x[n][2];
-      l[n][1] += x[n][1] + x[n][3];
+        for (int k = 0; k < 4; ++k) {
+          plain[k] = exp2_fast(x[n][k] - lift[k >> 1]);
+          x[n][k] = exp2_fast(x[n][k]) * value_part[k >> 1];
+        }
+        l[n][0] += plain[0] + plain[2];
+        l[n][1] += plain[1] + plain[3];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[n][k] = exp2_fast(x[n][k]);
+        l[n][0] += x[n][0] + x[n][2];
+        l[n][1] += x[n][1] + x[n][3];
+      }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         if constexpr (kTwoParts) {
@@ -891,12 +933,12 @@ int head_tiles(const TrisPagedKv& c, int group, int window) {
 }
 size_t part_floats(int ctas, int tile_heads, int head_dim) { return 2 * static_cast<size_t>(ctas) * tile_heads * (head_dim + 2); }
 
-template <typename T, bool FP8, int DP, int NT>
+template <typename T, bool FP8, bool SB, int DP, int NT>
 int launch_attention(AttnArgs& a, cudaStream_t stream) {
-  using S = Shape<T, FP8, DP, NT, kWarps>;
-  auto kernel = paged_attention_kernel<T, FP8, DP, NT, kWarps>;
+  using S = Shape<T, FP8, SB, DP, NT, kWarps>;
+  auto kernel = paged_attention_kernel<T, FP8, SB, DP, NT, kWarps>;
   const TrisPagedKv& c = a.cache;
-  if (int st = allow_shared_memory<paged_attention_kernel<T, FP8, DP, NT, kWarps>>(S::kMostSmem)) return st;
+  if (int st = allow_shared_memory<paged_attention_kernel<T, FP8, SB, DP, NT, kWarps>>(S::kMostSmem)) return st;
   TRIS_REQUIRE(sm_count() > 0, TRIS_ERR_CUDA, "paged_decode_attention: no device");
   a.resident = resident_ctas(c.head_dim, FP8, NT);
   a.rows_together = a.page_blocks && c.head_dim == DP && c.k_token_stride == DP && c.v_token_stride == DP;
@@ -904,9 +946,9 @@ int launch_attention(AttnArgs& a, cudaStream_t stream) {
   a.cluster = cluster_size(c, a.row_tiles, a.query.window, a.resident);
   const dim3 items(c.num_kv_heads * a.row_tiles, c.num_sequences, a.cluster);
   if (a.cluster == 1 && two_warps(c, a.row_tiles, a.query.window, a.resident)) {
-    using P = Shape<T, FP8, DP, NT, 2>;
-    if (int st = allow_shared_memory<paged_attention_kernel<T, FP8, DP, NT, 2>>(P::kMostSmem)) return st;
-    TRIS_CUDA(launch_step(paged_attention_kernel<T, FP8, DP, NT, 2>, items, dim3(64), P::kMostSmem, stream, pdl, 1, a));
+    using P = Shape<T, FP8, SB, DP, NT, 2>;
+    if (int st = allow_shared_memory<paged_attention_kernel<T, FP8, SB, DP, NT, 2>>(P::kMostSmem)) return st;
+    TRIS_CUDA(launch_step(paged_attention_kernel<T, FP8, SB, DP, NT, 2>, items, dim3(64), P::kMostSmem, stream, pdl, 1, a));
     return TRIS_OK;
   }
   if (a.cluster) {
@@ -923,11 +965,11 @@ int launch_attention(AttnArgs& a, cudaStream_t stream) {
   TRIS_CUDA(launch_step(paged_attention_join_kernel<T>, dim3(a.query.num_q_heads, c.num_sequences), dim3(kJoinThreads), 0, stream, true, 1, a, S::kHeads));
   return TRIS_OK;
 }
-template <typename T, bool FP8>
+template <typename T, bool FP8, bool SB>
 int launch_shape(AttnArgs& a, int tiles, cudaStream_t stream) {
   const int d = a.cache.head_dim;
-  if (tiles == 2) return d <= 64 ? launch_attention<T, FP8, 64, 2>(a, stream) : launch_attention<T, FP8, 128, 2>(a, stream);
-  return d <= 64 ? launch_attention<T, FP8, 64, 1>(a, stream) : d <= 128 ? launch_attention<T, FP8, 128, 1>(a, stream) : launch_attention<T, FP8, 256, 1>(a, stream);
+  if (tiles == 2) return d <= 64 ? launch_attention<T, FP8, SB, 64, 2>(a, stream) : launch_attention<T, FP8, SB, 128, 2>(a, stream);
+  return d <= 64 ? launch_attention<T, FP8, SB, 64, 1>(a, stream) : d <= 128 ? launch_attention<T, FP8, SB, 128, 1>(a, stream) : launch_attention<T, FP8, SB, 256, 1>(a, stream);
 }
 
 }  // namespace
@@ -975,6 +1017,13 @@ extern "C" int tris_paged_decode_attention(const TrisPagedKv* cache, const TrisP
     if (c.page_size == 1 << s) a.page_shift = s;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool q8 = c.dtype == TRIS_DTYPE_E4M3;
-  if (q.dtype == TRIS_DTYPE_F16) return q8 ? launch_shape<__half, true>(a, tiles, s) : launch_shape<__half, false>(a, tiles, s);
-  return q8 ? launch_shape<__nv_bfloat16, true>(a, tiles, s) : launch_shape<__nv_bfloat16, false>(a, tiles, s);
+  a.scale_shift = -1;
+  if (c.scale_tokens) {
+    a.page_scales = c.page_size / c.scale_tokens;
+    for (int i = 0; i < 31; ++i)
+      if (c.scale_tokens == 1 << i) a.scale_shift = i;
+    return q.dtype == TRIS_DTYPE_F16 ? launch_shape<__half, true, true>(a, tiles, s) : launch_shape<__nv_bfloat16, true, true>(a, tiles, s);
+  }
+  if (q.dtype == TRIS_DTYPE_F16) return q8 ? launch_shape<__half, true, false>(a, tiles, s) : launch_shape<__half, false, false>(a, tiles, s);
+  return q8 ? launch_shape<__nv_bfloat16, true, false>(a, tiles, s) : launch_shape<__nv_bfloat16, false, false>(a, tiles, s);
 }

@@ -25,6 +25,12 @@ int validate_paged_kv(const TrisPagedKv* c, const char* what) {
   const int sizes[3] = {c->num_pages, c->page_size, c->num_kv_heads};
   for (int i = 0; i < 6; ++i)  // of a size of 1 the stride is of no account
     TRIS_REQUIRE(sizes[i / 2] <= 1 || (strides[i] >= 0 && strides[i] * elt % 16 == 0), TRIS_ERR_UNSUPPORTED, "%s: strides of the pages must be multiples of 16 bytes", what);
+  TRIS_REQUIRE(c->scale_tokens >= 0, TRIS_ERR_INVALID_ARG, "%s: negative scale_tokens", what);
+  if (c->scale_tokens) {
+    TRIS_REQUIRE(c->dtype == TRIS_DTYPE_E4M3 && c->page_size % c->scale_tokens == 0, TRIS_ERR_INVALID_ARG, "%s: blocks of %d tokens belong to e4m3 pages of a multiple of that (%d)", what,
+                 c->scale_tokens, c->page_size);
+    TRIS_REQUIRE((c->k_scale && c->v_scale) || c->num_pages == 0, TRIS_ERR_INVALID_ARG, "%s: null scales of blocks", what);
+  }
   TRIS_REQUIRE(aligned_to(c->k_pages, 16) && aligned_to(c->v_pages, 16), TRIS_ERR_UNSUPPORTED, "%s: pages must start on a 16-byte boundary", what);
   return TRIS_OK;
 }
@@ -237,6 +243,7 @@ extern "C" int tris_paged_kv_append(const TrisPagedKv* cache, const TrisPagedApp
   TRIS_REQUIRE((r.q && r.q_out) || r.num_q_heads == 0, TRIS_ERR_INVALID_ARG, "paged_kv_append: null q or q_out");
   TRIS_REQUIRE(r.k && r.v && r.positions, TRIS_ERR_INVALID_ARG, "paged_kv_append: null k, v or positions");
 
+  if (c.scale_tokens) return append_block_scaled(c, r, rot, static_cast<cudaStream_t>(stream));
   AppendArgs a{c, r, 0, 1};
   a.rows.rotary_dim = rot;
   // 16-byte accesses need rows that start on such boundaries and chunks of 8 that do not straddle the halves or the rotated part

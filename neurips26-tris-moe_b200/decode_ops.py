@@ -11,7 +11,9 @@ Nor is there a backward pass: where gradients are recorded, inputs that require 
 Pages.  ``k_pages`` and ``v_pages`` are ``[num_pages, page_size, num_kv_heads, head_dim]`` with any
 strides that are multiples of 16 bytes and the head's dimensions side by side; fastest is one where a head's tokens of a page
 are, too (allocate ``[num_pages, num_kv_heads, page_size, head_dim]`` and pass ``.transpose(1, 2)``).  They hold the
-rows' type (fp16 or bf16) or ``torch.float8_e4m3fn`` with one scale per head.  Token ``i`` of sequence ``b`` is in page
+rows' type (fp16 or bf16) or ``torch.float8_e4m3fn`` with one scale per head or, ``k_scale`` and ``v_scale`` [num_pages, blocks, num_kv_heads] in
+fp32, one for each of ``blocks`` equal parts of a page and head: these belong to the cache, are written by ``append_paged_kv``, and need no
+calibration.  Token ``i`` of sequence ``b`` is in page
 ``block_table[b, i // page_size]``.  ``status`` is an optional int32 tensor of one element, zero
 at first: a page, position or length that does not fit sets it (``raise_on_status``).
 """
@@ -109,12 +111,18 @@ def _cache(what: str, k_pages, v_pages, block_table, k_scale, v_scale, status) -
         _fail(what, "block_table must have the pages of a sequence side by side")
     if (k_scale is not None or v_scale is not None) and dtype is not torch.float8_e4m3fn:
         _fail(what, "scales belong to e4m3 pages")
+    each, scale_tokens = (heads,), 0
+    if k_scale is not None and k_scale.dim() == 3:
+        blocks = k_scale.shape[1]
+        if v_scale is None or blocks == 0 or page_size % blocks:
+            _fail(what, f"scales of blocks go together, [{pages}, blocks, {heads}] with pages of {page_size} tokens cut evenly, got {tuple(k_scale.shape)}")
+        each, scale_tokens = (pages, blocks, heads), page_size // blocks
     packed = _PAGED_KV.pack(
         k_pages.data_ptr(), v_pages.data_ptr(), k0, k1, k2, v0, v1, v2,
-        0 if k_scale is None else _want(what, "k_scale", k_scale, torch.float32, (heads,)),
-        0 if v_scale is None else _want(what, "v_scale", v_scale, torch.float32, (heads,)),
+        0 if k_scale is None else _want(what, "k_scale", k_scale, torch.float32, each),
+        0 if v_scale is None else _want(what, "v_scale", v_scale, torch.float32, each),
         block_table.data_ptr(), t0, sequences, width, pages, page_size, heads, dim,
-        _DTYPES[dtype], 0, 0 if status is None else _want(what, "status", status, torch.int32, (1,)))
+        _DTYPES[dtype], scale_tokens, 0 if status is None else _want(what, "status", status, torch.int32, (1,)))
     return packed, (dtype, heads, dim, sequences, width, page_size)
 
 
@@ -137,7 +145,10 @@ def append_paged_kv(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     fine.  Token ``t`` belongs to sequence ``sequences[t]`` (int32; default: ``t``, of which the block table must have as many) and stands at ``positions[t]`` (int32 or
     int64; negative: padding, not written).  ``cos`` and ``sin`` [positions, rotary_dim / 2] in fp32 rotate the first ``rotary_dim``
     dimensions, pairs ``(i, i + rotary_dim / 2)`` or, ``interleaved``, ``(2 i, 2 i + 1)``; None: no rotation.  e4m3 pages get
-    ``x / scale``, saturated.  Tokens of one call must have different places.  Returns the rotated queries (None without ``q``),
+    ``x / scale``, saturated.  Tokens of one call must have different places.  Scales of blocks are written, too: the smallest power of two (2^-64 to 2^64) by which the
+    finite numbers of a block stay within 448.  A token at its block's first place begins it anew; one behind makes the scale larger where it has to, and
+    the block's tokens ahead of it are brought to that (exact, but for what falls below e4m3's smallest number).  In one call the tokens of a block follow one
+    another in the order of their positions.  Returns the rotated queries (None without ``q``),
     with ``return_key`` a pair with the rotated keys."""
     what = "append_paged_kv"
     dev = _same_device(what, k, v, q, k_pages, v_pages, block_table, positions, sequences, cos, sin, k_scale, v_scale, status)
