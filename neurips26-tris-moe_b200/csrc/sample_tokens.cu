@@ -4,19 +4,20 @@
 // p times those of the first k, and while its weight exp((z - max) / T) is at least min_p; of those kept, in the order of the vocabulary, the first
 // whose running sum exceeds u times the whole is drawn.  All three ends are one place in the order, so no order is made: a histogram over max - z
 // finds the interval in which the k-th token lies, or the one that ends the share p, and the few tokens of that interval are ranked one against another.
+// Where the first k tokens are few, all that follows is done on a list of them.
 //
 // Weights are integers, exp in units of 2^-46 of the largest (fewer bits for vocabularies beyond 65536): their sums are exact, so neither the order of
-// atomics nor that of threads counts, and u falls where it does in 64-bit arithmetic.  With 32-bit exponentials one row in some hundred would
-// draw a neighbour.  A row belongs to one CTA or, for few rows, to a cluster that cuts the vocabulary and reads one another's histograms; its logits are
-// read from memory once and some three times from L1.
+// atomics nor that of threads counts, and u falls where it does in 64-bit arithmetic.  (With 32-bit exponentials one row in some hundred would
+// draw a neighbour.)  A row belongs to one CTA or, for few rows, to a cluster that cuts the vocabulary and reads one another's histograms; its logits are
+// read from memory once and two or three times from L1.  Bound by instructions: some 30 for a weight, of which every token has one and every kept token two.
 #include "decode_step.cuh"
 
 namespace tris {
 namespace {
 
 constexpr int kThreads = 1024, kBins = kThreads, kFew = 256;
-constexpr int kMostCtas = 8;  // of a cluster
-constexpr int kTable = 256;   // powers 2^(i / kTable)
+constexpr int kMostCtas = 8;   // of a cluster
+constexpr int kTable = 1024;   // powers 2^(i / kTable)
 
 struct SampleArgs {
   TrisSampleTokens s;
@@ -82,17 +83,20 @@ __device__ __forceinline__ N scan(N v, N* red, N& total) {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid_constant__ SampleArgs args) {
-  __shared__ __align__(16) Histogram first, finer;
+  __shared__ union Buffer {
+    Histogram bins;
+    float kept[kThreads / 32][128];  // logits of a warp's tokens, one after the other
+  } buffer;
   __shared__ double powers[kTable];
+  __shared__ uint64_t sums[kThreads], red64[32], part;
   __shared__ uint64_t lists[2][kFew];  // tokens of the interval that was found, of this CTA
   __shared__ ulonglong2 merged[kFew];  // and of all, each with its weight
-  __shared__ uint32_t listed[2];
-  __shared__ uint64_t ends[2][2];  // the last and the first of them in the order, where they are many
+  __shared__ uint32_t listed[2], red32[32], best;
+  __shared__ uint64_t ends[2][2];  // the last and the first of them in the order
   __shared__ __align__(8) float extremes[2];
-  __shared__ uint64_t part, red64[32];
-  __shared__ uint32_t red32[32], best;
   __shared__ Found found;
-  __shared__ uint64_t cut, cut_weight;
+  __shared__ uint64_t cut;
+  Histogram& bins = buffer.bins;
   const TrisSampleTokens& s = args.s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.y;
@@ -102,9 +106,23 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
     else __syncthreads();
   };
   auto there = [&](const void* mine, int r) { return in_cta(smem_u32(mine), r); };
+  // The same word of every CTA of the cluster; all of them are asked for before the first has arrived.
+  auto words_of_all = [&](const uint32_t* mine, uint32_t (&v)[kMostCtas]) {
+#pragma unroll
+    for (int r = 0; r < kMostCtas; ++r) v[r] = 0;
+    if (ctas == 1) {
+      v[0] = *mine;
+      return;
+    }
+#pragma unroll
+    for (int r = 0; r < kMostCtas; ++r)
+      if (r < ctas) v[r] = load_cluster_u32(there(mine, r));
+  };
+  auto clear_bins = [&] { bins.count[tid] = bins.low[tid] = bins.high[tid] = 0; };
 
-  if (tid < kTable) powers[tid] = exp2(static_cast<double>(tid) / kTable);
-  first.count[tid] = first.low[tid] = first.high[tid] = 0;
+  powers[tid] = exp2(static_cast<double>(tid) / kTable);
+  static_assert(kTable == kThreads, "a power to a thread");
+  clear_bins();
   if (tid < 2) {
     listed[tid] = 0;
     ends[tid][0] = ~0ull;
@@ -114,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
   pdl_wait();
   pdl_launch_dependents();
   const T* in = static_cast<const T*>(s.logits) + row * s.logits_stride + v0;
-  // Four logits of the slice; what is not there, and what is not a number, is -inf.
+  // Four logits of the slice, -inf where there is none.  What is not a number fails every comparison below.
   auto fetch = [&](int at, float (&z)[4]) {
     if (args.wide && at + 4 <= n) {
       if constexpr (sizeof(T) == 4) {
@@ -129,47 +147,41 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
 #pragma unroll
       for (int k = 0; k < 4; ++k) z[k] = at + k < n ? to_float(in[at + k]) : -INFINITY;
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) z[k] = z[k] == z[k] ? z[k] : -INFINITY;
   };
   const float temperature = s.temperature ? s.temperature[row] : 1.f;
   const int top_k = s.top_k ? s.top_k[row] : 0;
   const float top_p = s.top_p ? s.top_p[row] : 1.f, min_p = s.min_p ? s.min_p[row] : 0.f;
+  const double u = fmax(static_cast<double>(s.random[row]), 0.);  // not a number: 0
 
-  // The largest logit, and the smallest that is one.
+  // The largest logit, and the smallest.
   float top = -INFINITY, low = INFINITY;
 #pragma unroll 4
   for (int at = 4 * tid; at < n; at += 4 * kThreads) {
     float z[4];
     fetch(at, z);
+    top = fmaxf(fmaxf(fmaxf(top, z[0]), fmaxf(z[1], z[2])), z[3]);
+    low = fminf(fminf(fminf(low, z[0]), fminf(z[1], z[2])), z[3]);
+  }
+  auto all_lanes = [&] {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      top = fmaxf(top, z[k]);
-      if (z[k] > -INFINITY) low = fminf(low, z[k]);
+    for (int d = 16; d; d >>= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+      low = fminf(low, __shfl_xor_sync(0xFFFFFFFFu, low, d));
     }
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    low = fminf(low, __shfl_xor_sync(0xFFFFFFFFu, low, d));
-  }
+  };
+  all_lanes();
   if (lane == 0) red64[warp] = (static_cast<uint64_t>(__float_as_uint(top)) << 32) | __float_as_uint(low);
   __syncthreads();
   top = __uint_as_float(static_cast<uint32_t>(red64[lane] >> 32));
   low = __uint_as_float(static_cast<uint32_t>(red64[lane]));
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    low = fminf(low, __shfl_xor_sync(0xFFFFFFFFu, low, d));
-  }
+  all_lanes();
   if (ctas > 1) {
     if (tid == 0) extremes[0] = top, extremes[1] = low;
     cluster_sync();
-    for (int r = 0; r < ctas; ++r) {
-      const float2 other = load_cluster_2(there(extremes, r));
-      top = fmaxf(top, other.x);
-      low = fminf(low, other.y);
-    }
+    float2 other = make_float2(top, low);
+    if (lane < ctas) other = load_cluster_2(there(extremes, lane));
+    top = other.x, low = other.y;
+    all_lanes();
   }
   if (top == -INFINITY) {  // nothing can be drawn
     if (blockIdx.z == 0 && tid == 0) s.out[row] = -1;
@@ -177,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
     return;
   }
 
-  if (!(temperature > 0.f) || top_k == 1 || top_p <= 0.f) {  // the first of the largest
+  if (!(temperature > 0.f) || top_k == 1 || top_p <= 0.f || top == INFINITY) {  // the first of the largest
     uint32_t mine = 0xFFFFFFFFu;
     for (int at = 4 * tid; at < n && mine == 0xFFFFFFFFu; at += 4 * kThreads) {
       float z[4];
@@ -198,220 +210,294 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
     return;
   }
 
-  // exp((z - top) / temperature) in units of 2^-bits.
-  const double per_unit = 1.4426950408889634074 / static_cast<double>(temperature);
+  // exp((z - top) / temperature) in units of 2^-bits.  (Rounded step by step, so that every place of the code finds the same weight.)
+  const double per_step = 1.4426950408889634074 * kTable / fmax(static_cast<double>(temperature), 1e-30);
+  const float per_power = static_cast<float>(per_step / kTable);
   auto weight_of = [&](float z) -> uint64_t {
-    if (z == top) return 1ull << args.bits;
-    // (rounded one by one, so that every place of the code finds the same weight)
-    const double y = __dmul_rn(static_cast<double>(z) - static_cast<double>(top), per_unit);
-    if (!(y > -60.)) return 0;
-    constexpr double kShift = 6755399441055744. / kTable;  // 1.5 * 2^52 / kTable: the last bit is 1 / kTable
-    const double t = __dadd_rn(y, kShift);
-    const int64_t steps = static_cast<int32_t>(__double_as_longlong(t));  // y * kTable, rounded
-    const double f = __dsub_rn(y, __dsub_rn(t, kShift));                   // up to 1 / (2 kTable)
-    // 2^f = sum of (f ln 2)^i / i!
-    const double p = fma(fma(fma(fma(9.6181291076284772e-3, f, 5.5504108664821580e-2), f, 2.4022650695910072e-1), f, 6.9314718055994531e-1), f, 1.);
-    const double w = __dmul_rn(powers[steps & (kTable - 1)], p);
-    const int64_t exponent = (steps >> 8) + args.bits;  // w * 2^exponent: the exponent's bits are added to
-    if (exponent < -2) return 0;
-    return static_cast<uint64_t>(__double2ull_rn(__longlong_as_double(__double_as_longlong(w) + (exponent << 52))));
+    if (!((z - top) * per_power > -50.f)) return 0;
+    constexpr double kRound = 6755399441055744.;  // 1.5 * 2^52: what is added to it is rounded to a whole number
+    const double y = __dmul_rn(static_cast<double>(z) - static_cast<double>(top), per_step);
+    const double t = __dadd_rn(y, kRound);
+    const int steps = __double2loint(t);
+    const double f = __dsub_rn(y, __dsub_rn(t, kRound));  // up to 1/2
+    // 2^(f / kTable) = sum of (f ln 2 / kTable)^i / i!
+    constexpr double c1 = 0.69314718055994531 / kTable, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;
+    const double w = __dmul_rn(powers[steps & (kTable - 1)], fma(fma(fma(c3, f, c2), f, c1), f, 1.));
+    static_assert(kTable == 1 << 10, "steps of a power");
+    const double scaled = __hiloint2double(__double2hiint(w) + (((steps >> 10) + args.bits) << 20), __double2loint(w));
+    return static_cast<uint64_t>(__double_as_longlong(__dadd_rn(scaled, 4503599627370496.))) & 0xFFFFFFFFFFFFFull;  // + 2^52
   };
-  static_assert(kTable == 256, "steps >> 8");
   const uint64_t least = min_p > 0.f ? static_cast<uint64_t>(ceil(fmin(static_cast<double>(min_p), 1.) * static_cast<double>(1ull << args.bits))) : 0;
+  // The tokens ahead of which less than p of `share` lies: weights that those ahead of the last one do not reach.
+  auto reach_of = [&](uint64_t share) {
+    const double to = ceil(static_cast<double>(top_p) * static_cast<double>(share));
+    return to <= 1. ? 1 : to >= static_cast<double>(share) ? share : static_cast<uint64_t>(to);
+  };
+  // What u falls on: the sum that the drawn token is the first to exceed.
+  auto target_of = [&](uint64_t whole) {
+    const double at = floor(u * static_cast<double>(whole));
+    return at >= static_cast<double>(whole) ? whole - 1 : min(static_cast<uint64_t>(at), whole - 1);
+  };
+  auto sum_of_all = [&](uint64_t v) {
+    uint64_t total;
+    scan(v, red64, total);
+    __syncthreads();
+    return total;
+  };
 
   uint64_t from = 0;  // the last place that is kept
   const bool by_count = top_k > 0 && top_k < s.vocab, by_weight = top_p < 1.f;
   if (by_count || by_weight) {
     const float range = fminf(40.f * temperature, top - low);
     const float per_bin = range > 0.f ? fminf(kBins / range, 1e30f) : 0.f;
-    auto bin_of = [&](float z) { return z == top ? 0 : static_cast<int>(fminf((top - z) * per_bin, kBins - 1.f)); };
-    auto enter = [&](Histogram& h, int bin, uint64_t w) {
-      atomicAdd(&h.count[bin], 1u);
+    auto bin_of = [&](float z) { return static_cast<int>(fminf((top - z) * per_bin, kBins - 1.f)); };
+    auto enter = [&](int bin, uint64_t w) {
       const uint32_t w_low = static_cast<uint32_t>(w);
       uint32_t w_high = static_cast<uint32_t>(w >> 32);
-      if (w_low) w_high += atomicAdd(&h.low[bin], w_low) + w_low < w_low;  // and what is carried
-      if (w_high) atomicAdd(&h.high[bin], w_high);
+      w_high += atomicAdd(&bins.low[bin], w_low) + w_low < w_low;  // and what is carried
+      if (w_high) atomicAdd(&bins.high[bin], w_high);
     };
-    // All CTAs' tokens and weights of bin `tid`, and those ahead of it.
-    uint32_t count, count_before, all_tokens;
-    uint64_t weight, weight_before, all_weight;
-    auto gather = [&](const Histogram& h) {
-      count = 0;
-      weight = 0;
-      for (int r = 0; r < ctas; ++r) {
-        count += load_cluster_u32(there(&h.count[tid], r));
-        weight += (static_cast<uint64_t>(load_cluster_u32(there(&h.high[tid], r))) << 32) + load_cluster_u32(there(&h.low[tid], r));
-      }
-      count_before = scan(count, red32, all_tokens);
-      weight_before = scan(weight, red64, all_weight);
-      __syncthreads();
-    };
+    // Adds to the list the tokens for which `inside` holds.
+    auto list_tokens = [&](int use, auto inside) {
+      uint64_t last = ~0ull, first = 0;
 #pragma unroll 2
-    for (int at = 4 * tid; at < n; at += 4 * kThreads) {
-      float z[4];
-      fetch(at, z);
+      for (int at = 4 * tid; at < n; at += 4 * kThreads) {
+        float z[4];
+        fetch(at, z);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (z[k] > -INFINITY) {
-          const uint64_t w = by_weight ? weight_of(z[k]) : 0;
-          if (by_count || w) enter(first, bin_of(z[k]), w);
+        for (int k = 0; k < 4; ++k)
+          if (inside(z[k], v0 + at + k)) {
+            const uint64_t place = place_of(z[k], v0 + at + k);
+            const uint32_t i = atomicAdd(&listed[use], 1u);
+            if (i < kFew) lists[use][i] = place;
+            last = min(last, place);
+            first = max(first, place);
+          }
+      }
+      if (first) {
+        atomicMin(reinterpret_cast<unsigned long long*>(&ends[use][0]), last);
+        atomicMax(reinterpret_cast<unsigned long long*>(&ends[use][1]), first);
+      }
+    };
+    // The lists of all CTAs as one, with weights; their number, or more than kFew.
+    auto merge_lists = [&](int use) {
+      uint32_t many[kMostCtas];
+      words_of_all(&listed[use], many);
+      uint32_t ahead = 0;
+#pragma unroll
+      for (int r = 0; r < kMostCtas; ++r) {
+        if (tid >= ahead && tid - ahead < min(many[r], kFew) && tid < kFew) {
+          const uint64_t place = ctas == 1 ? lists[use][tid] : load_cluster_u64(there(&lists[use][tid - ahead], r));
+          merged[tid] = make_ulonglong2(place, weight_of(logit_of(place)));
         }
-    }
-    meet();
-    gather(first);
-    const uint32_t count0 = count, count_before0 = count_before;
-    const uint64_t weight0 = weight, weight_before0 = weight_before;
+        ahead += many[r];
+      }
+      __syncthreads();
+      return ahead;
+    };
 
-    // The place of the token that is the count_to-th, or with which the weights reach weight_to; and the weights up to and with it.
-    auto select = [&](int use, uint32_t count_to, uint64_t weight_to, uint64_t& upto) -> uint64_t {
-      count = count0, count_before = count_before0, weight = weight0, weight_before = weight_before0;
-      uint64_t high = 0, shift = 0;  // of a finer histogram: the first place, and bits of a bin
-      uint64_t interval_low = 0, interval_high = 0;
-      bool finer_bins = false;
+    // The place of the token that is the count_to-th or, if that is 0, with which the weights of places >= from reach weight_to.
+    auto select = [&](int use, uint32_t count_to, uint64_t weight_to, uint64_t weight, uint64_t weight_before, uint32_t count, uint32_t count_before) -> uint64_t {
+      uint64_t last = 0, first = ~0ull, shift = 0;
+      bool places = false;  // whether the bins are intervals of places
       // every turn leaves a 1024th of the places, of which there are less than 2^62
       for (int turn = 0; turn < 8; ++turn) {
         const bool here = count_to ? count_before < count_to && count_before + count >= count_to : weight_before < weight_to && weight_before + weight >= weight_to;
         if (here) found = {tid, count, count_before, weight_before};
         __syncthreads();
         const Found f = found;
-        if (finer_bins) {
-          interval_high = high - (static_cast<uint64_t>(f.bin) << shift);
-          const uint64_t width = (1ull << shift) - 1;
-          interval_low = interval_high - interval_low < width ? interval_low : interval_high - width;
-        }
-        auto inside = [&](float z, uint64_t at) { return z > -INFINITY && (finer_bins ? at >= interval_low && at <= interval_high : bin_of(z) == f.bin); };
-        const bool few = f.tokens <= kFew;
-        if (!few && finer_bins) {
-          // the interval's bounds are known
+        if (!places) {
+          list_tokens(use, [&](float z, int token) { return z > -INFINITY && bin_of(z) == f.bin && (from == 0 || place_of(z, token) >= from); });
         } else {
-          uint64_t lo = ~0ull, hi = 0;
-#pragma unroll 2
-          for (int at = 4 * tid; at < n; at += 4 * kThreads) {
-            float z[4];
-            fetch(at, z);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint64_t place = place_of(z[k], v0 + at + k);
-              if (!inside(z[k], place) || (!count_to && weight_of(z[k]) == 0)) continue;
-              if (few) {
-                const uint32_t i = atomicAdd(&listed[use], 1u);
-                if (i < kFew) lists[use][i] = place;
-              }
-              lo = min(lo, place);
-              hi = max(hi, place);
-            }
-          }
-          if (!few) {
-#pragma unroll
-            for (int d = 16; d; d >>= 1) {
-              lo = min(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, d));
-              hi = max(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, d));
-            }
-            if (lane == 0) {
-              atomicMin(reinterpret_cast<unsigned long long*>(&ends[use][0]), lo);
-              atomicMax(reinterpret_cast<unsigned long long*>(&ends[use][1]), hi);
-            }
-          }
+          first -= static_cast<uint64_t>(f.bin) << shift;
+          const uint64_t width = (1ull << shift) - 1;
+          last = first - last < width ? last : first - width;
+          if (tid == 0) listed[use] = 0;
           meet();
-          if (few) {
-            // every CTA ranks them all
-            int ahead = 0;
-            for (int r = 0; r < ctas; ++r) {
-              const int many = min(static_cast<int>(load_cluster_u32(there(&listed[use], r))), kFew - ahead);
-              if (tid >= ahead && tid < ahead + many) {
-                const uint64_t place = load_cluster_u64(there(&lists[use][tid - ahead], r));
-                merged[tid] = make_ulonglong2(place, weight_of(logit_of(place)));
-              }
-              ahead += many;
-            }
-            __syncthreads();
-            if (tid < ahead) {
-              const uint64_t mine = merged[tid].x, own = merged[tid].y;
-              uint64_t sum = f.weight_before;
-              uint32_t rank = f.count_before;
-              for (int i = 0; i < ahead; ++i) {
-                const ulonglong2 other = merged[i];
-                rank += other.x > mine;
-                sum += other.x > mine ? other.y : 0;
-              }
-              if (count_to ? rank + 1 == count_to : sum < weight_to && sum + own >= weight_to) {
-                cut = mine;
-                cut_weight = sum + own;
-              }
-            }
-            __syncthreads();
-            const uint64_t place = cut;
-            upto = cut_weight;
-            __syncthreads();
-            return place;
-          }
-          interval_low = ~0ull;
-          interval_high = 0;
-          for (int r = 0; r < ctas; ++r) {
-            interval_low = min(interval_low, load_cluster_u64(there(&ends[use][0], r)));
-            interval_high = max(interval_high, load_cluster_u64(there(&ends[use][1], r)));
-          }
+          list_tokens(use, [&](float z, int token) {
+            const uint64_t place = place_of(z, token);
+            return z > -INFINITY && place >= last && place <= first;
+          });
         }
-        // too many: a histogram of this interval alone
-        finer_bins = true;
-        high = interval_high;
-        shift = 64 - __clzll(static_cast<long long>(interval_high - interval_low));
+        meet();
+        const uint32_t many = merge_lists(use);
+        if (many <= kFew) {
+          if (tid < many) {
+            const uint64_t mine = merged[tid].x, own = merged[tid].y;
+            uint64_t sum = f.weight_before;
+            uint32_t rank = f.count_before;
+            for (uint32_t i = 0; i < many; ++i) {
+              const ulonglong2 other = merged[i];
+              rank += other.x > mine;
+              sum += other.x > mine ? other.y : 0;
+            }
+            if (count_to ? rank + 1 == count_to : sum < weight_to && sum + own >= weight_to) cut = mine;
+          }
+          __syncthreads();
+          const uint64_t place = cut;
+          __syncthreads();
+          return place;
+        }
+        // too many: a histogram of their places alone
+        if (!places) {
+          for (int r = 0; r < ctas; ++r) {
+            last = r ? min(last, load_cluster_u64(there(&ends[use][0], r))) : load_cluster_u64(there(&ends[use][0], 0));
+            first = r ? max(first, load_cluster_u64(there(&ends[use][1], r))) : load_cluster_u64(there(&ends[use][1], 0));
+          }
+          places = true;
+        }
+        shift = 64 - __clzll(static_cast<long long>(first - last));
         shift = shift > 10 ? shift - 10 : 0;
-        static_assert(kBins == 1 << 10, "bins of a finer histogram");
-        finer.count[tid] = finer.low[tid] = finer.high[tid] = 0;
+        static_assert(kBins == 1 << 10, "bins of places");
+        clear_bins();
         __syncthreads();
-#pragma unroll 2
+#pragma unroll 1
         for (int at = 4 * tid; at < n; at += 4 * kThreads) {
           float z[4];
           fetch(at, z);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint64_t place = place_of(z[k], v0 + at + k);
-            if (z[k] > -INFINITY && place >= interval_low && place <= interval_high) {
-              const uint64_t w = by_weight ? weight_of(z[k]) : 0;
-              if (count_to || w) enter(finer, static_cast<int>((high - place) >> shift), w);
+            if (z[k] > -INFINITY && place >= last && place <= first) {
+              const int bin = static_cast<int>((first - place) >> shift);
+              if (count_to) atomicAdd(&bins.count[bin], 1u);
+              else enter(bin, weight_of(z[k]));
             }
           }
         }
         meet();
-        gather(finer);
-        count_before += f.count_before;
-        weight_before += f.weight_before;
-        meet();
+        uint32_t counts[kMostCtas], lows[kMostCtas], highs[kMostCtas], all_count;
+        uint64_t all_weight;
+        words_of_all(&bins.count[tid], counts);
+        words_of_all(&bins.low[tid], lows);
+        words_of_all(&bins.high[tid], highs);
+        count = 0, weight = 0;
+        for (int r = 0; r < kMostCtas; ++r) count += counts[r], weight += (static_cast<uint64_t>(highs[r]) << 32) + lows[r];
+        count_before = f.count_before + scan(count, red32, all_count);
+        weight_before = f.weight_before + scan(weight, red64, all_weight);
+        meet();  // nobody clears what another still reads
       }
       return 0;
     };
 
-    uint64_t share = all_weight;
-    const uint32_t tokens = all_tokens;
-    if (by_count && static_cast<uint32_t>(top_k) < tokens) from = select(0, top_k, 0, share);
+    if (by_count) {
+#pragma unroll 2
+      for (int at = 4 * tid; at < n; at += 4 * kThreads) {
+        float z[4];
+        fetch(at, z);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (z[k] > -INFINITY) atomicAdd(&bins.count[bin_of(z[k])], 1u);
+      }
+      meet();
+      uint32_t counts[kMostCtas], count = 0, all_count;
+      words_of_all(&bins.count[tid], counts);
+#pragma unroll
+      for (int r = 0; r < kMostCtas; ++r) count += counts[r];
+      const uint32_t before = scan(count, red32, all_count);
+      if (tid == 0) found.bin = -1;
+      __syncthreads();
+      const bool here = before < top_k && before + count >= top_k;
+      if (here) found = {tid, count, before, 0};
+      __syncthreads();
+      const Found f = found;  // bin -1: there are fewer tokens than that
+      const int last_bin = f.bin < 0 ? kBins - 1 : f.bin;
+      if ((f.bin < 0 ? all_count : f.count_before + f.tokens) <= kFew) {
+        // all that can be drawn fits a list
+        list_tokens(0, [&](float z, int) { return z > -INFINITY && bin_of(z) <= last_bin; });
+        meet();
+        if (blockIdx.z == 0) {
+          const uint32_t many = min(merge_lists(0), kFew);
+          uint32_t rank = 0;
+          uint64_t ahead = 0, own = 0;
+          ulonglong2 mine{0, 0};
+          if (tid < many) {
+            mine = merged[tid];
+#pragma unroll 4
+            for (uint32_t i = 0; i < many; ++i) {
+              const ulonglong2 other = merged[i];
+              rank += other.x > mine.x;
+              ahead += other.x > mine.x ? other.y : 0;
+            }
+            if (rank < top_k) own = mine.y;
+          }
+          if (by_weight) {
+            const uint64_t reach = reach_of(sum_of_all(own));
+            if (ahead >= reach) own = 0;
+          }
+          if (own < least) own = 0;
+          __syncthreads();
+          if (tid < many) merged[tid].y = own;
+          const uint64_t target = target_of(sum_of_all(own));
+          if (own) {
+            uint64_t upto = 0;  // in the order of the vocabulary
+#pragma unroll 4
+            for (uint32_t i = 0; i < many; ++i) {
+              const ulonglong2 other = merged[i];
+              upto += static_cast<uint32_t>(other.x) >= static_cast<uint32_t>(mine.x) ? other.y : 0;
+            }
+            if (upto > target && upto - own <= target) s.out[row] = 0xFFFFFFFFu - static_cast<uint32_t>(mine.x);
+          }
+        }
+        meet();
+        return;
+      }
+      if (f.bin >= 0) from = select(0, top_k, 0, 0, 0, count, before);
+      else meet();
+      clear_bins();
+      __syncthreads();
+    }
     if (by_weight) {
-      const double to = static_cast<double>(top_p) * static_cast<double>(share);
-      const uint64_t reach = to <= 1. ? 1 : static_cast<uint64_t>(ceil(to));
-      uint64_t upto;
-      from = max(from, select(1, 0, reach < share ? reach : share, upto));
+#pragma unroll 2
+      for (int at = 4 * tid; at < n; at += 4 * kThreads) {
+        float z[4];
+        fetch(at, z);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (from == 0 || place_of(z[k], v0 + at + k) >= from) {
+            const uint64_t w = weight_of(z[k]);
+            if (w) enter(bin_of(z[k]), w);
+          }
+      }
+      meet();
+      uint32_t lows[kMostCtas], highs[kMostCtas];
+      words_of_all(&bins.low[tid], lows);
+      words_of_all(&bins.high[tid], highs);
+      uint64_t weight = 0, share;
+#pragma unroll
+      for (int r = 0; r < kMostCtas; ++r) weight += (static_cast<uint64_t>(highs[r]) << 32) + lows[r];
+      const uint64_t before = scan(weight, red64, share);
+      from = max(from, select(1, 0, reach_of(share), weight, before, 0, 0));
     }
   }
 
-  // Sums of what is kept, chunk by chunk; a warp has a chunk.
-  auto kept_weight = [&](float z, int at) -> uint64_t {
-    if (!(z > -INFINITY) || place_of(z, v0 + at) < from) return 0;
+  // Sums of what is kept, chunk by chunk; a warp has a chunk.  Its kept tokens move together, so that few of them take few turns.
+  const float last_logit = from ? logit_of(from) : -INFINITY;
+  const int last_token = from ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(from)) : -1;
+  auto is_kept = [&](float z, int token) { return z > last_logit || (z == last_logit && token <= last_token); };
+  auto kept_weight = [&](float z) -> uint64_t {
     const uint64_t w = weight_of(z);
     return w >= least ? w : 0;
   };
-  if (tid == 0) part = 0;
-  uint64_t* sums = reinterpret_cast<uint64_t*>(&finer);  // kThreads of them
-  static_assert(sizeof(Histogram) >= kThreads * sizeof(uint64_t), "sums");
   __syncthreads();
   sums[tid] = 0;
   __syncthreads();
   for (int c = warp; c * args.chunk < n; c += kThreads / 32) {
     uint64_t sum = 0;
-    for (int at = c * args.chunk + 4 * lane; at < min(n, (c + 1) * args.chunk); at += 128) {
+    for (int at = c * args.chunk + 4 * lane; at - 4 * lane < min(n, (c + 1) * args.chunk); at += 128) {
       float z[4];
       fetch(at, z);
+      int many = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum += kept_weight(z[k], at + k);
+      for (int k = 0; k < 4; ++k) {
+        const bool kept = is_kept(z[k], v0 + at + k);
+        const uint32_t all = __ballot_sync(0xFFFFFFFFu, kept);
+        if (kept) buffer.kept[warp][many + __popc(all & ((1u << lane) - 1))] = z[k];
+        many += __popc(all);
+      }
+      __syncwarp();
+      for (int i = lane; i < many; i += 32) sum += kept_weight(buffer.kept[warp][i]);
+      __syncwarp();
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
@@ -431,9 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
       whole += other;
     }
   }
-  const double u = fmax(static_cast<double>(s.random[row]), 0.);  // not a number: 0
-  const double at_sum = floor(u * static_cast<double>(whole));
-  const uint64_t target = at_sum >= static_cast<double>(whole) ? whole - 1 : min(static_cast<uint64_t>(at_sum), whole - 1);
+  const uint64_t target = target_of(whole);
   if (tid == 0) found.bin = -1;
   __syncthreads();
   if (target >= ahead + before && target < ahead + before + mine) {
@@ -449,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
       fetch(at, z);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        w[k] = at + k < n ? kept_weight(z[k], at + k) : 0;
+        w[k] = is_kept(z[k], v0 + at + k) ? kept_weight(z[k]) : 0;
         sum += w[k];
       }
       uint64_t upto = sum;
