@@ -214,7 +214,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
   const double per_step = 1.4426950408889634074 * kTable / fmax(static_cast<double>(temperature), 1e-30);
   const float per_power = static_cast<float>(per_step / kTable);
   auto weight_of = [&](float z) -> uint64_t {
-    if (!((z - top) * per_power > -50.f)) return 0;
+    // (no branch: several of them are computed side by side)
+    const bool some = (z - top) * per_power > -50.f;
     constexpr double kRound = 6755399441055744.;  // 1.5 * 2^52: what is added to it is rounded to a whole number
     const double y = __dmul_rn(static_cast<double>(z) - static_cast<double>(top), per_step);
     const double t = __dadd_rn(y, kRound);
@@ -225,7 +226,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
     const double w = __dmul_rn(powers[steps & (kTable - 1)], fma(fma(fma(c3, f, c2), f, c1), f, 1.));
     static_assert(kTable == 1 << 10, "steps of a power");
     const double scaled = __hiloint2double(__double2hiint(w) + (((steps >> 10) + args.bits) << 20), __double2loint(w));
-    return static_cast<uint64_t>(__double_as_longlong(__dadd_rn(scaled, 4503599627370496.))) & 0xFFFFFFFFFFFFFull;  // + 2^52
+    const double whole = __dadd_rn(scaled, 4503599627370496.);  // + 2^52
+    const uint32_t high = some ? static_cast<uint32_t>(__double2hiint(whole)) & 0xFFFFFu : 0, low_part = some ? static_cast<uint32_t>(__double2loint(whole)) : 0;
+    return static_cast<uint64_t>(high) << 32 | low_part;
   };
   const uint64_t least = min_p > 0.f ? static_cast<uint64_t>(ceil(fmin(static_cast<double>(min_p), 1.) * static_cast<double>(1ull << args.bits))) : 0;
   // The tokens ahead of which less than p of `share` lies: weights that those ahead of the last one do not reach.
@@ -451,13 +454,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
 #pragma unroll 2
       for (int at = 4 * tid; at < n; at += 4 * kThreads) {
         float z[4];
+        uint64_t w[4];
         fetch(at, z);
 #pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = weight_of(z[k]);
+#pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (from == 0 || place_of(z[k], v0 + at + k) >= from) {
-            const uint64_t w = weight_of(z[k]);
-            if (w) enter(bin_of(z[k]), w);
-          }
+          if (w[k] && (from == 0 || place_of(z[k], v0 + at + k) >= from)) enter(bin_of(z[k]), w[k]);
       }
       meet();
       uint32_t lows[kMostCtas], highs[kMostCtas];
