@@ -5,10 +5,13 @@
 // to 32-bit sums in registers, times its scale.  Two TMEM tiles take turns: one is filled while the other is read.
 //
 // Roles: one warp asks for operands (TMA, a ring of stages), one issues the MMAs, and one or two groups of four warps add up.
-//   rows many: the 128 lanes of a tile are rows of x, its columns are features.  A thread has one row and its scale.
-//   rows few (kSwap): the lanes are features, the columns rows of x, so that a tile wastes nothing on rows that do not exist; a thread has one
-//   feature, and the rows' scales come from shared memory.  Bound by the weights' bytes; the groups are cut among the CTAs of a cluster, whose sums
+//   rows few (kFeatures): the 128 lanes of a tile are features, its columns rows of x, so that a tile wastes nothing on rows that do not exist; a thread has
+//   one feature, and the rows' scales come from shared memory.  Bound by the weights' bytes; the groups are cut among the CTAs of a cluster, whose sums
 //   are joined in the order of the CTAs over distributed shared memory.
+//   rows many (kRows): the lanes are rows of x, the columns features.  A thread has one row and its scales, four groups of them at a time.
+//   rows many, tiles enough (kPair): two CTAs of a cluster have one tile of 256 rows x 256 features, each 128 of its rows in TMEM and 128 of either operand in shared
+//   memory, which the MMAs of both read.  What counts there is the way from L2, which brings an SM some 64 bytes a cycle: a group of a tile of its own, 128 x 256,
+//   takes 48 KB and 512 cycles of the tensor core, half a pair's tile 32 KB.
 #include <type_traits>
 
 #include "decode_step.cuh"
@@ -18,35 +21,44 @@ namespace tris {
 
 // Row-major rows of `cols` bytes, `stride` bytes apart; one copy = 128 columns of box_rows rows, 128-byte-swizzled, zeros past the matrix (tc_gemm.cu).
 bool encode_bytes_map(CUtensorMap* map, const void* base, int rows, int cols, int64_t stride, int box_rows);
+// The same of outputs, elt bytes each: 128 bytes of 128 rows, nothing is written past the matrix.
+bool encode_output_map(CUtensorMap* map, const void* base, int rows, int cols, int elt, int64_t stride);
 
 namespace {
 
 constexpr int kGroup = 128;  // columns of a scale, and bytes of a swizzled line
 constexpr int kLanes = 128;  // rows of a tile's first operand
 
+enum class Mode { kFeatures, kRows, kPair };
+
 struct LinearArgs {
   TrisE4m3Linear a;
   int groups;       // of K
   int per_cta;      // of them, that a CTA adds up
   int row_tiles, feature_tiles;
-  int wide_store;   // whether 32 bytes of a row can be stored at once
+  int store_map;    // whether outputs go out by tensor copies
+  int wide_scales;  // whether four scales of a row can be read at once
 };
 struct LinearMaps {
-  CUtensorMap lanes, columns;
+  CUtensorMap lanes, columns, out;
 };
 
 // BN: columns of a tile.  WGS: groups of four warps that add up, each BN / WGS columns.
-template <int BN, int WGS, bool kSwap>
+template <int BN, int WGS, Mode M>
 struct LinearShape {
-  static constexpr int kStageBytes = (kLanes + BN) * kGroup;
+  static constexpr bool kSwap = M == Mode::kFeatures, kPair = M == Mode::kPair;
+  static constexpr int kLoaded = kPair ? BN / 2 : BN;  // rows of the second operand that a CTA loads
+  static constexpr int kStageBytes = (kLanes + kLoaded) * kGroup;
   static constexpr int kCtasPerSm = kSwap ? 2 : 1;
-  static constexpr int kStagesThatFit = ((228 / kCtasPerSm - 2) * 1024 - 1024 - 1024) / kStageBytes;
+  static constexpr int kOutBytes = kSwap ? 0 : WGS * kLanes * 128;  // 128 bytes of every row, for each group of warps
+  static constexpr int kStagesThatFit = ((kCtasPerSm == 1 ? 227 : 113) * 1024 - 1024 - 1280 - kOutBytes) / kStageBytes;  // less the boundary's part and what else there is
   static constexpr int kStages = kStagesThatFit > 8 ? 8 : kStagesThatFit;
   static constexpr int kWarps = 4 * WGS, kThreads = 32 * (kWarps + 2);
   static constexpr int kColumns = BN / WGS;  // of a thread
-  static constexpr int kTmem = 2 * BN < 32 ? 32 : 2 * BN;
-  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + 1024;
-  static_assert(kStages >= 3 && BN * kLanes * 4 <= kStages * kStageBytes, "a tile's sums lie where the stages were");
+  static constexpr int kTiles = BN == 256 ? 2 : 4;  // in TMEM, that take turns
+  static constexpr int kTmem = kTiles * BN;
+  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + kOutBytes + 1024;
+  static_assert(kStages >= 3 && (kPair || BN * kLanes * 4 <= kStages * kStageBytes), "a tile's sums lie where the stages were");
 };
 
 __device__ __forceinline__ void umma_f8_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
@@ -56,6 +68,39 @@ __device__ __forceinline__ void umma_f8_ss(uint32_t tmem_d, uint64_t desc_a, uin
       "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// By one thread for both CTAs of a pair: rows and columns of the operands from either one's shared memory, at the same places.
+__device__ __forceinline__ void umma_f8_ss_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives on the barrier at this place in both CTAs of a pair.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+// To this CTA's shared memory, with the bytes counted by a barrier of the pair's first CTA.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst_smem, const CUtensorMap* map, int c0, int c1, uint32_t bar_of_first) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst_smem)), "l"(map),
+               "r"(c0), "r"(c1), "r"(bar_of_first)
+               : "memory");
+}
+__device__ __forceinline__ void arrive_in_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int c0, int c1, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0), "r"(c1), "r"(src) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // 32 lanes x 32 columns of TMEM.
 __device__ __forceinline__ void tmem_ld_32(uint32_t taddr, float (&v)[32]) {
   asm volatile(
@@ -73,6 +118,16 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
   else tmem_ld_32(taddr, v);
 }
 
+// As mbar_wait_bounded; the timer, whose reading takes longer than most of these waits, is not looked at before 256 tries have failed.
+__device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < 256; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_bounded(bar, parity);
+}
+// The same by a whole warp, with one answer for all lanes.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait_one(bar, parity)); }
+
 __device__ __forceinline__ float bias_at(const TrisE4m3Linear& a, int n) {
   if (!a.bias) return 0.f;
   if (a.bias_dtype == TRIS_DTYPE_F32) return static_cast<const float*>(a.bias)[n];
@@ -83,57 +138,23 @@ __device__ __forceinline__ void store_output(const TrisE4m3Linear& a, int64_t at
   else if (a.dtype == TRIS_DTYPE_F16) static_cast<__half*>(a.out)[at] = __float2half_rn(v);
   else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
 }
-__device__ __forceinline__ void store_32_bytes(void* p, const uint32_t (&v)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-// Neighbouring features n, n + 1, ... of one row.
-template <int N>
-__device__ __forceinline__ void store_features(const LinearArgs& args, int64_t row, int n, const float (&v)[N]) {
-  const TrisE4m3Linear& a = args.a;
-  const int64_t at = row * a.out_stride + n;
-  static_assert(N % 16 == 0, "32 bytes of 16-bit numbers");
-  if (args.wide_store && n + N <= a.out_features) {
-#pragma unroll
-    for (int i = 0; i < N; i += 16) {
-      float f[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) f[j] = v[i + j] + (a.bias ? bias_at(a, n + i + j) : 0.f);
-      uint32_t r[8];
-      if (a.dtype == TRIS_DTYPE_F32) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(f[8 * h + j]);
-          store_32_bytes(static_cast<float*>(a.out) + at + i + 8 * h, r);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = a.dtype == TRIS_DTYPE_F16 ? Pair<__half>::pack(f[2 * j], f[2 * j + 1]) : Pair<__nv_bfloat16>::pack(f[2 * j], f[2 * j + 1]);
-        store_32_bytes(static_cast<__half*>(a.out) + at + i, r);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (n + i < a.out_features) store_output(a, at + i, v[i] + bias_at(a, n + i));
-  }
-}
-
-// grid (CTAs, 1, CTAs of a cluster).  A CTA walks over tiles; where the groups are cut among a cluster's CTAs it has one.
-template <int BN, int WGS, bool kSwap>
-__global__ void __launch_bounds__(LinearShape<BN, WGS, kSwap>::kThreads, LinearShape<BN, WGS, kSwap>::kCtasPerSm)
+// grid (CTAs, 1, CTAs of a cluster), or (2 pairs, 1, 1) in clusters of two.  A CTA (a pair) walks over tiles; where the groups are cut among a cluster's CTAs it has one.
+template <int BN, int WGS, Mode M>
+__global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape<BN, WGS, M>::kCtasPerSm)
     e4m3_linear_kernel(const __grid_constant__ LinearArgs args, const __grid_constant__ LinearMaps maps) {
-  using S = LinearShape<BN, WGS, kSwap>;
+  using S = LinearShape<BN, WGS, M>;
+  constexpr bool kSwap = S::kSwap, kPair = S::kPair;
   extern __shared__ uint4 smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>(smem_raw) + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  __shared__ uint64_t full[S::kStages], empty[S::kStages], tile_full[2], tile_empty[2];
+  __shared__ uint64_t full[S::kStages], empty[S::kStages], tile_full[S::kTiles], tile_empty[S::kTiles];
   __shared__ uint32_t tmem_base;
   __shared__ int timed_out;
   __shared__ __align__(16) float row_scales[2][kSwap ? BN : 4];
+  __shared__ __align__(16) float biases[kSwap ? 4 : BN];
   const TrisE4m3Linear& a = args.a;
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int tiles = args.row_tiles * args.feature_tiles;
+  const int rank = kPair ? blockIdx.x & 1 : 0, split = gridDim.z, walker = kPair ? blockIdx.x / 2 : blockIdx.x, walkers = kPair ? gridDim.x / 2 : gridDim.x;
   const int first = blockIdx.z * args.per_cta, count = min(args.per_cta, args.groups - first);  // groups of this CTA; at least one
 
   if (threadIdx.x == 0) {
@@ -141,16 +162,20 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, kSwap>::kThreads, LinearS
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < S::kTiles; ++i) {
       mbar_init(&tile_full[i], 1);
-      mbar_init(&tile_empty[i], S::kWarps);
+      mbar_init(&tile_empty[i], S::kWarps * (kPair ? 2 : 1));
     }
     fence_mbar_init();
     timed_out = 0;
   }
-  if (warp == 0) tmem_alloc(&tmem_base, S::kTmem);
+  if (warp == 0) {
+    if constexpr (kPair) tmem_alloc_pair(&tmem_base, S::kTmem);
+    else tmem_alloc(&tmem_base, S::kTmem);
+  }
   tcgen05_fence_before();
   __syncthreads();
+  if constexpr (kPair) cluster_sync();  // the other CTA's barriers are there
   tcgen05_fence_after();
   const uint32_t tmem = warp_uniform(tmem_base);
   pdl_wait();
@@ -158,7 +183,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, kSwap>::kThreads, LinearS
 
   // tiles in strips of 16 along the rows: what runs at one time shares rows and features
   auto place = [&](int tile, int& row_tile, int& feature_tile) {
-    constexpr int kStrip = 16;
+    constexpr int kStrip = kPair ? 8 : 16;
     const int strip = tile / (kStrip * args.feature_tiles), in = tile - strip * (kStrip * args.feature_tiles);
     const int height = min(kStrip, args.row_tiles - strip * kStrip);
     feature_tile = in / height;
@@ -169,42 +194,57 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, kSwap>::kThreads, LinearS
   if (warp == S::kWarps) {
     if (lane == 0) {
       bool ok = true;
-      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      for (int tile = walker; tile < tiles && ok; tile += walkers) {
         int rt, ft;
         place(tile, rt, ft);
-        const int lane0 = (kSwap ? ft : rt) * kLanes, column0 = (kSwap ? rt : ft) * BN;
+        const int lane0 = kSwap ? ft * kLanes : (rt * (kPair ? 2 : 1) + rank) * kLanes, column0 = (kSwap ? rt : ft) * BN + rank * S::kLoaded;
         for (int g = 0; g < count; ++g, ++asked) {
           const int s = asked % S::kStages;
-          if (asked >= S::kStages && !mbar_wait_bounded(&empty[s], (asked / S::kStages - 1) & 1)) {
+          if (asked >= S::kStages && !wait_one(&empty[s], (asked / S::kStages - 1) & 1)) {
             timed_out = 1;
             ok = false;
             break;
           }
           uint8_t* to = ring + s * S::kStageBytes;
-          mbar_arrive_expect_tx(&full[s], S::kStageBytes);
-          tma_load_2d(to, &maps.lanes, (first + g) * kGroup, lane0, &full[s]);
-          tma_load_2d(to + kLanes * kGroup, &maps.columns, (first + g) * kGroup, column0, &full[s]);
+          if constexpr (kPair) {
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * S::kStageBytes);  // the other CTA's bytes, too
+            const uint32_t bar = in_cta(smem_u32(&full[s]), 0);
+            tma_load_2d_pair(to, &maps.lanes, (first + g) * kGroup, lane0, bar);
+            tma_load_2d_pair(to + kLanes * kGroup, &maps.columns, (first + g) * kGroup, column0, bar);
+          } else {
+            mbar_arrive_expect_tx(&full[s], S::kStageBytes);
+            tma_load_2d(to, &maps.lanes, (first + g) * kGroup, lane0, &full[s]);
+            tma_load_2d(to + kLanes * kGroup, &maps.columns, (first + g) * kGroup, column0, &full[s]);
+          }
         }
       }
     }
     __syncwarp();
   } else if (warp == S::kWarps + 1) {
-    const uint32_t idesc = umma_idesc_f16(kLanes, BN);  // the same fields: fp32 sums, operand types 0 (here e4m3), K-major
+    const uint32_t idesc = umma_idesc_f16(kPair ? 2 * kLanes : kLanes, BN);  // the same fields: fp32 sums, operand types 0 (here e4m3), K-major
     bool ok = true;
     int i = 0;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+    for (int tile = walker; rank == 0 && tile < tiles && ok; tile += walkers) {
       for (int g = 0; g < count; ++g, ++i) {
-        const int s = i % S::kStages, half = i & 1;
-        ok = mbar_wait_warp(&full[s], (i / S::kStages) & 1) && (i < 2 || mbar_wait_warp(&tile_empty[half], (i / 2 - 1) & 1));
+        const int s = i % S::kStages, turn = i % S::kTiles;
+        ok = wait_for(&full[s], (i / S::kStages) & 1) && (i < S::kTiles || wait_for(&tile_empty[turn], (i / S::kTiles - 1) & 1));
         if (!ok) break;
         tcgen05_fence_after();
         const uint32_t at = smem_u32(ring + s * S::kStageBytes);
         const uint64_t da = umma_smem_desc_sw128(at), db = umma_smem_desc_sw128(at + kLanes * kGroup);
         if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < kGroup / 32; ++j) umma_f8_ss(tmem + half * BN, da + 2 * j, db + 2 * j, idesc, j > 0 ? 1u : 0u);
-          umma_commit(&empty[s]);
-          umma_commit(&tile_full[half]);
+          for (int j = 0; j < kGroup / 32; ++j) {
+            if constexpr (kPair) umma_f8_ss_pair(tmem + turn * BN, da + 2 * j, db + 2 * j, idesc, j > 0 ? 1u : 0u);
+            else umma_f8_ss(tmem + turn * BN, da + 2 * j, db + 2 * j, idesc, j > 0 ? 1u : 0u);
+          }
+          if constexpr (kPair) {
+            umma_commit_pair(&empty[s]);
+            umma_commit_pair(&tile_full[turn]);
+          } else {
+            umma_commit(&empty[s]);
+            umma_commit(&tile_full[turn]);
+          }
         }
         __syncwarp();
       }
@@ -214,57 +254,86 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, kSwap>::kThreads, LinearS
   } else {
     const int wg = warp >> 2, in_tile = 32 * (warp & 3) + lane;  // lane of the tile
     const uint32_t from = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + wg * S::kColumns;
-    constexpr int kPart = S::kColumns < 32 ? S::kColumns : 32;
+    constexpr int kPart = S::kColumns < 32 ? S::kColumns : 32, kQuad = kSwap ? 1 : 4;
+    uint8_t* out_stage = ring + S::kStages * S::kStageBytes + wg * kLanes * 128;
     bool ok = true;
     int i = 0;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    for (int tile = walker; tile < tiles; tile += walkers) {
       int rt, ft;
       place(tile, rt, ft);
-      // the scales of a thread's row, or of a row for each thread to pass on, and of the weights' block
-      const int row = kSwap ? rt * BN + static_cast<int>(threadIdx.x) : rt * kLanes + in_tile;
-      const int block = kSwap ? ft : (ft * BN + wg * S::kColumns) / kGroup;
+      // the scales of a thread's row, or of a row for each thread to pass on, and of the weights' block: kQuad groups, and the next ones on their way
+      const int row = kSwap ? rt * BN + static_cast<int>(threadIdx.x) : (rt * (kPair ? 2 : 1) + rank) * kLanes + in_tile;
+      const int feature0 = ft * BN + wg * S::kColumns;  // unless kSwap
+      const int block = kSwap ? ft : feature0 / kGroup;
       const bool has_row = row < a.rows && (!kSwap || threadIdx.x < BN), has_block = block * kGroup < a.out_features;
       const float* xs = a.x_scales + static_cast<int64_t>(has_row ? row : 0) * a.x_scales_stride + first;
       const float* ws = a.weight_scales + static_cast<int64_t>(has_block ? block : 0) * a.weight_scales_stride + first;
-      float x_next = has_row ? xs[0] : 0.f, w_next = ws[0];
+      float x_next[kQuad], w_next[kQuad];
+      auto fetch_scales = [&](int g) {
+        if (kQuad == 4 && args.wide_scales && g + 4 <= count) {
+          const float4 x = *reinterpret_cast<const float4*>(xs + g), w = *reinterpret_cast<const float4*>(ws + g);
+          x_next[0] = x.x, x_next[kQuad - 3] = x.y, x_next[kQuad - 2] = x.z, x_next[kQuad - 1] = x.w;
+          w_next[0] = w.x, w_next[kQuad - 3] = w.y, w_next[kQuad - 2] = w.z, w_next[kQuad - 1] = w.w;
+        } else {
+#pragma unroll
+          for (int q = 0; q < kQuad; ++q) {
+            x_next[q] = g + q < count ? xs[g + q] : 0.f;
+            w_next[q] = g + q < count ? ws[g + q] : 0.f;
+          }
+        }
+      };
+      fetch_scales(0);
+      if constexpr (!kSwap) {
+        // (a barrier lies between this and the last use of the tile before: the one behind the tile's last stores, or the warps' own below)
+        named_barrier_sync(1 + wg, 128);
+        if (in_tile < S::kColumns) biases[wg * S::kColumns + in_tile] = feature0 + in_tile < a.out_features ? bias_at(a, feature0 + in_tile) : 0.f;
+        named_barrier_sync(1 + wg, 128);
+      }
       uint64_t acc[S::kColumns / 2];
 #pragma unroll
       for (int c = 0; c < S::kColumns / 2; ++c) acc[c] = 0;
-      for (int g = 0; g < count; ++g, ++i) {
-        const int half = i & 1;
-        const float scale = x_next * w_next;
-        if (g + 1 < count) {
-          x_next = has_row ? xs[g + 1] : 0.f;
-          w_next = ws[g + 1];
-        }
-        if constexpr (kSwap) {
-          // two places take turns: who writes the next but one has met everybody who reads this one
-          if (threadIdx.x < BN) row_scales[half][threadIdx.x] = scale;
-          named_barrier_sync(1, 32 * S::kWarps);
-        }
-        if (ok) ok = mbar_wait_warp(&tile_full[half], (i / 2) & 1);
-        if (!ok) continue;
-        tcgen05_fence_after();
+      for (int g0 = 0; g0 < count; g0 += kQuad) {
+        float scales[kQuad];
 #pragma unroll
-        for (int c = 0; c < S::kColumns; c += kPart) {
-          float v[kPart];
-          tmem_ld<kPart>(from + half * BN + c, v);
-          if (c + kPart == S::kColumns) {
-            tcgen05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&tile_empty[half]);
-          }
+        for (int q = 0; q < kQuad; ++q) scales[q] = has_row ? x_next[q] * w_next[q] : 0.f;
+        if (g0 + kQuad < count) fetch_scales(g0 + kQuad);
+#pragma unroll
+        for (int q = 0; q < kQuad; ++q) {
+          if (g0 + q >= count) break;
+          const int half = i & 1, turn = i % S::kTiles, parity = (i / S::kTiles) & 1;
+          ++i;
           if constexpr (kSwap) {
+            // two places take turns: who writes the next but one has met everybody who reads this one
+            if (threadIdx.x < BN) row_scales[half][threadIdx.x] = scales[q];
+            named_barrier_sync(1, 32 * S::kWarps);
+          }
+          if (ok) ok = wait_for(&tile_full[turn], parity);
+          if (!ok) continue;
+          tcgen05_fence_after();
 #pragma unroll
-            for (int j = 0; j < kPart; j += 4) {
-              const float4 s = *reinterpret_cast<const float4*>(&row_scales[half][c + j]);
-              acc[(c + j) / 2] = fma_2(pack_2(v[j], v[j + 1]), pack_2(s.x, s.y), acc[(c + j) / 2]);
-              acc[(c + j) / 2 + 1] = fma_2(pack_2(v[j + 2], v[j + 3]), pack_2(s.z, s.w), acc[(c + j) / 2 + 1]);
+          for (int c = 0; c < S::kColumns; c += kPart) {
+            float v[kPart];
+            tmem_ld<kPart>(from + turn * BN + c, v);
+            if (c + kPart == S::kColumns) {
+              tcgen05_fence_before();
+              __syncwarp();
+              if (lane == 0) {
+                if constexpr (kPair) arrive_in_cluster(in_cta(smem_u32(&tile_empty[turn]), 0));
+                else mbar_arrive(&tile_empty[turn]);
+              }
             }
-          } else {
-            const uint64_t s = pack_2(scale, scale);
+            if constexpr (kSwap) {
 #pragma unroll
-            for (int j = 0; j < kPart; j += 2) acc[(c + j) / 2] = fma_2(pack_2(v[j], v[j + 1]), s, acc[(c + j) / 2]);
+              for (int j = 0; j < kPart; j += 4) {
+                const float4 s = *reinterpret_cast<const float4*>(&row_scales[half][c + j]);
+                acc[(c + j) / 2] = fma_2(pack_2(v[j], v[j + 1]), pack_2(s.x, s.y), acc[(c + j) / 2]);
+                acc[(c + j) / 2 + 1] = fma_2(pack_2(v[j + 2], v[j + 3]), pack_2(s.z, s.w), acc[(c + j) / 2 + 1]);
+              }
+            } else {
+              const uint64_t s = pack_2(scales[q], scales[q]);
+#pragma unroll
+              for (int j = 0; j < kPart; j += 2) acc[(c + j) / 2] = fma_2(pack_2(v[j], v[j + 1]), s, acc[(c + j) / 2]);
+            }
           }
         }
       }
@@ -278,7 +347,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, kSwap>::kThreads, LinearS
         asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(acc[c / 2]));
         return c & 1 ? hi : lo;
       };
-      if (gridDim.z > 1) {
+      if (split > 1) {
         // the ring is idle: this CTA's only tile has been multiplied
         float* part = reinterpret_cast<float*>(ring);
 #pragma unroll
@@ -293,26 +362,68 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, kSwap>::kThreads, LinearS
             if (t < a.rows) store_output(a, static_cast<int64_t>(t) * a.out_stride + n, sum(c) + bias);
           }
         }
-      } else if (row < a.rows) {
+      } else if (args.store_map) {
+        // 128 bytes of every row at a time, in the order that the tensor copy expects: 16-byte chunk c of row r at place c ^ (r & 7)
+        auto put = [&](int chunk, uint4 v) { *reinterpret_cast<uint4*>(out_stage + in_tile * 128 + ((chunk ^ (in_tile & 7)) << 4)) = v; };
+        const int row0 = row - in_tile;
+        auto stage_out = [&](int c0, int columns, auto write) {
+          if (in_tile == 0) tma_stores_read();
+          named_barrier_sync(1 + wg, 128);
+          write();
+          fence_proxy_async();
+          named_barrier_sync(1 + wg, 128);
+          if (in_tile == 0 && feature0 + c0 < a.out_features && row0 < a.rows) tma_store_2d(&maps.out, feature0 + c0, row0, smem_u32(out_stage));
+        };
+        if (a.dtype == TRIS_DTYPE_F32) {
 #pragma unroll
-        for (int c = 0; c < S::kColumns; c += 16) {
-          float v[16];
+          for (int c0 = 0; c0 < S::kColumns; c0 += 32)
+            stage_out(c0, 32, [&] {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = sum(c + j);
-          store_features(args, row, ft * BN + wg * S::kColumns + c, v);
+              for (int c = 0; c < 32; c += 4) {
+                const float4 b = *reinterpret_cast<const float4*>(&biases[wg * S::kColumns + c0 + c]);
+                put(c / 4, make_uint4(__float_as_uint(sum(c0 + c) + b.x), __float_as_uint(sum(c0 + c + 1) + b.y), __float_as_uint(sum(c0 + c + 2) + b.z), __float_as_uint(sum(c0 + c + 3) + b.w)));
+              }
+            });
+        } else {
+#pragma unroll
+          for (int c0 = 0; c0 < S::kColumns; c0 += 64)
+            stage_out(c0, 64, [&] {
+#pragma unroll
+              for (int c = 0; c < 64; c += 8) {
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const float2 b = *reinterpret_cast<const float2*>(&biases[wg * S::kColumns + c0 + c + 2 * k]);
+                  const float x = sum(c0 + c + 2 * k) + b.x, y = sum(c0 + c + 2 * k + 1) + b.y;
+                  w[k] = a.dtype == TRIS_DTYPE_F16 ? Pair<__half>::pack(x, y) : Pair<__nv_bfloat16>::pack(x, y);
+                }
+                put(c / 8, make_uint4(w[0], w[1], w[2], w[3]));
+              }
+            });
         }
+      } else if (row < a.rows) {
+        const int64_t at = static_cast<int64_t>(row) * a.out_stride + feature0;
+#pragma unroll
+        for (int c = 0; c < S::kColumns; ++c)
+          if (feature0 + c < a.out_features) store_output(a, at + c, sum(c) + biases[wg * S::kColumns + c]);
       }
     }
+    if (!kSwap && in_tile == 0) tma_stores_done();
   }
   __syncthreads();
   if (timed_out) {
     if (threadIdx.x == 0 && a.status_dev) atomicExch(a.status_dev, TRIS_ERR_TIMEOUT);
-    if (warp == S::kWarps && lane == 0)  // copies in flight have to land before this memory is another's
+    if (warp == S::kWarps && lane == 0 && rank == 0)  // copies in flight have to land before this memory is another's
       for (int s = 0; s < S::kStages && s < asked; ++s) mbar_wait_bounded(&full[s], ((asked - 1 - s) / S::kStages) & 1);
     __syncthreads();
   }
+  if constexpr (kPair) {
+    cluster_sync();  // neither CTA leaves, or gives back TMEM, while the other's products or barriers need it
+    if (warp == 0) tmem_dealloc_pair(tmem, S::kTmem);
+    return;
+  }
   if (warp == 0) tmem_dealloc(tmem, S::kTmem);
-  if (gridDim.z == 1) return;
+  if (split == 1) return;
 
   // every CTA of the cluster joins its share of the tile's columns, in the order of the CTAs
   cluster_sync();
@@ -321,43 +432,60 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, kSwap>::kThreads, LinearS
     place(blockIdx.x, rt, ft);
     const uint32_t local = smem_u32(ring);
     const int in_tile = threadIdx.x % kLanes, part = threadIdx.x / kLanes;
-    constexpr int kUnit = kSwap ? 1 : 16;  // columns at a time
-    for (int u = blockIdx.z * WGS + part; u < BN / kUnit; u += gridDim.z * WGS) {
-      const int t = kSwap ? rt * BN + u : rt * kLanes + in_tile, n = kSwap ? ft * kLanes + in_tile : ft * BN + u * kUnit;
+    for (int u = blockIdx.z * WGS + part; u < BN; u += split * WGS) {
+      const int t = kSwap ? rt * BN + u : rt * kLanes + in_tile, n = kSwap ? ft * kLanes + in_tile : ft * BN + u;
       if (t >= a.rows || n >= a.out_features) continue;
-      float v[kUnit];
-#pragma unroll
-      for (int j = 0; j < kUnit; ++j) v[j] = 0.f;
-      for (int r = 0; r < static_cast<int>(gridDim.z); ++r) {
-        const uint32_t there = in_cta(local, r);
-#pragma unroll
-        for (int j = 0; j < kUnit; ++j) v[j] += load_cluster(there + ((u * kUnit + j) * kLanes + in_tile) * 4);
-      }
-      if constexpr (kSwap) store_output(a, static_cast<int64_t>(t) * a.out_stride + n, v[0] + bias_at(a, n));
-      else store_features(args, t, n, v);
+      float v = 0.f;
+#pragma unroll 8
+      for (int r = 0; r < split; ++r) v += load_cluster(in_cta(local, r) + (u * kLanes + in_tile) * 4);
+      store_output(a, static_cast<int64_t>(t) * a.out_stride + n, v + (kSwap ? bias_at(a, n) : biases[kSwap ? 0 : u]));
     }
   }
   cluster_sync();  // nobody leaves while another reads its shared memory
 }
 
-template <int BN, int WGS, bool kSwap>
+template <int BN, int WGS, Mode M>
 int launch_linear(LinearArgs& args, int split, cudaStream_t stream) {
-  using S = LinearShape<BN, WGS, kSwap>;
-  constexpr auto kernel = e4m3_linear_kernel<BN, WGS, kSwap>;
-  if (int st = allow_shared_memory<e4m3_linear_kernel<BN, WGS, kSwap>>(static_cast<int>(S::kSmem))) return st;
+  using S = LinearShape<BN, WGS, M>;
+  constexpr bool kSwap = S::kSwap, kPair = S::kPair;
+  constexpr auto kernel = e4m3_linear_kernel<BN, WGS, M>;
+  if (int st = allow_shared_memory<e4m3_linear_kernel<BN, WGS, M>>(static_cast<int>(S::kSmem))) return st;
   const TrisE4m3Linear& a = args.a;
-  args.row_tiles = ceil_div(a.rows, kSwap ? BN : kLanes);
+  args.row_tiles = ceil_div(a.rows, kSwap ? BN : kPair ? 2 * kLanes : kLanes);
   args.feature_tiles = ceil_div(a.out_features, kSwap ? kLanes : BN);
   args.per_cta = ceil_div(args.groups, split);
   split = ceil_div(args.groups, args.per_cta);  // every CTA has a group
+  args.wide_scales = aligned_to(a.x_scales, 16) && aligned_to(a.weight_scales, 16) && (a.rows == 1 || a.x_scales_stride % 4 == 0) &&
+                     (a.out_features <= kGroup || a.weight_scales_stride % 4 == 0) && (split == 1 || args.per_cta % 4 == 0);
   LinearMaps maps;
   const bool ok = encode_bytes_map(&maps.lanes, kSwap ? a.weight : a.x, kSwap ? a.out_features : a.rows, a.in_features, kSwap ? a.weight_stride : a.x_stride, kLanes) &&
-                  encode_bytes_map(&maps.columns, kSwap ? a.x : a.weight, kSwap ? a.rows : a.out_features, a.in_features, kSwap ? a.x_stride : a.weight_stride, BN);
+                  encode_bytes_map(&maps.columns, kSwap ? a.x : a.weight, kSwap ? a.rows : a.out_features, a.in_features, kSwap ? a.x_stride : a.weight_stride, S::kLoaded);
   TRIS_REQUIRE(ok, TRIS_ERR_CUDA, "e4m3_linear: no tensor map for these matrices");
-  const int64_t tiles = static_cast<int64_t>(args.row_tiles) * args.feature_tiles, room = static_cast<int64_t>(sm_count()) * S::kCtasPerSm;
+  const int elt = dtype_size(a.dtype);
+  args.store_map = !kSwap && split == 1 && aligned_to(a.out, 16) && a.out_stride * elt % 16 == 0;
+  if (args.store_map)
+    TRIS_REQUIRE(encode_output_map(&maps.out, a.out, a.rows, a.out_features, elt, a.out_stride * elt), TRIS_ERR_CUDA, "e4m3_linear: no tensor map for the output");
+  const int64_t tiles = static_cast<int64_t>(args.row_tiles) * args.feature_tiles, room = static_cast<int64_t>(sm_count()) * S::kCtasPerSm / (kPair ? 2 : 1);
   TRIS_REQUIRE(tiles < (1ll << 31) - room, TRIS_ERR_UNSUPPORTED, "e4m3_linear: more than 2^31 tiles");
   const int ctas = static_cast<int>(split > 1 || tiles < room ? tiles : room);
-  TRIS_CUDA(launch_step(kernel, dim3(ctas, 1, split), dim3(S::kThreads), S::kSmem, stream, programmatic_launch_default(), split, args, maps));
+  if constexpr (kPair) {  // the CTAs of a pair are neighbours along x
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * ctas);
+    cfg.blockDim = dim3(S::kThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = 2;
+    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = programmatic_launch_default() ? 2 : 1;
+    TRIS_CUDA(cudaLaunchKernelEx(&cfg, kernel, args, maps));
+  } else {
+    TRIS_CUDA(launch_step(kernel, dim3(ctas, 1, split), dim3(S::kThreads), S::kSmem, stream, programmatic_launch_default(), split, args, maps));
+  }
   return TRIS_OK;
 }
 
@@ -394,18 +522,18 @@ extern "C" int tris_e4m3_linear(const TrisE4m3Linear* linear, void* stream) {
   if (a.rows == 1) args.a.x_stride = line;  // of no account, but a tensor map wants one
   if (a.out_features == 1) args.a.weight_stride = line;
   args.groups = ceil_div(a.in_features, kGroup);
-  args.wide_store = aligned_to(a.out, 32) && a.out_stride * dtype_size(a.dtype) % 32 == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int sms = sm_count();
   if (a.rows <= 64) {
     const int split = split_of(ceil_div(a.out_features, kLanes), 2 * sms, args.groups);
-    if (a.rows <= 16) return launch_linear<16, 1, true>(args, split, s);
-    if (a.rows <= 32) return launch_linear<32, 1, true>(args, split, s);
-    return launch_linear<64, 1, true>(args, split, s);
+    if (a.rows <= 16) return launch_linear<16, 1, Mode::kFeatures>(args, split, s);
+    if (a.rows <= 32) return launch_linear<32, 1, Mode::kFeatures>(args, split, s);
+    return launch_linear<64, 1, Mode::kFeatures>(args, split, s);
   }
-  const int64_t row_tiles = ceil_div(a.rows, kLanes), large = row_tiles * ceil_div(a.out_features, 256), small = row_tiles * ceil_div(a.out_features, 128);
-  // time of the whole, in MMAs of 128 x 128: large tiles unless small ones leave fewer SMs without work
-  const int64_t t_large = (large + sms - 1) / sms * 2, t_small = (small + sms - 1) / sms;
-  if (t_large <= t_small) return launch_linear<256, 2, false>(args, 1, s);
-  return launch_linear<128, 2, false>(args, split_of(small, sms, args.groups), s);
+  const int64_t pairs = static_cast<int64_t>(ceil_div(a.rows, 2 * kLanes)) * ceil_div(a.out_features, 256);
+  const int64_t small = static_cast<int64_t>(ceil_div(a.rows, kLanes)) * ceil_div(a.out_features, 128);
+  // rounds of all SMs; one of pairs takes twice as long as one of small tiles
+  const int64_t t_pairs = (pairs + sms / 2 - 1) / (sms / 2) * 2, t_small = (small + sms - 1) / sms;
+  if (a.rows > kLanes && t_pairs <= t_small) return launch_linear<256, 2, Mode::kPair>(args, 1, s);
+  return launch_linear<128, 2, Mode::kRows>(args, split_of(small, sms, args.groups), s);
 }
