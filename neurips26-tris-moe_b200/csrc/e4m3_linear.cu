@@ -50,14 +50,18 @@ struct LinearShape {
   static constexpr int kLoaded = kPair ? BN / 2 : BN;  // rows of the second operand that a CTA loads
   static constexpr int kStageBytes = (kLanes + kLoaded) * kGroup;
   static constexpr int kCtasPerSm = kSwap ? 2 : 1;
-  static constexpr int kOutBytes = kSwap ? 0 : WGS * kLanes * 128;  // 128 bytes of every row, for each group of warps
-  static constexpr int kStagesThatFit = ((kCtasPerSm == 1 ? 227 : 113) * 1024 - 1024 - 1280 - kOutBytes) / kStageBytes;  // less the boundary's part and what else there is
+  static constexpr int kOutBytes = kSwap ? 0 : WGS * kLanes * 128;       // 128 bytes of every row, for each group of warps
+  static constexpr int kScaleBytes = kSwap ? 0 : WGS * (kLanes + 4) * 32;  // twice four groups' scales, for each thread and warp
+  static constexpr int kStagesThatFit = ((kCtasPerSm == 1 ? 227 : 113) * 1024 - 1024 - 1280 - kOutBytes - kScaleBytes) / kStageBytes;  // less the boundary's part and what else there is
   static constexpr int kStages = kStagesThatFit > 8 ? 8 : kStagesThatFit;
   static constexpr int kWarps = 4 * WGS, kThreads = 32 * (kWarps + 2);
   static constexpr int kColumns = BN / WGS;  // of a thread
   static constexpr int kTiles = BN == 256 ? 2 : 4;  // in TMEM, that take turns
+  static constexpr int kHalves = kPair ? WGS : 1;    // of a tile that are multiplied, read and given back by themselves
+  static constexpr int kHalf = BN / kHalves;
   static constexpr int kTmem = kTiles * BN;
-  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + kOutBytes + 1024;
+  static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + kOutBytes + kScaleBytes + 1024;
+  static_assert(!kPair || (kHalf == kColumns && kHalf == kGroup), "a group of warps has a half, and one block's scale");
   static_assert(kStages >= 3 && (kPair || BN * kLanes * 4 <= kStages * kStageBytes), "a tile's sums lie where the stages were");
 };
 
@@ -93,7 +97,10 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst_smem, const CUtensorM
                "r"(c0), "r"(c1), "r"(bar_of_first)
                : "memory");
 }
-__device__ __forceinline__ void arrive_in_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void cp_async_4(void* dst_smem, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst_smem)), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void arrive_in_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int c0, int c1, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0), "r"(c1), "r"(src) : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
@@ -118,12 +125,13 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
   else tmem_ld_32(taddr, v);
 }
 
-// As mbar_wait_bounded; the timer, whose reading takes longer than most of these waits, is not looked at before 256 tries have failed.
+// Waits for the phase with the given parity, giving up after 2^20 tries, each of which waits itself up to a limit of the hardware's.  (The timer takes longer to read
+// than most of these waits, and code that may read it costs registers.)
 __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity) {
+  bool done = false;
 #pragma unroll 1
-  for (int i = 0; i < 256; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait_bounded(bar, parity);
+  for (int i = 0; !done && i < (1 << 20); ++i) done = mbar_try_wait(bar, parity);
+  return done;
 }
 // The same by a whole warp, with one answer for all lanes.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait_one(bar, parity)); }
@@ -146,7 +154,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
   constexpr bool kSwap = S::kSwap, kPair = S::kPair;
   extern __shared__ uint4 smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>(smem_raw) + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  __shared__ uint64_t full[S::kStages], empty[S::kStages], tile_full[S::kTiles], tile_empty[S::kTiles];
+  __shared__ uint64_t full[S::kStages], empty[S::kStages], tile_full[S::kTiles][S::kHalves], tile_empty[S::kTiles][S::kHalves];
   __shared__ uint32_t tmem_base;
   __shared__ int timed_out;
   __shared__ __align__(16) float row_scales[2][kSwap ? BN : 4];
@@ -162,10 +170,11 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < S::kTiles; ++i) {
-      mbar_init(&tile_full[i], 1);
-      mbar_init(&tile_empty[i], S::kWarps * (kPair ? 2 : 1));
-    }
+    for (int i = 0; i < S::kTiles; ++i)
+      for (int h = 0; h < S::kHalves; ++h) {
+        mbar_init(&tile_full[i][h], 1);
+        mbar_init(&tile_empty[i][h], S::kWarps / S::kHalves * (kPair ? 2 : 1));
+      }
     fence_mbar_init();
     timed_out = 0;
   }
@@ -197,7 +206,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
       for (int tile = walker; tile < tiles && ok; tile += walkers) {
         int rt, ft;
         place(tile, rt, ft);
-        const int lane0 = kSwap ? ft * kLanes : (rt * (kPair ? 2 : 1) + rank) * kLanes, column0 = (kSwap ? rt : ft) * BN + rank * S::kLoaded;
+        const int lane0 = kSwap ? ft * kLanes : (rt * (kPair ? 2 : 1) + rank) * kLanes, column0 = (kSwap ? rt : ft) * BN + rank * (S::kLoaded / S::kHalves);
         for (int g = 0; g < count; ++g, ++asked) {
           const int s = asked % S::kStages;
           if (asked >= S::kStages && !wait_one(&empty[s], (asked / S::kStages - 1) & 1)) {
@@ -210,7 +219,9 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
             if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * S::kStageBytes);  // the other CTA's bytes, too
             const uint32_t bar = in_cta(smem_u32(&full[s]), 0);
             tma_load_2d_pair(to, &maps.lanes, (first + g) * kGroup, lane0, bar);
-            tma_load_2d_pair(to + kLanes * kGroup, &maps.columns, (first + g) * kGroup, column0, bar);
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h)  // of either half's columns one half
+              tma_load_2d_pair(to + (kLanes + h * (S::kHalf / 2)) * kGroup, &maps.columns, (first + g) * kGroup, column0 + h * S::kHalf, bar);
           } else {
             mbar_arrive_expect_tx(&full[s], S::kStageBytes);
             tma_load_2d(to, &maps.lanes, (first + g) * kGroup, lane0, &full[s]);
@@ -221,32 +232,38 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
     }
     __syncwarp();
   } else if (warp == S::kWarps + 1) {
-    const uint32_t idesc = umma_idesc_f16(kPair ? 2 * kLanes : kLanes, BN);  // the same fields: fp32 sums, operand types 0 (here e4m3), K-major
+    const uint32_t idesc = umma_idesc_f16(kPair ? 2 * kLanes : kLanes, S::kHalf);  // the same fields: fp32 sums, operand types 0 (here e4m3), K-major
     bool ok = true;
     int i = 0;
     for (int tile = walker; rank == 0 && tile < tiles && ok; tile += walkers) {
       for (int g = 0; g < count; ++g, ++i) {
         const int s = i % S::kStages, turn = i % S::kTiles;
-        ok = wait_for(&full[s], (i / S::kStages) & 1) && (i < S::kTiles || wait_for(&tile_empty[turn], (i / S::kTiles - 1) & 1));
-        if (!ok) break;
-        tcgen05_fence_after();
+        ok = wait_for(&full[s], (i / S::kStages) & 1);
         const uint32_t at = smem_u32(ring + s * S::kStageBytes);
         const uint64_t da = umma_smem_desc_sw128(at), db = umma_smem_desc_sw128(at + kLanes * kGroup);
-        if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < kGroup / 32; ++j) {
-            if constexpr (kPair) umma_f8_ss_pair(tmem + turn * BN, da + 2 * j, db + 2 * j, idesc, j > 0 ? 1u : 0u);
-            else umma_f8_ss(tmem + turn * BN, da + 2 * j, db + 2 * j, idesc, j > 0 ? 1u : 0u);
+        for (int h = 0; h < S::kHalves; ++h) {
+          ok = ok && (i < S::kTiles || wait_for(&tile_empty[turn][h], (i / S::kTiles - 1) & 1));
+          if (!ok) break;
+          tcgen05_fence_after();
+          if (elect_one()) {
+            const uint32_t to = tmem + turn * BN + h * S::kHalf;
+#pragma unroll
+            for (int j = 0; j < kGroup / 32; ++j) {
+              if constexpr (kPair) umma_f8_ss_pair(to, da + 2 * j, db + 2 * j + h * (S::kHalf / 2 * kGroup / 16), idesc, j > 0 ? 1u : 0u);
+              else umma_f8_ss(to, da + 2 * j, db + 2 * j, idesc, j > 0 ? 1u : 0u);
+            }
+            if constexpr (kPair) {
+              if (h == S::kHalves - 1) umma_commit_pair(&empty[s]);
+              umma_commit_pair(&tile_full[turn][h]);
+            } else {
+              umma_commit(&empty[s]);
+              umma_commit(&tile_full[turn][h]);
+            }
           }
-          if constexpr (kPair) {
-            umma_commit_pair(&empty[s]);
-            umma_commit_pair(&tile_full[turn]);
-          } else {
-            umma_commit(&empty[s]);
-            umma_commit(&tile_full[turn]);
-          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
       }
     }
     if (!ok && lane == 0) timed_out = 1;
@@ -254,8 +271,13 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
   } else {
     const int wg = warp >> 2, in_tile = 32 * (warp & 3) + lane;  // lane of the tile
     const uint32_t from = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + wg * S::kColumns;
-    constexpr int kPart = S::kColumns < 32 ? S::kColumns : 32, kQuad = kSwap ? 1 : 4;
+    constexpr int kPart = S::kColumns < 32 ? S::kColumns : 32;  // columns that leave TMEM at a time
+    constexpr int kQuad = kSwap ? 1 : 4;
     uint8_t* out_stage = ring + S::kStages * S::kStageBytes + wg * kLanes * 128;
+    // Scales of four groups: this thread's row's, and the weights' block's for its warp.  They are asked for by asynchronous copies of their own, four groups ahead:
+    // loads to registers kept eight of them occupied, and the sums went to local memory.
+    float4* x_scales = reinterpret_cast<float4*>(ring + S::kStages * S::kStageBytes + S::kOutBytes) + threadIdx.x;
+    float4* w_scales = reinterpret_cast<float4*>(ring + S::kStages * S::kStageBytes + S::kOutBytes) + 2 * 32 * S::kWarps + warp;
     bool ok = true;
     int i = 0;
     for (int tile = walker; tile < tiles; tile += walkers) {
@@ -268,46 +290,69 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
       const bool has_row = row < a.rows && (!kSwap || threadIdx.x < BN), has_block = block * kGroup < a.out_features;
       const float* xs = a.x_scales + static_cast<int64_t>(has_row ? row : 0) * a.x_scales_stride + first;
       const float* ws = a.weight_scales + static_cast<int64_t>(has_block ? block : 0) * a.weight_scales_stride + first;
-      float x_next[kQuad], w_next[kQuad];
-      auto fetch_scales = [&](int g) {
-        if (kQuad == 4 && args.wide_scales && g + 4 <= count) {
-          const float4 x = *reinterpret_cast<const float4*>(xs + g), w = *reinterpret_cast<const float4*>(ws + g);
-          x_next[0] = x.x, x_next[kQuad - 3] = x.y, x_next[kQuad - 2] = x.z, x_next[kQuad - 1] = x.w;
-          w_next[0] = w.x, w_next[kQuad - 3] = w.y, w_next[kQuad - 2] = w.z, w_next[kQuad - 1] = w.w;
-        } else {
+      float x_next = 0.f, w_next = 0.f;
+      auto ask_scales = [&](int g) {
+        float4 *x_to = x_scales + (g / 4 & 1) * 32 * S::kWarps, *w_to = w_scales + (g / 4 & 1) * S::kWarps;
+        if (g < count) {
+          if (args.wide_scales && g + 4 <= count) {
+            cp_async_16(x_to, xs + g, has_row);
+            if (lane == 0) cp_async_16(w_to, ws + g);
+          } else {
 #pragma unroll
-          for (int q = 0; q < kQuad; ++q) {
-            x_next[q] = g + q < count ? xs[g + q] : 0.f;
-            w_next[q] = g + q < count ? ws[g + q] : 0.f;
+            for (int q = 0; q < 4; ++q) {
+              const bool there = g + q < count;
+              cp_async_4(reinterpret_cast<float*>(x_to) + q, there ? xs + g + q : xs, there && has_row);
+              if (lane == 0) cp_async_4(reinterpret_cast<float*>(w_to) + q, there ? ws + g + q : ws, there);
+            }
           }
         }
+        cp_async_commit();
       };
-      fetch_scales(0);
+      if constexpr (kSwap) {
+        x_next = has_row ? xs[0] : 0.f;
+        w_next = ws[0];
+      } else {
+        ask_scales(0);
+      }
       if constexpr (!kSwap) {
         // (a barrier lies between this and the last use of the tile before: the one behind the tile's last stores, or the warps' own below)
         named_barrier_sync(1 + wg, 128);
         if (in_tile < S::kColumns) biases[wg * S::kColumns + in_tile] = feature0 + in_tile < a.out_features ? bias_at(a, feature0 + in_tile) : 0.f;
         named_barrier_sync(1 + wg, 128);
       }
-      uint64_t acc[S::kColumns / 2];
+      float acc[S::kColumns];
 #pragma unroll
-      for (int c = 0; c < S::kColumns / 2; ++c) acc[c] = 0;
+      for (int c = 0; c < S::kColumns; ++c) acc[c] = 0.f;
+#pragma unroll 1
       for (int g0 = 0; g0 < count; g0 += kQuad) {
         float scales[kQuad];
-#pragma unroll
-        for (int q = 0; q < kQuad; ++q) scales[q] = has_row ? x_next[q] * w_next[q] : 0.f;
-        if (g0 + kQuad < count) fetch_scales(g0 + kQuad);
+        if constexpr (kSwap) {
+          scales[0] = x_next * w_next;
+          if (g0 + 1 < count) {
+            x_next = has_row ? xs[g0 + 1] : 0.f;
+            w_next = ws[g0 + 1];
+          }
+          // two places take turns: who writes the next but one has met everybody who reads this one
+          if (threadIdx.x < BN) row_scales[i & 1][threadIdx.x] = scales[0];
+          named_barrier_sync(1, 32 * S::kWarps);
+        } else {
+          __syncwarp();  // the last four have been read
+          ask_scales(g0 + 4);
+          cp_async_wait<1>();
+          __syncwarp();
+          const float4 x = x_scales[(g0 / 4 & 1) * 32 * S::kWarps], w = w_scales[(g0 / 4 & 1) * S::kWarps];
+          scales[0] = has_row ? x.x * w.x : 0.f;
+          scales[kQuad - 3] = has_row ? x.y * w.y : 0.f;
+          scales[kQuad - 2] = has_row ? x.z * w.z : 0.f;
+          scales[kQuad - 1] = has_row ? x.w * w.w : 0.f;
+        }
 #pragma unroll
         for (int q = 0; q < kQuad; ++q) {
           if (g0 + q >= count) break;
           const int half = i & 1, turn = i % S::kTiles, parity = (i / S::kTiles) & 1;
+          const float scale = scales[q];
           ++i;
-          if constexpr (kSwap) {
-            // two places take turns: who writes the next but one has met everybody who reads this one
-            if (threadIdx.x < BN) row_scales[half][threadIdx.x] = scales[q];
-            named_barrier_sync(1, 32 * S::kWarps);
-          }
-          if (ok) ok = wait_for(&tile_full[turn], parity);
+          if (ok) ok = wait_for(&tile_full[turn][kPair ? wg : 0], parity);
           if (!ok) continue;
           tcgen05_fence_after();
 #pragma unroll
@@ -318,21 +363,22 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
               tcgen05_fence_before();
               __syncwarp();
               if (lane == 0) {
-                if constexpr (kPair) arrive_in_cluster(in_cta(smem_u32(&tile_empty[turn]), 0));
-                else mbar_arrive(&tile_empty[turn]);
+                if constexpr (kPair) arrive_in_cluster(in_cta(smem_u32(&tile_empty[turn][wg]), 0));
+                else mbar_arrive(&tile_empty[turn][0]);
               }
             }
             if constexpr (kSwap) {
 #pragma unroll
               for (int j = 0; j < kPart; j += 4) {
                 const float4 s = *reinterpret_cast<const float4*>(&row_scales[half][c + j]);
-                acc[(c + j) / 2] = fma_2(pack_2(v[j], v[j + 1]), pack_2(s.x, s.y), acc[(c + j) / 2]);
-                acc[(c + j) / 2 + 1] = fma_2(pack_2(v[j + 2], v[j + 3]), pack_2(s.z, s.w), acc[(c + j) / 2 + 1]);
+                acc[c + j] = fmaf(v[j], s.x, acc[c + j]);
+                acc[c + j + 1] = fmaf(v[j + 1], s.y, acc[c + j + 1]);
+                acc[c + j + 2] = fmaf(v[j + 2], s.z, acc[c + j + 2]);
+                acc[c + j + 3] = fmaf(v[j + 3], s.w, acc[c + j + 3]);
               }
             } else {
-              const uint64_t s = pack_2(scales[q], scales[q]);
 #pragma unroll
-              for (int j = 0; j < kPart; j += 2) acc[(c + j) / 2] = fma_2(pack_2(v[j], v[j + 1]), s, acc[(c + j) / 2]);
+              for (int j = 0; j < kPart; ++j) acc[c + j] = fmaf(v[j], scale, acc[c + j]);
             }
           }
         }
@@ -340,18 +386,13 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
       if (!ok) {  // a wait has run out: what is stored says so
         timed_out = 1;
 #pragma unroll
-        for (int c = 0; c < S::kColumns / 2; ++c) acc[c] = pack_2(NAN, NAN);
+        for (int c = 0; c < S::kColumns; ++c) acc[c] = NAN;
       }
-      auto sum = [&](int c) {
-        float lo, hi;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(acc[c / 2]));
-        return c & 1 ? hi : lo;
-      };
       if (split > 1) {
         // the ring is idle: this CTA's only tile has been multiplied
         float* part = reinterpret_cast<float*>(ring);
 #pragma unroll
-        for (int c = 0; c < S::kColumns; ++c) part[(wg * S::kColumns + c) * kLanes + in_tile] = sum(c);
+        for (int c = 0; c < S::kColumns; ++c) part[(wg * S::kColumns + c) * kLanes + in_tile] = acc[c];
       } else if constexpr (kSwap) {
         const int n = ft * kLanes + in_tile;
         if (n < a.out_features) {
@@ -359,7 +400,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
 #pragma unroll
           for (int c = 0; c < S::kColumns; ++c) {
             const int t = rt * BN + c;
-            if (t < a.rows) store_output(a, static_cast<int64_t>(t) * a.out_stride + n, sum(c) + bias);
+            if (t < a.rows) store_output(a, static_cast<int64_t>(t) * a.out_stride + n, acc[c] + bias);
           }
         }
       } else if (args.store_map) {
@@ -381,7 +422,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
 #pragma unroll
               for (int c = 0; c < 32; c += 4) {
                 const float4 b = *reinterpret_cast<const float4*>(&biases[wg * S::kColumns + c0 + c]);
-                put(c / 4, make_uint4(__float_as_uint(sum(c0 + c) + b.x), __float_as_uint(sum(c0 + c + 1) + b.y), __float_as_uint(sum(c0 + c + 2) + b.z), __float_as_uint(sum(c0 + c + 3) + b.w)));
+                put(c / 4, make_uint4(__float_as_uint(acc[c0 + c] + b.x), __float_as_uint(acc[c0 + c + 1] + b.y), __float_as_uint(acc[c0 + c + 2] + b.z), __float_as_uint(acc[c0 + c + 3] + b.w)));
               }
             });
         } else {
@@ -394,7 +435,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                   const float2 b = *reinterpret_cast<const float2*>(&biases[wg * S::kColumns + c0 + c + 2 * k]);
-                  const float x = sum(c0 + c + 2 * k) + b.x, y = sum(c0 + c + 2 * k + 1) + b.y;
+                  const float x = acc[c0 + c + 2 * k] + b.x, y = acc[c0 + c + 2 * k + 1] + b.y;
                   w[k] = a.dtype == TRIS_DTYPE_F16 ? Pair<__half>::pack(x, y) : Pair<__nv_bfloat16>::pack(x, y);
                 }
                 put(c / 8, make_uint4(w[0], w[1], w[2], w[3]));
@@ -405,7 +446,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
         const int64_t at = static_cast<int64_t>(row) * a.out_stride + feature0;
 #pragma unroll
         for (int c = 0; c < S::kColumns; ++c)
-          if (feature0 + c < a.out_features) store_output(a, at + c, sum(c) + biases[wg * S::kColumns + c]);
+          if (feature0 + c < a.out_features) store_output(a, at + c, acc[c] + biases[wg * S::kColumns + c]);
       }
     }
     if (!kSwap && in_tile == 0) tma_stores_done();
@@ -459,7 +500,7 @@ int launch_linear(LinearArgs& args, int split, cudaStream_t stream) {
                      (a.out_features <= kGroup || a.weight_scales_stride % 4 == 0) && (split == 1 || args.per_cta % 4 == 0);
   LinearMaps maps;
   const bool ok = encode_bytes_map(&maps.lanes, kSwap ? a.weight : a.x, kSwap ? a.out_features : a.rows, a.in_features, kSwap ? a.weight_stride : a.x_stride, kLanes) &&
-                  encode_bytes_map(&maps.columns, kSwap ? a.x : a.weight, kSwap ? a.rows : a.out_features, a.in_features, kSwap ? a.x_stride : a.weight_stride, S::kLoaded);
+                  encode_bytes_map(&maps.columns, kSwap ? a.x : a.weight, kSwap ? a.rows : a.out_features, a.in_features, kSwap ? a.x_stride : a.weight_stride, S::kLoaded / S::kHalves);
   TRIS_REQUIRE(ok, TRIS_ERR_CUDA, "e4m3_linear: no tensor map for these matrices");
   const int elt = dtype_size(a.dtype);
   args.store_map = !kSwap && split == 1 && aligned_to(a.out, 16) && a.out_stride * elt % 16 == 0;
@@ -534,6 +575,6 @@ extern "C" int tris_e4m3_linear(const TrisE4m3Linear* linear, void* stream) {
   const int64_t small = static_cast<int64_t>(ceil_div(a.rows, kLanes)) * ceil_div(a.out_features, 128);
   // rounds of all SMs; one of pairs takes twice as long as one of small tiles
   const int64_t t_pairs = (pairs + sms / 2 - 1) / (sms / 2) * 2, t_small = (small + sms - 1) / sms;
-  if (a.rows > kLanes && t_pairs <= t_small) return launch_linear<256, 2, Mode::kPair>(args, 1, s);
+  if (a.rows > kLanes && 3 * t_pairs <= 5 * t_small) return launch_linear<256, 2, Mode::kPair>(args, 1, s);
   return launch_linear<128, 2, Mode::kRows>(args, split_of(small, sms, args.groups), s);
 }
