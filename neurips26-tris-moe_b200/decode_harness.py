@@ -11,8 +11,10 @@ is captured into a CUDA graph and replayed ``output_length - 1`` times with no h
 
 With ``page_size`` the decoder runs on the operators of ``decode_ops``: keys and values go to a paged
 cache (fp16 or e4m3), one new token attends over the tokens that are there and no others, and the
-residual is added by the norm that follows it.  ``run_exact_generation`` takes ``logit_controls``
-(penalties, biases, grammar masks) either way.
+residual is added by the norm that follows it.  ``cache_scale_tokens`` gives an e4m3 cache a scale for each block of that
+many tokens, and ``linear_dtype=torch.float8_e4m3fn`` runs the projections and the logits' product in 8 bits: the
+norm's output goes into them as it is.  ``run_exact_generation`` takes ``logit_controls`` (penalties, biases, grammar
+masks) and ``sampling`` (temperature, top-k, top-p, min-p) either way.
 """
 from __future__ import annotations
 
@@ -24,7 +26,9 @@ from typing import List, Optional
 import torch
 import torch.nn.functional as F
 
-from .decode_ops import add_rms_norm, append_paged_kv, apply_logit_controls, paged_decode_attention, raise_on_status
+from .decode_ops import (add_rms_norm, add_rms_norm_e4m3, append_paged_kv, apply_logit_controls, paged_decode_attention, raise_on_status,
+                         sample_tokens)
+from .e4m3_ops import GROUP, linear_e4m3, quantize_e4m3
 from .moe_block import TrisSparseMoeBlock
 
 
@@ -60,10 +64,12 @@ def _rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor
 class TrisDecoder(torch.nn.Module):
     """``len(moe_blocks)`` decoder layers: RMSNorm -> attention (fp16, KV cache) -> RMSNorm -> MoE.  ``page_size``: the cache is
     paged and the layers run on ``decode_ops``; ``cache_dtype`` is fp16 or ``torch.float8_e4m3fn`` (scale 1: normalised keys and
-    values are a few units large)."""
+    values are a few units large; with ``cache_scale_tokens``: one scale for each block of that many tokens and head).  ``linear_dtype``:
+    ``torch.float8_e4m3fn`` holds the attention's projections and the logits' matrix in 8 bits with block scales."""
 
     def __init__(self, moe_blocks: List[TrisSparseMoeBlock], shape: DecoderShape, max_length: int, max_batch: int,
-                 device, seed: int = 0, page_size: Optional[int] = None, cache_dtype: torch.dtype = torch.float16):
+                 device, seed: int = 0, page_size: Optional[int] = None, cache_dtype: torch.dtype = torch.float16,
+                 cache_scale_tokens: Optional[int] = None, linear_dtype: torch.dtype = torch.float16):
         super().__init__()
         self.shape, self.blocks = shape, list(moe_blocks)
         self.max_length, self.max_batch = int(max_length), int(max_batch)
@@ -78,6 +84,13 @@ class TrisDecoder(torch.nn.Module):
         self.key_index = torch.arange(self.max_length, device=dev)[None, None, None, :]
         self.layers = []
         self.page_size = page_size
+        self.scale_tokens = cache_scale_tokens
+        self.linear8 = linear_dtype == torch.float8_e4m3fn
+        what = "trismoe_b200 decode harness: "
+        if cache_scale_tokens and (cache_dtype != torch.float8_e4m3fn or not page_size or page_size % cache_scale_tokens):
+            raise RuntimeError(what + "scales of blocks belong to a paged cache in 8 bits, whose pages are whole blocks")
+        if linear_dtype not in (torch.float16, torch.float8_e4m3fn) or (self.linear8 and (not page_size or H % GROUP)):
+            raise RuntimeError(what + f"projections are fp16, or, with a paged cache and a hidden size that is a multiple of {GROUP}, e4m3")
         if page_size:
             width = -(-self.max_length // page_size)
             # a sequence's pages one after the other: an allocator would hand them out in any order
@@ -94,6 +107,14 @@ class TrisDecoder(torch.nn.Module):
                 "wqkv": rnd((nh + 2 * nkv) * hd, H, std=1.0 / math.sqrt(H)), "wo": rnd(H, nh * hd, std=1.0 / math.sqrt(nh * hd)),
                 "k": pages(), "v": pages(),
             })
+            if cache_scale_tokens:
+                scales = lambda: torch.zeros((max_batch * width, page_size // cache_scale_tokens, nkv), dtype=torch.float32, device=dev)
+                self.layers[-1].update(k_scale=scales(), v_scale=scales())
+        if self.linear8:
+            quantized = lambda w: quantize_e4m3(w, group_rows=GROUP)
+            self.lm_head = quantized(self.lm_head)
+            for layer in self.layers:
+                layer.update(wqkv=quantized(layer["wqkv"]), wo=quantized(layer["wo"]))
 
     def _attention(self, layer: dict, x: torch.Tensor, positions: torch.Tensor, batch: int, rope, mask) -> torch.Tensor:
         """x [B, S, H]; positions [B, S] absolute positions of these tokens.  Writes K/V at the
@@ -115,22 +136,42 @@ class TrisDecoder(torch.nn.Module):
         out = F.scaled_dot_product_attention(q, keys, vals, attn_mask=mask)
         return F.linear(out.transpose(1, 2).reshape(B, S, nq * s.head_dim), layer["wo"])
 
-    def _paged_attention(self, layer: dict, x: torch.Tensor, positions: torch.Tensor, sequences, lengths, mask) -> torch.Tensor:
+    def _linear(self, x, weight, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+        """``x`` as the weight takes it: rows in fp16 or, in 8 bits, those or values with their scales."""
+        if not self.linear8:
+            return F.linear(x, weight).to(dtype)
+        return linear_e4m3(*(x if isinstance(x, tuple) else quantize_e4m3(x)), *weight, dtype=dtype)
+
+    def _norm(self, x: torch.Tensor, h: Optional[torch.Tensor], weight: torch.Tensor):
+        """The residual norm ahead of a product: its rows as ``_linear`` takes them, and the new residual."""
+        if not self.linear8:
+            return add_rms_norm(x, h, weight, self.shape.rms_eps)
+        values, scales, h = add_rms_norm_e4m3(x, h, weight, self.shape.rms_eps, group_size=GROUP)
+        return (values, scales), h
+
+    def _paged_attention(self, layer: dict, x, positions: torch.Tensor, sequences, lengths, mask) -> torch.Tensor:
         """The same over pages.  One new token per sequence attends through the block table; several (a prompt) over the pages
         gathered to the dense form."""
         s = self.shape
-        B, S, _ = x.shape
+        B, S = positions.shape
         nq, nkv, hd = s.num_heads, s.num_kv_heads, s.head_dim
-        qkv = F.linear(x, layer["wqkv"]).view(B * S, nq + 2 * nkv, hd)
+        qkv = self._linear(x, layer["wqkv"]).view(B * S, nq + 2 * nkv, hd)
         table = self.block_table[:B]
+        scales = {name: layer.get(name) for name in ("k_scale", "v_scale")}
         q = append_paged_kv(qkv[:, :nq], qkv[:, nq: nq + nkv], qkv[:, nq + nkv:], layer["k"], layer["v"], table, positions.reshape(-1), sequences,
-                            cos=self.rope_cos, sin=self.rope_sin, status=self.cache_status)
+                            cos=self.rope_cos, sin=self.rope_sin, status=self.cache_status, **scales)
         if S == 1:
-            out = paged_decode_attention(q, layer["k"], layer["v"], table, lengths, status=self.cache_status)
+            out = paged_decode_attention(q, layer["k"], layer["v"], table, lengths, status=self.cache_status, **scales)
         else:
-            dense = lambda pages: pages[table].reshape(B, -1, nkv, hd)[:, : self.max_length].transpose(1, 2).to(q.dtype).repeat_interleave(nq // nkv, dim=1)
-            out = F.scaled_dot_product_attention(q.view(B, S, nq, hd).transpose(1, 2), dense(layer["k"]), dense(layer["v"]), attn_mask=mask).transpose(1, 2)
-        return F.linear(out.reshape(B, S, nq * hd), layer["wo"])
+            def dense(pages, scale):
+                rows = pages[table]
+                if scale is not None:
+                    rows = rows.float() * scale[table].repeat_interleave(self.scale_tokens, 2)[..., None]
+                return rows.reshape(B, -1, nkv, hd)[:, : self.max_length].transpose(1, 2).to(q.dtype).repeat_interleave(nq // nkv, dim=1)
+
+            k, v = dense(layer["k"], scales["k_scale"]), dense(layer["v"], scales["v_scale"])
+            out = F.scaled_dot_product_attention(q.view(B, S, nq, hd).transpose(1, 2), k, v, attn_mask=mask).transpose(1, 2)
+        return self._linear(out.reshape(B, S, nq * hd), layer["wo"])
 
     def _paged_forward(self, token_ids: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         B, S = token_ids.shape
@@ -141,12 +182,13 @@ class TrisDecoder(torch.nn.Module):
         else:
             sequences = torch.arange(B, dtype=torch.int32, device=h.device).repeat_interleave(S)
             mask = self.key_index <= positions[:, None, :, None]
-        x, _ = add_rms_norm(h, None, self.layers[0]["ln1"], eps)
+        x, _ = self._norm(h, None, self.layers[0]["ln1"])
         for i, (layer, blk) in enumerate(zip(self.layers, self.blocks)):
             x, h = add_rms_norm(self._paged_attention(layer, x, positions, sequences, lengths, mask), h, layer["ln2"], eps)
             y, _ = blk(x)
-            x, h = add_rms_norm(y, h, self.layers[i + 1]["ln1"] if i + 1 < len(self.layers) else self.final_norm, eps)
-        return F.linear(x[:, -1], self.lm_head).float()
+            x, h = self._norm(y, h, self.layers[i + 1]["ln1"] if i + 1 < len(self.layers) else self.final_norm)
+        last = tuple(part[:, -1] for part in x) if self.linear8 else x[:, -1]
+        return self._linear(last, self.lm_head, torch.float32)
 
     def raise_on_kernel_status(self) -> None:
         """Raises if a paged operator met a page, position or length that does not fit (waits for the GPU)."""
@@ -170,11 +212,12 @@ class TrisDecoder(torch.nn.Module):
 
 
 def run_exact_generation(model: TrisDecoder, input_ids: torch.Tensor, output_length: int, use_graph: bool = True,
-                         measure_latency: bool = True, logit_controls: Optional[dict] = None) -> dict:
-    """Prefill ``input_ids`` [B, L], then generate exactly ``output_length`` tokens greedily.  Returns the
+                         measure_latency: bool = True, logit_controls: Optional[dict] = None, sampling: Optional[dict] = None) -> dict:
+    """Prefill ``input_ids`` [B, L], then generate exactly ``output_length`` tokens, greedily or drawn.  Returns the
     reference benchmark's fields (prefill_ms, decode_ms, decode_tokens_per_s, ...) and the tokens.  ``logit_controls``: arguments of
     ``apply_logit_controls`` (``repetition``, ``presence``, ``frequency``, ``bias_ids``, ``bias_values``, ``allowed``) for every step; the
-    history of prompt and answer is kept here."""
+    history of prompt and answer is kept here.  ``sampling``: ``random`` (fp32 [output_length, B], a row for each step) and arguments of
+    ``sample_tokens`` (``temperature``, ``top_k``, ``top_p``, ``min_p``); a sequence none of whose tokens can be drawn gets token 0."""
     dev = input_ids.device
     B, L = (int(v) for v in input_ids.shape)
     if L + output_length > model.max_length or B > model.max_batch:
@@ -189,11 +232,23 @@ def run_exact_generation(model: TrisDecoder, input_ids: torch.Tensor, output_len
         known = torch.full((B,), L, dtype=torch.int32, device=dev)
         prompt = known.clone()
 
-    def choose(logits):
-        """Greedy token [B, 1] under the controls, noted in the history."""
-        if history is None:
+    random = None
+    if sampling is not None:
+        sampling = dict(sampling)
+        random = sampling.pop("random")
+        if random.shape != (output_length, B) or random.dtype is not torch.float32:
+            raise RuntimeError(f"trismoe_b200 decode harness: sampling needs random numbers, fp32 [{output_length}, {B}]")
+
+    def pick(logits):
+        if random is None:
             return logits.argmax(dim=-1, keepdim=True)
-        chosen = apply_logit_controls(logits, tokens=history, token_lengths=known, prompt_lengths=prompt, out=logits, **logit_controls).argmax(dim=-1, keepdim=True)
+        return sample_tokens(logits, random.index_select(0, step_index).view(B), **sampling).clamp_(min=0)[:, None]
+
+    def choose(logits):
+        """Token [B, 1] under the controls, noted in the history."""
+        if history is None:
+            return pick(logits)
+        chosen = pick(apply_logit_controls(logits, tokens=history, token_lengths=known, prompt_lengths=prompt, out=logits, **logit_controls))
         history.index_copy_(1, step_index + L, chosen.to(torch.int32))
         known.add_(1)
         return chosen
