@@ -361,6 +361,7 @@ int launch_blocks(const BlockArgs& a, Form form, cudaStream_t stream) {
 
 // Arguments have been checked (tris_paged_kv_append).
 int append_block_scaled(const TrisPagedKv& c, const TrisPagedAppend& r, int rotary_dim, cudaStream_t stream) {
+  TRIS_REQUIRE(r.sequences || r.num_tokens <= c.num_sequences, TRIS_ERR_INVALID_ARG, "paged_kv_append: %d tokens without sequences for a block table of %d", r.num_tokens, c.num_sequences);
   BlockArgs a{c, r};
   a.rows.rotary_dim = rotary_dim;
   a.page_shift = a.block_mask = -1;
