@@ -5,9 +5,10 @@
 // (but for what becomes smaller than e4m3 can be), however often it happens.  Bound by bytes for prompts, by the chain position -> page -> scale -> store for
 // a decode step.
 //
-// Tokens that follow one another in a block are a run, and one warp has all of a run for one head's keys or values: it finds the largest
-// magnitude, then scales and stores.  Up to kHeld rows for each of its row places stay in registers in between; longer runs are read again, from L1 or L2.
-// Whoever has the chunk of tokens in which a run begins has all of it.  Queries are only rotated, head by head.
+// Tokens that follow one another in a block are a run.  A CTA has the rows of some neighbouring tokens, whole runs, and some heads: a thread has the same 16 dimensions
+// of its row for one head after the other - two chunks of eight that rotate together - so that its cosines and sines are read once.  Two heads are rotated, their rows' largest
+// magnitudes meet in shared memory, and while they do the next two are on their way.  A run longer than a CTA's rows is read twice, the second time from L2.
+// (A warp for each run and head, which had the rows' cosines to read for every head, took 75 us for 4 prompts of 2047 tokens.)
 #include <float.h>
 
 #include "decode_step.cuh"
@@ -15,340 +16,423 @@
 namespace tris {
 namespace {
 
-constexpr int kWarps = 4, kHeld = 8;
+constexpr int kHeads = 2;  // at a time
 
 struct BlockArgs {
   TrisPagedKv cache;
   TrisPagedAppend rows;
-  int chunk;        // tokens that a warp looks at: 1 to 32
-  int shares;       // CTAs that share a chunk's heads
+  int lanes;        // that have a row, 16 dimensions each: a power of two
+  int window;       // rows of a CTA, up to 32
   int page_shift;   // log2(page_size), or -1
   int block_mask;   // scale_tokens - 1 where that is a power of two, or -1
   int page_scales;  // scales of a page and head
-  int lanes;        // that have a row, eight dimensions each: a power of two
 };
 
 // Which pairs of dimensions rotate together, and whether eight elements and four cosines can be read, and eight results written, at once: (i, i + half) with
-// half a multiple of 8, so that the other element is in another lane at the same place; (2 i, 2 i + 1); and whatever else there is.
+// half a multiple of 8; (2 i, 2 i + 1); and whatever else there is.
 enum class Form { kHalves, kPairs, kAny };
 
-// The biased exponent of the smallest power of two s with top <= 448 s, from 2^-64 to 2^64.
+// The smallest power of two s with top <= 448 s, from 2^-64 to 2^64.
 __device__ __forceinline__ float block_scale(float top) {
   const uint32_t bits = __float_as_uint(top);
   const int e = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);  // 448 = 1.75 * 2^8
   return __uint_as_float(static_cast<uint32_t>(min(max(e, 127 - 64), 127 + 64)) << 23);
 }
 
-// A warp has some of the heads' rows (queries, keys, values) of one chunk of tokens, and what it needs of the next head is on its way while it does one.  Raw rows
-// wait in shared memory, where a lane finds what it has asked for itself; in registers they would cost half of the warps that are resident.
+// grid (windows of tokens, shares of the heads), window * lanes threads, a multiple of 32.
 template <typename T, Form F>
-__global__ void __launch_bounds__(kWarps * 32, 4) paged_kv_append_blocks_kernel(const __grid_constant__ BlockArgs a) {
-  __shared__ uint4 staged[kWarps][2][kHeld][32];
+__global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __grid_constant__ BlockArgs a) {
+  __shared__ __align__(16) float tops[2][kHeads][32];  // largest magnitude of every row; two turns
   pdl_wait();
   pdl_launch_dependents();
   const TrisPagedAppend& r = a.rows;
   const TrisPagedKv& c = a.cache;
-  const int lane = threadIdx.x & 31, hq = r.num_q_heads, hkv = c.num_kv_heads, items = hq + 2 * hkv;
-  const int first_item = blockIdx.y * kWarps + (threadIdx.x >> 5), item_step = gridDim.y * kWarps;
-  if (first_item >= items) return;
-  const int D = c.head_dim, rot = r.rotary_dim, half = rot / 2, block = c.scale_tokens;
+  const int tid = threadIdx.x, lane = tid & 31, L = a.lanes, R = a.window, row = tid / L, u = tid % L;
+  const int hq = r.num_q_heads, hkv = c.num_kv_heads, D = c.head_dim, rot = r.rotary_dim, half = rot / 2, block = c.scale_tokens;
   const int64_t room = static_cast<int64_t>(c.table_width) * c.page_size;
-  const int t0 = blockIdx.x * a.chunk, t1 = min(r.num_tokens, t0 + a.chunk);
+  const bool active = 16 * u < D;
+  // this thread's two chunks of eight dimensions
+  const bool pairs_up = F == Form::kHalves && u < half / 8;
+  const int c0 = pairs_up ? u : 2 * u, c1 = pairs_up ? u + half / 8 : 2 * u + 1;
 
   auto position = [&](int t) -> int64_t { return r.positions_are_64bit ? reinterpret_cast<const int64_t*>(r.positions)[t] : reinterpret_cast<const int32_t*>(r.positions)[t]; };
-  auto page_of = [&](int pos) { return a.page_shift >= 0 ? pos >> a.page_shift : pos / c.page_size; };
   auto in_block = [&](int pos) { return a.block_mask >= 0 ? pos & a.block_mask : pos % block; };  // pages are whole blocks
-  // Whether token t, which has a place at `pos`, goes on where the token before it in the call is.
-  auto follows_at = [&](int t, int64_t pos) {
-    return t > 0 && r.sequences && in_block(static_cast<int>(pos)) && position(t - 1) == pos - 1 && r.sequences[t - 1] == r.sequences[t];
-  };
-  // What a lane knows of token t0 + lane: its position (-1: padding, -2: it has no place), its page, and whether it follows.
-  struct Token {
-    int pos, page;
-    bool follows;
-  };
-  auto look = [&](int t) {
-    Token k{-1, -1, false};
+  auto slot_of = [&](int pos) { return a.page_shift >= 0 ? pos & (c.page_size - 1) : pos % c.page_size; };
+  // Whether token t begins a run: it does not go on, inside a block, where the token before it in the call is.
+  auto begins = [&](int t) {
+    if (t >= r.num_tokens || t == 0 || !r.sequences) return true;
     const int64_t pos = position(t);
+    return pos < 0 || pos >= room || in_block(static_cast<int>(pos)) == 0 || position(t - 1) != pos - 1 || r.sequences[t - 1] != r.sequences[t];
+  };
+  auto beginnings = [&](int w) { return __ballot_sync(0xFFFFFFFFu, lane < R && begins(w + lane)); };
+
+  // What a thread knows of its row's token.
+  int t = 0, pos = 0, page = 0;
+  bool placed = false, turns = false;  // whether it goes to the cache, and out as something else than zeros
+  float cs[8], sn[8];
+  auto enter = [&](int token, bool there) {
+    t = token;
+    placed = turns = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cs[i] = 1.f, sn[i] = 0.f;
+    if (!there) return;
+    const int64_t p = position(t);
     const int seq = r.sequences ? r.sequences[t] : t;
-    if (pos < 0) return k;
-    bool fits = seq >= 0 && seq < c.num_sequences && pos < room;
-    const bool turns = !r.cos || pos < r.max_positions;
+    turns = p >= 0 && (!r.cos || p < r.max_positions);
+    pos = static_cast<int>(min(p, static_cast<int64_t>(0x7FFFFFFF)));
+    if (turns && rot && active && (F == Form::kHalves ? pairs_up : F == Form::kPairs)) {
+      const int64_t table = p * half;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {  // kHalves: the eight frequencies of both chunks; kPairs: four of each
+        const int f = F == Form::kHalves ? 8 * c0 + 4 * k : 4 * (c0 + k);
+        if (f >= half) break;
+        const float4 x = *reinterpret_cast<const float4*>(r.cos + table + f), y = *reinterpret_cast<const float4*>(r.sin + table + f);
+        cs[4 * k] = x.x, cs[4 * k + 1] = x.y, cs[4 * k + 2] = x.z, cs[4 * k + 3] = x.w;
+        sn[4 * k] = y.x, sn[4 * k + 1] = y.y, sn[4 * k + 2] = y.z, sn[4 * k + 3] = y.w;
+      }
+    }
+    if (p < 0) return;
+    bool fits = seq >= 0 && seq < c.num_sequences && p < room;
     if (fits) {
-      k.page = c.block_table[seq * c.table_stride + page_of(static_cast<int>(pos))];
-      fits = k.page >= 0 && k.page < c.num_pages;
+      page = c.block_table[seq * c.table_stride + (a.page_shift >= 0 ? pos >> a.page_shift : pos / c.page_size)];
+      fits = page >= 0 && page < c.num_pages;
     }
-    if (!fits || !turns) {
-      if (c.status_dev) *c.status_dev = TRIS_ERR_CORRUPT;
-      k.pos = turns ? -2 : -1;  // one without a place is still rotated, as long as the tables have its position
-      if (turns) k.page = static_cast<int>(min(pos, static_cast<int64_t>(0x7FFFFFFF)));
-      return k;
-    }
-    k.pos = static_cast<int>(pos);
-    k.follows = follows_at(t, pos);
-    return k;
+    placed = fits && turns;
+    if (!placed && c.status_dev) *c.status_dev = TRIS_ERR_CORRUPT;
   };
 
-  const int l = lane % a.lanes, place = lane / a.lanes, places = 32 / a.lanes, d0 = 8 * l;
-  const bool active = d0 < D;
   struct Source {
     const T* rows;
     int64_t stride;
-    int kind, head;  // 0: queries, 1: keys, 2: values
   };
-  auto source = [&](int item) {
-    const int kind = item < hq ? 0 : item < hq + hkv ? 1 : 2, head = item - (kind == 0 ? 0 : kind == 1 ? hq : hq + hkv);
+  auto source = [&](int kind, int head) {  // 0: queries, 1: keys, 2: values
     const T* base = static_cast<const T*>(kind == 0 ? r.q : kind == 1 ? r.k : r.v);
-    return Source{base + head * (kind == 0 ? r.q_head_stride : kind == 1 ? r.k_head_stride : r.v_head_stride), kind == 0 ? r.q_token_stride : kind == 1 ? r.k_token_stride : r.v_token_stride, kind, head};
+    return Source{base + head * (kind == 0 ? r.q_head_stride : kind == 1 ? r.k_head_stride : r.v_head_stride), kind == 0 ? r.q_token_stride : kind == 1 ? r.k_token_stride : r.v_token_stride};
   };
-  // Rows [from, to) of a source, as many as a buffer holds; a lane has row from + i * places + place at step i.
-  auto ask = [&](int buffer, const Source& src, int from, int to) {
-    uint4* dst = &staged[threadIdx.x >> 5][buffer][0][lane];
-    const T* p = src.rows + static_cast<int64_t>(from + place) * src.stride + d0;
+  auto source_of = [&](int item) { return item < hkv ? source(1, item) : source(2, item - hkv); };  // keys' heads, then values'
+  auto fetch = [&](const Source& src, uint4 (&raw)[2]) {
+    raw[0] = raw[1] = make_uint4(0, 0, 0, 0);
+    if (!turns || !active) return;
+    const T* p = src.rows + t * src.stride;
+    if constexpr (F != Form::kAny) {
+      raw[0] = *reinterpret_cast<const uint4*>(p + 8 * c0);
+      raw[1] = *reinterpret_cast<const uint4*>(p + 8 * c1);
+    } else {
+      const uint16_t* e = reinterpret_cast<const uint16_t*>(p) + 16 * u;
+      uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      if (from + i * places >= to) break;
-      const bool there = active && from + i * places + place < to;
-      if constexpr (F != Form::kAny) {
-        cp_async_16(dst + i * 32, there ? p + i * places * src.stride : src.rows, there);
-      } else {
-        uint32_t w[4] = {0, 0, 0, 0};
-        const uint16_t* e = reinterpret_cast<const uint16_t*>(p + i * places * src.stride);
-        for (int k = 0; there && k < 4; ++k) w[k] = e[2 * k] | (static_cast<uint32_t>(e[2 * k + 1]) << 16);
-        dst[i * 32] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+      for (int k = 0; k < 8; ++k) w[k] = e[2 * k] | (static_cast<uint32_t>(e[2 * k + 1]) << 16);
+      raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      raw[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
-    cp_async_commit();
   };
-  // Step i's eight dimensions of token t at position pos, rotated; zeros where the buffer has no row (t and pos are those of another one then).  By a whole warp.
-  const bool turns_here = active && d0 < rot;
-  const int partner = !turns_here ? lane : d0 < half ? lane + half / 8 : lane - half / 8, f0 = F == Form::kPairs ? d0 / 2 : d0 < half ? d0 : d0 - half;
-  const uint32_t flip = d0 < half ? 0x80008000u : 0;  // a cos - b sin, b cos + a sin
-  auto turned = [&](const Source& src, int buffer, int i, int t, int pos, float (&v)[8]) {
-    const uint4 raw = staged[threadIdx.x >> 5][buffer][i][lane];
-    unpack_8<T>(raw, v);
-    if (rot == 0) return;
-    uint4 pair;
-    if constexpr (F == Form::kHalves)
-      pair = make_uint4(__shfl_sync(0xFFFFFFFFu, raw.x, partner) ^ flip, __shfl_sync(0xFFFFFFFFu, raw.y, partner) ^ flip, __shfl_sync(0xFFFFFFFFu, raw.z, partner) ^ flip,
-                        __shfl_sync(0xFFFFFFFFu, raw.w, partner) ^ flip);
-    if (!turns_here) return;
-    const int64_t table = static_cast<int64_t>(pos) * half + f0;
+  auto rotate = [&](const Source& src, float (&x)[8], float (&y)[8]) {
+    if (!rot) return;
     if constexpr (F == Form::kHalves) {
-      float other[8];
-      unpack_8<T>(pair, other);
+      if (pairs_up) {
 #pragma unroll
-      for (int k = 0; k < 8; k += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(r.cos + table + k), y = *reinterpret_cast<const float4*>(r.sin + table + k);
-        v[k] = fmaf(v[k], x.x, other[k] * y.x);
-        v[k + 1] = fmaf(v[k + 1], x.y, other[k + 1] * y.y);
-        v[k + 2] = fmaf(v[k + 2], x.z, other[k + 2] * y.z);
-        v[k + 3] = fmaf(v[k + 3], x.w, other[k + 3] * y.w);
+        for (int k = 0; k < 8; ++k) {
+          const float p = x[k], q = y[k];
+          x[k] = p * cs[k] - q * sn[k];
+          y[k] = q * cs[k] + p * sn[k];
+        }
       }
     } else if constexpr (F == Form::kPairs) {
-      const float4 x = *reinterpret_cast<const float4*>(r.cos + table), y = *reinterpret_cast<const float4*>(r.sin + table);
-      const float cs[4] = {x.x, x.y, x.z, x.w}, sn[4] = {y.x, y.y, y.z, y.w};
+      // (dimensions behind the rotated ones stay as they are: by a cosine of 1 and a sine of 0 an infinity would spoil its neighbour)
+      if (8 * c0 < rot) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float p = v[2 * k], q = v[2 * k + 1];
-        v[2 * k] = p * cs[k] - q * sn[k];
-        v[2 * k + 1] = q * cs[k] + p * sn[k];
+        for (int k = 0; k < 4; ++k) {
+          const float p = x[2 * k], q = x[2 * k + 1];
+          x[2 * k] = p * cs[k] - q * sn[k];
+          x[2 * k + 1] = q * cs[k] + p * sn[k];
+        }
+      }
+      if (8 * c1 < rot) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float p = y[2 * k], q = y[2 * k + 1];
+          y[2 * k] = p * cs[4 + k] - q * sn[4 + k];
+          y[2 * k + 1] = q * cs[4 + k] + p * sn[4 + k];
+        }
       }
     } else {
+      if (!turns || !active) return;
       const T* p = src.rows + t * src.stride;
       const float *cr = r.cos + static_cast<int64_t>(pos) * half, *sr = r.sin + static_cast<int64_t>(pos) * half;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int d = d0 + k;
+      for (int k = 0; k < 16; ++k) {
+        const int d = 16 * u + k;
         if (d >= rot) break;
         const bool up = r.interleaved ? d & 1 : d >= half;
         const int f = r.interleaved ? d / 2 : up ? d - half : d, with = r.interleaved ? d ^ 1 : up ? d - half : d + half;
-        const float x = to_float(p[with]) * sr[f];
-        v[k] = v[k] * cr[f] + (up ? x : -x);
+        const float other = to_float(p[with]) * sr[f];
+        float& v = k < 8 ? x[k & 7] : y[k & 7];
+        v = v * cr[f] + (up ? other : -other);
       }
     }
   };
-  auto put_row = [&](void* out, int64_t row, const float (&v)[8]) {  // of q_out or k_out
+  auto put_row = [&](void* out, int heads, int head, const float (&x)[8], const float (&y)[8]) {  // of q_out or k_out
     if (!active) return;
-    T* p = static_cast<T*>(out) + row * D + d0;
+    T* p = static_cast<T*>(out) + (static_cast<int64_t>(t) * heads + head) * D;
     if constexpr (F != Form::kAny) {
-      store_8(p, v);
+      store_8(p + 8 * c0, x);
+      store_8(p + 8 * c1, y);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) store_float(p + i, v[i]);
+      for (int k = 0; k < 8; ++k) {
+        store_float(p + 16 * u + k, x[k]);
+        store_float(p + 16 * u + 8 + k, y[k]);
+      }
+    }
+  };
+  auto row_top = [&](const float (&x)[8], const float (&y)[8], bool finite) {  // over the row's lanes
+    float top = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      top = fmaxf(top, !finite || fabsf(x[k]) <= FLT_MAX ? fabsf(x[k]) : 0.f);
+      top = fmaxf(top, !finite || fabsf(y[k]) <= FLT_MAX ? fabsf(y[k]) : 0.f);
+    }
+    for (int d = 1; d < L; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    return top;
+  };
+  // Where a block of a head's keys or values lies: its first token's row, and its scale.
+  struct Place {
+    uint8_t* row;
+    int64_t stride;
+    float* scale;
+  };
+  auto place_of = [&](int item, int slot) {  // slot: that of one of its tokens in the page
+    const bool keys = item < hkv;
+    const int head = keys ? item : item - hkv, at = in_block(slot);
+    uint8_t* p = static_cast<uint8_t*>(keys ? c.k_pages : c.v_pages) + head * (keys ? c.k_head_stride : c.v_head_stride) + page * (keys ? c.k_page_stride : c.v_page_stride);
+    const int64_t stride = keys ? c.k_token_stride : c.v_token_stride;
+    return Place{p + (slot - at) * stride, stride, const_cast<float*>(keys ? c.k_scale : c.v_scale) + (static_cast<int64_t>(page) * a.page_scales + (slot - at) / block) * hkv + head};
+  };
+  // The block's tokens ahead of the run are brought to its new scale, by the run's rows in turn.
+  auto bring_along = [&](const Place& to, int ahead, int from, int step, float by) {
+    for (int k = from; k < ahead; k += step) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint2* at = reinterpret_cast<uint2*>(to.row + k * to.stride + 8 * (h ? c1 : c0));
+        const uint2 was = *at;
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((i < 2 ? was.x : was.y) >> (16 * (i & 1))), __NV_E4M3);
+          const float2 pair = __half22float2(__half2(two));
+          f[2 * i] = pair.x * by, f[2 * i + 1] = pair.y * by;
+        }
+        *at = make_uint2(e4m3_pack4(f[0], f[1], f[2], f[3]), e4m3_pack4(f[4], f[5], f[6], f[7]));
+      }
+    }
+  };
+  auto known = [](float held) { return held > 0.f && held <= FLT_MAX ? held : 0.f; };
+  auto store_row = [&](const Place& to, int at, float scale, float (&x)[8], float (&y)[8]) {
+    // x / scale: by a power of two, which a scale is unless the caller has put in another, the product with its reciprocal
+    const uint32_t bits = __float_as_uint(scale);
+    if ((bits & 0x7FFFFFu) == 0) {
+      const float up = __uint_as_float((254u << 23) - bits);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] *= up, y[k] *= up;
+    } else {
+      const DivideBy divide(scale);
+      divide(x, INFINITY);
+      divide(y, INFINITY);
+    }
+    uint8_t* p = to.row + at * to.stride;
+    store_8(reinterpret_cast<__nv_fp8_e4m3*>(p + 8 * c0), x);
+    store_8(reinterpret_cast<__nv_fp8_e4m3*>(p + 8 * c1), y);
+  };
+
+  const int share = blockIdx.y * kHeads, shares = gridDim.y * kHeads, items = 2 * hkv;
+  auto queries = [&](bool there) {
+    if (share >= hq) return;
+    uint4 next[kHeads][2];
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k) fetch(source(0, min(share + k, hq - 1)), next[k]);
+#pragma unroll 1
+    for (int h0 = share; h0 < hq; h0 += shares) {
+      float x[kHeads][8], y[kHeads][8];
+#pragma unroll
+      for (int k = 0; k < kHeads; ++k) {
+        unpack_8<T>(next[k][0], x[k]);
+        unpack_8<T>(next[k][1], y[k]);
+      }
+      if (h0 + shares < hq) {
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k) fetch(source(0, min(h0 + shares + k, hq - 1)), next[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < kHeads; ++k) {
+        if (h0 + k >= hq) break;
+        rotate(source(0, h0 + k), x[k], y[k]);
+        if (there) put_row(r.q_out, hq, h0 + k, x[k], y[k]);
+      }
     }
   };
 
-  // Rows that are rotated and go out as they are: queries, and keys that the caller asks for.
-  const int goes_out = r.k_out ? hq + hkv : hq;
-  const int window = kHeld * places;  // rows of a buffer
-  if (first_item < goes_out) ask(0, source(first_item), t0, min(t1, t0 + window));
-  Token own{-1, -1, false};
-  if (t0 + lane < t1) own = look(t0 + lane);
-  int buffer = 0;
-#pragma unroll 1
-  for (int item = first_item; item < goes_out; item += item_step) {
-    const Source src = source(item);
-#pragma unroll 1
-    for (int from = t0; from < t1; from += window) {
-      if (from + window < t1) ask(buffer ^ 1, src, from + window, min(t1, from + 2 * window));
-      else if (item + item_step < goes_out) ask(buffer ^ 1, source(item + item_step), t0, min(t1, t0 + window));
-      else cp_async_commit();
-      cp_async_wait<1>();
-#pragma unroll 2
-      for (int i = 0; i < kHeld; ++i) {
-        if (from + i * places >= t1) break;
-        const int t = min(from + i * places + place, t1 - 1);
-        const int pos = __shfl_sync(0xFFFFFFFFu, own.pos == -2 ? own.page : own.pos, t - t0);
-        float v[8];
-        turned(src, buffer, i, t, max(pos, 0), v);
-        if (pos < 0) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = 0.f;
-        }
-        if (from + i * places + place < t1) put_row(src.kind == 0 ? r.q_out : r.k_out, static_cast<int64_t>(t) * (src.kind == 0 ? hq : hkv) + src.head, v);
-      }
-      buffer ^= 1;
-    }
+  const int end = min((static_cast<int>(blockIdx.x) + 1) * R, r.num_tokens);
+  int w = blockIdx.x * R, turn = 0;
+  uint32_t starts = beginnings(w);
+  if (!starts) return;  // all of these tokens belong to a run that begins ahead of them
+  if (!(starts & 1)) {
+    w += __ffs(starts) - 1;
+    if (w < end) starts = beginnings(w);
   }
-  // Keys and values.
-  const int first_cached = first_item + (first_item < hq ? (hq - first_item + item_step - 1) / item_step * item_step : 0);
-  if (first_cached >= items) return;
-  const uint32_t placed = __ballot_sync(0xFFFFFFFFu, own.pos >= 0), follows = __ballot_sync(0xFFFFFFFFu, own.follows);
 #pragma unroll 1
-  for (uint32_t runs = placed & ~follows; runs; runs &= runs - 1) {
-    const int lead = __ffs(runs) - 1;
-    const int pos0 = __shfl_sync(0xFFFFFFFFu, own.pos, lead), page = __shfl_sync(0xFFFFFFFFu, own.page, lead), first = t0 + lead;
-    // its length: tokens that follow, in this chunk and behind it
-    const uint32_t behind = lead == 31 ? 0 : ~follows >> (lead + 1);  // (bits behind the chunk's last token are 0 in follows)
-    int length = behind ? __ffs(behind) : 32 - lead;
-    const int slot0 = pos0 - page_of(pos0) * c.page_size, ahead = in_block(pos0);  // tokens of the block ahead of the run
-    const int room_left = block - ahead, most = min(room_left, r.num_tokens - first);
-    if (first + length == t1) {
-      while (length < most) {
-        // the block's next tokens have places where its first one has, but for the rotation's tables
-        const int t = first + length + lane, pos = pos0 + length + lane;
-        const bool on = length + lane < most && position(t) == pos && (!r.cos || pos < r.max_positions) && follows_at(t, pos);
-        const uint32_t more = ~__ballot_sync(0xFFFFFFFFu, on);
-        length += more ? __ffs(more) - 1 : 32;
-        if (more) break;
+  while (w < end) {
+    // the rows of whole runs that a window holds
+    const uint32_t behind = starts & ~1u;
+    const int count = begins(w + R) ? R : behind ? 31 - __clz(behind) : 0;
+    if (count) {
+      const int first = 31 - __clz(starts & (row < 31 ? (2u << row) - 1 : ~0u));  // of this row's run
+      const uint32_t above = row < 31 ? starts >> (row + 1) : 0;
+      const int last = min(above ? row + __ffs(above) : R, count);  // behind it
+      const bool there = row < count && w + row < r.num_tokens;
+      enter(min(w + row, r.num_tokens - 1), there);
+      queries(there);
+      const int ahead = in_block(pos) - (row - first);  // tokens of the block ahead of the run
+      const bool whole = first == 0 && last == R && R >= 4;  // four rows at a time
+      uint4 next[kHeads][2];
+      if (share < items) {
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k) fetch(source_of(min(share + k, items - 1)), next[k]);
       }
+#pragma unroll 1
+      for (int i0 = share; i0 < items; i0 += shares, turn ^= 1) {
+        float x[kHeads][8], y[kHeads][8], held[kHeads];
+        bool infinite = false;
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k) {
+          const int item = min(i0 + k, items - 1);
+          unpack_8<T>(next[k][0], x[k]);
+          unpack_8<T>(next[k][1], y[k]);
+          if (item < hkv) rotate(source_of(item), x[k], y[k]);
+          held[k] = placed && ahead > 0 ? *place_of(item, slot_of(pos)).scale : 0.f;
+          const float top = row_top(x[k], y[k], false);
+          infinite |= placed && top == INFINITY;
+          if (u == 0) tops[turn][k][row] = placed ? top : 0.f;
+        }
+        if (i0 + shares < items) {
+#pragma unroll
+          for (int k = 0; k < kHeads; ++k) fetch(source_of(min(i0 + shares + k, items - 1)), next[k]);
+        }
+        if (__syncthreads_or(infinite)) {  // rare: the largest of the finite ones alone
+#pragma unroll
+          for (int k = 0; k < kHeads; ++k) {
+            const float top = row_top(x[k], y[k], true);
+            if (u == 0) tops[turn][k][row] = placed ? top : 0.f;
+          }
+          __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k) {
+          const int item = i0 + k;
+          if (item >= items) break;
+          float all = 0.f;
+          if (whole) {
+            for (int n = 0; n < R; n += 4) {
+              const float4 m = *reinterpret_cast<const float4*>(&tops[turn][k][n]);
+              all = fmaxf(fmaxf(fmaxf(all, m.x), fmaxf(m.y, m.z)), m.w);
+            }
+          } else {
+            for (int n = first; n < last; ++n) all = fmaxf(all, tops[turn][k][n]);
+          }
+          if (item < hkv && r.k_out && there) put_row(r.k_out, hkv, item, x[k], y[k]);
+          if (!placed || !active) continue;
+          const float old = known(held[k]), scale = fmaxf(block_scale(all), old);
+          const Place to = place_of(item, slot_of(pos));
+          if (ahead > 0 && old < scale) bring_along(to, ahead, row - first, last - first, old / scale);
+          store_row(to, in_block(pos), scale, x[k], y[k]);
+          if (row == first && u == 0 && scale != held[k]) *to.scale = scale;
+        }
+      }
+      w += count;
+    } else {
+      // one run, longer than a window: its length first
+      int length = R;
+      for (;;) {
+        const uint32_t more = beginnings(w + length);
+        if (more) {
+          length += __ffs(more) - 1;
+          break;
+        }
+        length += R;
+      }
+      for (int at = 0; at < length; at += R) {
+        enter(w + min(at + row, length - 1), at + row < length);
+        queries(at + row < length);
+      }
+#pragma unroll 1
+      for (int i0 = share; i0 < items; i0 += shares, turn ^= 1) {
+        const int many = min(kHeads, items - i0);
+        float most[kHeads] = {}, scale[kHeads] = {};
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+          for (int at = 0; at < length; at += R) {
+            const bool there = at + row < length;
+            enter(w + min(at + row, length - 1), there);
+#pragma unroll
+            for (int k = 0; k < kHeads; ++k) {
+              if (k >= many) break;
+              uint4 raw[2];
+              float x[8], y[8];
+              const Source src = source_of(i0 + k);
+              fetch(src, raw);
+              unpack_8<T>(raw[0], x);
+              unpack_8<T>(raw[1], y);
+              if (i0 + k < hkv) rotate(src, x, y);
+              if (pass == 0) {
+                const float top = row_top(x, y, true);
+                if (placed) most[k] = fmaxf(most[k], top);
+              } else {
+                if (i0 + k < hkv && r.k_out && there) put_row(r.k_out, hkv, i0 + k, x, y);
+                if (placed && active) store_row(place_of(i0 + k, slot_of(pos)), in_block(pos), scale[k], x, y);
+              }
+            }
+          }
+          if (pass == 1) break;
+          enter(w, true);  // the run's first token, for all
+          const int ahead = in_block(pos);
+#pragma unroll
+          for (int k = 0; k < kHeads; ++k)
+            if (u == 0) tops[turn][k][row] = most[k];
+          __syncthreads();
+          float held[kHeads] = {};
+#pragma unroll
+          for (int k = 0; k < kHeads; ++k) {
+            float all = 0.f;
+            for (int n = 0; n < R; ++n) all = fmaxf(all, tops[turn][k][n]);
+            if (k >= many || !placed) continue;
+            const Place to = place_of(i0 + k, slot_of(pos));
+            held[k] = ahead ? *to.scale : 0.f;
+            const float old = known(held[k]);
+            scale[k] = fmaxf(block_scale(all), old);
+            if (active && ahead && old < scale[k]) bring_along(to, ahead, row, R, old / scale[k]);
+          }
+          __syncthreads();  // all have read the scales that are written now
+#pragma unroll
+          for (int k = 0; k < kHeads; ++k)
+            if (k < many && placed && tid == 0 && scale[k] != held[k]) *place_of(i0 + k, slot_of(pos)).scale = scale[k];
+        }
+      }
+      w += length;
     }
-    length = min(length, most);
-    const int64_t scale_index = (static_cast<int64_t>(page) * a.page_scales + (slot0 - ahead) / block) * hkv;
-    const bool whole = length <= window;  // a buffer holds the run
-    auto rows_from = [&](int k) { return min(first + length, first + k + window); };
-    ask(buffer, source(first_cached), first, rows_from(0));
-#pragma unroll 1
-    for (int item = first_cached; item < items; item += item_step) {
-      const Source src = source(item);
-      const bool keys = src.kind == 1;
-      float* scale_at = const_cast<float*>(keys ? c.k_scale : c.v_scale) + scale_index + src.head;
-      const float held = ahead ? *scale_at : 0.f;
-      // Step i of the rows from `base` on.
-      float v[kHeld][8];
-      auto row_of = [&](int base, int i) { return min(base + i * places + place, length - 1); };
-      auto load_window = [&](int base) {
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-          if (base + i * places >= length) break;
-          if (keys) turned(src, buffer, i, first + row_of(base, i), pos0 + row_of(base, i), v[i]);
-          else unpack_8<T>(staged[threadIdx.x >> 5][buffer][i][lane], v[i]);
-        }
-      };
-      // The largest magnitude, of finite numbers alone where there are others, too.
-      auto largest = [&](int base, float top, bool finite) {
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-          if (base + i * places >= length) break;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, !finite || fabsf(v[i][e]) <= FLT_MAX ? fabsf(v[i][e]) : 0.f);
-        }
-        return top;
-      };
-      auto of_all = [&](float top) {
-#pragma unroll
-        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-        return top;
-      };
-      float top = 0.f;
-      if (whole) {
-        if (item + item_step < items) ask(buffer ^ 1, source(item + item_step), first, rows_from(0));
-        else cp_async_commit();
-        cp_async_wait<1>();
-        load_window(0);
-        top = of_all(largest(0, 0.f, false));
-        if (top == INFINITY) top = of_all(largest(0, 0.f, true));
-      } else {
-#pragma unroll 1
-        for (int base = 0; base < length; base += window) {
-          if (base) ask(buffer, src, first + base, rows_from(base));
-          cp_async_wait<0>();
-          load_window(base);
-          top = largest(base, top, true);
-        }
-        top = of_all(top);
-      }
-      const float need = block_scale(top), old = held > 0.f && held <= FLT_MAX ? held : 0.f, scale = fmaxf(need, old);
-      uint8_t* rows = static_cast<uint8_t*>(keys ? c.k_pages : c.v_pages) + src.head * (keys ? c.k_head_stride : c.v_head_stride) + page * (keys ? c.k_page_stride : c.v_page_stride) + d0;
-      const int64_t token_stride = keys ? c.k_token_stride : c.v_token_stride;
-      if (ahead && old < scale) {  // what the block holds already
-        const float by = old / scale;
-#pragma unroll 4
-        for (int k = place; k < ahead; k += places) {
-          if (!active) continue;
-          uint2* at = reinterpret_cast<uint2*>(rows + (slot0 - ahead + k) * token_stride);
-          const uint2 was = *at;
-          float f[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((i < 2 ? was.x : was.y) >> (16 * (i & 1))), __NV_E4M3);
-            const float2 pair = __half22float2(__half2(two));
-            f[2 * i] = pair.x * by, f[2 * i + 1] = pair.y * by;
-          }
-          *at = make_uint2(e4m3_pack4(f[0], f[1], f[2], f[3]), e4m3_pack4(f[4], f[5], f[6], f[7]));
-        }
-      }
-      // x / scale: by a power of two, which a scale is unless the caller has put in another, the product with its reciprocal
-      const uint32_t scale_bits = __float_as_uint(scale);
-      const bool shifts = (scale_bits & 0x7FFFFFu) == 0;
-      const float up = __uint_as_float((254u << 23) - scale_bits);
-#pragma unroll 1
-      for (int base = 0; base < length; base += window) {
-        if (!whole) {
-          ask(buffer, src, first + base, rows_from(base));
-          cp_async_wait<0>();
-          load_window(base);
-        }
-        if (!shifts) {
-          const DivideBy divide(scale);
-#pragma unroll
-          for (int i = 0; i < kHeld; ++i) {
-            if (base + i * places >= length) break;
-            divide(v[i], INFINITY);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-          const int k = base + i * places + place;
-          if (base + i * places >= length) break;
-          if (shifts) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] *= up;
-          }
-          if (k < length && active) store_8(reinterpret_cast<__nv_fp8_e4m3*>(rows + (slot0 + k) * token_stride), v[i]);
-        }
-      }
-      if (lane == 0 && scale != held) *scale_at = scale;
-      if (whole) buffer ^= 1;
-      else if (item + item_step < items) ask(buffer, source(item + item_step), first, rows_from(0));
-    }
+    if (w < end) starts = beginnings(w);
   }
 }
 
 template <typename T, Form F>
 int launch_blocks(const BlockArgs& a, cudaStream_t stream) {
-  TRIS_CUDA(launch_step(paged_kv_append_blocks_kernel<T, F>, dim3(ceil_div(a.rows.num_tokens, a.chunk), a.shares), dim3(kWarps * 32), 0, stream, programmatic_launch_default(), 1, a));
+  const int heads = a.rows.num_q_heads > 2 * a.cache.num_kv_heads ? a.rows.num_q_heads : 2 * a.cache.num_kv_heads;
+  // CTAs that share a window's heads: all of them where there are few windows, else until a thread has kWalk heads of queries and as many of keys and values
+  constexpr int kWalk = 8;
+  const int64_t windows = (static_cast<int64_t>(a.rows.num_tokens) + a.window - 1) / a.window;
+  const int most = ceil_div(heads, kHeads), few = ceil_div(heads, kWalk);
+  const int shares = windows * most <= 16 * static_cast<int64_t>(sm_count()) ? most : few;
+  TRIS_REQUIRE(shares <= 65535, TRIS_ERR_UNSUPPORTED, "paged_kv_append: too many heads");
+  TRIS_CUDA(launch_step(paged_kv_append_blocks_kernel<T, F>, dim3(static_cast<unsigned>(windows), shares), dim3(a.window * a.lanes), 0, stream, programmatic_launch_default(), 1, a));
   return TRIS_OK;
 }
 
@@ -370,21 +454,17 @@ int append_block_scaled(const TrisPagedKv& c, const TrisPagedAppend& r, int rota
     if (c.scale_tokens == 1 << i) a.block_mask = c.scale_tokens - 1;
   }
   a.page_scales = c.page_size / c.scale_tokens;
-  a.lanes = 2;
-  while (8 * a.lanes < c.head_dim) a.lanes *= 2;
+  a.lanes = 1;
+  while (16 * a.lanes < c.head_dim) a.lanes *= 2;
   bool wide = (!r.q_out || aligned_to(r.q_out, 16)) && (!r.k_out || aligned_to(r.k_out, 16)) && aligned_to(r.cos, 16) && aligned_to(r.sin, 16);
   const void* src[3] = {r.num_q_heads ? r.q : nullptr, r.k, r.v};
   const int64_t strides[3][2] = {{r.q_token_stride, r.q_head_stride}, {r.k_token_stride, r.k_head_stride}, {r.v_token_stride, r.v_head_stride}};
   for (int i = 0; i < 3; ++i)
     if (src[i]) wide = wide && aligned_to(src[i], 16) && strides[i][0] % 8 == 0 && strides[i][1] % 8 == 0;
   const Form form = wide && rotary_dim % (r.interleaved ? 8 : 16) == 0 ? (r.interleaved ? Form::kPairs : Form::kHalves) : Form::kAny;
-  // a token to a warp where there are few (a decode step), 32 where there are many
+  // a warp's rows to a CTA where there are few tokens (a decode step), else 16 or, of short rows, 32
   const int64_t items = r.num_q_heads + 2 * c.num_kv_heads;
-  a.chunk = r.num_tokens * items <= 64 * static_cast<int64_t>(sm_count()) ? 1 : 32;
-  // and as many CTAs to a chunk as a warp has kHeads heads
-  constexpr int kHeads = 2;
-  a.shares = ceil_div(static_cast<int>(items), kWarps * (a.chunk == 1 ? 1 : kHeads));
-  TRIS_REQUIRE(items <= 65535 * kWarps, TRIS_ERR_UNSUPPORTED, "paged_kv_append: too many heads");
+  a.window = r.num_tokens * items <= 64 * static_cast<int64_t>(sm_count()) ? 32 / a.lanes : a.lanes >= 8 ? 16 : 32;
   return r.dtype == TRIS_DTYPE_F16 ? launch_blocks<__half>(a, form, stream) : launch_blocks<__nv_bfloat16>(a, form, stream);
 }
 
