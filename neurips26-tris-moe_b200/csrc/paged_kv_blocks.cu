@@ -57,7 +57,6 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
 
   auto position = [&](int t) -> int64_t { return r.positions_are_64bit ? reinterpret_cast<const int64_t*>(r.positions)[t] : reinterpret_cast<const int32_t*>(r.positions)[t]; };
   auto in_block = [&](int pos) { return a.block_mask >= 0 ? pos & a.block_mask : pos % block; };  // pages are whole blocks
-  auto slot_of = [&](int pos) { return a.page_shift >= 0 ? pos & (c.page_size - 1) : pos % c.page_size; };
   // Whether token t begins a run: it does not go on, inside a block, where the token before it in the call is.
   auto begins = [&](int t) {
     if (t >= r.num_tokens || t == 0 || !r.sequences) return true;
@@ -102,18 +101,16 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
   };
 
   struct Source {
-    const T* rows;
-    int64_t stride;
+    const T* row;    // this thread's, of some head
+    int64_t stride;  // to the next head
   };
   auto source = [&](int kind, int head) {  // 0: queries, 1: keys, 2: values
-    const T* base = static_cast<const T*>(kind == 0 ? r.q : kind == 1 ? r.k : r.v);
-    return Source{base + head * (kind == 0 ? r.q_head_stride : kind == 1 ? r.k_head_stride : r.v_head_stride), kind == 0 ? r.q_token_stride : kind == 1 ? r.k_token_stride : r.v_token_stride};
+    const int64_t stride = kind == 0 ? r.q_head_stride : kind == 1 ? r.k_head_stride : r.v_head_stride;
+    return Source{static_cast<const T*>(kind == 0 ? r.q : kind == 1 ? r.k : r.v) + t * (kind == 0 ? r.q_token_stride : kind == 1 ? r.k_token_stride : r.v_token_stride) + head * stride, stride};
   };
-  auto source_of = [&](int item) { return item < hkv ? source(1, item) : source(2, item - hkv); };  // keys' heads, then values'
-  auto fetch = [&](const Source& src, uint4 (&raw)[2]) {
+  auto fetch = [&](const T* p, uint4 (&raw)[2]) {
     raw[0] = raw[1] = make_uint4(0, 0, 0, 0);
     if (!turns || !active) return;
-    const T* p = src.rows + t * src.stride;
     if constexpr (F != Form::kAny) {
       raw[0] = *reinterpret_cast<const uint4*>(p + 8 * c0);
       raw[1] = *reinterpret_cast<const uint4*>(p + 8 * c1);
@@ -126,7 +123,12 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
       raw[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
   };
-  auto rotate = [&](const Source& src, float (&x)[8], float (&y)[8]) {
+  // The next heads' rows; behind the last head its own once more, so that no branch lies between the loads.
+  auto fetch_heads = [&](const T* p, int64_t stride, int left, uint4 (&raw)[kHeads][2]) {
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k) fetch(p + min(k, left - 1) * stride, raw[k]);
+  };
+  auto rotate = [&](const T* p, float (&x)[8], float (&y)[8]) {
     if (!rot) return;
     if constexpr (F == Form::kHalves) {
       if (pairs_up) {
@@ -157,7 +159,6 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
       }
     } else {
       if (!turns || !active) return;
-      const T* p = src.rows + t * src.stride;
       const float *cr = r.cos + static_cast<int64_t>(pos) * half, *sr = r.sin + static_cast<int64_t>(pos) * half;
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
@@ -195,25 +196,28 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
     for (int d = 1; d < L; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
     return top;
   };
-  // Where a block of a head's keys or values lies: its first token's row, and its scale.
+  // Where a block of a head's keys or values lies: its first token's row, and its scale; both for the next head, too.
   struct Place {
     uint8_t* row;
-    int64_t stride;
     float* scale;
+    int64_t token_stride, head_stride;
   };
-  auto place_of = [&](int item, int slot) {  // slot: that of one of its tokens in the page
-    const bool keys = item < hkv;
-    const int head = keys ? item : item - hkv, at = in_block(slot);
-    uint8_t* p = static_cast<uint8_t*>(keys ? c.k_pages : c.v_pages) + head * (keys ? c.k_head_stride : c.v_head_stride) + page * (keys ? c.k_page_stride : c.v_page_stride);
-    const int64_t stride = keys ? c.k_token_stride : c.v_token_stride;
-    return Place{p + (slot - at) * stride, stride, const_cast<float*>(keys ? c.k_scale : c.v_scale) + (static_cast<int64_t>(page) * a.page_scales + (slot - at) / block) * hkv + head};
+  auto place_of = [&](bool keys, int head) {  // of the block that this thread's row is in
+    const int slot = a.page_shift >= 0 ? pos & (c.page_size - 1) : pos % c.page_size, at = in_block(slot);
+    Place to;
+    to.token_stride = keys ? c.k_token_stride : c.v_token_stride;
+    to.head_stride = keys ? c.k_head_stride : c.v_head_stride;
+    to.row = static_cast<uint8_t*>(keys ? c.k_pages : c.v_pages) + page * (keys ? c.k_page_stride : c.v_page_stride) + (slot - at) * to.token_stride + head * to.head_stride;
+    to.scale = const_cast<float*>(keys ? c.k_scale : c.v_scale) + (static_cast<int64_t>(page) * a.page_scales + (slot - at) / block) * hkv + head;
+    return to;
   };
   // The block's tokens ahead of the run are brought to its new scale, by the run's rows in turn.
-  auto bring_along = [&](const Place& to, int ahead, int from, int step, float by) {
+  auto bring_along = [&](uint8_t* rows, int64_t stride, int ahead, int from, int step, float by) {
+#pragma unroll 1
     for (int k = from; k < ahead; k += step) {
-#pragma unroll
+#pragma unroll 1
       for (int h = 0; h < 2; ++h) {
-        uint2* at = reinterpret_cast<uint2*>(to.row + k * to.stride + 8 * (h ? c1 : c0));
+        uint2* at = reinterpret_cast<uint2*>(rows + k * stride + 8 * (h ? c1 : c0));
         const uint2 was = *at;
         float f[8];
 #pragma unroll
@@ -227,7 +231,7 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
     }
   };
   auto known = [](float held) { return held > 0.f && held <= FLT_MAX ? held : 0.f; };
-  auto store_row = [&](const Place& to, int at, float scale, float (&x)[8], float (&y)[8]) {
+  auto store_row = [&](uint8_t* p, float scale, float (&x)[8], float (&y)[8]) {
     // x / scale: by a power of two, which a scale is unless the caller has put in another, the product with its reciprocal
     const uint32_t bits = __float_as_uint(scale);
     if ((bits & 0x7FFFFFu) == 0) {
@@ -239,17 +243,16 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
       divide(x, INFINITY);
       divide(y, INFINITY);
     }
-    uint8_t* p = to.row + at * to.stride;
     store_8(reinterpret_cast<__nv_fp8_e4m3*>(p + 8 * c0), x);
     store_8(reinterpret_cast<__nv_fp8_e4m3*>(p + 8 * c1), y);
   };
 
-  const int share = blockIdx.y * kHeads, shares = gridDim.y * kHeads, items = 2 * hkv;
+  const int share = blockIdx.y * kHeads, shares = gridDim.y * kHeads;
   auto queries = [&](bool there) {
     if (share >= hq) return;
+    Source src = source(0, share);
     uint4 next[kHeads][2];
-#pragma unroll
-    for (int k = 0; k < kHeads; ++k) fetch(source(0, min(share + k, hq - 1)), next[k]);
+    fetch_heads(src.row, src.stride, hq - share, next);
 #pragma unroll 1
     for (int h0 = share; h0 < hq; h0 += shares) {
       float x[kHeads][8], y[kHeads][8];
@@ -258,14 +261,13 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
         unpack_8<T>(next[k][0], x[k]);
         unpack_8<T>(next[k][1], y[k]);
       }
-      if (h0 + shares < hq) {
-#pragma unroll
-        for (int k = 0; k < kHeads; ++k) fetch(source(0, min(h0 + shares + k, hq - 1)), next[k]);
-      }
+      const T* now = src.row;
+      src.row += shares * src.stride;
+      if (h0 + shares < hq) fetch_heads(src.row, src.stride, hq - h0 - shares, next);
 #pragma unroll
       for (int k = 0; k < kHeads; ++k) {
         if (h0 + k >= hq) break;
-        rotate(source(0, h0 + k), x[k], y[k]);
+        rotate(now + k * src.stride, x[k], y[k]);
         if (there) put_row(r.q_out, hq, h0 + k, x[k], y[k]);
       }
     }
@@ -293,58 +295,61 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
       queries(there);
       const int ahead = in_block(pos) - (row - first);  // tokens of the block ahead of the run
       const bool whole = first == 0 && last == R && R >= 4;  // four rows at a time
-      uint4 next[kHeads][2];
-      if (share < items) {
-#pragma unroll
-        for (int k = 0; k < kHeads; ++k) fetch(source_of(min(share + k, items - 1)), next[k]);
-      }
+      const int sharers = r.cos ? min(last - first, r.max_positions - (pos - (row - first))) : last - first;  // rows of the run that have a place
 #pragma unroll 1
-      for (int i0 = share; i0 < items; i0 += shares, turn ^= 1) {
-        float x[kHeads][8], y[kHeads][8], held[kHeads];
-        bool infinite = false;
-#pragma unroll
-        for (int k = 0; k < kHeads; ++k) {
-          const int item = min(i0 + k, items - 1);
-          unpack_8<T>(next[k][0], x[k]);
-          unpack_8<T>(next[k][1], y[k]);
-          if (item < hkv) rotate(source_of(item), x[k], y[k]);
-          held[k] = placed && ahead > 0 ? *place_of(item, slot_of(pos)).scale : 0.f;
-          const float top = row_top(x[k], y[k], false);
-          infinite |= placed && top == INFINITY;
-          if (u == 0) tops[turn][k][row] = placed ? top : 0.f;
-        }
-        if (i0 + shares < items) {
-#pragma unroll
-          for (int k = 0; k < kHeads; ++k) fetch(source_of(min(i0 + shares + k, items - 1)), next[k]);
-        }
-        if (__syncthreads_or(infinite)) {  // rare: the largest of the finite ones alone
+      for (int kind = 1; kind <= 2 && share < hkv; ++kind) {
+        Source src = source(kind, share);
+        Place to = place_of(kind == 1, share);
+        const int64_t own_row = in_block(pos) * to.token_stride;
+        uint4 next[kHeads][2];
+        fetch_heads(src.row, src.stride, hkv - share, next);
+#pragma unroll 1
+        for (int h0 = share; h0 < hkv; h0 += shares, turn ^= 1) {
+          float x[kHeads][8], y[kHeads][8], held[kHeads];
+          bool infinite = false;
 #pragma unroll
           for (int k = 0; k < kHeads; ++k) {
-            const float top = row_top(x[k], y[k], true);
+            unpack_8<T>(next[k][0], x[k]);
+            unpack_8<T>(next[k][1], y[k]);
+            const int within = min(k, hkv - 1 - h0);
+            if (kind == 1) rotate(src.row + within * src.stride, x[k], y[k]);
+            held[k] = placed && ahead > 0 ? to.scale[within] : 0.f;
+            const float top = row_top(x[k], y[k], false);
+            infinite |= placed && top == INFINITY;
             if (u == 0) tops[turn][k][row] = placed ? top : 0.f;
           }
-          __syncthreads();
-        }
-#pragma unroll
-        for (int k = 0; k < kHeads; ++k) {
-          const int item = i0 + k;
-          if (item >= items) break;
-          float all = 0.f;
-          if (whole) {
-            for (int n = 0; n < R; n += 4) {
-              const float4 m = *reinterpret_cast<const float4*>(&tops[turn][k][n]);
-              all = fmaxf(fmaxf(fmaxf(all, m.x), fmaxf(m.y, m.z)), m.w);
+          src.row += shares * src.stride;
+          if (h0 + shares < hkv) fetch_heads(src.row, src.stride, hkv - h0 - shares, next);
+          if (__syncthreads_or(infinite)) {  // rare: the largest of the finite ones alone
+#pragma unroll 1
+            for (int k = 0; k < kHeads; ++k) {
+              const float top = k ? row_top(x[1], y[1], true) : row_top(x[0], y[0], true);
+              if (u == 0) tops[turn][k][row] = placed ? top : 0.f;
             }
-          } else {
-            for (int n = first; n < last; ++n) all = fmaxf(all, tops[turn][k][n]);
+            __syncthreads();
           }
-          if (item < hkv && r.k_out && there) put_row(r.k_out, hkv, item, x[k], y[k]);
-          if (!placed || !active) continue;
-          const float old = known(held[k]), scale = fmaxf(block_scale(all), old);
-          const Place to = place_of(item, slot_of(pos));
-          if (ahead > 0 && old < scale) bring_along(to, ahead, row - first, last - first, old / scale);
-          store_row(to, in_block(pos), scale, x[k], y[k]);
-          if (row == first && u == 0 && scale != held[k]) *to.scale = scale;
+#pragma unroll
+          for (int k = 0; k < kHeads; ++k) {
+            if (h0 + k >= hkv) break;
+            float all = 0.f;
+            if (whole) {
+              for (int n = 0; n < R; n += 4) {
+                const float4 m = *reinterpret_cast<const float4*>(&tops[turn][k][n]);
+                all = fmaxf(fmaxf(fmaxf(all, m.x), fmaxf(m.y, m.z)), m.w);
+              }
+            } else {
+              for (int n = first; n < last; ++n) all = fmaxf(all, tops[turn][k][n]);
+            }
+            if (kind == 1 && r.k_out && there) put_row(r.k_out, hkv, h0 + k, x[k], y[k]);
+            if (!placed || !active) continue;
+            uint8_t* rows = to.row + k * to.head_stride;
+            const float old = known(held[k]), scale = fmaxf(block_scale(all), old);
+            if (ahead > 0 && old < scale) bring_along(rows, to.token_stride, ahead, row - first, sharers, old / scale);
+            store_row(rows + own_row, scale, x[k], y[k]);
+            if (row == first && u == 0 && scale != held[k]) to.scale[k] = scale;
+          }
+          to.row += shares * to.head_stride;
+          to.scale += shares;
         }
       }
       w += count;
@@ -364,57 +369,50 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
         queries(at + row < length);
       }
 #pragma unroll 1
-      for (int i0 = share; i0 < items; i0 += shares, turn ^= 1) {
-        const int many = min(kHeads, items - i0);
-        float most[kHeads] = {}, scale[kHeads] = {};
+      for (int item = blockIdx.y; item < 2 * hkv; item += gridDim.y, turn ^= 1) {  // one head at a time
+        const bool keys = item < hkv;
+        const int head = keys ? item : item - hkv;
+        float most = 0.f, scale = 0.f;
 #pragma unroll 1
         for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll 1
           for (int at = 0; at < length; at += R) {
             const bool there = at + row < length;
             enter(w + min(at + row, length - 1), there);
-#pragma unroll
-            for (int k = 0; k < kHeads; ++k) {
-              if (k >= many) break;
-              uint4 raw[2];
-              float x[8], y[8];
-              const Source src = source_of(i0 + k);
-              fetch(src, raw);
-              unpack_8<T>(raw[0], x);
-              unpack_8<T>(raw[1], y);
-              if (i0 + k < hkv) rotate(src, x, y);
-              if (pass == 0) {
-                const float top = row_top(x, y, true);
-                if (placed) most[k] = fmaxf(most[k], top);
-              } else {
-                if (i0 + k < hkv && r.k_out && there) put_row(r.k_out, hkv, i0 + k, x, y);
-                if (placed && active) store_row(place_of(i0 + k, slot_of(pos)), in_block(pos), scale[k], x, y);
+            uint4 raw[2];
+            float x[8], y[8];
+            const T* from = source(keys ? 1 : 2, head).row;
+            fetch(from, raw);
+            unpack_8<T>(raw[0], x);
+            unpack_8<T>(raw[1], y);
+            if (keys) rotate(from, x, y);
+            if (pass == 0) {
+              const float top = row_top(x, y, true);
+              if (placed) most = fmaxf(most, top);
+            } else {
+              if (keys && r.k_out && there) put_row(r.k_out, hkv, head, x, y);
+              if (placed && active) {
+                const Place to = place_of(keys, head);
+                store_row(to.row + in_block(pos) * to.token_stride, scale, x, y);
               }
             }
           }
           if (pass == 1) break;
           enter(w, true);  // the run's first token, for all
-          const int ahead = in_block(pos);
-#pragma unroll
-          for (int k = 0; k < kHeads; ++k)
-            if (u == 0) tops[turn][k][row] = most[k];
+          if (u == 0) tops[turn][0][row] = most;
           __syncthreads();
-          float held[kHeads] = {};
-#pragma unroll
-          for (int k = 0; k < kHeads; ++k) {
-            float all = 0.f;
-            for (int n = 0; n < R; ++n) all = fmaxf(all, tops[turn][k][n]);
-            if (k >= many || !placed) continue;
-            const Place to = place_of(i0 + k, slot_of(pos));
-            held[k] = ahead ? *to.scale : 0.f;
-            const float old = known(held[k]);
-            scale[k] = fmaxf(block_scale(all), old);
-            if (active && ahead && old < scale[k]) bring_along(to, ahead, row, R, old / scale[k]);
+          float all = 0.f, held = 0.f;
+          for (int n = 0; n < R; ++n) all = fmaxf(all, tops[turn][0][n]);
+          if (placed) {
+            const int ahead = in_block(pos);
+            const Place to = place_of(keys, head);
+            held = ahead ? *to.scale : 0.f;
+            const float old = known(held);
+            scale = fmaxf(block_scale(all), old);
+            if (active && ahead && old < scale) bring_along(to.row, to.token_stride, ahead, row, R, old / scale);
           }
-          __syncthreads();  // all have read the scales that are written now
-#pragma unroll
-          for (int k = 0; k < kHeads; ++k)
-            if (k < many && placed && tid == 0 && scale[k] != held[k]) *place_of(i0 + k, slot_of(pos)).scale = scale[k];
+          __syncthreads();  // all have read the scale that is written now
+          if (placed && tid == 0 && scale != held) *place_of(keys, head).scale = scale;
         }
       }
       w += length;
@@ -425,9 +423,9 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
 
 template <typename T, Form F>
 int launch_blocks(const BlockArgs& a, cudaStream_t stream) {
-  const int heads = a.rows.num_q_heads > 2 * a.cache.num_kv_heads ? a.rows.num_q_heads : 2 * a.cache.num_kv_heads;
-  // CTAs that share a window's heads: all of them where there are few windows, else until a thread has kWalk heads of queries and as many of keys and values
-  constexpr int kWalk = 8;
+  const int heads = a.rows.num_q_heads > a.cache.num_kv_heads ? a.rows.num_q_heads : a.cache.num_kv_heads;
+  // CTAs that share a window's heads: all of them where there are few windows, else until a thread has kWalk heads of queries, keys and values each
+  constexpr int kWalk = 4;
   const int64_t windows = (static_cast<int64_t>(a.rows.num_tokens) + a.window - 1) / a.window;
   const int most = ceil_div(heads, kHeads), few = ceil_div(heads, kWalk);
   const int shares = windows * most <= 16 * static_cast<int64_t>(sm_count()) ? most : few;
