@@ -363,8 +363,8 @@ def sample_tokens(logits: torch.Tensor, random: torch.Tensor, *, temperature: Op
     if len(shape) != 2 or dtype not in _LOGIT_TYPES or (logits.stride(1) != 1 and shape[1] > 1):
         _fail(what, "logits must be fp16, bf16 or fp32 [rows, vocab] with a row's logits side by side")
     rows, vocab = shape
-    out = torch.empty((rows,), dtype=torch.int64, device=dev)
     each, f32 = (rows,), torch.float32
+    out = logits.new_empty(each, dtype=torch.int64)
     args = _SAMPLE.pack(logits.data_ptr(), _want(what, "random", random, f32, each),
                         0 if temperature is None else _want(what, "temperature", temperature, f32, each),
                         0 if top_k is None else _want(what, "top_k", top_k, torch.int32, each),

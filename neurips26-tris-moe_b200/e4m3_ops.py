@@ -15,6 +15,7 @@ import torch
 from .decode_ops import _DTYPES, _LOGIT_TYPES, _ROWS, _fail, _launch, _matrix, _same_device
 
 GROUP = 128  # columns of a scale
+_E4M3 = torch.float8_e4m3fn
 _QUANTIZE = struct.Struct("@3Q3q4i")
 _LINEAR = struct.Struct("@7Q5q6i")
 
@@ -33,24 +34,25 @@ def quantize_e4m3(x: torch.Tensor, *, group_rows: int = 1):
     magnitude / 448) for each 128 columns of a row - scales [..., ceil(columns / 128)] - or, ``group_rows=128``, of 128 rows of a matrix: weights, scales
     [ceil(rows / 128), ceil(columns / 128)].  The last groups may be smaller.  Rows of values start on 16-byte boundaries, as ``linear_e4m3`` wants them."""
     what = "quantize_e4m3"
-    dev = _same_device(what, x)
-    if x.dtype not in _ROWS:
+    _same_device(what, x)
+    dtype, x2 = x.dtype, x
+    if dtype not in _ROWS:
         _fail(what, "x must be fp16 or bf16")
-    if group_rows not in (1, GROUP):
-        _fail(what, f"a scale is for 1 or {GROUP} rows, not {group_rows}")
-    if group_rows == GROUP and x.dim() != 2:
-        _fail(what, "blocks of 128 x 128 are those of a matrix")
-    x2 = _rows(what, "x", x)
+    if group_rows != 1 and (group_rows != GROUP or x.dim() != 2):
+        _fail(what, f"a scale is for 1 row, or for {GROUP} of a matrix, not {group_rows} of {tuple(x.shape)}")
+    if x.dim() != 2 or x.stride(1) != 1:
+        x2 = _rows(what, "x", x)
     rows, columns = x2.shape
-    line = -(-columns // 16) * 16
-    values = torch.empty((rows, line), dtype=torch.float8_e4m3fn, device=dev)
-    if line != columns:
-        values = values[:, :columns]
-    scales = torch.empty((-(-rows // group_rows), -(-columns // GROUP)), dtype=torch.float32, device=dev)
-    _launch(what, "tris_quantize_e4m3", dev, _QUANTIZE.pack(x2.data_ptr(), values.data_ptr(), scales.data_ptr(), x2.stride(0), line, scales.shape[1],
-                                                            rows, columns, group_rows, _DTYPES[x.dtype]))
+    groups, line = (columns + GROUP - 1) // GROUP, (columns + 15) // 16 * 16
+    if line == columns:
+        values = torch.empty_like(x2, dtype=_E4M3, memory_format=torch.contiguous_format)
+    else:
+        values = x2.new_empty((rows, line), dtype=_E4M3)[:, :columns]
+    scales = x2.new_empty((rows if group_rows == 1 else (rows + GROUP - 1) // GROUP, groups), dtype=torch.float32)
+    _launch(what, "tris_quantize_e4m3", x.device, _QUANTIZE.pack(x2.data_ptr(), values.data_ptr(), scales.data_ptr(), x2.stride(0), line, groups, rows, columns, group_rows,
+                                                                 _DTYPES[dtype]))
     if x.dim() != 2:
-        return values.view(x.shape), scales.view(x.shape[:-1] + scales.shape[1:])
+        return values.view(x.shape), scales.view(x.shape[:-1] + (groups,))
     return values, scales
 
 
@@ -62,34 +64,34 @@ def linear_e4m3(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, w
     [..., ceil(in_features / 128)] and ``weight_scales`` [ceil(out_features / 128), ceil(in_features / 128)] in fp32; ``bias`` [out_features] in fp16, bf16 or fp32.
     ``status``: optional int32 tensor of one element, zero at first, set where a kernel gives up a wait (``raise_on_status``)."""
     what = "linear_e4m3"
-    dev = _same_device(what, x, x_scales, weight, weight_scales, bias, status)
-    e4m3 = torch.float8_e4m3fn
-    if x.dtype is not e4m3 or weight.dtype is not e4m3 or weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
-        _fail(what, f"x [..., in_features] and weight [out_features, in_features] must be {e4m3}, got {x.dtype} {tuple(x.shape)} and {weight.dtype} {tuple(weight.shape)}")
+    _same_device(what, x, x_scales, weight, weight_scales, bias, status)
+    shape, x2, xs2 = x.shape, x, x_scales
+    if x.dtype is not _E4M3 or weight.dtype is not _E4M3 or len(weight.shape) != 2 or not shape or shape[-1] != weight.shape[1]:
+        _fail(what, f"x [..., in_features] and weight [out_features, in_features] must be {_E4M3}, got {x.dtype} {tuple(shape)} and {weight.dtype} {tuple(weight.shape)}")
     if dtype not in _LOGIT_TYPES:
         _fail(what, f"outputs are fp16, bf16 or fp32, not {dtype}")
     outputs, inputs = weight.shape
-    groups = -(-inputs // GROUP)
-    x2, xs2 = _rows(what, "x", x), x_scales
-    if x_scales.dim() != x.dim() or x_scales.shape[:-1] != x.shape[:-1]:
-        _fail(what, f"x_scales must be {tuple(x.shape[:-1])} x {groups}, got {tuple(x_scales.shape)}")
-    if x.dim() != 2:
-        xs2 = _rows(what, "x_scales", x_scales)
+    groups = (inputs + GROUP - 1) // GROUP
+    if len(shape) != 2 or x.stride(1) != 1:
+        if x_scales.shape[:-1] != shape[:-1]:
+            _fail(what, f"x_scales must be {tuple(shape[:-1])} x {groups}, got {tuple(x_scales.shape)}")
+        x2, xs2 = _rows(what, "x", x), _rows(what, "x_scales", x_scales)
     rows = x2.shape[0]
     xs_at, xs_stride, _ = _matrix(what, "x_scales", xs2, torch.float32, rows, groups)
-    w_at, w_stride, _ = _matrix(what, "weight", weight, e4m3, outputs, inputs)
-    ws_at, ws_stride, _ = _matrix(what, "weight_scales", weight_scales, torch.float32, -(-outputs // GROUP), groups)
-    bias_at, bias_type = 0, 0
+    ws_at, ws_stride, _ = _matrix(what, "weight_scales", weight_scales, torch.float32, (outputs + GROUP - 1) // GROUP, groups)
+    w_stride, along = weight.stride()
+    if along != 1 and inputs > 1:
+        _fail(what, "weight must have a row side by side")
+    bias_at = bias_type = status_at = 0
     if bias is not None:
         if bias.dtype not in _LOGIT_TYPES or bias.shape != (outputs,) or not bias.is_contiguous():
             _fail(what, f"bias must be contiguous fp16, bf16 or fp32 [{outputs}], got {bias.dtype} {tuple(bias.shape)}")
         bias_at, bias_type = bias.data_ptr(), _DTYPES[bias.dtype]
-    status_at = 0
     if status is not None:
         if status.dtype is not torch.int32 or status.numel() != 1:
             _fail(what, "status must be an int32 tensor of one element")
         status_at = status.data_ptr()
-    out = torch.empty((rows, outputs), dtype=dtype, device=dev)
-    _launch(what, "tris_e4m3_linear", dev, _LINEAR.pack(x2.data_ptr(), xs_at, w_at, ws_at, bias_at, out.data_ptr(), status_at, x2.stride(0), xs_stride, w_stride, ws_stride,
-                                                        outputs, rows, inputs, outputs, _DTYPES[dtype], bias_type, 0))
-    return out if x.dim() == 2 else out.view(x.shape[:-1] + (outputs,))
+    out = x2.new_empty((rows, outputs), dtype=dtype)
+    _launch(what, "tris_e4m3_linear", x.device, _LINEAR.pack(x2.data_ptr(), xs_at, weight.data_ptr(), ws_at, bias_at, out.data_ptr(), status_at, x2.stride(0), xs_stride, w_stride,
+                                                             ws_stride, outputs, rows, inputs, outputs, _DTYPES[dtype], bias_type, 0))
+    return out if len(shape) == 2 else out.view(shape[:-1] + (outputs,))
