@@ -15,7 +15,7 @@
 namespace tris {
 namespace {
 
-constexpr int kThreads = 1024, kBins = kThreads, kFew = 256;
+constexpr int kThreads = 1024, kBins = kThreads, kFew = 512;
 constexpr int kMostCtas = 8;   // of a cluster
 constexpr int kTable = 1024;   // powers 2^(i / kTable)
 
@@ -88,15 +88,20 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
     float kept[kThreads / 32][128];  // logits of a warp's tokens, one after the other
   } buffer;
   __shared__ double powers[kTable];
-  __shared__ uint64_t sums[kThreads], red64[32], part;
-  __shared__ uint64_t lists[2][kFew];  // tokens of the interval that was found, of this CTA
-  __shared__ ulonglong2 merged[kFew];  // and of all, each with its weight
+  __shared__ union Second {
+    uint64_t sums[kThreads];   // of a chunk's weights
+    ulonglong2 merged[kFew];  // tokens of the interval that was found, of all CTAs, each with its weight
+  } second;
+  __shared__ uint64_t red64[32], part;
+  __shared__ uint64_t lists[2][kFew];  // those of this CTA
   __shared__ uint32_t listed[2], red32[32], best;
   __shared__ uint64_t ends[2][2];  // the last and the first of them in the order
   __shared__ __align__(8) float extremes[2];
   __shared__ Found found;
   __shared__ uint64_t cut;
   Histogram& bins = buffer.bins;
+  auto& sums = second.sums;
+  auto& merged = second.merged;
   const TrisSampleTokens& s = args.s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.y;
@@ -253,7 +258,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
   if (by_count || by_weight) {
     const float range = fminf(40.f * temperature, top - low);
     const float per_bin = range > 0.f ? fminf(kBins / range, 1e30f) : 0.f;
-    auto bin_of = [&](float z) { return static_cast<int>(fminf((top - z) * per_bin, kBins - 1.f)); };
+    // (rounded by what is added to it, which takes no turn of the slow pipe for conversions)
+    auto bin_of = [&](float z) { return static_cast<int>(__float_as_uint(fminf((top - z) * per_bin, kBins - 1.f) + 12582912.f) & (2 * kBins - 1)); };
     auto enter = [&](int bin, uint64_t w) {
       const uint32_t w_low = static_cast<uint32_t>(w);
       uint32_t w_high = static_cast<uint32_t>(w >> 32);
@@ -262,7 +268,6 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
     };
     // Adds to the list the tokens for which `inside` holds.
     auto list_tokens = [&](int use, auto inside) {
-      uint64_t last = ~0ull, first = 0;
 #pragma unroll 2
       for (int at = 4 * tid; at < n; at += 4 * kThreads) {
         float z[4];
@@ -270,18 +275,35 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (inside(z[k], v0 + at + k)) {
-            const uint64_t place = place_of(z[k], v0 + at + k);
             const uint32_t i = atomicAdd(&listed[use], 1u);
-            if (i < kFew) lists[use][i] = place;
-            last = min(last, place);
-            first = max(first, place);
+            if (i < kFew) lists[use][i] = place_of(z[k], v0 + at + k);
           }
       }
-      if (first) {
+    };
+    // The last and the first of them in the order, for too many of them to be listed.
+    auto find_ends = [&](int use, auto inside) {
+      uint64_t last = ~0ull, first = 0;
+      for (int at = 4 * tid; at < n; at += 4 * kThreads) {
+        float z[4];
+        fetch(at, z);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (inside(z[k], v0 + at + k)) {
+            last = min(last, place_of(z[k], v0 + at + k));
+            first = max(first, place_of(z[k], v0 + at + k));
+          }
+      }
+#pragma unroll
+      for (int d = 16; d; d >>= 1) {
+        last = min(last, __shfl_xor_sync(0xFFFFFFFFu, last, d));
+        first = max(first, __shfl_xor_sync(0xFFFFFFFFu, first, d));
+      }
+      if (lane == 0 && first) {
         atomicMin(reinterpret_cast<unsigned long long*>(&ends[use][0]), last);
         atomicMax(reinterpret_cast<unsigned long long*>(&ends[use][1]), first);
       }
     };
+
     // The lists of all CTAs as one, with weights; their number, or more than kFew.
     auto merge_lists = [&](int use) {
       uint32_t many[kMostCtas];
@@ -309,8 +331,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
         if (here) found = {tid, count, count_before, weight_before};
         __syncthreads();
         const Found f = found;
+        // a bin's tokens: what is rounded to its number
+        auto in_bin = [&](float z, int token) { return bin_of(z) == f.bin && z > -INFINITY && (from == 0 || place_of(z, token) >= from); };
         if (!places) {
-          list_tokens(use, [&](float z, int token) { return z > -INFINITY && bin_of(z) == f.bin && (from == 0 || place_of(z, token) >= from); });
+          list_tokens(use, in_bin);
         } else {
           first -= static_cast<uint64_t>(f.bin) << shift;
           const uint64_t width = (1ull << shift) - 1;
@@ -329,6 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
             const uint64_t mine = merged[tid].x, own = merged[tid].y;
             uint64_t sum = f.weight_before;
             uint32_t rank = f.count_before;
+#pragma unroll 4
             for (uint32_t i = 0; i < many; ++i) {
               const ulonglong2 other = merged[i];
               rank += other.x > mine;
@@ -343,6 +368,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
         }
         // too many: a histogram of their places alone
         if (!places) {
+          find_ends(use, in_bin);
+          meet();
           for (int r = 0; r < ctas; ++r) {
             last = r ? min(last, load_cluster_u64(there(&ends[use][0], r))) : load_cluster_u64(there(&ends[use][0], 0));
             first = r ? max(first, load_cluster_u64(there(&ends[use][1], r))) : load_cluster_u64(there(&ends[use][1], 0));
@@ -485,26 +512,41 @@ __global__ void __launch_bounds__(kThreads, 1) sample_tokens_kernel(const __grid
   __syncthreads();
   sums[tid] = 0;
   __syncthreads();
-  for (int c = warp; c * args.chunk < n; c += kThreads / 32) {
-    uint64_t sum = 0;
-    for (int at = c * args.chunk + 4 * lane; at - 4 * lane < min(n, (c + 1) * args.chunk); at += 128) {
-      float z[4];
-      fetch(at, z);
-      int many = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const bool kept = is_kept(z[k], v0 + at + k);
-        const uint32_t all = __ballot_sync(0xFFFFFFFFu, kept);
-        if (kept) buffer.kept[warp][many + __popc(all & ((1u << lane) - 1))] = z[k];
-        many += __popc(all);
-      }
-      __syncwarp();
-      for (int i = lane; i < many; i += 32) sum += kept_weight(buffer.kept[warp][i]);
-      __syncwarp();
+  // A warp's pieces of 128 tokens, chunk after chunk; the next one's logits are on their way.
+  auto next_piece = [&](int& c, int& at) {
+    at += 128;
+    if (at >= (c + 1) * args.chunk || at >= n) {
+      c += kThreads / 32;
+      at = c * args.chunk;
     }
+  };
+  int chunk = warp, piece = warp * args.chunk;
+  float next[4];
+  if (piece < n) fetch(piece + 4 * lane, next);
+  uint64_t sum = 0;
+#pragma unroll 1
+  while (piece < n) {
+    const float z[4] = {next[0], next[1], next[2], next[3]};
+    const int at = piece + 4 * lane, now = chunk;
+    next_piece(chunk, piece);
+    if (piece < n) fetch(piece + 4 * lane, next);
+    int many = 0;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-    if (lane == 0) sums[c] = sum;
+    for (int k = 0; k < 4; ++k) {
+      const bool kept = is_kept(z[k], v0 + at + k);
+      const uint32_t all = __ballot_sync(0xFFFFFFFFu, kept);
+      if (kept) buffer.kept[warp][many + __popc(all & ((1u << lane) - 1))] = z[k];
+      many += __popc(all);
+    }
+    __syncwarp();
+    for (int i = lane; i < many; i += 32) sum += kept_weight(buffer.kept[warp][i]);
+    __syncwarp();
+    if (chunk != now) {
+#pragma unroll
+      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+      if (lane == 0) sums[now] = sum;
+      sum = 0;
+    }
   }
   __syncthreads();
   uint64_t mine = sums[tid], all;
