@@ -22,7 +22,7 @@ struct BlockArgs {
   TrisPagedKv cache;
   TrisPagedAppend rows;
   int lanes;        // that have a row, 16 dimensions each: a power of two
-  int window;       // rows of a CTA, up to 32
+  int window;       // rows of a CTA, up to 16
   int page_shift;   // log2(page_size), or -1
   int block_mask;   // scale_tokens - 1 where that is a power of two, or -1
   int page_scales;  // scales of a page and head
@@ -42,7 +42,7 @@ __device__ __forceinline__ float block_scale(float top) {
 // grid (windows of tokens, shares of the heads), window * lanes threads, a multiple of 32.
 template <typename T, Form F>
 __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __grid_constant__ BlockArgs a) {
-  __shared__ __align__(16) float tops[2][kHeads][32];  // largest magnitude of every row; two turns
+  __shared__ __align__(16) float tops[2][kHeads][16];  // largest magnitude of every row; two turns
   pdl_wait();
   pdl_launch_dependents();
   const TrisPagedAppend& r = a.rows;
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
     const int64_t pos = position(t);
     return pos < 0 || pos >= room || in_block(static_cast<int>(pos)) == 0 || position(t - 1) != pos - 1 || r.sequences[t - 1] != r.sequences[t];
   };
-  auto beginnings = [&](int w) { return __ballot_sync(0xFFFFFFFFu, lane < R && begins(w + lane)); };
+  auto beginnings = [&](int w) { return __ballot_sync(0xFFFFFFFFu, begins(w + lane)); };  // among 32 tokens, of which a window has up to 16
 
   // What a thread knows of its row's token.
   int t = 0, pos = 0, page = 0;
@@ -275,21 +275,19 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
 
   const int end = min((static_cast<int>(blockIdx.x) + 1) * R, r.num_tokens);
   int w = blockIdx.x * R, turn = 0;
+  const uint32_t rows = (1u << R) - 1;
   uint32_t starts = beginnings(w);
-  if (!starts) return;  // all of these tokens belong to a run that begins ahead of them
-  if (!(starts & 1)) {
-    w += __ffs(starts) - 1;
-    if (w < end) starts = beginnings(w);
-  }
+  if (!(starts & rows)) return;  // all of these tokens belong to a run that begins ahead of them
+  w += __ffs(starts) - 1;
+  starts >>= __ffs(starts) - 1;
 #pragma unroll 1
   while (w < end) {
     // the rows of whole runs that a window holds
-    const uint32_t behind = starts & ~1u;
-    const int count = begins(w + R) ? R : behind ? 31 - __clz(behind) : 0;
+    const uint32_t behind = starts & rows & ~1u;
+    const int count = (starts >> R) & 1 ? R : behind ? 31 - __clz(behind) : 0;
     if (count) {
-      const int first = 31 - __clz(starts & (row < 31 ? (2u << row) - 1 : ~0u));  // of this row's run
-      const uint32_t above = row < 31 ? starts >> (row + 1) : 0;
-      const int last = min(above ? row + __ffs(above) : R, count);  // behind it
+      const int first = 31 - __clz(starts & ((2u << row) - 1));  // of this row's run
+      const int last = min(row + __ffs(starts >> (row + 1)), count);  // behind it; a run begins at row `count`
       const bool there = row < count && w + row < r.num_tokens;
       enter(min(w + row, r.num_tokens - 1), there);
       queries(there);
@@ -358,11 +356,8 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
       int length = R;
       for (;;) {
         const uint32_t more = beginnings(w + length);
-        if (more) {
-          length += __ffs(more) - 1;
-          break;
-        }
-        length += R;
+        length += more ? __ffs(more) - 1 : 32;
+        if (more) break;
       }
       for (int at = 0; at < length; at += R) {
         enter(w + min(at + row, length - 1), at + row < length);
@@ -452,7 +447,7 @@ int append_block_scaled(const TrisPagedKv& c, const TrisPagedAppend& r, int rota
     if (c.scale_tokens == 1 << i) a.block_mask = c.scale_tokens - 1;
   }
   a.page_scales = c.page_size / c.scale_tokens;
-  a.lanes = 1;
+  a.lanes = 2;
   while (16 * a.lanes < c.head_dim) a.lanes *= 2;
   bool wide = (!r.q_out || aligned_to(r.q_out, 16)) && (!r.k_out || aligned_to(r.k_out, 16)) && aligned_to(r.cos, 16) && aligned_to(r.sin, 16);
   const void* src[3] = {r.num_q_heads ? r.q : nullptr, r.k, r.v};
@@ -460,9 +455,9 @@ int append_block_scaled(const TrisPagedKv& c, const TrisPagedAppend& r, int rota
   for (int i = 0; i < 3; ++i)
     if (src[i]) wide = wide && aligned_to(src[i], 16) && strides[i][0] % 8 == 0 && strides[i][1] % 8 == 0;
   const Form form = wide && rotary_dim % (r.interleaved ? 8 : 16) == 0 ? (r.interleaved ? Form::kPairs : Form::kHalves) : Form::kAny;
-  // a warp's rows to a CTA where there are few tokens (a decode step), else 16 or, of short rows, 32
+  // a warp's rows to a CTA where there are few tokens (a decode step), else 16
   const int64_t items = r.num_q_heads + 2 * c.num_kv_heads;
-  a.window = r.num_tokens * items <= 64 * static_cast<int64_t>(sm_count()) ? 32 / a.lanes : a.lanes >= 8 ? 16 : 32;
+  a.window = r.num_tokens * items <= 64 * static_cast<int64_t>(sm_count()) ? 32 / a.lanes : 16;
   return r.dtype == TRIS_DTYPE_F16 ? launch_blocks<__half>(a, form, stream) : launch_blocks<__nv_bfloat16>(a, form, stream);
 }
 

@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const __grid_co
 
 // A CTA has a block of 128 x 128.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const __grid_constant__ QuantizeArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) quantize_blocks_kernel(const __grid_constant__ QuantizeArgs a) {
   __shared__ uint32_t tops[kThreads / 32];
   pdl_wait();
   pdl_launch_dependents();
