@@ -915,7 +915,7 @@ int tris_logit_controls(const TrisLogitControls* args, void* stream);
  * are less than top_p times those of the first top_k, and its weight w = exp((z - max) / temperature) is at least min_p; of those kept, in the order of
  * the vocabulary, the first is drawn whose running sum exceeds random times the whole.  temperature <= 0: the first of the largest.  Off: top_k <= 0,
  * top_p >= 1, min_p <= 0, and NULL (temperature 1).  Weights are counted in units of 2^-46 of the largest (vocabularies beyond 65536: 2^-(62 - log2)).
- * Logits of -inf and NaN are never drawn; a row without others gives -1.
+ * Logits of -inf and NaN are never drawn, the first of +inf always is; a row without others gives -1.
  */
 typedef struct TrisSampleTokens {
   const void* logits;               /* [rows, vocab]                                       */

@@ -2,7 +2,7 @@
 //
 // y[t, n] = sum_g xs[t, g] ws[n / 128, g] sum_{k in g} x[t, k] w[n, k] + bias[n].  The inner sums are products of 128 columns on the tensor cores
 // (tcgen05.mma, kind::f8f6f4, fp32 accumulators in TMEM); the scales differ from one group to the next, so every group's tile leaves TMEM and is added
-// to 32-bit sums in registers, times its scale.  Two TMEM tiles take turns: one is filled while the other is read.
+// to 32-bit sums in registers, times its scale.  TMEM tiles take turns: one is filled while another is read.
 //
 // Roles: one warp asks for operands (TMA, a ring of stages), one issues the MMAs, and one or two groups of four warps add up.
 //   rows few (kFeatures): the 128 lanes of a tile are features, its columns rows of x, so that a tile wastes nothing on rows that do not exist; a thread has
@@ -10,8 +10,12 @@
 //   are joined in the order of the CTAs over distributed shared memory.
 //   rows many (kRows): the lanes are rows of x, the columns features.  A thread has one row and its scales, four groups of them at a time.
 //   rows many, tiles enough (kPair): two CTAs of a cluster have one tile of 256 rows x 256 features, each 128 of its rows in TMEM and 128 of either operand in shared
-//   memory, which the MMAs of both read.  What counts there is the way from L2, which brings an SM some 64 bytes a cycle: a group of a tile of its own, 128 x 256,
-//   takes 48 KB and 512 cycles of the tensor core, half a pair's tile 32 KB.
+//   memory, which the MMAs of both read.  The way from L2 brings an SM some 50 bytes a cycle: a group of a tile of 128 x 256 is 48 KB for 512 cycles of the tensor core,
+//   half a pair's tile 32 KB.  The tile's halves are multiplied, read and given back by themselves, a half for each group of warps.
+// 8192 rows of 4096 to 14336 features in bf16: 470 to 550 us by the clock that the power limit leaves (1.7 to 2.0 PFLOP/s; tiles of 128 x 128 640 us, of 128 x 256 without pairs
+// 570), of which loads and products alone take 332; the rest is the sums: 128 columns of a thread leave TMEM in four loads that wait, some 1000 cycles a group with what is around
+// them, at two warps a scheduler.  Tried, us beside 471: four groups of warps 520, 16 columns a load 512, packed sums 540, more registers for the sums by setmaxnreg 484.
+// 64 rows of 4096 to 32000 in fp32: 30 us, 131 MB of weights; streaming them alone takes 24.  One row of 2048 to 6144: 6.1 us, a chain of launch, loads, products and join.
 #include <type_traits>
 
 #include "decode_step.cuh"
@@ -125,13 +129,20 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
   else tmem_ld_32(taddr, v);
 }
 
-// Waits for the phase with the given parity, giving up after 2^20 tries, each of which waits itself up to a limit of the hardware's.  (The timer takes longer to read
-// than most of these waits, and code that may read it costs registers.)
+// Waits for the phase with the given parity, giving up after 2^20 tries of a microsecond each at most: about a second.  The first tries are plain ones, which come back sooner
+// (509 rows of 2048 to 6144: 13.8 us, 14.8 without them).  (The timer takes longer to read than most of these waits, and code that may read it costs registers.)
 __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity) {
-  bool done = false;
+  uint32_t done = 0;
 #pragma unroll 1
-  for (int i = 0; !done && i < (1 << 20); ++i) done = mbar_try_wait(bar, parity);
-  return done;
+  for (int i = 0; !done && i < 64; ++i) done = mbar_try_wait(bar, parity);
+#pragma unroll 1
+  for (int i = 0; !done && i < (1 << 20); ++i)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000)
+        : "memory");
+  return done != 0;
 }
 // The same by a whole warp, with one answer for all lanes.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait_one(bar, parity)); }
@@ -146,6 +157,7 @@ __device__ __forceinline__ void store_output(const TrisE4m3Linear& a, int64_t at
   else if (a.dtype == TRIS_DTYPE_F16) static_cast<__half*>(a.out)[at] = __float2half_rn(v);
   else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
 }
+
 // grid (CTAs, 1, CTAs of a cluster), or (2 pairs, 1, 1) in clusters of two.  A CTA (a pair) walks over tiles; where the groups are cut among a cluster's CTAs it has one.
 template <int BN, int WGS, Mode M>
 __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape<BN, WGS, M>::kCtasPerSm)
@@ -315,8 +327,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
         ask_scales(0);
       }
       if constexpr (!kSwap) {
-        // (a barrier lies between this and the last use of the tile before: the one behind the tile's last stores, or the warps' own below)
-        named_barrier_sync(1 + wg, 128);
+        named_barrier_sync(1 + wg, 128);  // the biases of the tile before have been read
         if (in_tile < S::kColumns) biases[wg * S::kColumns + in_tile] = feature0 + in_tile < a.out_features ? bias_at(a, feature0 + in_tile) : 0.f;
         named_barrier_sync(1 + wg, 128);
       }

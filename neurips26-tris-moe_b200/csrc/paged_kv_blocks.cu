@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
   const TrisPagedKv& c = a.cache;
   const int tid = threadIdx.x, lane = tid & 31, L = a.lanes, R = a.window, row = tid / L, u = tid % L;
   const int hq = r.num_q_heads, hkv = c.num_kv_heads, D = c.head_dim, rot = r.rotary_dim, half = rot / 2, block = c.scale_tokens;
-  const int64_t room = static_cast<int64_t>(c.table_width) * c.page_size;
+  const int64_t room = min(static_cast<int64_t>(c.table_width) * c.page_size, static_cast<int64_t>(0x7FFFFFFF));  // positions are 32-bit numbers from here on
   const bool active = 16 * u < D;
   // this thread's two chunks of eight dimensions
   const bool pairs_up = F == Form::kHalves && u < half / 8;
@@ -439,6 +439,7 @@ int launch_blocks(const BlockArgs& a, Form form, cudaStream_t stream) {
 // Arguments have been checked (tris_paged_kv_append).
 int append_block_scaled(const TrisPagedKv& c, const TrisPagedAppend& r, int rotary_dim, cudaStream_t stream) {
   TRIS_REQUIRE(r.sequences || r.num_tokens <= c.num_sequences, TRIS_ERR_INVALID_ARG, "paged_kv_append: %d tokens without sequences for a block table of %d", r.num_tokens, c.num_sequences);
+  TRIS_REQUIRE(r.num_tokens <= 1 << 30, TRIS_ERR_UNSUPPORTED, "paged_kv_append: too many tokens in one call");
   BlockArgs a{c, r};
   a.rows.rotary_dim = rotary_dim;
   a.page_shift = a.block_mask = -1;

@@ -356,7 +356,7 @@ def sample_tokens(logits: torch.Tensor, random: torch.Tensor, *, temperature: Op
     * ``min_p`` (fp32 [rows]): its weight is at least ``min_p`` times the largest; 0 or less: off.
 
     ``temperature`` (fp32 [rows], default 1): 0 or less takes the first of the largest logits.  Weights are counted in units of 2^-46 of the
-    largest, so the sums are exact and a draw is the same on every run.  Logits of -inf and NaN are never drawn; a row without any other gives -1."""
+    largest, so the sums are exact and a draw is the same on every run.  Logits of -inf and NaN are never drawn, the first of +inf always is; a row without any other gives -1."""
     what = "sample_tokens"
     dev = _same_device(what, logits, random, temperature, top_k, top_p, min_p)
     shape, dtype = logits.shape, logits.dtype
