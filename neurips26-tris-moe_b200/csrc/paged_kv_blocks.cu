@@ -16,12 +16,12 @@
 namespace tris {
 namespace {
 
-constexpr int kHeads = 2;  // at a time
+constexpr int kHeads = 1;  // at a time
 
 struct BlockArgs {
   TrisPagedKv cache;
   TrisPagedAppend rows;
-  int lanes;        // that have a row, 16 dimensions each: a power of two
+  int lanes;        // that have a row, 16 dimensions each: a power of two from 2 to 16
   int window;       // rows of a CTA, up to 16
   int page_shift;   // log2(page_size), or -1
   int block_mask;   // scale_tokens - 1 where that is a power of two, or -1
@@ -40,14 +40,15 @@ __device__ __forceinline__ float block_scale(float top) {
 }
 
 // grid (windows of tokens, shares of the heads), window * lanes threads, a multiple of 32.
-template <typename T, Form F>
-__global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __grid_constant__ BlockArgs a) {
+// L: lanes that have a row, 16 dimensions each.
+template <typename T, Form F, int L>
+__global__ void __launch_bounds__(16 * L, L == 16 ? 3 : L == 8 ? 6 : 12) paged_kv_append_blocks_kernel(const __grid_constant__ BlockArgs a) {
   __shared__ __align__(16) float tops[2][kHeads][16];  // largest magnitude of every row; two turns
   pdl_wait();
   pdl_launch_dependents();
   const TrisPagedAppend& r = a.rows;
   const TrisPagedKv& c = a.cache;
-  const int tid = threadIdx.x, lane = tid & 31, L = a.lanes, R = a.window, row = tid / L, u = tid % L;
+  const int tid = threadIdx.x, lane = tid & 31, R = a.window, row = tid / L, u = tid % L;
   const int hq = r.num_q_heads, hkv = c.num_kv_heads, D = c.head_dim, rot = r.rotary_dim, half = rot / 2, block = c.scale_tokens;
   const int64_t room = min(static_cast<int64_t>(c.table_width) * c.page_size, static_cast<int64_t>(0x7FFFFFFF));  // positions are 32-bit numbers from here on
   const bool active = 16 * u < D;
@@ -193,6 +194,7 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
       top = fmaxf(top, !finite || fabsf(x[k]) <= FLT_MAX ? fabsf(x[k]) : 0.f);
       top = fmaxf(top, !finite || fabsf(y[k]) <= FLT_MAX ? fabsf(y[k]) : 0.f);
     }
+#pragma unroll
     for (int d = 1; d < L; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
     return top;
   };
@@ -319,9 +321,9 @@ __global__ void __launch_bounds__(256, 2) paged_kv_append_blocks_kernel(const __
           src.row += shares * src.stride;
           if (h0 + shares < hkv) fetch_heads(src.row, src.stride, hkv - h0 - shares, next);
           if (__syncthreads_or(infinite)) {  // rare: the largest of the finite ones alone
-#pragma unroll 1
+#pragma unroll
             for (int k = 0; k < kHeads; ++k) {
-              const float top = k ? row_top(x[1], y[1], true) : row_top(x[0], y[0], true);
+              const float top = row_top(x[k], y[k], true);
               if (u == 0) tops[turn][k][row] = placed ? top : 0.f;
             }
             __syncthreads();
@@ -425,7 +427,9 @@ int launch_blocks(const BlockArgs& a, cudaStream_t stream) {
   const int most = ceil_div(heads, kHeads), few = ceil_div(heads, kWalk);
   const int shares = windows * most <= 16 * static_cast<int64_t>(sm_count()) ? most : few;
   TRIS_REQUIRE(shares <= 65535, TRIS_ERR_UNSUPPORTED, "paged_kv_append: too many heads");
-  TRIS_CUDA(launch_step(paged_kv_append_blocks_kernel<T, F>, dim3(static_cast<unsigned>(windows), shares), dim3(a.window * a.lanes), 0, stream, programmatic_launch_default(), 1, a));
+  auto kernel = a.lanes == 2 ? paged_kv_append_blocks_kernel<T, F, 2> : a.lanes == 4 ? paged_kv_append_blocks_kernel<T, F, 4> : a.lanes == 8 ? paged_kv_append_blocks_kernel<T, F, 8>
+                                                                                                                                              : paged_kv_append_blocks_kernel<T, F, 16>;
+  TRIS_CUDA(launch_step(kernel, dim3(static_cast<unsigned>(windows), shares), dim3(a.window * a.lanes), 0, stream, programmatic_launch_default(), 1, a));
   return TRIS_OK;
 }
 
