@@ -66,7 +66,8 @@ struct LinearShape {
   static constexpr int kTmem = kTiles * BN;
   static constexpr size_t kSmem = static_cast<size_t>(kStages) * kStageBytes + kOutBytes + kScaleBytes + 1024;
   static_assert(!kPair || (kHalf == kColumns && kHalf == kGroup), "a group of warps has a half, and one block's scale");
-  static_assert(kStages >= 3 && (kPair || BN * kLanes * 4 <= kStages * kStageBytes), "a tile's sums lie where the stages were");
+  static constexpr int kPitch = kSwap ? kLanes : kLanes + 1;  // of a column of sums, for the join; rows of it are read across, too, where they are rows of x
+  static_assert(kStages >= 3 && (kPair || BN * kPitch * 4 <= kStages * kStageBytes), "a tile's sums lie where the stages were");
 };
 
 __device__ __forceinline__ void umma_f8_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
@@ -403,7 +404,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
         // the ring is idle: this CTA's only tile has been multiplied
         float* part = reinterpret_cast<float*>(ring);
 #pragma unroll
-        for (int c = 0; c < S::kColumns; ++c) part[(wg * S::kColumns + c) * kLanes + in_tile] = acc[c];
+        for (int c = 0; c < S::kColumns; ++c) part[(wg * S::kColumns + c) * S::kPitch + in_tile] = acc[c];
       } else if constexpr (kSwap) {
         const int n = ft * kLanes + in_tile;
         if (n < a.out_features) {
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
         // 128 bytes of every row at a time, in the order that the tensor copy expects: 16-byte chunk c of row r at place c ^ (r & 7)
         auto put = [&](int chunk, uint4 v) { *reinterpret_cast<uint4*>(out_stage + in_tile * 128 + ((chunk ^ (in_tile & 7)) << 4)) = v; };
         const int row0 = row - in_tile;
-        auto stage_out = [&](int c0, int columns, auto write) {
+        auto stage_out = [&](int c0, auto write) {
           if (in_tile == 0) tma_stores_read();
           named_barrier_sync(1 + wg, 128);
           write();
@@ -429,7 +430,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
         if (a.dtype == TRIS_DTYPE_F32) {
 #pragma unroll
           for (int c0 = 0; c0 < S::kColumns; c0 += 32)
-            stage_out(c0, 32, [&] {
+            stage_out(c0, [&] {
 #pragma unroll
               for (int c = 0; c < 32; c += 4) {
                 const float4 b = *reinterpret_cast<const float4*>(&biases[wg * S::kColumns + c0 + c]);
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
         } else {
 #pragma unroll
           for (int c0 = 0; c0 < S::kColumns; c0 += 64)
-            stage_out(c0, 64, [&] {
+            stage_out(c0, [&] {
 #pragma unroll
               for (int c = 0; c < 64; c += 8) {
                 uint32_t w[4];
@@ -477,20 +478,50 @@ __global__ void __launch_bounds__(LinearShape<BN, WGS, M>::kThreads, LinearShape
   if (warp == 0) tmem_dealloc(tmem, S::kTmem);
   if (split == 1) return;
 
-  // every CTA of the cluster joins its share of the tile's columns, in the order of the CTAs
+  // Every CTA of the cluster joins its share of the tile's columns, in the order of the CTAs.  A thread has some of them on their way, of up to four CTAs.
+  // (us, and with one of a thread after the other and rows of x written across: 64 x 2048 to 6144 9.3 and 15.9, 256 x 14336 to 4096 33.5 and 45.0.)
   cluster_sync();
   if (warp < S::kWarps) {
     int rt, ft;
     place(blockIdx.x, rt, ft);
+    float* const mine = reinterpret_cast<float*>(ring);
     const uint32_t local = smem_u32(ring);
-    const int in_tile = threadIdx.x % kLanes, part = threadIdx.x / kLanes;
-    for (int u = blockIdx.z * WGS + part; u < BN; u += split * WGS) {
-      const int t = kSwap ? rt * BN + u : rt * kLanes + in_tile, n = kSwap ? ft * kLanes + in_tile : ft * BN + u;
-      if (t >= a.rows || n >= a.out_features) continue;
-      float v = 0.f;
-#pragma unroll 8
-      for (int r = 0; r < split; ++r) v += load_cluster(in_cta(local, r) + (u * kLanes + in_tile) * 4);
-      store_output(a, static_cast<int64_t>(t) * a.out_stride + n, v + (kSwap ? bias_at(a, n) : biases[kSwap ? 0 : u]));
+    const int rows = min(a.rows - rt * (kSwap ? BN : kLanes), kSwap ? BN : kLanes), features = min(a.out_features - ft * (kSwap ? kLanes : BN), kSwap ? kLanes : BN);
+    const int lanes_there = kSwap ? features : rows, columns_there = kSwap ? rows : features, share = (columns_there + split - 1) / split;
+    const int in_tile = threadIdx.x % kLanes, u0 = blockIdx.z * share, u1 = min(u0 + share, columns_there);
+    constexpr int kAtOnce = 4;
+    for (int u = u0 + static_cast<int>(threadIdx.x) / kLanes; u < u1; u += kAtOnce * WGS) {
+      float v[kAtOnce] = {};
+      for (int r0 = 0; r0 < split; r0 += 4) {
+        float w[4][kAtOnce];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k) w[r][k] = r0 + r < split && u + k * WGS < u1 ? load_cluster(in_cta(local, r0 + r) + ((u + k * WGS) * S::kPitch + in_tile) * 4) : 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k) v[k] += w[r][k];
+      }
+      if constexpr (kSwap) {
+        if (in_tile >= lanes_there) continue;
+        const int n = ft * kLanes + in_tile;
+        const float bias = bias_at(a, n);
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k)
+          if (u + k * WGS < u1) store_output(a, static_cast<int64_t>(rt * BN + u + k * WGS) * a.out_stride + n, v[k] + bias);
+      } else {  // no other CTA reads this one's share
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k)
+          if (u + k * WGS < u1) mine[(u + k * WGS) * S::kPitch + in_tile] = v[k] + biases[u + k * WGS];
+      }
+    }
+    if constexpr (!kSwap) {  // and out, features side by side
+      named_barrier_sync(1 + WGS, 32 * S::kWarps);
+      const int wide = 1 << (31 - __clz(max(1, min(32, share)))), across = threadIdx.x % wide;
+      for (int row = threadIdx.x / wide; row < lanes_there; row += 32 * S::kWarps / wide)
+        for (int u = u0 + across; u < u1; u += wide)
+          store_output(a, static_cast<int64_t>(rt * kLanes + row) * a.out_stride + ft * BN + u, mine[u * S::kPitch + row]);
     }
   }
   cluster_sync();  // nobody leaves while another reads its shared memory
@@ -541,11 +572,13 @@ int launch_linear(LinearArgs& args, int split, cudaStream_t stream) {
   return TRIS_OK;
 }
 
-// CTAs of a cluster that cut the groups of a tile among themselves: a power of two up to 8, as many as run at one time.  (1 x 2048 to 6144, 48 tiles of 16 groups, us:
-// 7.4 uncut, 6.4 by two, 6.7 by three, 6.1 by four; 10.0 by six and 8.9 by eight, which no more run at one time.)
-int split_of(int64_t tiles, int room, int groups) {
+// CTAs of a cluster that cut the groups of a tile among themselves: a power of two up to 8, as many as run at one time, each with `least` groups to itself.
+//   kFeatures, 4: 1 x 2048 to 6144, 48 tiles of 16 groups, us: 7.4 uncut, 6.4 by two, 6.7 by three, 6.1 by four; 10.0 by six and 8.9 by eight, which no more run at
+//   one time.  64 x 14336 to 4096, 32 tiles of 112 groups: 43.0 uncut, 15.6 by eight.
+//   kRows, 16: its join has 128 rows.  128 x 2048 to 6144: 10.9 uncut, 14.1 by two; 128 x 14336 to 4096: 48.4 uncut, 21.1 by four.
+int split_of(int64_t tiles, int room, int groups, int least) {
   int split = 1;
-  while (split < 8 && 2 * tiles * split <= room && groups >= 4 * split) split *= 2;
+  while (split < 8 && 2 * tiles * split <= room && groups >= 2 * least * split) split *= 2;
   return split;
 }
 
@@ -577,16 +610,19 @@ extern "C" int tris_e4m3_linear(const TrisE4m3Linear* linear, void* stream) {
   args.groups = ceil_div(a.in_features, kGroup);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int sms = sm_count();
+  // Features along the lanes while one tile has all rows.  us, features and rows along the lanes: 64 x 2048 to 6144 9.3 and 10.5, 64 x 14336 to 4096 15.6 and 20.6, 64 x 4096 to
+  // 14336 20 either way; 128 rows in two such tiles 28, 29 and 44, rows along the lanes 11, 21 and 19.  (One row as a tile of 64 columns instead of 16: 7.9 and 14.6 for 6.2 and 11.2.)
   if (a.rows <= 64) {
-    const int split = split_of(ceil_div(a.out_features, kLanes), 2 * sms, args.groups);
+    const int split = split_of(ceil_div(a.out_features, kLanes), 2 * sms, args.groups, 4);
     if (a.rows <= 16) return launch_linear<16, 1, Mode::kFeatures>(args, split, s);
     if (a.rows <= 32) return launch_linear<32, 1, Mode::kFeatures>(args, split, s);
     return launch_linear<64, 1, Mode::kFeatures>(args, split, s);
   }
   const int64_t pairs = static_cast<int64_t>(ceil_div(a.rows, 2 * kLanes)) * ceil_div(a.out_features, 256);
   const int64_t small = static_cast<int64_t>(ceil_div(a.rows, kLanes)) * ceil_div(a.out_features, 128);
-  // rounds of all SMs; one of pairs takes twice as long as one of small tiles
-  const int64_t t_pairs = (pairs + sms / 2 - 1) / (sms / 2) * 2, t_small = (small + sms - 1) / sms;
-  if (a.rows > kLanes && 3 * t_pairs <= 5 * t_small) return launch_linear<256, 2, Mode::kPair>(args, 1, s);
-  return launch_linear<128, 2, Mode::kRows>(args, split_of(small, sms, args.groups), s);
+  // Rounds of all SMs; one of pairs takes six fifths of one of small tiles.  us, pairs and small tiles: 256 x 2048 to 6144, a round either way, 14.0 and 11.1; 512 x 2048 to 6144,
+  // one round and two, 14.4 and 18.2; 768 x 14336 to 4096, one and two, 60 and 92; 8192 x 4096 to 14336, 25 and 49, 550 and 690.
+  const int64_t rounds_of_pairs = (pairs + sms / 2 - 1) / (sms / 2), rounds_of_small = (small + sms - 1) / sms;
+  if (a.rows > kLanes && 6 * rounds_of_pairs <= 5 * rounds_of_small) return launch_linear<256, 2, Mode::kPair>(args, 1, s);
+  return launch_linear<128, 2, Mode::kRows>(args, split_of(small, sms, args.groups, 16), s);
 }
