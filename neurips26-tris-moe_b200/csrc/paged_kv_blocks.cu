@@ -6,9 +6,12 @@
 // a decode step.
 //
 // Tokens that follow one another in a block are a run.  A CTA has the rows of some neighbouring tokens, whole runs, and some heads: a thread has the same 16 dimensions
-// of its row for one head after the other - two chunks of eight that rotate together - so that its cosines and sines are read once.  Two heads are rotated, their rows' largest
-// magnitudes meet in shared memory, and while they do the next two are on their way.  A run longer than a CTA's rows is read twice, the second time from L2.
-// (A warp for each run and head, which had the rows' cosines to read for every head, took 75 us for 4 prompts of 2047 tokens.)
+// of its row for one head after the other - two chunks of eight that rotate together - so that its cosines and sines are read once.  A head is rotated, its rows' largest
+// magnitudes meet in shared memory, and while they do the next head's are on their way.  A run longer than a CTA's rows is read twice, the second time from L2.
+//
+// 32/8 heads of 128 in bf16, blocks of 16 tokens, replayed: one token 5.0 us, 64 sequences' 5.5, a prompt of 512 tokens 6.8, of 2048 14, 4 of 2047 57 to 60 (165 MB, 2.8 TB/s:
+// some 40 instructions for every 16 bytes that are read hold the rest back).  Two heads at a time, 8.2 for one token and 59 for 4 of 2047; a warp for each run and head, which had the
+// rows' cosines to read for every head, 75.
 #include <float.h>
 
 #include "decode_step.cuh"
@@ -16,13 +19,12 @@
 namespace tris {
 namespace {
 
-constexpr int kHeads = 1;  // at a time
+constexpr int kWindow = 16;  // rows of a CTA
 
 struct BlockArgs {
   TrisPagedKv cache;
   TrisPagedAppend rows;
   int lanes;        // that have a row, 16 dimensions each: a power of two from 2 to 16
-  int window;       // rows of a CTA, up to 16
   int page_shift;   // log2(page_size), or -1
   int block_mask;   // scale_tokens - 1 where that is a power of two, or -1
   int page_scales;  // scales of a page and head
@@ -39,16 +41,17 @@ __device__ __forceinline__ float block_scale(float top) {
   return __uint_as_float(static_cast<uint32_t>(min(max(e, 127 - 64), 127 + 64)) << 23);
 }
 
-// grid (windows of tokens, shares of the heads), window * lanes threads, a multiple of 32.
+// grid (windows of tokens, shares of the heads), kWindow * L threads.
 // L: lanes that have a row, 16 dimensions each.
 template <typename T, Form F, int L>
-__global__ void __launch_bounds__(16 * L, L == 16 ? 3 : L == 8 ? 6 : 12) paged_kv_append_blocks_kernel(const __grid_constant__ BlockArgs a) {
-  __shared__ __align__(16) float tops[2][kHeads][16];  // largest magnitude of every row; two turns
+__global__ void __launch_bounds__(kWindow * L, L == 16 ? 3 : L == 8 ? 6 : 12) paged_kv_append_blocks_kernel(const __grid_constant__ BlockArgs a) {
+  __shared__ __align__(16) float tops[2][kWindow];  // largest magnitude of every row; two turns
   pdl_wait();
   pdl_launch_dependents();
   const TrisPagedAppend& r = a.rows;
   const TrisPagedKv& c = a.cache;
-  const int tid = threadIdx.x, lane = tid & 31, R = a.window, row = tid / L, u = tid % L;
+  const int tid = threadIdx.x, lane = tid & 31, row = tid / L, u = tid % L;
+  constexpr int R = kWindow;
   const int hq = r.num_q_heads, hkv = c.num_kv_heads, D = c.head_dim, rot = r.rotary_dim, half = rot / 2, block = c.scale_tokens;
   const int64_t room = min(static_cast<int64_t>(c.table_width) * c.page_size, static_cast<int64_t>(0x7FFFFFFF));  // positions are 32-bit numbers from here on
   const bool active = 16 * u < D;
@@ -64,7 +67,7 @@ __global__ void __launch_bounds__(16 * L, L == 16 ? 3 : L == 8 ? 6 : 12) paged_k
     const int64_t pos = position(t);
     return pos < 0 || pos >= room || in_block(static_cast<int>(pos)) == 0 || position(t - 1) != pos - 1 || r.sequences[t - 1] != r.sequences[t];
   };
-  auto beginnings = [&](int w) { return __ballot_sync(0xFFFFFFFFu, begins(w + lane)); };  // among 32 tokens, of which a window has up to 16
+  auto beginnings = [&](int w) { return __ballot_sync(0xFFFFFFFFu, begins(w + lane)); };  // among 32 tokens, of which a window has 16
 
   // What a thread knows of its row's token.
   int t = 0, pos = 0, page = 0;
@@ -123,11 +126,6 @@ __global__ void __launch_bounds__(16 * L, L == 16 ? 3 : L == 8 ? 6 : 12) paged_k
       raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
       raw[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
-  };
-  // The next heads' rows; behind the last head its own once more, so that no branch lies between the loads.
-  auto fetch_heads = [&](const T* p, int64_t stride, int left, uint4 (&raw)[kHeads][2]) {
-#pragma unroll
-    for (int k = 0; k < kHeads; ++k) fetch(p + min(k, left - 1) * stride, raw[k]);
   };
   auto rotate = [&](const T* p, float (&x)[8], float (&y)[8]) {
     if (!rot) return;
@@ -249,29 +247,22 @@ __global__ void __launch_bounds__(16 * L, L == 16 ? 3 : L == 8 ? 6 : 12) paged_k
     store_8(reinterpret_cast<__nv_fp8_e4m3*>(p + 8 * c1), y);
   };
 
-  const int share = blockIdx.y * kHeads, shares = gridDim.y * kHeads;
+  const int share = blockIdx.y, shares = gridDim.y;
   auto queries = [&](bool there) {
     if (share >= hq) return;
     Source src = source(0, share);
-    uint4 next[kHeads][2];
-    fetch_heads(src.row, src.stride, hq - share, next);
+    uint4 next[2];
+    fetch(src.row, next);
 #pragma unroll 1
-    for (int h0 = share; h0 < hq; h0 += shares) {
-      float x[kHeads][8], y[kHeads][8];
-#pragma unroll
-      for (int k = 0; k < kHeads; ++k) {
-        unpack_8<T>(next[k][0], x[k]);
-        unpack_8<T>(next[k][1], y[k]);
-      }
+    for (int h = share; h < hq; h += shares) {
+      float x[8], y[8];
+      unpack_8<T>(next[0], x);
+      unpack_8<T>(next[1], y);
       const T* now = src.row;
       src.row += shares * src.stride;
-      if (h0 + shares < hq) fetch_heads(src.row, src.stride, hq - h0 - shares, next);
-#pragma unroll
-      for (int k = 0; k < kHeads; ++k) {
-        if (h0 + k >= hq) break;
-        rotate(now + k * src.stride, x[k], y[k]);
-        if (there) put_row(r.q_out, hq, h0 + k, x[k], y[k]);
-      }
+      if (h + shares < hq) fetch(src.row, next);
+      rotate(now, x, y);
+      if (there) put_row(r.q_out, hq, h, x, y);
     }
   };
 
@@ -294,59 +285,47 @@ __global__ void __launch_bounds__(16 * L, L == 16 ? 3 : L == 8 ? 6 : 12) paged_k
       enter(min(w + row, r.num_tokens - 1), there);
       queries(there);
       const int ahead = in_block(pos) - (row - first);  // tokens of the block ahead of the run
-      const bool whole = first == 0 && last == R && R >= 4;  // four rows at a time
+      const bool whole = first == 0 && last == R;
       const int sharers = r.cos ? min(last - first, r.max_positions - (pos - (row - first))) : last - first;  // rows of the run that have a place
 #pragma unroll 1
       for (int kind = 1; kind <= 2 && share < hkv; ++kind) {
         Source src = source(kind, share);
         Place to = place_of(kind == 1, share);
         const int64_t own_row = in_block(pos) * to.token_stride;
-        uint4 next[kHeads][2];
-        fetch_heads(src.row, src.stride, hkv - share, next);
+        uint4 next[2];
+        fetch(src.row, next);
 #pragma unroll 1
-        for (int h0 = share; h0 < hkv; h0 += shares, turn ^= 1) {
-          float x[kHeads][8], y[kHeads][8], held[kHeads];
-          bool infinite = false;
-#pragma unroll
-          for (int k = 0; k < kHeads; ++k) {
-            unpack_8<T>(next[k][0], x[k]);
-            unpack_8<T>(next[k][1], y[k]);
-            const int within = min(k, hkv - 1 - h0);
-            if (kind == 1) rotate(src.row + within * src.stride, x[k], y[k]);
-            held[k] = placed && ahead > 0 ? to.scale[within] : 0.f;
-            const float top = row_top(x[k], y[k], false);
-            infinite |= placed && top == INFINITY;
-            if (u == 0) tops[turn][k][row] = placed ? top : 0.f;
-          }
+        for (int h = share; h < hkv; h += shares, turn ^= 1) {
+          float x[8], y[8];
+          unpack_8<T>(next[0], x);
+          unpack_8<T>(next[1], y);
+          if (kind == 1) rotate(src.row, x, y);
+          const float held = placed && ahead > 0 ? *to.scale : 0.f;
+          const float top = row_top(x, y, false);
+          if (u == 0) tops[turn][row] = placed ? top : 0.f;
           src.row += shares * src.stride;
-          if (h0 + shares < hkv) fetch_heads(src.row, src.stride, hkv - h0 - shares, next);
-          if (__syncthreads_or(infinite)) {  // rare: the largest of the finite ones alone
-#pragma unroll
-            for (int k = 0; k < kHeads; ++k) {
-              const float top = row_top(x[k], y[k], true);
-              if (u == 0) tops[turn][k][row] = placed ? top : 0.f;
-            }
+          if (h + shares < hkv) fetch(src.row, next);
+          if (__syncthreads_or(placed && top == INFINITY)) {  // rare: the largest of the finite ones alone
+            const float finite = row_top(x, y, true);
+            if (u == 0) tops[turn][row] = placed ? finite : 0.f;
             __syncthreads();
           }
+          float all = 0.f;
+          if (whole) {
 #pragma unroll
-          for (int k = 0; k < kHeads; ++k) {
-            if (h0 + k >= hkv) break;
-            float all = 0.f;
-            if (whole) {
-              for (int n = 0; n < R; n += 4) {
-                const float4 m = *reinterpret_cast<const float4*>(&tops[turn][k][n]);
-                all = fmaxf(fmaxf(fmaxf(all, m.x), fmaxf(m.y, m.z)), m.w);
-              }
-            } else {
-              for (int n = first; n < last; ++n) all = fmaxf(all, tops[turn][k][n]);
+            for (int n = 0; n < R; n += 4) {
+              const float4 m = *reinterpret_cast<const float4*>(&tops[turn][n]);
+              all = fmaxf(fmaxf(fmaxf(all, m.x), fmaxf(m.y, m.z)), m.w);
             }
-            if (kind == 1 && r.k_out && there) put_row(r.k_out, hkv, h0 + k, x[k], y[k]);
-            if (!placed || !active) continue;
-            uint8_t* rows = to.row + k * to.head_stride;
-            const float old = known(held[k]), scale = fmaxf(block_scale(all), old);
-            if (ahead > 0 && old < scale) bring_along(rows, to.token_stride, ahead, row - first, sharers, old / scale);
-            store_row(rows + own_row, scale, x[k], y[k]);
-            if (row == first && u == 0 && scale != held[k]) to.scale[k] = scale;
+          } else {
+            for (int n = first; n < last; ++n) all = fmaxf(all, tops[turn][n]);
+          }
+          if (kind == 1 && r.k_out && there) put_row(r.k_out, hkv, h, x, y);
+          if (placed && active) {
+            const float old = known(held), scale = fmaxf(block_scale(all), old);
+            if (ahead > 0 && old < scale) bring_along(to.row, to.token_stride, ahead, row - first, sharers, old / scale);
+            store_row(to.row + own_row, scale, x, y);
+            if (row == first && u == 0 && scale != held) *to.scale = scale;
           }
           to.row += shares * to.head_stride;
           to.scale += shares;
@@ -396,10 +375,10 @@ __global__ void __launch_bounds__(16 * L, L == 16 ? 3 : L == 8 ? 6 : 12) paged_k
           }
           if (pass == 1) break;
           enter(w, true);  // the run's first token, for all
-          if (u == 0) tops[turn][0][row] = most;
+          if (u == 0) tops[turn][row] = most;
           __syncthreads();
           float all = 0.f, held = 0.f;
-          for (int n = 0; n < R; ++n) all = fmaxf(all, tops[turn][0][n]);
+          for (int n = 0; n < R; ++n) all = fmaxf(all, tops[turn][n]);
           if (placed) {
             const int ahead = in_block(pos);
             const Place to = place_of(keys, head);
@@ -421,15 +400,15 @@ __global__ void __launch_bounds__(16 * L, L == 16 ? 3 : L == 8 ? 6 : 12) paged_k
 template <typename T, Form F>
 int launch_blocks(const BlockArgs& a, cudaStream_t stream) {
   const int heads = a.rows.num_q_heads > a.cache.num_kv_heads ? a.rows.num_q_heads : a.cache.num_kv_heads;
-  // CTAs that share a window's heads: all of them where there are few windows, else until a thread has kWalk heads of queries, keys and values each
+  // CTAs that share a window's heads: one for each head where there are few windows, else until a thread has kWalk heads of queries, keys and values each.  us, the first and the
+  // second: one token 5.0 and 5.6, 512 tokens 6.8 and 7.1, 1024 10.0 and 8.4, 8188 77 and 60.  (A walk of 2 heads 62 for 8188, of 8 heads 64.)
   constexpr int kWalk = 4;
-  const int64_t windows = (static_cast<int64_t>(a.rows.num_tokens) + a.window - 1) / a.window;
-  const int most = ceil_div(heads, kHeads), few = ceil_div(heads, kWalk);
-  const int shares = windows * most <= 16 * static_cast<int64_t>(sm_count()) ? most : few;
+  const int64_t windows = (static_cast<int64_t>(a.rows.num_tokens) + kWindow - 1) / kWindow;
+  const int shares = windows * heads <= 8 * static_cast<int64_t>(sm_count()) ? heads : ceil_div(heads, kWalk);
   TRIS_REQUIRE(shares <= 65535, TRIS_ERR_UNSUPPORTED, "paged_kv_append: too many heads");
   auto kernel = a.lanes == 2 ? paged_kv_append_blocks_kernel<T, F, 2> : a.lanes == 4 ? paged_kv_append_blocks_kernel<T, F, 4> : a.lanes == 8 ? paged_kv_append_blocks_kernel<T, F, 8>
                                                                                                                                               : paged_kv_append_blocks_kernel<T, F, 16>;
-  TRIS_CUDA(launch_step(kernel, dim3(static_cast<unsigned>(windows), shares), dim3(a.window * a.lanes), 0, stream, programmatic_launch_default(), 1, a));
+  TRIS_CUDA(launch_step(kernel, dim3(static_cast<unsigned>(windows), shares), dim3(kWindow * a.lanes), 0, stream, programmatic_launch_default(), 1, a));
   return TRIS_OK;
 }
 
@@ -460,9 +439,6 @@ int append_block_scaled(const TrisPagedKv& c, const TrisPagedAppend& r, int rota
   for (int i = 0; i < 3; ++i)
     if (src[i]) wide = wide && aligned_to(src[i], 16) && strides[i][0] % 8 == 0 && strides[i][1] % 8 == 0;
   const Form form = wide && rotary_dim % (r.interleaved ? 8 : 16) == 0 ? (r.interleaved ? Form::kPairs : Form::kHalves) : Form::kAny;
-  // a warp's rows to a CTA where there are few tokens (a decode step), else 16
-  const int64_t items = r.num_q_heads + 2 * c.num_kv_heads;
-  a.window = r.num_tokens * items <= 64 * static_cast<int64_t>(sm_count()) ? 32 / a.lanes : 16;
   return r.dtype == TRIS_DTYPE_F16 ? launch_blocks<__half>(a, form, stream) : launch_blocks<__nv_bfloat16>(a, form, stream);
 }
 

@@ -2,6 +2,7 @@
 //
 // s = max |x| / 448 of a group, and x / s, both rounded as divisions round them.  Bound by bytes (2 read and 1 written an element), by latency for a few
 // rows.  A half-warp has 128 columns of a row, eight a lane; for blocks a CTA has all of one in its registers, so that x is read once.
+// Replayed, bf16: rows of 4096, 64 of them 1.7 us, 1024 4.8, 8192 27 (101 MB, 3.7 TB/s); blocks of 14336 x 4096 30 to 35 us (176 MB, 5.0 to 5.9 TB/s).
 #include "decode_step.cuh"
 
 namespace tris {
@@ -49,37 +50,27 @@ __device__ __forceinline__ uint32_t top_of(const uint4& raw) {
   return __float_as_uint(Pair<T>::unpack(top).x);
 }
 
-// A half-warp has a group of one row, and UNITS of them on their way.
-template <typename T, int UNITS>
+// A half-warp has a group of one row.  (Four of them, for more loads on their way: 64 rows of 4096 3.2 us, 8192 27.5.)
+template <typename T>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const __grid_constant__ QuantizeArgs a) {
   pdl_wait();
   pdl_launch_dependents();
   const int l = threadIdx.x % kLanes;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / kLanes), first = blockIdx.x * static_cast<int64_t>(kThreads / kLanes) + threadIdx.x / kLanes;
-  uint4 raw[UNITS];
+  const int64_t unit = blockIdx.x * static_cast<int64_t>(kThreads / kLanes) + threadIdx.x / kLanes, here = min(unit, a.units - 1), row = here / a.groups;
+  const int group = static_cast<int>(here - row * a.groups);
+  const uint4 raw = fetch_8<T>(a, row, group * kGroup + 8 * l);
+  uint32_t top = top_of<T>(raw);
 #pragma unroll
-  for (int i = 0; i < UNITS; ++i) {
-    const int64_t unit = min(first + i * step, a.units - 1), row = unit / a.groups;
-    raw[i] = fetch_8<T>(a, row, static_cast<int>(unit - row * a.groups) * kGroup + 8 * l);
-  }
-#pragma unroll
-  for (int i = 0; i < UNITS; ++i) {
-    const int64_t unit = first + i * step, row = unit / a.groups;
-    const int group = static_cast<int>(unit - row * a.groups);
-    uint32_t top = top_of<T>(raw[i]);
-#pragma unroll
-    for (int d = 1; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    float v[8];
-    unpack_8<T>(raw[i], v);
-    const float scale = quantize_8(v, top);
-    if (unit < a.units) {
-      put_8(a, row, group * kGroup + 8 * l, v);
-      if (l == 0) a.q.scales[row * a.q.scales_stride + group] = scale;
-    }
-  }
+  for (int d = 1; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+  float v[8];
+  unpack_8<T>(raw, v);
+  const float scale = quantize_8(v, top);
+  if (unit >= a.units) return;
+  put_8(a, row, group * kGroup + 8 * l, v);
+  if (l == 0) a.q.scales[row * a.q.scales_stride + group] = scale;
 }
 
-// A CTA has a block of 128 x 128.
+// A CTA has a block of 128 x 128.  (Five CTAs an SM 29.8 us for 14336 x 4096; four 31.8, six 32.5, eight, which leave too few registers, 40.8.)
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 5) quantize_blocks_kernel(const __grid_constant__ QuantizeArgs a) {
   __shared__ uint32_t tops[kThreads / 32];
@@ -120,13 +111,8 @@ int launch_quantize(const QuantizeArgs& a, cudaStream_t stream) {
     TRIS_CUDA(launch_step(quantize_blocks_kernel<T>, dim3(a.groups, ceil_div(a.q.rows, kGroup)), dim3(kThreads), 0, stream, pdl, 1, a));
     return TRIS_OK;
   }
-  // four groups to a half-warp where there are enough for all SMs, one where there are few
-  constexpr int kMany = 4, kPerCta = kThreads / kLanes;
-  if (a.units >= static_cast<int64_t>(kMany) * kPerCta * 8 * sm_count()) {
-    TRIS_CUDA(launch_step(quantize_rows_kernel<T, kMany>, dim3(static_cast<unsigned>((a.units + kMany * kPerCta - 1) / (kMany * kPerCta))), dim3(kThreads), 0, stream, pdl, 1, a));
-  } else {
-    TRIS_CUDA(launch_step(quantize_rows_kernel<T, 1>, dim3(static_cast<unsigned>((a.units + kPerCta - 1) / kPerCta)), dim3(kThreads), 0, stream, pdl, 1, a));
-  }
+  constexpr int kPerCta = kThreads / kLanes;
+  TRIS_CUDA(launch_step(quantize_rows_kernel<T>, dim3(static_cast<unsigned>((a.units + kPerCta - 1) / kPerCta)), dim3(kThreads), 0, stream, pdl, 1, a));
   return TRIS_OK;
 }
 
