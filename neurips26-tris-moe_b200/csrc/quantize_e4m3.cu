@@ -1,8 +1,8 @@
 // Rows and weights to e4m3, with a scale for each 128 columns of a row or for each block of 128 x 128.
 //
 // s = max |x| / 448 of a group, and x / s, both rounded as divisions round them.  Bound by bytes (2 read and 1 written an element), by latency for a few
-// rows.  A half-warp has 128 columns of a row, eight a lane; for blocks a CTA has all of one in its registers, so that x is read once.
-// Replayed, bf16: rows of 4096, 64 of them 1.7 us, 1024 4.8, 8192 27 (101 MB, 3.7 TB/s); blocks of 14336 x 4096 30 to 35 us (176 MB, 5.0 to 5.9 TB/s).
+// rows.  A quarter-warp has 128 columns of a row; for blocks a CTA has all of one in its registers, so that x is read once.
+// Replayed, bf16: rows of 4096, 64 of them 1.8 us, 1024 3.6, 8192 18.5 (101 MB, 5.5 TB/s); blocks of 14336 x 4096 30 to 35 us (176 MB, 5.0 to 5.9 TB/s).
 #include "decode_step.cuh"
 
 namespace tris {
@@ -10,6 +10,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kGroup = 128, kLanes = kGroup / 8;  // columns of a scale, and lanes that have them
+constexpr int kRowLanes = 8;  // of a group of one row
 
 struct QuantizeArgs {
   TrisQuantizeE4m3 q;
@@ -50,23 +51,33 @@ __device__ __forceinline__ uint32_t top_of(const uint4& raw) {
   return __float_as_uint(Pair<T>::unpack(top).x);
 }
 
-// A half-warp has a group of one row.  (Four of them, for more loads on their way: 64 rows of 4096 3.2 us, 8192 27.5.)
+// A quarter-warp has a group of one row, a lane two vectors of it.  (us for 64 and for 8192 rows of 4096: 16 lanes to a group 1.6 and 24.0, eight 1.8 and 18.5, four 2.2 and 17.3; four
+// groups of sixteen lanes each, one after the other, 3.2 and 27.5.)
 template <typename T>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const __grid_constant__ QuantizeArgs a) {
   pdl_wait();
   pdl_launch_dependents();
-  const int l = threadIdx.x % kLanes;
-  const int64_t unit = blockIdx.x * static_cast<int64_t>(kThreads / kLanes) + threadIdx.x / kLanes, here = min(unit, a.units - 1), row = here / a.groups;
+  const int l = threadIdx.x % kRowLanes;
+  const int64_t unit = blockIdx.x * static_cast<int64_t>(kThreads / kRowLanes) + threadIdx.x / kRowLanes, here = min(unit, a.units - 1), row = here / a.groups;
   const int group = static_cast<int>(here - row * a.groups);
-  const uint4 raw = fetch_8<T>(a, row, group * kGroup + 8 * l);
-  uint32_t top = top_of<T>(raw);
+  constexpr int kSteps = kLanes / kRowLanes;
+  uint4 raw[kSteps];
 #pragma unroll
-  for (int d = 1; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-  float v[8];
-  unpack_8<T>(raw, v);
-  const float scale = quantize_8(v, top);
+  for (int i = 0; i < kSteps; ++i) raw[i] = fetch_8<T>(a, row, group * kGroup + 8 * (i * kRowLanes + l));
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) top = max(top, top_of<T>(raw[i]));
+#pragma unroll
+  for (int d = 1; d < kRowLanes; d <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
   if (unit >= a.units) return;
-  put_8(a, row, group * kGroup + 8 * l, v);
+  float scale = 0.f;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    float v[8];
+    unpack_8<T>(raw[i], v);
+    scale = quantize_8(v, top);
+    put_8(a, row, group * kGroup + 8 * (i * kRowLanes + l), v);
+  }
   if (l == 0) a.q.scales[row * a.q.scales_stride + group] = scale;
 }
 
@@ -111,7 +122,7 @@ int launch_quantize(const QuantizeArgs& a, cudaStream_t stream) {
     TRIS_CUDA(launch_step(quantize_blocks_kernel<T>, dim3(a.groups, ceil_div(a.q.rows, kGroup)), dim3(kThreads), 0, stream, pdl, 1, a));
     return TRIS_OK;
   }
-  constexpr int kPerCta = kThreads / kLanes;
+  constexpr int kPerCta = kThreads / kRowLanes;
   TRIS_CUDA(launch_step(quantize_rows_kernel<T>, dim3(static_cast<unsigned>((a.units + kPerCta - 1) / kPerCta)), dim3(kThreads), 0, stream, pdl, 1, a));
   return TRIS_OK;
 }
