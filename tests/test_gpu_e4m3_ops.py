@@ -78,6 +78,20 @@ def test_bias_and_leading_dimensions(lib, rows, outputs, inputs, bias):
     _close(y[0], *_product_64(x, xs, w, ws, b), inputs)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32], ids=str)
+@pytest.mark.parametrize("rows,outputs,inputs", [(5, 40, 9000), (17, 5, 1030), (33, 140, 16384), (64, 513, 14336), (65, 130, 4096), (100, 257, 5000), (128, 1, 4224), (129, 300, 14336), (200, 129, 8300)])
+def test_products_cut_among_blocks(lib, rows, outputs, inputs, dtype):
+    """Few tiles and many groups: a cluster's blocks have some groups each and join a share of the columns, some of which do not exist."""
+    import trismoe_b200 as tm
+
+    x, xs, w, ws = _operands(rows, outputs, inputs, seed=21)
+    b = torch.randn((outputs,), generator=_gen(22), device="cuda") * 100
+    y = tm.linear_e4m3(x, xs, w, ws, b, dtype=dtype)
+    _close(y, *_product_64(x, xs, w, ws, b), inputs)
+    for _ in range(3):
+        assert torch.equal(tm.linear_e4m3(x, xs, w, ws, b, dtype=dtype).view(torch.uint8), y.view(torch.uint8))
+
+
 @pytest.mark.parametrize("rows", [3, 90, 400])
 def test_rows_and_scales_that_are_parts_of_larger_ones(lib, rows):
     """Any stride: rows 16 bytes apart from one another's ends, scales that start anywhere."""
