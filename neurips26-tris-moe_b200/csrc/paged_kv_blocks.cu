@@ -5,7 +5,7 @@
 // (but for what becomes smaller than e4m3 can be), however often it happens.  Bound by bytes for prompts, by the chain position -> page -> scale -> store for
 // a decode step.
 //
-// Tokens that follow one another in a block are a run.  A CTA has the rows of some neighbouring tokens, whole runs, and some heads: a thread has the same 16 dimensions
+// Tokens that follow one another in a block are a run.  A CTA has the rows of some neighbouring tokens, whole runs that begin among its 16 tokens, and some heads: a thread has the same 16 dimensions
 // of its row for one head after the other - two chunks of eight that rotate together - so that its cosines and sines are read once.  A head is rotated, its rows' largest
 // magnitudes meet in shared memory, and while they do the next head's are on their way.  A run longer than a CTA's rows is read twice, the second time from L2.
 //
@@ -14,6 +14,7 @@
 // rows' cosines to read for every head, 75.
 #include <float.h>
 
+#include "block_runs.cuh"
 #include "decode_step.cuh"
 
 namespace tris {
@@ -268,18 +269,15 @@ __global__ void __launch_bounds__(kWindow * L, L == 16 ? 3 : L == 8 ? 6 : 12) pa
 
   const int end = min((static_cast<int>(blockIdx.x) + 1) * R, r.num_tokens);
   int w = blockIdx.x * R, turn = 0;
-  const uint32_t rows = (1u << R) - 1;
   uint32_t starts = beginnings(w);
-  if (!(starts & rows)) return;  // all of these tokens belong to a run that begins ahead of them
-  w += __ffs(starts) - 1;
-  starts >>= __ffs(starts) - 1;
+  if (!(starts & ((1u << R) - 1))) return;  // all of these tokens belong to a run that begins ahead of them
+  w += lowest_bit(starts);
+  starts >>= lowest_bit(starts);
 #pragma unroll 1
   while (w < end) {
-    // the rows of whole runs that a window holds
-    const uint32_t behind = starts & rows & ~1u;
-    const int count = (starts >> R) & 1 ? R : behind ? 31 - __clz(behind) : 0;
+    const int count = tokens_of_whole_runs(starts, end - w, R);
     if (count) {
-      const int first = 31 - __clz(starts & ((2u << row) - 1));  // of this row's run
+      const int first = highest_bit(starts & ((2u << row) - 1));  // of this row's run
       const int last = min(row + __ffs(starts >> (row + 1)), count);  // behind it; a run begins at row `count`
       const bool there = row < count && w + row < r.num_tokens;
       enter(min(w + row, r.num_tokens - 1), there);
