@@ -140,7 +140,7 @@ class TrisDecoder(torch.nn.Module):
         """``x`` as the weight takes it: rows in fp16 or, in 8 bits, those or values with their scales."""
         if not self.linear8:
             return F.linear(x, weight).to(dtype)
-        return linear_e4m3(*(x if isinstance(x, tuple) else quantize_e4m3(x)), *weight, dtype=dtype)
+        return linear_e4m3(*(x if isinstance(x, tuple) else quantize_e4m3(x)), *weight, dtype=dtype, status=self.cache_status)
 
     def _norm(self, x: torch.Tensor, h: Optional[torch.Tensor], weight: torch.Tensor):
         """The residual norm ahead of a product: its rows as ``_linear`` takes them, and the new residual."""
@@ -191,7 +191,8 @@ class TrisDecoder(torch.nn.Module):
         return self._linear(last, self.lm_head, torch.float32)
 
     def raise_on_kernel_status(self) -> None:
-        """Raises if a paged operator met a page, position or length that does not fit (waits for the GPU)."""
+        """Raises if a paged operator met a page, position or length that does not fit, or a product in 8 bits gave up a wait: its logits are NaN then, and a token
+        drawn from them is 0 (waits for the GPU)."""
         if self.page_size:
             raise_on_status(self.cache_status)
 
