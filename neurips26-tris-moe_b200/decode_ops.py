@@ -15,7 +15,8 @@ rows' type (fp16 or bf16) or ``torch.float8_e4m3fn`` with one scale per head or,
 fp32, one for each of ``blocks`` equal parts of a page and head: these belong to the cache, are written by ``append_paged_kv``, and need no
 calibration.  Token ``i`` of sequence ``b`` is in page
 ``block_table[b, i // page_size]``.  ``status`` is an optional int32 tensor of one element, zero
-at first: a page, position or length that does not fit sets it (``raise_on_status``).
+at first: a page, position or length that does not fit sets it, as does a product of ``e4m3_ops`` that gives up a wait
+(``raise_on_status``).
 """
 from __future__ import annotations
 
@@ -126,12 +127,19 @@ def _cache(what: str, k_pages, v_pages, block_table, k_scale, v_scale, status) -
     return packed, (dtype, heads, dim, sequences, width, page_size)
 
 
-def raise_on_status(status: torch.Tensor, what: str = "paged cache") -> None:
+# what a status word says: whose it is, unless the caller says so, and what has happened
+_REPORTS = {
+    4: ("paged cache", "a page, position or length outside the cache, its block table or the rotation tables"),
+    6: ("product in 8 bits", "a wait ran out: what that call returned is NaN in part"),
+}
+
+
+def raise_on_status(status: torch.Tensor, what: Optional[str] = None) -> None:
     """Reads a status word (waits for the GPU), and raises if an operator has set it."""
     word = int(status.item())
     if word:
-        raise RuntimeError(f"trismoe_b200 {what}: a kernel reported {_native.STATUS_NAMES.get(word, word)} "
-                           "(a page, position or length outside the cache, its block table or the rotation tables)")
+        whose, why = _REPORTS.get(word, ("status word", "no status of these operators"))
+        raise RuntimeError(f"trismoe_b200 {what or whose}: a kernel reported {_native.STATUS_NAMES.get(word, word)} ({why})")
 
 
 def append_paged_kv(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
