@@ -209,7 +209,7 @@ class TrisDecoder(torch.nn.Module):
             y, _ = blk(_rms_norm(h, layer["ln2"], self.shape.rms_eps))
             h = h + y
         last = _rms_norm(h[:, -1], self.final_norm, self.shape.rms_eps)
-        return F.linear(last, self.lm_head).float()
+        return self._linear(last, self.lm_head, torch.float32)
 
 
 def run_exact_generation(model: TrisDecoder, input_ids: torch.Tensor, output_length: int, use_graph: bool = True,
