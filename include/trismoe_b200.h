@@ -774,7 +774,9 @@ typedef struct TrisPagedKv {
  * [max_positions, rotary_dim / 2] - pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved - in fp32 and rounded once.
  * Scales of blocks: a block's scale is the smallest power of two by which its finite values stay within 448.  A token at the block's first place begins it anew;
  * one behind makes the scale larger where it has to, and the tokens ahead of it are brought to the new scale (exact, but for what falls below
- * the smallest number of e4m3).  The tokens of one block follow one another in the call, in the order of their positions.
+ * the smallest number of e4m3).  The tokens of one block are one stretch of the call: neighbours at rising positions without a gap, and no other token between them,
+ * padding included.  A stretch right behind another one of its block, or inside a block with nothing but padding in between, is not written and sets status_dev
+ * (TRIS_ERR_CORRUPT); one behind another sequence's tokens is not looked for.
  */
 typedef struct TrisPagedAppend {
   const void* q;                    /* NULL (with num_q_heads 0): keys and values only     */

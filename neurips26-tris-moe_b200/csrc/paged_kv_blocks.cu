@@ -9,7 +9,7 @@
 // of its row for one head after the other - two chunks of eight that rotate together - so that its cosines and sines are read once.  A head is rotated, its rows' largest
 // magnitudes meet in shared memory, and while they do the next head's are on their way.  A run longer than a CTA's rows is read twice, the second time from L2.
 //
-// 32/8 heads of 128 in bf16, blocks of 16 tokens, replayed: one token 5.0 us, 64 sequences' 5.5, a prompt of 512 tokens 6.8, of 2048 14, 4 of 2047 57 to 60 (165 MB, 2.8 TB/s:
+// 32/8 heads of 128 in bf16, blocks of 16 tokens, replayed: one token 5.3 us, 64 sequences' 5.7, a prompt of 512 tokens 6.9, of 2048 14, 4 of 2047 55 to 60 (165 MB, 2.8 TB/s:
 // some 40 instructions for every 16 bytes that are read hold the rest back).  Two heads at a time, 8.2 for one token and 59 for 4 of 2047; a warp for each run and head, which had the
 // rows' cosines to read for every head, 75.
 #include <float.h>
@@ -62,19 +62,47 @@ __global__ void __launch_bounds__(kWindow * L, L == 16 ? 3 : L == 8 ? 6 : 12) pa
 
   auto position = [&](int t) -> int64_t { return r.positions_are_64bit ? reinterpret_cast<const int64_t*>(r.positions)[t] : reinterpret_cast<const int32_t*>(r.positions)[t]; };
   auto in_block = [&](int pos) { return a.block_mask >= 0 ? pos & a.block_mask : pos % block; };  // pages are whole blocks
-  // Whether token t begins a run: it does not go on, inside a block, where the token before it in the call is.
-  auto begins = [&](int t) {
-    if (t >= r.num_tokens || t == 0 || !r.sequences) return true;
-    const int64_t pos = position(t);
-    return pos < 0 || pos >= room || in_block(static_cast<int>(pos)) == 0 || position(t - 1) != pos - 1 || r.sequences[t - 1] != r.sequences[t];
+  auto outside = [&](int64_t pos) { return pos < 0 || pos >= room; };
+  // Which of 32 tokens, of which a window has 16, begin runs: those that do not go on, inside a block, where the token before them in the call is.  And which of these are refused, as
+  // the call's tokens ahead of them, padding aside, are in the same block: two runs of one block would both bring it to a new scale.
+  uint32_t refused = 0;
+  auto beginnings = [&](int w) {
+    const int t = w + lane;
+    bool begins = true, again = false, hidden = false;
+    if (t < r.num_tokens && t > 0 && r.sequences) {
+      const int64_t pos = position(t), before = position(t - 1);
+      const bool same = r.sequences[t - 1] == r.sequences[t];
+      if (!outside(pos)) {
+        const int at = in_block(static_cast<int>(pos));
+        begins = at == 0 || before != pos - 1 || !same;
+        hidden = at && outside(before);
+        again = begins && same && !outside(before) && before - in_block(static_cast<int>(before)) == pos - at;
+      }
+    }
+#pragma unroll 1
+    for (uint32_t ask = __ballot_sync(0xFFFFFFFFu, hidden); ask; ask &= ask - 1) {  // a token inside a block behind padding: what is ahead of that
+      const int token = w + lowest_bit(ask);
+      const int64_t pos = position(token);
+#pragma unroll 1
+      for (int t0 = token - 2;; t0 -= 32) {
+        const int64_t before = t0 - lane >= 0 ? position(t0 - lane) : 0;
+        const uint32_t found = __ballot_sync(0xFFFFFFFFu, t0 - lane < 0 || !outside(before));
+        if (!found) continue;
+        const bool it = lane == lowest_bit(found) && t0 - lane >= 0;
+        const bool here = it && r.sequences[t0 - lane] == r.sequences[token] && before - in_block(static_cast<int>(before)) == pos - in_block(static_cast<int>(pos));
+        if (__any_sync(0xFFFFFFFFu, here) && w + lane == token) again = true;
+        break;
+      }
+    }
+    refused = __ballot_sync(0xFFFFFFFFu, again);
+    return __ballot_sync(0xFFFFFFFFu, begins);
   };
-  auto beginnings = [&](int w) { return __ballot_sync(0xFFFFFFFFu, begins(w + lane)); };  // among 32 tokens, of which a window has 16
 
   // What a thread knows of its row's token.
   int t = 0, pos = 0, page = 0;
   bool placed = false, turns = false;  // whether it goes to the cache, and out as something else than zeros
   float cs[8], sn[8];
-  auto enter = [&](int token, bool there) {
+  auto enter = [&](int token, bool there, bool again) {
     t = token;
     placed = turns = false;
 #pragma unroll
@@ -101,7 +129,7 @@ __global__ void __launch_bounds__(kWindow * L, L == 16 ? 3 : L == 8 ? 6 : 12) pa
       page = c.block_table[seq * c.table_stride + (a.page_shift >= 0 ? pos >> a.page_shift : pos / c.page_size)];
       fits = page >= 0 && page < c.num_pages;
     }
-    placed = fits && turns;
+    placed = fits && turns && !again;
     if (!placed && c.status_dev) *c.status_dev = TRIS_ERR_CORRUPT;
   };
 
@@ -272,6 +300,7 @@ __global__ void __launch_bounds__(kWindow * L, L == 16 ? 3 : L == 8 ? 6 : 12) pa
   uint32_t starts = beginnings(w);
   if (!(starts & ((1u << R) - 1))) return;  // all of these tokens belong to a run that begins ahead of them
   w += lowest_bit(starts);
+  refused >>= lowest_bit(starts);
   starts >>= lowest_bit(starts);
 #pragma unroll 1
   while (w < end) {
@@ -280,7 +309,7 @@ __global__ void __launch_bounds__(kWindow * L, L == 16 ? 3 : L == 8 ? 6 : 12) pa
       const int first = highest_bit(starts & ((2u << row) - 1));  // of this row's run
       const int last = min(row + __ffs(starts >> (row + 1)), count);  // behind it; a run begins at row `count`
       const bool there = row < count && w + row < r.num_tokens;
-      enter(min(w + row, r.num_tokens - 1), there);
+      enter(min(w + row, r.num_tokens - 1), there, (refused >> first) & 1);
       queries(there);
       const int ahead = in_block(pos) - (row - first);  // tokens of the block ahead of the run
       const bool whole = first == 0 && last == R;
@@ -332,6 +361,7 @@ __global__ void __launch_bounds__(kWindow * L, L == 16 ? 3 : L == 8 ? 6 : 12) pa
       w += count;
     } else {
       // one run, longer than a window: its length first
+      const bool again = refused & 1;
       int length = R;
       for (;;) {
         const uint32_t more = beginnings(w + length);
@@ -339,7 +369,7 @@ __global__ void __launch_bounds__(kWindow * L, L == 16 ? 3 : L == 8 ? 6 : 12) pa
         if (more) break;
       }
       for (int at = 0; at < length; at += R) {
-        enter(w + min(at + row, length - 1), at + row < length);
+        enter(w + min(at + row, length - 1), at + row < length, again);
         queries(at + row < length);
       }
 #pragma unroll 1
@@ -352,7 +382,7 @@ __global__ void __launch_bounds__(kWindow * L, L == 16 ? 3 : L == 8 ? 6 : 12) pa
 #pragma unroll 1
           for (int at = 0; at < length; at += R) {
             const bool there = at + row < length;
-            enter(w + min(at + row, length - 1), there);
+            enter(w + min(at + row, length - 1), there, again);
             uint4 raw[2];
             float x[8], y[8];
             const T* from = source(keys ? 1 : 2, head).row;
@@ -372,7 +402,7 @@ __global__ void __launch_bounds__(kWindow * L, L == 16 ? 3 : L == 8 ? 6 : 12) pa
             }
           }
           if (pass == 1) break;
-          enter(w, true);  // the run's first token, for all
+          enter(w, true, again);  // the run's first token, for all
           if (u == 0) tops[turn][row] = most;
           __syncthreads();
           float all = 0.f, held = 0.f;

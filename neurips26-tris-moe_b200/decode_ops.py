@@ -155,8 +155,9 @@ def append_paged_kv(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     dimensions, pairs ``(i, i + rotary_dim / 2)`` or, ``interleaved``, ``(2 i, 2 i + 1)``; None: no rotation.  e4m3 pages get
     ``x / scale``, saturated.  Tokens of one call must have different places.  Scales of blocks are written, too: the smallest power of two (2^-64 to 2^64) by which the
     finite numbers of a block stay within 448.  A token at its block's first place begins it anew; one behind makes the scale larger where it has to, and
-    the block's tokens ahead of it are brought to that (exact, but for what falls below e4m3's smallest number).  In one call the tokens of a block follow one
-    another in the order of their positions.  Returns the rotated queries (None without ``q``),
+    the block's tokens ahead of it are brought to that (exact, but for what falls below e4m3's smallest number).  In one call the tokens of a block are
+    one stretch: neighbours at rising positions without a gap, and no other token between them, padding included.  A stretch right behind another one of its block, or inside a
+    block with nothing but padding in between, is not written and sets ``status``; one behind another sequence's tokens is not looked for.  Returns the rotated queries (None without ``q``),
     with ``return_key`` a pair with the rotated keys."""
     what = "append_paged_kv"
     dev = _same_device(what, k, v, q, k_pages, v_pages, block_table, positions, sequences, cos, sin, k_scale, v_scale, status)
