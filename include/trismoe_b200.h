@@ -8,6 +8,7 @@
  * workspaces and derived indexes are caller-owned buffers.  Nothing here falls back to
  * the CPU; a launch that cannot run returns a non-zero status and `tris_last_error()`
  * holds the reason for the calling thread.
+ * Structs are cleared before their fields are set: reserved fields are 0, and one may get a meaning later (TrisPagedKv.scale_tokens was reserved0).
  *
  * Reference interfaces these entry points stand in for are cited per declaration as
  * path:line inside the TriS-MoE source tree
@@ -763,7 +764,7 @@ typedef struct TrisPagedKv {
   int32_t num_kv_heads;
   int32_t head_dim;
   int32_t dtype;                    /* F16, BF16 (that of the rows) or E4M3                */
-  int32_t scale_tokens;             /* 0: a scale for each head; else tokens of a block, of which page_size is a multiple */
+  int32_t scale_tokens;             /* 0: a scale for each head; else tokens of a block, of which page_size is a multiple (reserved0 once: callers that left it unset have to clear it) */
   int32_t* status_dev;
 } TrisPagedKv;
 
