@@ -451,6 +451,7 @@ int launch_blocks(const BlockArgs& a, Form form, cudaStream_t stream) {
 int append_block_scaled(const TrisPagedKv& c, const TrisPagedAppend& r, int rotary_dim, cudaStream_t stream) {
   TRIS_REQUIRE(r.sequences || r.num_tokens <= c.num_sequences, TRIS_ERR_INVALID_ARG, "paged_kv_append: %d tokens without sequences for a block table of %d", r.num_tokens, c.num_sequences);
   TRIS_REQUIRE(r.num_tokens <= 1 << 30, TRIS_ERR_UNSUPPORTED, "paged_kv_append: too many tokens in one call");
+  TRIS_REQUIRE(c.k_scale != c.v_scale || c.num_pages == 0, TRIS_ERR_INVALID_ARG, "paged_kv_append: keys and values with the same scales of blocks");
   BlockArgs a{c, r};
   a.rows.rotary_dim = rotary_dim;
   a.page_shift = a.block_mask = -1;

@@ -6,6 +6,7 @@ import subprocess
 
 import pytest
 
+from test_decode_ops_checks import A, _cache, _call
 from test_kernel_sources import CSRC
 
 WINDOW = 16
@@ -84,3 +85,16 @@ def test_the_kernel_asks_the_rule():
     """The window that the kernel looks at is the one that is tried here."""
     text = open(os.path.join(CSRC, "paged_kv_blocks.cu")).read()
     assert f"kWindow = {WINDOW};" in text and text.count("tokens_of_whole_runs(starts, end - w, R)") == 1
+
+
+def test_keys_and_values_need_scales_of_their_own(lib):
+    """An append writes both; attention may read the same ones."""
+    import trismoe_b200 as tm
+
+    n = tm._native
+    base = dict(dtype=3, k_page_stride=4096, v_page_stride=4096, scale_tokens=4)
+    args = n.TrisPagedAppend(k=A, v=A, positions=A, num_tokens=1)
+    st, message = _call(lib, "tris_paged_kv_append", _cache(tm, **base, k_scale=A, v_scale=A), args)
+    assert st == 1 and "the same scales" in message, message
+    st, message = _call(lib, "tris_paged_kv_append", _cache(tm, **base, num_pages=0), n.TrisPagedAppend(k=A, v=A, positions=A, num_tokens=3))
+    assert st == 1 and "without sequences" in message, message  # a cache without pages has none of either
