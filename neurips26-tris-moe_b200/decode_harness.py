@@ -236,8 +236,8 @@ def run_exact_generation(model: TrisDecoder, input_ids: torch.Tensor, output_len
     random = None
     if sampling is not None:
         sampling = dict(sampling)
-        random = sampling.pop("random")
-        if random.shape != (output_length, B) or random.dtype is not torch.float32:
+        random = sampling.pop("random", None)
+        if random is None or random.shape != (output_length, B) or random.dtype is not torch.float32:
             raise RuntimeError(f"trismoe_b200 decode harness: sampling needs random numbers, fp32 [{output_length}, {B}]")
 
     def pick(logits):

@@ -1,6 +1,7 @@
 """CPU tests of what the decode harness hands to its operators."""
 import types
 
+import pytest
 import torch
 
 
@@ -31,3 +32,13 @@ def test_a_decoder_without_layers_has_its_logits_in_8_bits(monkeypatch):
     want, got = plain(ids, positions), eight(ids, positions)
     assert got.dtype is want.dtype is torch.float32 and got.shape == (2, 32)
     assert float((got - want).abs().max()) <= 2.0 ** -10 * float(want.abs().max())  # the plain logits are rounded to 16 bits
+
+
+@pytest.mark.parametrize("sampling", [{}, {"random": None}, {"random": torch.zeros(4, 3)}, {"random": torch.zeros(5, 2, dtype=torch.float64)}], ids=["none", "None", "shape", "type"])
+def test_sampling_without_its_random_numbers_is_refused(sampling):
+    """Before the prompt runs, in the harness's own words."""
+    from trismoe_b200 import decode_harness as dh
+
+    model = types.SimpleNamespace(max_length=20, max_batch=4)
+    with pytest.raises(RuntimeError, match=r"random numbers, fp32 \[5, 2\]"):
+        dh.run_exact_generation(model, torch.zeros((2, 3), dtype=torch.long), 5, sampling=sampling)
