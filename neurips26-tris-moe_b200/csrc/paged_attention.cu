@@ -8,7 +8,7 @@
 // steps of a warp take 21 500, nine tenths of the rate of a copy, the reads ahead of them, which depend on one another, 6 600, and the joins 9 700.
 // Scales of blocks (SB) cost a step two more loads; a key's scale is multiplied into its score, a value's into its token's weight - its power of two into the exponent, which
 // the largest s counts in, so that neither weights nor sums leave their range:
-// 64 sequences of 1 to 16384 tokens of 32/8 heads of 128 in 8 bits with a scale for 16 tokens, 0.9 GB, 170 us.
+// 64 sequences of 1 to 16384 tokens of 32/8 heads of 128 in 8 bits with a scale for 32 tokens, 0.9 GB, 182 us.
 //
 // Work.  Short sequences: a cluster of CTAs has one key/value head of one sequence and cuts its tokens evenly (cluster_size has the rule).
 // Long ones: the tokens of every (sequence, key/value head) are cut into blocks of 16, all blocks are numbered through, and each warp of the grid
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(W * 32, Shape<T, FP8, SB, DP, NT, W>::kCtasPer
   // Range of the weights, to base 2.  bf16 ones are not lifted: they lose nothing below 1, and values may go up to the end of 32 bits themselves.
   constexpr float kLift = std::is_same_v<M, __half> ? 7.f : 0.f, kMostWeight = kLift + 8.f;
   // Two 16-bit numbers of a weight, so that a result is rounded once.  (bf16 queries over 8-bit pages with a scale for each head have one, good to 2^-12 of each weight.  With scales of
-  // blocks the second takes no time: 64 sequences of 1 to 16384 tokens of 32/8 heads of 128 186 us, 188 with one.)
+  // blocks one took, replayed, 171 us for 64 sequences of 1 to 16384 tokens of 32/8 heads of 128, 32.2 for 32 of 700 of 16/16 and 8.2 for one of 513; two 182, 33.6 and 8.2.)
   constexpr bool kTwoParts = !FP8 || SB || std::is_same_v<T, __half>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Piece pieces[2 * W];
