@@ -12,8 +12,8 @@
 //   rows many, tiles enough (kPair): two CTAs of a cluster have one tile of 256 rows x 256 features, each 128 of its rows in TMEM and 128 of either operand in shared
 //   memory, which the MMAs of both read.  The way from L2 brings an SM some 50 bytes a cycle: a group of a tile of 128 x 256 is 48 KB for 512 cycles of the tensor core,
 //   half a pair's tile 32 KB.  The tile's halves are multiplied, read and given back by themselves, a half for each group of warps.
-// 8192 rows of 4096 to 14336 features in bf16: 470 to 550 us by the clock that the power limit leaves (1.7 to 2.0 PFLOP/s; tiles of 128 x 128 640 us, of 128 x 256 without pairs
-// 570), of which loads and products alone take 332; the rest is the sums: 128 columns of a thread leave TMEM in four loads that wait, some 1000 cycles a group with what is around
+// 8192 rows of 4096 to 14336 features in bf16: 0.9 million cycles: 560 to 585 us in a loop (563 at 1590 MHz, 576 at 1560, which the power limit leaves), 470 to 515 after a pause (1.65 to 2.0 PFLOP/s;
+// beside 471 us tiles of 128 x 128 took 640 and of 128 x 256 without pairs 570), of which loads and products alone take 332; the rest is the sums: 128 columns of a thread leave TMEM in four loads that wait, some 1000 cycles a group with what is around
 // them, at two warps a scheduler.  Tried, us beside 471: four groups of warps 520, 16 columns a load 512, packed sums 540, more registers for the sums by setmaxnreg 484.
 // 64 rows of 4096 to 32000 in fp32: 30 us, 131 MB of weights; streaming them alone takes 24.  One row of 2048 to 6144: 6.1 us, a chain of launch, loads, products and join.
 #include <type_traits>
@@ -131,7 +131,7 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
 }
 
 // Waits for the phase with the given parity, giving up after 2^20 tries of a microsecond each at most: about a second.  The first tries are plain ones, which come back sooner
-// (509 rows of 2048 to 6144: 13.8 us, 14.8 without them).  (The timer takes longer to read than most of these waits, and code that may read it costs registers.)
+// (509 rows of 2048 to 6144: 1 us less than without them, of 15).  (The timer takes longer to read than most of these waits, and code that may read it costs registers.)
 __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity) {
   uint32_t done = 0;
 #pragma unroll 1
@@ -620,8 +620,8 @@ extern "C" int tris_e4m3_linear(const TrisE4m3Linear* linear, void* stream) {
   }
   const int64_t pairs = static_cast<int64_t>(ceil_div(a.rows, 2 * kLanes)) * ceil_div(a.out_features, 256);
   const int64_t small = static_cast<int64_t>(ceil_div(a.rows, kLanes)) * ceil_div(a.out_features, 128);
-  // Rounds of all SMs; one of pairs takes six fifths of one of small tiles.  us, pairs and small tiles: 256 x 2048 to 6144, a round either way, 14.0 and 11.1; 512 x 2048 to 6144,
-  // one round and two, 14.4 and 18.2; 768 x 14336 to 4096, one and two, 60 and 92; 8192 x 4096 to 14336, 25 and 49, 550 and 690.
+  // Rounds of all SMs; one of pairs takes six fifths of one of small tiles.  us, pairs and small tiles: 256 x 2048 to 6144, a round either way, 13.9 and 11.1; 512 x 2048 to 6144,
+  // one round and two, 14.3 and 18.1; 768 x 14336 to 4096, one and two, 60 and 95; 8192 x 4096 to 14336, 25 and 49, at one clock 546 and 728.
   const int64_t rounds_of_pairs = (pairs + sms / 2 - 1) / (sms / 2), rounds_of_small = (small + sms - 1) / sms;
   if (a.rows > kLanes && 6 * rounds_of_pairs <= 5 * rounds_of_small) return launch_linear<256, 2, Mode::kPair>(args, 1, s);
   return launch_linear<128, 2, Mode::kRows>(args, split_of(small, sms, args.groups, 16), s);

@@ -10,7 +10,8 @@
 // magnitudes meet in shared memory, and while they do the next head's are on their way.  A run longer than a CTA's rows is read twice, the second time from L2.
 //
 // 32/8 heads of 128 in bf16, blocks of 16 tokens, replayed: one token 5.3 us, 64 sequences' 5.7, a prompt of 512 tokens 6.9, of 2048 14, 4 of 2047 55 to 60 (165 MB, 2.8 TB/s:
-// some 40 instructions for every 16 bytes that are read hold the rest back).  Two heads at a time, 8.2 for one token and 59 for 4 of 2047; a warp for each run and head, which had the
+// 270 instructions for the 16 dimensions that a lane reads, at 20 warps an SM and 45 % of the issue slots, so latency holds the rest back).  Blocks of more than 16 tokens take a CTA a run, one window after the
+// other: 4 of 2047 tokens of 16/16 heads 58 us with blocks of 16, 120, 137 and 246 with 32, 64 and 128.  A decode step of 64 sequences whose blocks all get a larger scale, with some 8 tokens to bring along, takes 20 us.  Two heads at a time, 8.2 for one token and 59 for 4 of 2047; a warp for each run and head, which had the
 // rows' cosines to read for every head, 75.
 #include <float.h>
 
