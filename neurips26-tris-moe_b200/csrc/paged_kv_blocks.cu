@@ -69,30 +69,38 @@ __global__ void __launch_bounds__(kWindow * L, L == 16 ? 3 : L == 8 ? 6 : 12) pa
   uint32_t refused = 0;
   auto beginnings = [&](int w) {
     const int t = w + lane;
-    bool begins = true, again = false, hidden = false;
+    bool begins = true, again = false, hidden = false, valid = false;
+    int seq = 0, at_block = 0;  // of a token that has a place: its sequence and its block's first position
     if (t < r.num_tokens && t > 0 && r.sequences) {
       const int64_t pos = position(t), before = position(t - 1);
-      const bool same = r.sequences[t - 1] == r.sequences[t];
+      seq = r.sequences[t];
+      const bool same = r.sequences[t - 1] == seq;
       if (!outside(pos)) {
         const int at = in_block(static_cast<int>(pos));
+        valid = true;
+        at_block = static_cast<int>(pos) - at;
         begins = at == 0 || before != pos - 1 || !same;
         hidden = at && outside(before);
-        again = begins && same && !outside(before) && before - in_block(static_cast<int>(before)) == pos - at;
+        again = begins && same && !outside(before) && before - in_block(static_cast<int>(before)) == at_block;
       }
     }
+    if (__any_sync(0xFFFFFFFFu, hidden)) {  // tokens inside a block behind padding: what is ahead of that, among these 32 or, for the first of them, wherever it is
+      const uint32_t ahead = __ballot_sync(0xFFFFFFFFu, valid) & ((1u << lane) - 1);
+      const int from = ahead ? highest_bit(ahead) : 0;
+      const int ahead_seq = __shfl_sync(0xFFFFFFFFu, seq, from), ahead_block = __shfl_sync(0xFFFFFFFFu, at_block, from);  // (by all lanes, whatever is compared)
+      if (hidden && ahead) again = ahead_seq == seq && ahead_block == at_block;
+      const uint32_t ask = __ballot_sync(0xFFFFFFFFu, hidden && !ahead);  // one at most
+      if (ask) {
+        const int whose = lowest_bit(ask), want_seq = __shfl_sync(0xFFFFFFFFu, seq, whose), want_block = __shfl_sync(0xFFFFFFFFu, at_block, whose);
+        uint32_t found = 0;
 #pragma unroll 1
-    for (uint32_t ask = __ballot_sync(0xFFFFFFFFu, hidden); ask; ask &= ask - 1) {  // a token inside a block behind padding: what is ahead of that
-      const int token = w + lowest_bit(ask);
-      const int64_t pos = position(token);
-#pragma unroll 1
-      for (int t0 = token - 2;; t0 -= 32) {
-        const int64_t before = t0 - lane >= 0 ? position(t0 - lane) : 0;
-        const uint32_t found = __ballot_sync(0xFFFFFFFFu, t0 - lane < 0 || !outside(before));
-        if (!found) continue;
-        const bool it = lane == lowest_bit(found) && t0 - lane >= 0;
-        const bool here = it && r.sequences[t0 - lane] == r.sequences[token] && before - in_block(static_cast<int>(before)) == pos - in_block(static_cast<int>(pos));
-        if (__any_sync(0xFFFFFFFFu, here) && w + lane == token) again = true;
-        break;
+        for (int t0 = w + whose - 2; !found; t0 -= 32) {
+          const int other = t0 - lane;
+          const int64_t pos = other >= 0 ? position(other) : 0;
+          found = __ballot_sync(0xFFFFFFFFu, other < 0 || !outside(pos));
+          const bool here = found && lane == lowest_bit(found) && other >= 0 && r.sequences[other] == want_seq && pos - in_block(static_cast<int>(pos)) == want_block;
+          if (__any_sync(0xFFFFFFFFu, here) && lane == whose) again = true;
+        }
       }
     }
     refused = __ballot_sync(0xFFFFFFFFu, again);

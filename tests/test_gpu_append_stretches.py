@@ -70,6 +70,23 @@ def test_padded_batches_are_whole(lib):
         _check([s if p >= 0 else 99 for s, p in zip(seqs, positions)], positions, [])
 
 
+def test_free_slots_between_the_tokens_of_a_step(lib):
+    """A decode step of slots, some of them free, whose tokens stand inside blocks; and the same with one sequence twice, behind free slots near and far."""
+    slots = [(b, 3 + b % 9) if b % 3 else (b, -1) for b in range(80)]
+    seqs, positions = [b for b, _ in slots], [p for _, p in slots]
+    written, _, _, status = _append(seqs, positions, 16, 16, sequences=80)
+    assert status == 0 and written == {(b, p) for b, p in slots if p >= 0}
+    for at, gap in ((5, 1), (20, 7), (31, 1), (32, 1), (33, 40)):  # the slot at `at`, free slots, then its sequence once more
+        again = at + gap + 1
+        s, p = list(seqs), list(positions)
+        p[at] = 5
+        for i in range(at + 1, again):
+            p[i] = -1
+        s[again], p[again] = s[at], 7
+        written, _, _, status = _append(s, p, 16, 16, sequences=80)
+        assert written == {(s[i], p[i]) for i in range(80) if p[i] >= 0 and i != again} and status != 0, (at, gap)
+
+
 def test_other_sequences_at_the_same_positions(lib):
     _check([0, 1, 2, 3], [3, 3, 3, 3], [])
     _check([0, 0, 1, 1, 1], [3, 4, 4, 5, 6], [])
