@@ -9,7 +9,7 @@
 // of its row for one head after the other - two chunks of eight that rotate together - so that its cosines and sines are read once.  A head is rotated, its rows' largest
 // magnitudes meet in shared memory, and while they do the next head's are on their way.  A run longer than a CTA's rows is read twice, the second time from L2.
 //
-// 32/8 heads of 128 in bf16, blocks of 16 tokens, replayed: one token 5.3 us, 64 sequences' 5.7, a prompt of 512 tokens 6.9, of 2048 14, 4 of 2047 55 to 60 (165 MB, 2.8 TB/s:
+// 32/8 heads of 128 in bf16, blocks of 16 tokens, replayed: one token 5.1 us, 64 sequences' 5.7 (half of the slots free: 6.0), a prompt of 512 tokens 6.9, of 2048 14, 4 of 2047 55 to 60 (165 MB, 2.8 TB/s:
 // 270 instructions for the 16 dimensions that a lane reads, at 20 warps an SM and 45 % of the issue slots, so latency holds the rest back).  Blocks of more than 16 tokens take a CTA a run, one window after the
 // other: 4 of 2047 tokens of 16/16 heads 58 us with blocks of 16, 120, 137 and 246 with 32, 64 and 128.  A decode step of 64 sequences whose blocks all get a larger scale, with some 8 tokens to bring along, takes 20 us.  Two heads at a time, 8.2 for one token and 59 for 4 of 2047; a warp for each run and head, which had the
 // rows' cosines to read for every head, 75.
